@@ -349,6 +349,88 @@ tecoopsStatus_t tecoopsGemvInt8(tecoopsHandle_t handle, const int8_t *weight,
                                 const void *scales, const void *x, void *y,
                                 int batch, int n, int k);
 
+/* ---- operators of a decoder layer around attention.  Work on no rows (m or
+ *      num_tokens 0) is done without a launch. ---- */
+
+typedef enum {
+    TECOOPS_ACTIVATION_NONE = 0,
+    TECOOPS_ACTIVATION_RELU = 1,
+    TECOOPS_ACTIVATION_SILU = 2,
+    TECOOPS_ACTIVATION_GELU = 3,      /* v Phi(v) */
+    TECOOPS_ACTIVATION_GELU_TANH = 4, /* its tanh form */
+} tecoopsActivation_t;
+
+/* Matrix product with its epilogue, fp32 accumulation and one rounding:
+ *   out[m, n] = act(sum_k x[m, k] W[n, k] + bias[n]) + residual[m, n].
+ * gated != 0: weight holds n gate rows, then n up rows, bias [2n] likewise, and
+ *   out[m, n] = act(gate[m, n]) * up[m, n] + residual[m, n].
+ * x [m, k], residual and out [m, n] with row strides in elements (elements of a
+ * row adjacent); weight [n or 2n, k] packed; bias and residual may be NULL.
+ * residual may be out itself (same pointer and stride); other overlaps of out
+ * with an input are not allowed.  dataType HALF or BFLOAT16, any sizes (rows
+ * of x and W in whole, aligned 16-byte words are fastest) up to k and x_stride
+ * 2^21 and n 2^30.
+ * workspace: tecoopsGetLinearWorkspaceSize() bytes for the same sizes let few
+ * tiles be split along k; with less, or NULL, the call runs with fewer splits
+ * (slower, the same result up to fp32 rounding).  Nothing is allocated. */
+tecoopsStatus_t tecoopsLinear(tecoopsHandle_t handle, const void *x, long long x_stride,
+                              const void *weight, const void *bias,
+                              const void *residual, long long residual_stride,
+                              void *out, long long out_stride, int m, int n, int k,
+                              tecoopsActivation_t activation, int gated,
+                              void *workspace, size_t workspace_bytes,
+                              tecoopsDataType_t dataType);
+tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, int gated, size_t *bytes);
+
+/* Rotary positions of several axes (time, height, width of images and video).
+ * As tecoopsRotaryEmbedding, but positions is int64 [axes, num_tokens] (rows
+ * position_stride elements apart, at least num_tokens) and pair i of a head
+ * turns by the position of one axis.  sections (host, [axes]) are the axes'
+ * numbers of frequencies; their sum has to be rot_dim / 2.
+ *   CONTIGUOUS   the first sections[0] pairs to axis 0, the next to axis 1, ...;
+ *                pair i at base^(-2i/rot_dim)
+ *   INTERLEAVED  pair i to axis a = i % axes while i < axes * sections[a], else
+ *                to axis 0; pair i at base^(-2i/rot_dim).  The last pair of each
+ *                axis but the first has to lie within rot_dim / 2.
+ *   PER_AXIS     in ranges as CONTIGUOUS, but the j-th of an axis' n pairs at
+ *                base^(-j/n)
+ * With a cos_sin_cache (float32 [max_position, rot_dim]) column i of either half
+ * is pair i; a token with any position outside it is left as it is.  Without,
+ * angles are computed in 64 bits. */
+#define TECOOPS_ROTARY_MAX_AXES 4
+typedef enum {
+    TECOOPS_ROTARY_CONTIGUOUS = 0,
+    TECOOPS_ROTARY_INTERLEAVED = 1,
+    TECOOPS_ROTARY_PER_AXIS = 2,
+} tecoopsRotaryLayout_t;
+
+tecoopsStatus_t tecoopsRotaryEmbeddingAxes(tecoopsHandle_t handle, const int64_t *positions,
+                                           long long position_stride, int axes,
+                                           const int *sections, tecoopsRotaryLayout_t layout,
+                                           void *query, void *key, int num_tokens, int num_heads,
+                                           int num_kv_heads, int head_size, int rot_dim,
+                                           long long query_stride, long long key_stride,
+                                           const float *cos_sin_cache, int max_position,
+                                           float base, int is_neox, tecoopsDataType_t dataType);
+
+/* The same fused with the store into the paged caches, as
+ * tecoopsRotaryReshapeAndCache; the cached values are bit-identical to the two
+ * calls in sequence. */
+tecoopsStatus_t tecoopsRotaryAxesReshapeAndCache(tecoopsHandle_t handle, const int64_t *positions,
+                                                 long long position_stride, int axes,
+                                                 const int *sections,
+                                                 tecoopsRotaryLayout_t layout, void *query,
+                                                 void *key, const void *value,
+                                                 const int64_t *slot_mapping, void *key_cache,
+                                                 void *value_cache, int num_tokens, int num_heads,
+                                                 int num_kv_heads, int head_size, int rot_dim,
+                                                 long long query_stride, long long key_stride,
+                                                 long long value_stride,
+                                                 const float *cos_sin_cache, int max_position,
+                                                 float base, int is_neox, int num_blocks,
+                                                 int block_size, int write_key,
+                                                 tecoopsDataType_t dataType);
+
 #ifdef __cplusplus
 }
 #endif

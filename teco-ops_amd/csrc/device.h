@@ -101,6 +101,13 @@ __device__ __forceinline__ float half_swap_sum(float x) {
            __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
 }
 
+// Lane l + 32's value in lanes l < 32.
+__device__ __forceinline__ float from_upper_half(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
+}
+
 // Lane l combined with the lane that dpp_ctrl CTRL selects within its row of
 // 16 (a DPP operand of the VALU op, no LDS round trip).
 template <int CTRL>

@@ -32,12 +32,14 @@ inline long long gemv_batch_bytes(long long n, int r, int staged, bool i8, int c
 // 16-bit rows of a multiple of 32 KiB keep off 48, and off 16 in several rounds
 // (waves of 16 rows then queue on the same memory channels: [12288, 16384]
 // batch 8 81.2 at 48, 59.7 at 64, [10240, 16384] batch 3 67.1 at 16, 55.3 at 8).
-inline int gemv_batch_rows(int n, int k, int batch, bool i8, int cus) {
+// `fewest`: the smallest size that will do (gated products pair rows within
+// tiles of 16).
+inline int gemv_batch_rows(int n, int k, int batch, bool i8, int cus, int fewest = 8) {
     const int staged = gemv_batch_staged(batch);
     int best = 0;
     long long least = 0;
     for (int r : {128, 112, 96, 64, 48, 32, 16, 8}) {
-        if (r == 48 && staged > 8) continue;
+        if (r < fewest || (r == 48 && staged > 8)) continue;
         if (!i8 && k % 16384 == 0 && (r == 48 || (r == 16 && n > 16 * cus))) continue;
         if (r < 32 && i8 && staged > 32) continue;
         const long long bytes = gemv_batch_bytes(n, r, staged, i8, cus);
@@ -55,5 +57,13 @@ inline int gemv_batch_rows(int n, int k, int batch, bool i8, int cus) {
 // INTERNAL_ERROR when a launch fails.
 tecoopsStatus_t gemv_batch(hipStream_t s, const void *W, const void *scales, const void *x,
                            void *y, int batch, int n, int k, tecoopsDataType_t dataType, bool i8);
+
+struct Epilogue;  // epilogue.h
+
+// The same for up to 64 rows of x, x_stride elements apart, with an epilogue:
+// W of `wrows` 16-bit rows (gate and up together when e.gated).
+tecoopsStatus_t gemv_batch_epilogue(hipStream_t s, const void *W, const void *x, long long x_stride,
+                                    void *y, int batch, int wrows, int k,
+                                    tecoopsDataType_t dataType, const Epilogue &e);
 
 }  // namespace tecoops

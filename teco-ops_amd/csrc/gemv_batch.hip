@@ -29,10 +29,12 @@
 
 #include "common.h"
 #include "device.h"
+#include "epilogue.h"
 
 namespace {
 
 using namespace tecoops::dev;
+using tecoops::Epilogue;
 using tecoops::gemv_batch_rows;
 
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
@@ -127,11 +129,16 @@ struct Shape {
 // With RS > 1 one barrier per stage publishes the x copies of the other waves
 // and, since every wave passes it after reading stage i - 1, frees the slot
 // the next copies go to.  With RS = 1 a wave reads only what it copied.
-template <typename T, bool I8, int XR, int WR, int RS, int KS>
+//
+// EPI: rows of x are x_stride bytes apart and the sums end in `epi`.  Gated
+// products hold 8 gate rows and the 8 up rows of the same outputs in each tile
+// of 16, so that the two sums of an output meet 32 lanes apart; N is then the
+// number of outputs, half the rows of W.
+template <typename T, bool I8, int XR, int WR, int RS, int KS, bool EPI>
 __global__ void __launch_bounds__(RS * KS * 64)
 gemv_batch_kernel(const char *__restrict__ W, const uint16_t *__restrict__ scales,
-                  const char *__restrict__ x, uint16_t *__restrict__ y, int N, int K, int B,
-                  int pairs) {
+                  const char *__restrict__ x, uint16_t *y, int N, int K, int B,
+                  int pairs, long long x_stride, Epilogue epi) {
     using S = Shape<I8, XR, WR, RS, KS>;
     constexpr int NW = S::NW, CT = S::CT, RT = S::RT, D = S::D, WC = S::WC, XC = S::XC, PER = S::PER;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -149,7 +156,10 @@ gemv_batch_kernel(const char *__restrict__ W, const uint16_t *__restrict__ scale
 #pragma unroll
     for (int m = 0; m < WC; ++m) {
         const int row = 4 * m + (lane >> 4);
-        wsrc[m] = W + static_cast<long long>(min(n0 + row, N - 1)) * kw * 16;
+        int from = min(n0 + row, N - 1);
+        if (EPI && epi.gated)
+            from = min(n0 / 2 + (row >> 4) * 8 + (row & 7), N - 1) + ((row & 8) ? N : 0);
+        wsrc[m] = W + static_cast<long long>(from) * kw * 16;
         wch[m] = kp * nst * 16 + ((lane & 15) ^ (row & 7));
     }
     // x copy q: rows (1024 / XROW) q + lane / XCH, slot lane % XCH; a K part's
@@ -160,7 +170,7 @@ gemv_batch_kernel(const char *__restrict__ W, const uint16_t *__restrict__ scale
     for (int m = 0; m < XC; ++m) {
         const int q = (rs + m * RS) % S::XN;
         const int row = (1024 / S::XROW) * q + lane / XCH;
-        xsrc[m] = x + static_cast<long long>(min(row, B - 1)) * kx * 16;
+        xsrc[m] = x + min(row, B - 1) * (EPI ? x_stride : kx * 16LL);
         xch[m] = kp * nst * XCH + ((lane % XCH) ^ (row & 7));
         xdst[m] = q * 1024;
     }
@@ -255,6 +265,18 @@ gemv_batch_kernel(const char *__restrict__ W, const uint16_t *__restrict__ scale
     }
     // lane l holds column l % 16 of rows 4 (l / 16) .. + 3 of each tile
     const auto put = [&](int n, int col, f32x4_t s) {
+        if constexpr (EPI) {
+            f32x4_t u = s;
+            if (epi.gated) {
+                n = n / 16 * 8 + (n & 7);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) u[v] = from_upper_half(s[v]);
+            }
+            if (col >= B || (epi.gated && g >= 2) || (WR < 16 && g >= WR / 4)) return;
+            const float sv[4] = {s[0], s[1], s[2], s[3]}, uv[4] = {u[0], u[1], u[2], u[3]};
+            finish4<T>(epi, y, col, n, N, sv, uv);
+            return;
+        }
         if (col >= B || n >= N || (WR < 16 && g >= WR / 4)) return;
         if constexpr (I8) {
 #pragma unroll
@@ -295,17 +317,30 @@ gemv_batch_kernel(const char *__restrict__ W, const uint16_t *__restrict__ scale
     }
 }
 
-template <typename T, bool I8, int XR, int WR, int RS, int KS>
-bool launch(const void *W, const void *sc, const void *x, void *y, int B, int N, int K,
-            hipStream_t s) {
+// A product's operands; N counts the rows of W.
+struct Product {
+    const void *W, *scales, *x;
+    void *y;
+    int N, K;
+    long long x_stride;  // elements
+    const Epilogue *epi;  // null: the sums are stored as they are
+    hipStream_t stream;
+};
+
+template <typename T, bool I8, int XR, int WR, int RS, int KS, bool EPI>
+bool launch(const Product &p, int B) {
     using S = Shape<I8, XR, WR, RS, KS>;
     static_assert(S::D >= 2, "two stages fit in LDS");
-    auto *kern = &gemv_batch_kernel<T, I8, XR, WR, RS, KS>;
+    auto *kern = &gemv_batch_kernel<T, I8, XR, WR, RS, KS, EPI>;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), S::LDS)) return false;
-    const int pairs = N % 4 == 0 && tecoops::aligned(y, 8);
-    hipLaunchKernelGGL(kern, dim3(tecoops::ceil_div(N, WR * RS)), dim3(S::NW * 64), S::LDS, s,
-                       static_cast<const char *>(W), static_cast<const uint16_t *>(sc),
-                       static_cast<const char *>(x), static_cast<uint16_t *>(y), N, K, B, pairs);
+    const int pairs = p.N % 4 == 0 && tecoops::aligned(p.y, 8);
+    Epilogue e;
+    if (EPI) e = *p.epi;
+    hipLaunchKernelGGL(kern, dim3(tecoops::ceil_div(p.N, WR * RS)), dim3(S::NW * 64), S::LDS,
+                       p.stream, static_cast<const char *>(p.W),
+                       static_cast<const uint16_t *>(p.scales), static_cast<const char *>(p.x),
+                       static_cast<uint16_t *>(p.y), EPI && e.gated ? p.N / 2 : p.N, p.K, B, pairs,
+                       p.x_stride * 2, e);
     return true;
 }
 
@@ -328,54 +363,53 @@ bool launch(const void *W, const void *sc, const void *x, void *y, int B, int N,
 // 64 rows: two waves of 32 for 16-bit W (one LDS read of x serves two row
 // tiles), four of 16 for int8 ([14336, 4096] batch 8: fp16 19.1 / 21.6, int8
 // 13.6 / 12.3 µs).
-template <typename T, bool I8, int XR>
-bool launch_rows(const void *W, const void *sc, const void *x, void *y, int B, int N, int K,
-                 hipStream_t s) {
+template <typename T, bool I8, int XR, bool EPI>
+bool launch_rows(const Product &p, int B) {
+    const int N = p.N, K = p.K;
     // int8 stages hold twice the x: above 32 rows of x two of them fit only
     // with K split two ways, and 16 rows of W per workgroup are then no
     // faster than 32 ([4096, 14336] batch 64: 43.4 / 41.8 µs)
     constexpr bool kShortX = I8 && XR > 32;
     const int stages = (K / (I8 ? 16 : 8) + 15) / 16;
     const int cus = tecoops::device_cus();
-    switch (gemv_batch_rows(N, K, B, I8, cus)) {
+    switch (gemv_batch_rows(N, K, B, I8, cus, EPI && p.epi->gated ? 16 : 8)) {
         case 8:
             if constexpr (I8 && XR <= 8)
-                if (stages >= 16) return launch<T, I8, XR, 8, 1, 8>(W, sc, x, y, B, N, K, s);
-            if constexpr (!kShortX) return launch<T, I8, XR, 8, 1, 4>(W, sc, x, y, B, N, K, s);
+                if (stages >= 16) return launch<T, I8, XR, 8, 1, 8, EPI>(p, B);
+            if constexpr (!kShortX) return launch<T, I8, XR, 8, 1, 4, EPI>(p, B);
             return false;
         case 16:
             if constexpr (XR <= 8)
-                if (stages >= 32) return launch<T, I8, XR, 16, 1, 8>(W, sc, x, y, B, N, K, s);
-            if constexpr (!kShortX) return launch<T, I8, XR, 16, 1, 4>(W, sc, x, y, B, N, K, s);
+                if (stages >= 32) return launch<T, I8, XR, 16, 1, 8, EPI>(p, B);
+            if constexpr (!kShortX) return launch<T, I8, XR, 16, 1, 4, EPI>(p, B);
             return false;
         case 32:
             if constexpr (I8 && XR <= 8)
                 if (stages >= (XR <= 4 ? 32 : 16) && N <= 24 * cus)
-                    return launch<T, I8, XR, 16, 2, 4>(W, sc, x, y, B, N, K, s);
-            return launch<T, I8, XR, 16, 2, 2>(W, sc, x, y, B, N, K, s);
+                    return launch<T, I8, XR, 16, 2, 4, EPI>(p, B);
+            return launch<T, I8, XR, 16, 2, 2, EPI>(p, B);
         case 48:
-            if constexpr (XR <= 8) return launch<T, I8, XR, 16, 3, 2>(W, sc, x, y, B, N, K, s);
+            if constexpr (XR <= 8) return launch<T, I8, XR, 16, 3, 2, EPI>(p, B);
             return false;
         case 64:
             if constexpr (I8)
-                return launch<T, I8, XR, 16, 4, (kShortX ? 1 : 2)>(W, sc, x, y, B, N, K, s);
+                return launch<T, I8, XR, 16, 4, (kShortX ? 1 : 2), EPI>(p, B);
             else
-                return launch<T, I8, XR, 32, 2, 2>(W, sc, x, y, B, N, K, s);
-        case 96: return launch<T, I8, XR, 16, 6, 1>(W, sc, x, y, B, N, K, s);
-        case 112: return launch<T, I8, XR, 16, 7, 1>(W, sc, x, y, B, N, K, s);
-        default: return launch<T, I8, XR, 16, 8, 1>(W, sc, x, y, B, N, K, s);
+                return launch<T, I8, XR, 32, 2, 2, EPI>(p, B);
+        case 96: return launch<T, I8, XR, 16, 6, 1, EPI>(p, B);
+        case 112: return launch<T, I8, XR, 16, 7, 1, EPI>(p, B);
+        default: return launch<T, I8, XR, 16, 8, 1, EPI>(p, B);
     }
 }
 
-template <typename T, bool I8>
-bool launch_batch(const void *W, const void *sc, const void *x, void *y, int B, int N, int K,
-                  hipStream_t s) {
-    if (B <= 4) return launch_rows<T, I8, 4>(W, sc, x, y, B, N, K, s);
-    if (B <= 8) return launch_rows<T, I8, 8>(W, sc, x, y, B, N, K, s);
-    if (B <= 16) return launch_rows<T, I8, 16>(W, sc, x, y, B, N, K, s);
-    if (B <= 32) return launch_rows<T, I8, 32>(W, sc, x, y, B, N, K, s);
-    if (B <= 48) return launch_rows<T, I8, 48>(W, sc, x, y, B, N, K, s);
-    return launch_rows<T, I8, 64>(W, sc, x, y, B, N, K, s);
+template <typename T, bool I8, bool EPI>
+bool launch_batch(const Product &p, int B) {
+    if (B <= 4) return launch_rows<T, I8, 4, EPI>(p, B);
+    if (B <= 8) return launch_rows<T, I8, 8, EPI>(p, B);
+    if (B <= 16) return launch_rows<T, I8, 16, EPI>(p, B);
+    if (B <= 32) return launch_rows<T, I8, 32, EPI>(p, B);
+    if (B <= 48) return launch_rows<T, I8, 48, EPI>(p, B);
+    return launch_rows<T, I8, 64, EPI>(p, B);
 }
 
 }  // namespace
@@ -386,14 +420,25 @@ tecoopsStatus_t tecoops::gemv_batch(hipStream_t s, const void *W, const void *sc
     constexpr int kSlice = 64;
     for (int b0 = 0; b0 < batch; b0 += kSlice) {
         const int nb = batch - b0 < kSlice ? batch - b0 : kSlice;
-        const void *xb = static_cast<const uint16_t *>(x) + static_cast<long long>(b0) * k;
-        void *yb = static_cast<uint16_t *>(y) + static_cast<long long>(b0) * n;
-        const bool ok = i8 ? launch_batch<f16, true>(W, scales, xb, yb, nb, n, k, s)
-                        : dataType == TECOOPS_DATA_HALF
-                            ? launch_batch<f16, false>(W, nullptr, xb, yb, nb, n, k, s)
-                            : launch_batch<bf16, false>(W, nullptr, xb, yb, nb, n, k, s);
+        Product p{W, scales, static_cast<const uint16_t *>(x) + static_cast<long long>(b0) * k,
+                  static_cast<uint16_t *>(y) + static_cast<long long>(b0) * n, n, k, k, nullptr, s};
+        const bool ok = i8 ? launch_batch<f16, true, false>(p, nb)
+                        : dataType == TECOOPS_DATA_HALF ? launch_batch<f16, false, false>(p, nb)
+                                                        : launch_batch<bf16, false, false>(p, nb);
         if (!ok) return TECOOPS_STATUS_INTERNAL_ERROR;
         TECO_CHECK_LAUNCH("gemv");
     }
+    return TECOOPS_STATUS_SUCCESS;
+}
+
+tecoopsStatus_t tecoops::gemv_batch_epilogue(hipStream_t s, const void *W, const void *x,
+                                             long long x_stride, void *y, int batch, int wrows,
+                                             int k, tecoopsDataType_t dataType, const Epilogue &e) {
+    if (batch > 64) return TECOOPS_STATUS_INTERNAL_ERROR;
+    Product p{W, nullptr, x, y, wrows, k, x_stride, &e, s};
+    const bool ok = dataType == TECOOPS_DATA_HALF ? launch_batch<f16, false, true>(p, batch)
+                                                  : launch_batch<bf16, false, true>(p, batch);
+    if (!ok) return TECOOPS_STATUS_INTERNAL_ERROR;
+    TECO_CHECK_LAUNCH("linear");
     return TECOOPS_STATUS_SUCCESS;
 }

@@ -15,6 +15,10 @@
 // loads of several tasks before any store (one memory round trip per batch
 // instead of per task).  HBM-bound: every byte of q and k is read once and
 // written once.
+//
+// Positions of several axes (time, height, width of images and video): pair i
+// turns by the position of the axis its frequency belongs to.  Only the angles
+// of a token differ, so the same kernels run with another source of them.
 #include "common.h"
 #include "device.h"
 
@@ -24,6 +28,102 @@ using namespace tecoops::dev;
 
 constexpr int kThreads = 256;
 constexpr int kMaxHalf = 256;  // rot_dim <= 512
+
+// Where the angles of token t come from: angle(t, i) is (cos, sin) of pair i,
+// skipped(t) whether the token is left unturned.
+
+// One position per token; angles computed in fp32, or read from the table
+// float32 [max_position, rot_dim], cos then sin.
+struct OnePosition {
+    const int64_t *__restrict__ positions;
+    const float *__restrict__ cos_sin_cache;
+    int max_position, rot_dim;
+    float log2_base;
+
+    // tokens outside the table turn by nothing in the fused kernel: pairs with
+    // an infinity become NaN there
+    static constexpr bool kCopySkipped = false;
+
+    __device__ __forceinline__ float2 angle(int t, int i) const {
+        const int half = rot_dim >> 1;
+        const int64_t pos = positions[t];
+        float c = 1.0f, s = 0.0f;
+        if (cos_sin_cache != nullptr) {
+            if (pos >= 0 && pos < max_position) {
+                c = cos_sin_cache[pos * rot_dim + i];
+                s = cos_sin_cache[pos * rot_dim + half + i];
+            }
+        } else {
+            const float inv_freq = exp2f(-(2.0f * i / static_cast<float>(rot_dim)) * log2_base);
+            sincosf(static_cast<float>(pos) * inv_freq, &s, &c);
+        }
+        return make_float2(c, s);
+    }
+    __device__ __forceinline__ bool skipped(int t) const {
+        if (cos_sin_cache == nullptr) return false;
+        const int64_t pos = positions[t];
+        return pos < 0 || pos >= max_position;
+    }
+};
+
+// One position per token and axis, positions[axis * stride + t].  first[a] is
+// the first frequency of axis a in ranges of them, first[a + 1] - first[a] its
+// number of frequencies.  Angles are computed in turns in 64 bits and reduced
+// to half a turn before sin and cos, so that far positions lose nothing: in 32
+// bits an angle of 200000 is off by up to 0.008.
+struct AxisPositions {
+    const int64_t *__restrict__ positions;
+    long long stride;
+    const float *__restrict__ cos_sin_cache;
+    int max_position, rot_dim, axes, layout;
+    int first[TECOOPS_ROTARY_MAX_AXES + 1];
+    double log2_base;
+
+    static constexpr bool kCopySkipped = true;  // as they are, whatever they hold
+
+    __device__ __forceinline__ float2 angle(int t, int i) const {
+        const int half = rot_dim >> 1;
+        int axis = 0, from = 0, n = first[1];
+        if (layout == TECOOPS_ROTARY_INTERLEAVED) {
+            const int a = i % axes;
+#pragma unroll
+            for (int b = 1; b < TECOOPS_ROTARY_MAX_AXES; ++b)
+                if (a == b && i < axes * (first[b + 1] - first[b])) axis = b;
+        } else {
+#pragma unroll
+            for (int b = 1; b < TECOOPS_ROTARY_MAX_AXES; ++b)
+                if (b < axes && i >= first[b]) {
+                    axis = b;
+                    from = first[b];
+                    n = first[b + 1] - first[b];
+                }
+        }
+        const int64_t pos = positions[axis * stride + t];
+        float c = 1.0f, s = 0.0f;
+        if (cos_sin_cache != nullptr) {
+            if (pos >= 0 && pos < max_position) {
+                c = cos_sin_cache[pos * rot_dim + i];
+                s = cos_sin_cache[pos * rot_dim + half + i];
+            }
+            return make_float2(c, s);
+        }
+        const double power = layout == TECOOPS_ROTARY_PER_AXIS
+                                 ? static_cast<double>(i - from) / n
+                                 : static_cast<double>(i) / half;
+        const double turns = static_cast<double>(pos) * (exp2(-power * log2_base) * 0.15915494309189535);
+        sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
+        return make_float2(c, s);
+    }
+    __device__ __forceinline__ bool skipped(int t) const {
+        if (cos_sin_cache == nullptr) return false;
+        bool out = false;
+        for (int a = 0; a < axes; ++a) {
+            const int64_t pos = positions[a * stride + t];
+            out = out || pos < 0 || pos >= max_position;
+        }
+        return out;
+    }
+};
 
 // One token per workgroup, each thread's (at most two) tasks loaded together
 // before any store.  More tokens per workgroup put more of q and k in flight
@@ -102,12 +202,11 @@ __device__ __forceinline__ void rot_pair(uint16_t x1b, uint16_t x2b, float2 cc, 
 
 // VW: 0 one pair per task; 1 four pairs (8-byte NeoX / 16-byte GPT-J words);
 // 2 eight NeoX pairs (16-byte words).  q and k are streamed (non-temporal).
-template <typename T, bool NEOX, int VW>
+template <typename T, bool NEOX, int VW, typename Angles>
 __global__ void __launch_bounds__(kThreads)
-rotary_kernel(const int64_t *__restrict__ positions, uint16_t *__restrict__ query,
-              uint16_t *__restrict__ key, int num_tokens, int num_heads, int num_kv_heads,
-              int head_size, int rot_dim, long long q_stride, long long k_stride,
-              const float *__restrict__ cos_sin_cache, int max_position, float log2_base) {
+rotary_kernel(Angles angles, uint16_t *__restrict__ query, uint16_t *__restrict__ key,
+              int num_tokens, int num_heads, int num_kv_heads, int head_size, int rot_dim,
+              long long q_stride, long long k_stride) {
     __shared__ float2 cs[kTokensPerBlock][kMaxHalf];
     __shared__ int skip[kTokensPerBlock];
     const int half = rot_dim >> 1;
@@ -116,27 +215,11 @@ rotary_kernel(const int64_t *__restrict__ positions, uint16_t *__restrict__ quer
         const int tt = e / half, i = e - tt * half;
         const int t = tbase + tt;
         if (t >= num_tokens) continue;
-        const int64_t pos = positions[t];
-        float c = 1.0f, s = 0.0f;
-        if (cos_sin_cache != nullptr) {
-            if (pos >= 0 && pos < max_position) {
-                c = cos_sin_cache[pos * rot_dim + i];
-                s = cos_sin_cache[pos * rot_dim + half + i];
-            }
-        } else {
-            const float inv_freq = exp2f(-(2.0f * i / static_cast<float>(rot_dim)) * log2_base);
-            sincosf(static_cast<float>(pos) * inv_freq, &s, &c);
-        }
-        cs[tt][i] = make_float2(c, s);
+        cs[tt][i] = angles.angle(t, i);
     }
     if (threadIdx.x < kTokensPerBlock) {
         const int t = tbase + threadIdx.x;
-        int sk = t >= num_tokens;
-        if (!sk && cos_sin_cache != nullptr) {
-            const int64_t pos = positions[t];
-            sk = pos < 0 || pos >= max_position;
-        }
-        skip[threadIdx.x] = sk;
+        skip[threadIdx.x] = t >= num_tokens || angles.skipped(t);
     }
     __syncthreads();
     constexpr int P = VW == 2 ? 8 : VW == 1 ? 4 : 1;  // pairs per lane-task
@@ -230,7 +313,6 @@ rotary_kernel(const int64_t *__restrict__ positions, uint16_t *__restrict__ quer
 // rotated (identity), as in rotary_kernel, but is still cached; slots < 0 or
 // >= num_blocks * block_size are not cached, as in reshape_and_cache.
 struct FusedArgs {
-    const int64_t *positions;
     uint16_t *query;
     uint16_t *key;
     const uint16_t *value;
@@ -239,16 +321,13 @@ struct FusedArgs {
     uint16_t *vcache;
     int num_tokens, num_heads, num_kv_heads, head_size, rot_dim;
     long long q_stride, k_stride, v_stride;
-    const float *cos_sin_cache;
-    int max_position;
-    float log2_base;
     int block_size, lbs;  // lbs = log2(block_size) or -1
     long long capacity;   // num_blocks * block_size
     int write_key;
 };
 
-template <typename T, bool NEOX, int VW>
-__global__ void __launch_bounds__(kThreads) rotary_cache_kernel(FusedArgs a) {
+template <typename T, bool NEOX, int VW, typename Angles>
+__global__ void __launch_bounds__(kThreads) rotary_cache_kernel(Angles angles, FusedArgs a) {
     __shared__ float2 cs[kTokensPerBlock][kMaxHalf];
     __shared__ long long crow[kTokensPerBlock];  // first element of the token's cache row, or -1
     const int half = a.rot_dim >> 1;
@@ -258,18 +337,7 @@ __global__ void __launch_bounds__(kThreads) rotary_cache_kernel(FusedArgs a) {
         const int tt = e / half, i = e - tt * half;
         const int t = tbase + tt;
         if (t >= a.num_tokens) continue;
-        const int64_t pos = a.positions[t];
-        float c = 1.0f, sn = 0.0f;
-        if (a.cos_sin_cache != nullptr) {
-            if (pos >= 0 && pos < a.max_position) {
-                c = a.cos_sin_cache[pos * a.rot_dim + i];
-                sn = a.cos_sin_cache[pos * a.rot_dim + half + i];
-            }
-        } else {
-            const float inv_freq = exp2f(-(2.0f * i / static_cast<float>(a.rot_dim)) * a.log2_base);
-            sincosf(static_cast<float>(pos) * inv_freq, &sn, &c);
-        }
-        cs[tt][i] = make_float2(c, sn);
+        cs[tt][i] = angles.angle(t, i);
     }
     if (threadIdx.x < kTokensPerBlock) {
         const int t = tbase + threadIdx.x;
@@ -286,6 +354,19 @@ __global__ void __launch_bounds__(kThreads) rotary_cache_kernel(FusedArgs a) {
         crow[threadIdx.x] = r;
     }
     __syncthreads();
+    if constexpr (Angles::kCopySkipped) {
+        static_assert(kTokensPerBlock == 1, "the whole workgroup's token");
+        if (angles.skipped(tbase)) {
+            if (crow[0] < 0) return;
+            for (int e = threadIdx.x; e < a.num_kv_heads * D; e += blockDim.x) {
+                const int h = e / D, d = e - h * D;
+                const long long at = crow[0] + h * static_cast<long long>(a.block_size) * D + d;
+                a.kcache[at] = a.key[tbase * a.k_stride + e];
+                a.vcache[at] = a.value[tbase * a.v_stride + e];
+            }
+            return;
+        }
+    }
     constexpr bool VEC = VW >= 1;
     constexpr int P = VW == 2 ? 8 : VW == 1 ? 4 : 1;  // rotation pairs per task
     constexpr int CV = VEC ? 8 : 1;                   // elements per copy task
@@ -497,154 +578,143 @@ __global__ void __launch_bounds__(kThreads) rotary_cache_kernel(FusedArgs a) {
     }
 }
 
-template <typename T, bool NEOX, int VW>
-void launch_vw(int T_, hipStream_t s, const int64_t *pos, void *q, void *k, int H, int Hkv, int D,
-               int rot, long long qs, long long ks, const float *cache, int maxpos, float lb) {
-    const unsigned grid = tecoops::ceil_div(T_, kTokensPerBlock);
-    hipLaunchKernelGGL((rotary_kernel<T, NEOX, VW>), dim3(grid), dim3(kThreads), 0, s, pos,
-                       static_cast<uint16_t *>(q), static_cast<uint16_t *>(k), T_, H, Hkv, D, rot,
-                       qs, ks, cache, maxpos, lb);
+// Heads and strides of a call, and the widest words it can be done in.
+struct Rows {
+    void *query, *key;
+    int num_tokens, num_heads, num_kv_heads, head_size, rot_dim;
+    long long query_stride, key_stride;
+};
+
+template <typename T, bool NEOX, int VW, typename Angles>
+void launch_vw(const Angles &an, const Rows &r, hipStream_t s) {
+    const unsigned grid = tecoops::ceil_div(r.num_tokens, kTokensPerBlock);
+    hipLaunchKernelGGL((rotary_kernel<T, NEOX, VW, Angles>), dim3(grid), dim3(kThreads), 0, s, an,
+                       static_cast<uint16_t *>(r.query), static_cast<uint16_t *>(r.key),
+                       r.num_tokens, r.num_heads, r.num_kv_heads, r.head_size, r.rot_dim,
+                       r.query_stride, r.key_stride);
 }
 
-template <typename T, bool NEOX>
-void launch(int vw, int T_, hipStream_t s, const int64_t *pos, void *q, void *k, int H,
-            int Hkv, int D, int rot, long long qs, long long ks, const float *cache, int maxpos,
-            float lb) {
+template <typename T, bool NEOX, typename Angles>
+void launch(int vw, const Angles &an, const Rows &r, hipStream_t s) {
     if (vw == 2)
-        launch_vw<T, NEOX, NEOX ? 2 : 1>(T_, s, pos, q, k, H, Hkv, D, rot, qs, ks, cache, maxpos, lb);
+        launch_vw<T, NEOX, NEOX ? 2 : 1>(an, r, s);
     else if (vw == 1)
-        launch_vw<T, NEOX, 1>(T_, s, pos, q, k, H, Hkv, D, rot, qs, ks, cache, maxpos, lb);
+        launch_vw<T, NEOX, 1>(an, r, s);
     else
-        launch_vw<T, NEOX, 0>(T_, s, pos, q, k, H, Hkv, D, rot, qs, ks, cache, maxpos, lb);
+        launch_vw<T, NEOX, 0>(an, r, s);
 }
 
-}  // namespace
-
-extern "C" tecoopsStatus_t tecoopsRotaryEmbedding(tecoopsHandle_t handle,
-                                                  const int64_t *positions, void *query,
-                                                  void *key, int num_tokens, int num_heads,
-                                                  int num_kv_heads, int head_size, int rot_dim,
-                                                  long long query_stride, long long key_stride,
-                                                  const float *cos_sin_cache, int max_position,
-                                                  float base, int is_neox,
-                                                  tecoopsDataType_t dataType) {
-    if (handle == nullptr) return TECOOPS_STATUS_NOT_INITIALIZED;
-    if (positions == nullptr || query == nullptr) return TECOOPS_STATUS_BAD_PARAM;
-    if (num_tokens <= 0 || num_heads <= 0 || head_size <= 0) return TECOOPS_STATUS_BAD_PARAM;
-    if (key != nullptr && num_kv_heads <= 0) return TECOOPS_STATUS_BAD_PARAM;
-    if (rot_dim <= 0 || (rot_dim & 1) || rot_dim > head_size || rot_dim / 2 > kMaxHalf)
+// Arguments that both kinds of positions share.
+tecoopsStatus_t check_rows(const Rows &r, const void *positions, const float *cos_sin_cache,
+                           int max_position, float base, tecoopsDataType_t dataType) {
+    if (positions == nullptr || r.query == nullptr) return TECOOPS_STATUS_BAD_PARAM;
+    if (r.num_tokens <= 0 || r.num_heads <= 0 || r.head_size <= 0) return TECOOPS_STATUS_BAD_PARAM;
+    if (r.key != nullptr && r.num_kv_heads <= 0) return TECOOPS_STATUS_BAD_PARAM;
+    if (r.rot_dim <= 0 || (r.rot_dim & 1) || r.rot_dim > r.head_size || r.rot_dim / 2 > kMaxHalf)
         return TECOOPS_STATUS_BAD_PARAM;
-    if (query_stride < static_cast<long long>(num_heads) * head_size) return TECOOPS_STATUS_BAD_PARAM;
-    if (key != nullptr && key_stride < static_cast<long long>(num_kv_heads) * head_size)
+    if (r.query_stride < static_cast<long long>(r.num_heads) * r.head_size)
+        return TECOOPS_STATUS_BAD_PARAM;
+    if (r.key != nullptr && r.key_stride < static_cast<long long>(r.num_kv_heads) * r.head_size)
         return TECOOPS_STATUS_BAD_PARAM;
     if (cos_sin_cache != nullptr && max_position <= 0) return TECOOPS_STATUS_BAD_PARAM;
     if (cos_sin_cache == nullptr && !(base > 0.0f)) return TECOOPS_STATUS_BAD_PARAM;
     if (!tecoops::is_16bit_float(dataType)) return TECOOPS_STATUS_BAD_PARAM;
-    const int half = rot_dim / 2;
+    return TECOOPS_STATUS_SUCCESS;
+}
+
+template <typename Angles>
+tecoopsStatus_t run_rotary(const Angles &an, Rows r, int is_neox, tecoopsDataType_t dataType,
+                           hipStream_t s) {
+    const int half = r.rot_dim / 2;
     // Vector paths: 4 pairs per lane with naturally aligned 8 / 16 byte
     // accesses, or 8 NeoX pairs per lane in 16-byte words.
     const size_t align = is_neox ? 8 : 16;
-    bool vec = (half % 4) == 0 && (head_size % 4) == 0 && (query_stride % 4) == 0 &&
-               tecoops::aligned(query, align);
-    if (key != nullptr) vec = vec && (key_stride % 4) == 0 && tecoops::aligned(key, align);
-    if (!is_neox) vec = vec && (head_size % 8) == 0 && (query_stride % 8) == 0 &&
-                        (key == nullptr || (key_stride % 8) == 0);
+    bool vec = (half % 4) == 0 && (r.head_size % 4) == 0 && (r.query_stride % 4) == 0 &&
+               tecoops::aligned(r.query, align);
+    if (r.key != nullptr) vec = vec && (r.key_stride % 4) == 0 && tecoops::aligned(r.key, align);
+    if (!is_neox) vec = vec && (r.head_size % 8) == 0 && (r.query_stride % 8) == 0 &&
+                        (r.key == nullptr || (r.key_stride % 8) == 0);
     // NeoX with 8 pairs per lane: both halves in 16-byte words
-    bool wide = is_neox && vec && (half % 8) == 0 && (head_size % 8) == 0 &&
-                (query_stride % 8) == 0 && tecoops::aligned(query, 16);
-    if (key != nullptr) wide = wide && (key_stride % 8) == 0 && tecoops::aligned(key, 16);
+    bool wide = is_neox && vec && (half % 8) == 0 && (r.head_size % 8) == 0 &&
+                (r.query_stride % 8) == 0 && tecoops::aligned(r.query, 16);
+    if (r.key != nullptr) wide = wide && (r.key_stride % 8) == 0 && tecoops::aligned(r.key, 16);
     const int vw = wide ? 2 : vec ? 1 : 0;
-    const float lb = cos_sin_cache ? 0.0f : log2f(base);
-    const int Hkv = key ? num_kv_heads : 0;
+    if (r.key == nullptr) r.num_kv_heads = 0;
     using tecoops::dev::bf16;
     using tecoops::dev::f16;
-    hipStream_t s = handle->stream;
     if (dataType == TECOOPS_DATA_HALF) {
-        if (is_neox) launch<f16, true>(vw, num_tokens, s, positions, query, key, num_heads, Hkv,
-                                       head_size, rot_dim, query_stride, key_stride,
-                                       cos_sin_cache, max_position, lb);
-        else launch<f16, false>(vw, num_tokens, s, positions, query, key, num_heads, Hkv,
-                                head_size, rot_dim, query_stride, key_stride, cos_sin_cache,
-                                max_position, lb);
+        if (is_neox) launch<f16, true>(vw, an, r, s);
+        else launch<f16, false>(vw, an, r, s);
     } else {
-        if (is_neox) launch<bf16, true>(vw, num_tokens, s, positions, query, key, num_heads, Hkv,
-                                        head_size, rot_dim, query_stride, key_stride,
-                                        cos_sin_cache, max_position, lb);
-        else launch<bf16, false>(vw, num_tokens, s, positions, query, key, num_heads, Hkv,
-                                 head_size, rot_dim, query_stride, key_stride, cos_sin_cache,
-                                 max_position, lb);
+        if (is_neox) launch<bf16, true>(vw, an, r, s);
+        else launch<bf16, false>(vw, an, r, s);
     }
     TECO_CHECK_LAUNCH("rotary_embedding");
     return TECOOPS_STATUS_SUCCESS;
 }
 
-extern "C" tecoopsStatus_t tecoopsRotaryReshapeAndCache(
-    tecoopsHandle_t handle, const int64_t *positions, void *query, void *key, const void *value,
-    const int64_t *slot_mapping, void *key_cache, void *value_cache, int num_tokens,
-    int num_heads, int num_kv_heads, int head_size, int rot_dim, long long query_stride,
-    long long key_stride, long long value_stride, const float *cos_sin_cache, int max_position,
-    float base, int is_neox, int num_blocks, int block_size, int write_key,
-    tecoopsDataType_t dataType) {
-    if (handle == nullptr) return TECOOPS_STATUS_NOT_INITIALIZED;
-    if (positions == nullptr || query == nullptr || key == nullptr || value == nullptr ||
-        slot_mapping == nullptr || key_cache == nullptr || value_cache == nullptr)
+// The paged caches that the fused kernel writes to.
+struct Pages {
+    const void *value;
+    const int64_t *slot_mapping;
+    void *key_cache, *value_cache;
+    long long value_stride;
+    int num_blocks, block_size, write_key;
+};
+
+tecoopsStatus_t check_pages(const Rows &r, const Pages &g) {
+    if (r.key == nullptr || g.value == nullptr || g.slot_mapping == nullptr ||
+        g.key_cache == nullptr || g.value_cache == nullptr)
         return TECOOPS_STATUS_BAD_PARAM;
-    if (num_tokens <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 ||
-        num_blocks <= 0 || block_size <= 0)
+    if (g.num_blocks <= 0 || g.block_size <= 0) return TECOOPS_STATUS_BAD_PARAM;
+    if (g.value_stride < static_cast<long long>(r.num_kv_heads) * r.head_size)
         return TECOOPS_STATUS_BAD_PARAM;
-    if (rot_dim <= 0 || (rot_dim & 1) || rot_dim > head_size || rot_dim / 2 > kMaxHalf)
-        return TECOOPS_STATUS_BAD_PARAM;
-    if (query_stride < static_cast<long long>(num_heads) * head_size ||
-        key_stride < static_cast<long long>(num_kv_heads) * head_size ||
-        value_stride < static_cast<long long>(num_kv_heads) * head_size)
-        return TECOOPS_STATUS_BAD_PARAM;
-    if (cos_sin_cache != nullptr && max_position <= 0) return TECOOPS_STATUS_BAD_PARAM;
-    if (cos_sin_cache == nullptr && !(base > 0.0f)) return TECOOPS_STATUS_BAD_PARAM;
-    if (!tecoops::is_16bit_float(dataType)) return TECOOPS_STATUS_BAD_PARAM;
-    const long long capacity = static_cast<long long>(num_blocks) * block_size;
-    if (capacity >= (1ll << 31)) return TECOOPS_STATUS_NOT_SUPPORTED;
+    if (static_cast<long long>(g.num_blocks) * g.block_size >= (1ll << 31))
+        return TECOOPS_STATUS_NOT_SUPPORTED;
+    return TECOOPS_STATUS_SUCCESS;
+}
+
+template <typename Angles>
+tecoopsStatus_t run_fused(const Angles &an, const Rows &r, const Pages &g, int is_neox,
+                          tecoopsDataType_t dataType, hipStream_t s) {
     FusedArgs a{};
-    a.positions = positions;
-    a.query = static_cast<uint16_t *>(query);
-    a.key = static_cast<uint16_t *>(key);
-    a.value = static_cast<const uint16_t *>(value);
-    a.slots = slot_mapping;
-    a.kcache = static_cast<uint16_t *>(key_cache);
-    a.vcache = static_cast<uint16_t *>(value_cache);
-    a.num_tokens = num_tokens;
-    a.num_heads = num_heads;
-    a.num_kv_heads = num_kv_heads;
-    a.head_size = head_size;
-    a.rot_dim = rot_dim;
-    a.q_stride = query_stride;
-    a.k_stride = key_stride;
-    a.v_stride = value_stride;
-    a.cos_sin_cache = cos_sin_cache;
-    a.max_position = max_position;
-    a.log2_base = cos_sin_cache ? 0.0f : log2f(base);
-    a.block_size = block_size;
-    a.lbs = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
-    a.capacity = capacity;
-    a.write_key = write_key;
+    a.query = static_cast<uint16_t *>(r.query);
+    a.key = static_cast<uint16_t *>(r.key);
+    a.value = static_cast<const uint16_t *>(g.value);
+    a.slots = g.slot_mapping;
+    a.kcache = static_cast<uint16_t *>(g.key_cache);
+    a.vcache = static_cast<uint16_t *>(g.value_cache);
+    a.num_tokens = r.num_tokens;
+    a.num_heads = r.num_heads;
+    a.num_kv_heads = r.num_kv_heads;
+    a.head_size = r.head_size;
+    a.rot_dim = r.rot_dim;
+    a.q_stride = r.query_stride;
+    a.k_stride = r.key_stride;
+    a.v_stride = g.value_stride;
+    a.block_size = g.block_size;
+    a.lbs = (g.block_size & (g.block_size - 1)) == 0 ? __builtin_ctz(g.block_size) : -1;
+    a.capacity = static_cast<long long>(g.num_blocks) * g.block_size;
+    a.write_key = g.write_key;
     // Vector path: 4 (or 8) pairs per rotation task and 16-byte value / tail
     // copies, all naturally aligned.
-    const int half = rot_dim / 2;
+    const int half = r.rot_dim / 2;
     const size_t ra = is_neox ? 8 : 16;
-    bool vec = (half % 4) == 0 && (head_size % 8) == 0 && ((head_size - rot_dim) % 8) == 0 &&
-               (query_stride % 8) == 0 && (key_stride % 8) == 0 && (value_stride % 8) == 0 &&
-               tecoops::aligned(query, ra) && tecoops::aligned(key, ra) &&
-               tecoops::aligned(value, 16) && tecoops::aligned(key_cache, 16) &&
-               tecoops::aligned(value_cache, 16);
+    bool vec = (half % 4) == 0 && (r.head_size % 8) == 0 && ((r.head_size - r.rot_dim) % 8) == 0 &&
+               (r.query_stride % 8) == 0 && (r.key_stride % 8) == 0 && (g.value_stride % 8) == 0 &&
+               tecoops::aligned(r.query, ra) && tecoops::aligned(r.key, ra) &&
+               tecoops::aligned(g.value, 16) && tecoops::aligned(g.key_cache, 16) &&
+               tecoops::aligned(g.value_cache, 16);
     // NeoX with 8 pairs per lane: both halves in 16-byte words
-    const bool wide = is_neox && vec && (half % 8) == 0 && tecoops::aligned(query, 16) &&
-                      tecoops::aligned(key, 16);
-    const unsigned grid = tecoops::ceil_div(num_tokens, kTokensPerBlock);
+    const bool wide = is_neox && vec && (half % 8) == 0 && tecoops::aligned(r.query, 16) &&
+                      tecoops::aligned(r.key, 16);
+    const unsigned grid = tecoops::ceil_div(r.num_tokens, kTokensPerBlock);
     using tecoops::dev::bf16;
     using tecoops::dev::f16;
-    hipStream_t s = handle->stream;
     const bool h16 = dataType == TECOOPS_DATA_HALF;
-#define TECO_ROT_CACHE(TT, NX, VV) \
-    hipLaunchKernelGGL((rotary_cache_kernel<TT, NX, VV>), dim3(grid), dim3(kThreads), 0, s, a)
+#define TECO_ROT_CACHE(TT, NX, VV)                                                              \
+    hipLaunchKernelGGL((rotary_cache_kernel<TT, NX, VV, Angles>), dim3(grid), dim3(kThreads), 0, \
+                       s, an, a)
     if (h16) {
         if (is_neox) {
             if (wide) TECO_ROT_CACHE(f16, true, 2);
@@ -665,4 +735,124 @@ extern "C" tecoopsStatus_t tecoopsRotaryReshapeAndCache(
 #undef TECO_ROT_CACHE
     TECO_CHECK_LAUNCH("rotary_reshape_and_cache");
     return TECOOPS_STATUS_SUCCESS;
+}
+
+OnePosition one_position(const int64_t *positions, const float *cos_sin_cache, int max_position,
+                         int rot_dim, float base) {
+    return {positions, cos_sin_cache, max_position, rot_dim, cos_sin_cache ? 0.0f : log2f(base)};
+}
+
+// The axes' frequencies have to fill the rotated half; interleaved, frequency
+// i belongs to axis i % axes while that axis has any left, so every axis but
+// the first has to find its last one inside the half.
+tecoopsStatus_t axis_positions(AxisPositions *out, const int64_t *positions,
+                               long long position_stride, int axes, const int *sections, int layout,
+                               const Rows &r, const float *cos_sin_cache, int max_position,
+                               float base) {
+    if (axes < 1 || axes > TECOOPS_ROTARY_MAX_AXES || sections == nullptr)
+        return TECOOPS_STATUS_BAD_PARAM;
+    if (layout < TECOOPS_ROTARY_CONTIGUOUS || layout > TECOOPS_ROTARY_PER_AXIS)
+        return TECOOPS_STATUS_BAD_PARAM;
+    if (axes > 1 && position_stride < r.num_tokens) return TECOOPS_STATUS_BAD_PARAM;
+    const int half = r.rot_dim / 2;
+    int sum = 0;
+    for (int a = 0; a < TECOOPS_ROTARY_MAX_AXES; ++a) {
+        out->first[a] = sum;
+        if (a >= axes) continue;
+        if (sections[a] < 0 || sections[a] > half - sum) return TECOOPS_STATUS_BAD_PARAM;
+        if (layout == TECOOPS_ROTARY_INTERLEAVED && a > 0 && sections[a] > 0 &&
+            axes * (sections[a] - 1) + a >= half)
+            return TECOOPS_STATUS_BAD_PARAM;
+        sum += sections[a];
+    }
+    out->first[TECOOPS_ROTARY_MAX_AXES] = sum;
+    if (sum != half) return TECOOPS_STATUS_BAD_PARAM;
+    out->positions = positions;
+    out->stride = position_stride;
+    out->cos_sin_cache = cos_sin_cache;
+    out->max_position = max_position;
+    out->rot_dim = r.rot_dim;
+    out->axes = axes;
+    out->layout = layout;
+    out->log2_base = cos_sin_cache ? 0.0 : log2(static_cast<double>(base));
+    return TECOOPS_STATUS_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" tecoopsStatus_t tecoopsRotaryEmbedding(tecoopsHandle_t handle,
+                                                  const int64_t *positions, void *query,
+                                                  void *key, int num_tokens, int num_heads,
+                                                  int num_kv_heads, int head_size, int rot_dim,
+                                                  long long query_stride, long long key_stride,
+                                                  const float *cos_sin_cache, int max_position,
+                                                  float base, int is_neox,
+                                                  tecoopsDataType_t dataType) {
+    if (handle == nullptr) return TECOOPS_STATUS_NOT_INITIALIZED;
+    const Rows r{query, key, num_tokens, num_heads, num_kv_heads, head_size, rot_dim, query_stride,
+                 key_stride};
+    const tecoopsStatus_t st = check_rows(r, positions, cos_sin_cache, max_position, base, dataType);
+    if (st != TECOOPS_STATUS_SUCCESS) return st;
+    return run_rotary(one_position(positions, cos_sin_cache, max_position, rot_dim, base), r,
+                      is_neox, dataType, handle->stream);
+}
+
+extern "C" tecoopsStatus_t tecoopsRotaryReshapeAndCache(
+    tecoopsHandle_t handle, const int64_t *positions, void *query, void *key, const void *value,
+    const int64_t *slot_mapping, void *key_cache, void *value_cache, int num_tokens,
+    int num_heads, int num_kv_heads, int head_size, int rot_dim, long long query_stride,
+    long long key_stride, long long value_stride, const float *cos_sin_cache, int max_position,
+    float base, int is_neox, int num_blocks, int block_size, int write_key,
+    tecoopsDataType_t dataType) {
+    if (handle == nullptr) return TECOOPS_STATUS_NOT_INITIALIZED;
+    const Rows r{query, key, num_tokens, num_heads, num_kv_heads, head_size, rot_dim, query_stride,
+                 key_stride};
+    const Pages g{value, slot_mapping, key_cache, value_cache, value_stride, num_blocks, block_size,
+                  write_key};
+    tecoopsStatus_t st = check_rows(r, positions, cos_sin_cache, max_position, base, dataType);
+    if (st == TECOOPS_STATUS_SUCCESS) st = check_pages(r, g);
+    if (st != TECOOPS_STATUS_SUCCESS) return st;
+    return run_fused(one_position(positions, cos_sin_cache, max_position, rot_dim, base), r, g,
+                     is_neox, dataType, handle->stream);
+}
+
+extern "C" tecoopsStatus_t tecoopsRotaryEmbeddingAxes(
+    tecoopsHandle_t handle, const int64_t *positions, long long position_stride, int axes,
+    const int *sections, tecoopsRotaryLayout_t layout, void *query, void *key, int num_tokens,
+    int num_heads, int num_kv_heads, int head_size, int rot_dim, long long query_stride,
+    long long key_stride, const float *cos_sin_cache, int max_position, float base, int is_neox,
+    tecoopsDataType_t dataType) {
+    if (handle == nullptr) return TECOOPS_STATUS_NOT_INITIALIZED;
+    const Rows r{query, key, num_tokens, num_heads, num_kv_heads, head_size, rot_dim, query_stride,
+                 key_stride};
+    AxisPositions an{};
+    tecoopsStatus_t st = check_rows(r, positions, cos_sin_cache, max_position, base, dataType);
+    if (st == TECOOPS_STATUS_SUCCESS)
+        st = axis_positions(&an, positions, position_stride, axes, sections, layout, r,
+                            cos_sin_cache, max_position, base);
+    if (st != TECOOPS_STATUS_SUCCESS) return st;
+    return run_rotary(an, r, is_neox, dataType, handle->stream);
+}
+
+extern "C" tecoopsStatus_t tecoopsRotaryAxesReshapeAndCache(
+    tecoopsHandle_t handle, const int64_t *positions, long long position_stride, int axes,
+    const int *sections, tecoopsRotaryLayout_t layout, void *query, void *key, const void *value,
+    const int64_t *slot_mapping, void *key_cache, void *value_cache, int num_tokens,
+    int num_heads, int num_kv_heads, int head_size, int rot_dim, long long query_stride,
+    long long key_stride, long long value_stride, const float *cos_sin_cache, int max_position,
+    float base, int is_neox, int num_blocks, int block_size, int write_key,
+    tecoopsDataType_t dataType) {
+    if (handle == nullptr) return TECOOPS_STATUS_NOT_INITIALIZED;
+    const Rows r{query, key, num_tokens, num_heads, num_kv_heads, head_size, rot_dim, query_stride,
+                 key_stride};
+    const Pages g{value, slot_mapping, key_cache, value_cache, value_stride, num_blocks, block_size,
+                  write_key};
+    AxisPositions an{};
+    tecoopsStatus_t st = check_rows(r, positions, cos_sin_cache, max_position, base, dataType);
+    if (st == TECOOPS_STATUS_SUCCESS) st = check_pages(r, g);
+    if (st == TECOOPS_STATUS_SUCCESS)
+        st = axis_positions(&an, positions, position_stride, axes, sections, layout, r,
+                            cos_sin_cache, max_position, base);
+    if (st != TECOOPS_STATUS_SUCCESS) return st;
+    return run_fused(an, r, g, is_neox, dataType, handle->stream);
 }

@@ -13,6 +13,7 @@
 // softmax_scale / causal and takes the element type (fp16 or bf16) from q;
 // causal_conv1d_fn_torch reads the [dim, tokens] layout in place instead of
 // two transposing copies (torch_ext.cpp:186-205).
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 #include <ATen/ATen.h>
@@ -304,6 +305,182 @@ void gemv_int8(const Tensor &weight, const Tensor &scales, const Tensor &x, Tens
           "gemv_int8");
 }
 
+// Rows packed, any distance apart: the distance in elements.
+int64_t row_stride(const Tensor &t, int64_t rows, int64_t width, const char *name) {
+    TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == width &&
+                    (width <= 1 || t.stride(1) == 1) && (rows <= 1 || t.stride(0) >= width),
+                "tecoops: ", name, " must be [", rows, ", ", width, "] with packed rows");
+    return rows > 1 ? t.stride(0) : width;
+}
+
+void same_device(const Tensor &x, std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        if (t && t->defined())
+            TORCH_CHECK(t->device() == x.device(), "tecoops: tensors must be on one device");
+}
+
+const Tensor *given(const c10::optional<Tensor> &t) { return t.has_value() ? &*t : nullptr; }
+
+int fits_int(int64_t v, const char *name) {
+    TORCH_CHECK(v >= 0 && v <= 0x7fffffff, "tecoops: ", name, " is too large");
+    return static_cast<int>(v);
+}
+
+tecoopsActivation_t activation_of(c10::string_view s) {
+    if (s == "none") return TECOOPS_ACTIVATION_NONE;
+    if (s == "relu") return TECOOPS_ACTIVATION_RELU;
+    if (s == "silu") return TECOOPS_ACTIVATION_SILU;
+    if (s == "gelu") return TECOOPS_ACTIVATION_GELU;
+    if (s == "gelu_tanh") return TECOOPS_ACTIVATION_GELU_TANH;
+    TORCH_CHECK(false, "tecoops: activation must be none, relu, silu, gelu or gelu_tanh, got ", s);
+}
+
+Tensor workspace_of(size_t bytes, const Tensor &like) {
+    return bytes ? at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)) : Tensor();
+}
+
+void linear(const Tensor &x, const Tensor &weight, Tensor &out, const c10::optional<Tensor> &bias,
+            const c10::optional<Tensor> &residual, c10::string_view activation, bool gated) {
+    const Tensor *b = given(bias), *r = given(residual);
+    need_cuda({&x, &weight, &out, b, r});
+    same_device(x, {&weight, &out, b, r});
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    const tecoopsDataType_t dt = dtype_of(x);
+    TORCH_CHECK(x.dim() == 2 && weight.dim() == 2 && out.dim() == 2,
+                "linear: x [M, K], weight [N, K], out [M, N]");
+    const int m = fits_int(out.size(0), "M"), n = fits_int(out.size(1), "N"),
+              k = fits_int(weight.size(1), "K");
+    TORCH_CHECK(weight.size(0) == (gated ? 2LL * n : n), "linear: weight must hold N rows, 2 N gated");
+    need_contiguous({&weight, b});
+    need_dtype(weight, x.scalar_type(), "weight");
+    need_dtype(out, x.scalar_type(), "out");
+    if (b) {
+        need_dtype(*b, x.scalar_type(), "bias");
+        TORCH_CHECK(b->numel() == weight.size(0), "linear: bias must hold an element per row of weight");
+    }
+    if (r) need_dtype(*r, x.scalar_type(), "residual");
+    const int64_t xs = row_stride(x, m, k, "x"), os = row_stride(out, m, n, "out");
+    const int64_t rs = r ? row_stride(*r, m, n, "residual") : 0;
+    const tecoopsActivation_t act = activation_of(activation);
+    if (m == 0) return;
+    size_t bytes = 0;
+    check(tecoopsGetLinearWorkspaceSize(m, n, k, gated, &bytes), "linear");
+    const Tensor ws = workspace_of(bytes, x);
+    check(tecoopsLinear(handle_for(x), x.data_ptr(), xs, weight.data_ptr(), b ? b->data_ptr() : nullptr,
+                        r ? r->data_ptr() : nullptr, rs, out.data_ptr(), os, m, n, k, act, gated,
+                        bytes ? ws.data_ptr() : nullptr, bytes, dt),
+          "linear");
+}
+
+// The arguments of the rotary functions of several axes, checked.
+struct AxesArgs {
+    std::vector<int> sections;
+    tecoopsRotaryLayout_t layout;
+    int tokens, heads, kv_heads, rot_dim;
+    int64_t position_stride, query_stride, key_stride;
+    const float *table;
+    int max_position;
+
+    AxesArgs(const Tensor &positions, const Tensor &query, const Tensor *key, int64_t head_size,
+             at::IntArrayRef sec, const Tensor *cos_sin_cache, int64_t rot, c10::string_view lay) {
+        need_cuda({&positions, &query, key, cos_sin_cache});
+        same_device(query, {&positions, key, cos_sin_cache});
+        need_dtype(positions, at::kLong, "positions");
+        TORCH_CHECK(head_size > 0, "tecoops: head_size must be positive");
+        TORCH_CHECK(positions.dim() == 2 && positions.size(0) == static_cast<int64_t>(sec.size()) &&
+                        (positions.size(1) <= 1 || positions.stride(1) == 1),
+                    "tecoops: positions must be [axes, tokens] with adjacent tokens, one axis per section");
+        tokens = fits_int(positions.size(1), "tokens");
+        position_stride = sec.size() > 1 ? positions.stride(0) : tokens;
+        for (int64_t s : sec) sections.push_back(static_cast<int>(std::min<int64_t>(std::max<int64_t>(s, -1), 1 << 20)));
+        heads = rows(query, query, head_size, "query", &query_stride);
+        kv_heads = 0;
+        key_stride = 0;
+        if (key) kv_heads = rows(*key, query, head_size, "key", &key_stride);
+        table = nullptr;
+        max_position = 0;
+        rot_dim = fits_int(rot > 0 ? rot : head_size, "rot_dim");
+        if (cos_sin_cache) {
+            need_dtype(*cos_sin_cache, at::kFloat, "cos_sin_cache");
+            need_contiguous({cos_sin_cache});
+            TORCH_CHECK(cos_sin_cache->dim() == 2 && (rot <= 0 || rot == cos_sin_cache->size(1)),
+                        "tecoops: cos_sin_cache must be [positions, rot_dim]");
+            rot_dim = fits_int(cos_sin_cache->size(1), "rot_dim");
+            table = cos_sin_cache->data_ptr<float>();
+            max_position = fits_int(cos_sin_cache->size(0), "positions of cos_sin_cache");
+        }
+        if (lay == "contiguous") layout = TECOOPS_ROTARY_CONTIGUOUS;
+        else if (lay == "interleaved") layout = TECOOPS_ROTARY_INTERLEAVED;
+        else if (lay == "per_axis") layout = TECOOPS_ROTARY_PER_AXIS;
+        else TORCH_CHECK(false, "tecoops: layout must be contiguous, interleaved or per_axis, got ", lay);
+    }
+
+    int rows(const Tensor &t, const Tensor &query, int64_t head_size, const char *name,
+             int64_t *stride) const {
+        need_dtype(t, query.scalar_type(), name);
+        const int64_t row = tokens ? t.numel() / tokens : head_size;
+        TORCH_CHECK((t.dim() == 2 || t.dim() == 3) && t.size(0) == tokens && row > 0 &&
+                        row % head_size == 0,
+                    "tecoops: ", name, " must be [tokens, heads * head_size] or [tokens, heads, head_size]");
+        TORCH_CHECK((t.dim() == 2 || t.size(1) <= 1 || t.stride(1) == t.size(2)) &&
+                        (t.size(-1) <= 1 || t.stride(-1) == 1),
+                    "tecoops: the heads of a token of ", name, " must be adjacent");
+        *stride = tokens > 1 ? t.stride(0) : row;
+        return fits_int(row / head_size, "heads");
+    }
+};
+
+void rotary_embedding_axes(const Tensor &positions, Tensor &query, const c10::optional<Tensor> &key,
+                           int64_t head_size, at::IntArrayRef sections,
+                           const c10::optional<Tensor> &cos_sin_cache, bool is_neox, double base,
+                           int64_t rot_dim, c10::string_view layout) {
+    const Tensor *k = given(key);
+    const AxesArgs a(positions, query, k, head_size, sections, given(cos_sin_cache), rot_dim, layout);
+    if (a.tokens == 0) return;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(query.device());
+    check(tecoopsRotaryEmbeddingAxes(
+              handle_for(query), positions.data_ptr<int64_t>(), a.position_stride,
+              static_cast<int>(a.sections.size()), a.sections.data(), a.layout, query.data_ptr(),
+              k ? k->data_ptr() : nullptr, a.tokens, a.heads, a.kv_heads, head_size, a.rot_dim,
+              a.query_stride, a.key_stride, a.table, a.max_position, static_cast<float>(base),
+              is_neox ? 1 : 0, dtype_of(query)),
+          "rotary_embedding_axes");
+}
+
+void rotary_axes_reshape_and_cache(const Tensor &positions, Tensor &query, Tensor &key,
+                                   const Tensor &value, const Tensor &slot_mapping,
+                                   Tensor &key_cache, Tensor &value_cache, int64_t head_size,
+                                   at::IntArrayRef sections,
+                                   const c10::optional<Tensor> &cos_sin_cache, bool is_neox,
+                                   double base, int64_t rot_dim, c10::string_view layout,
+                                   bool write_key) {
+    const AxesArgs a(positions, query, &key, head_size, sections, given(cos_sin_cache), rot_dim, layout);
+    need_cuda({&value, &slot_mapping, &key_cache, &value_cache});
+    same_device(query, {&value, &slot_mapping, &key_cache, &value_cache});
+    need_contiguous({&slot_mapping, &key_cache, &value_cache});
+    need_dtype(slot_mapping, at::kLong, "slot_mapping");
+    need_dtype(key_cache, query.scalar_type(), "key_cache");
+    need_dtype(value_cache, query.scalar_type(), "value_cache");
+    TORCH_CHECK(slot_mapping.numel() == a.tokens, "tecoops: slot_mapping must hold a slot per token");
+    TORCH_CHECK(key_cache.dim() == 4 && key_cache.size(1) == a.kv_heads && key_cache.size(3) == head_size &&
+                    value_cache.sizes() == key_cache.sizes(),
+                "tecoops: caches must be [num_blocks, kv heads, block_size, head_size]");
+    int64_t value_stride = 0;
+    TORCH_CHECK(a.rows(value, query, head_size, "value", &value_stride) == a.kv_heads,
+                "tecoops: value must match key");
+    if (a.tokens == 0) return;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(query.device());
+    check(tecoopsRotaryAxesReshapeAndCache(
+              handle_for(query), positions.data_ptr<int64_t>(), a.position_stride,
+              static_cast<int>(a.sections.size()), a.sections.data(), a.layout, query.data_ptr(),
+              key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr<int64_t>(),
+              key_cache.data_ptr(), value_cache.data_ptr(), a.tokens, a.heads, a.kv_heads, head_size,
+              a.rot_dim, a.query_stride, a.key_stride, value_stride, a.table, a.max_position,
+              static_cast<float>(base), is_neox ? 1 : 0, fits_int(key_cache.size(0), "num_blocks"),
+              fits_int(key_cache.size(2), "block_size"), write_key ? 1 : 0, dtype_of(query)),
+          "rotary_axes_reshape_and_cache");
+}
+
 void memset_(Tensor &t, int64_t value) {
     need_cuda({&t});
     check(tecoopsMemset(handle_for(t), t.data_ptr(), static_cast<int>(value),
@@ -335,6 +512,15 @@ TORCH_LIBRARY(tecoops, m) {
           "bool write_key) -> ()");
     m.def("gemv(Tensor weight, Tensor x, Tensor(a!) out) -> ()");
     m.def("gemv_int8(Tensor weight, Tensor scales, Tensor x, Tensor(a!) out) -> ()");
+    m.def("linear(Tensor x, Tensor weight, Tensor(a!) out, Tensor? bias, Tensor? residual, "
+          "str activation, bool gated) -> ()");
+    m.def("rotary_embedding_axes(Tensor positions, Tensor(a!) query, Tensor(b!)? key, "
+          "int head_size, int[] sections, Tensor? cos_sin_cache, bool is_neox, float base, "
+          "int rot_dim, str layout) -> ()");
+    m.def("rotary_axes_reshape_and_cache(Tensor positions, Tensor(a!) query, Tensor(b!) key, "
+          "Tensor value, Tensor slot_mapping, Tensor(c!) key_cache, Tensor(d!) value_cache, "
+          "int head_size, int[] sections, Tensor? cos_sin_cache, bool is_neox, float base, "
+          "int rot_dim, str layout, bool write_key) -> ()");
     m.def("memset(Tensor(a!) t, int value) -> ()");
 }
 
@@ -348,5 +534,8 @@ TORCH_LIBRARY_IMPL(tecoops, CUDA, m) {
     m.impl("rotary_reshape_and_cache", &rotary_reshape_and_cache);
     m.impl("gemv", &gemv);
     m.impl("gemv_int8", &gemv_int8);
+    m.impl("linear", &linear);
+    m.impl("rotary_embedding_axes", &rotary_embedding_axes);
+    m.impl("rotary_axes_reshape_and_cache", &rotary_axes_reshape_and_cache);
     m.impl("memset", &memset_);
 }

@@ -41,7 +41,7 @@ __all__ = [
     "flash_attn_varlen_func", "causal_conv1d_fn_torch",
     # extensions
     "rotary_embedding", "rotary_reshape_and_cache", "gemv", "gemv_int8", "causal_conv1d",
-    "memset", "ops",
+    "memset", "linear", "rotary_embedding_axes", "rotary_axes_reshape_and_cache", "ops",
 ]
 
 _tls = threading.local()   # per thread: {device index: _Handle}
@@ -114,6 +114,39 @@ def _check_dtype(t, name, *dtypes):
     if t is not None and t.dtype not in dtypes:
         raise TypeError(f"tecoops: {name} must be {' or '.join(str(d) for d in dtypes)}, "
                         f"got {t.dtype}")
+
+
+def _check_device(device, **ts):
+    for name, t in ts.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"tecoops: {name} must be on {device}, got {t.device}")
+
+
+def _check_rows(t, name, width):
+    """A [rows, width] tensor whose rows are packed (rows may be any distance
+    apart): the distance in elements."""
+    if t.dim() != 2 or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        raise ValueError(f"tecoops: {name} must be [rows, {width}] with packed rows")
+    if t.shape[0] > 1 and t.stride(0) < width:
+        raise ValueError(f"tecoops: rows of {name} must not overlap")
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+def _choice(table, value, what):
+    try:
+        return table[value]
+    except (KeyError, TypeError):
+        raise ValueError(f"tecoops: {what} must be one of "
+                         f"{', '.join(str(k) for k in table)}, got {value!r}") from None
+
+
+def _call_on(device, name, *args):
+    """_lib.call with `device` current: a launch goes to the current device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args)
 
 
 class _Desc:
@@ -345,6 +378,163 @@ def gemv_int8(weight, scales, x, out):
         raise ValueError(f"tecoops.gemv_int8: x must be [B, {K}], out [B, {N}], scales [{N}]")
     _lib.call("tecoopsGemvInt8", _handle(x.device), _ptr(weight), _ptr(scales), _ptr(x),
               _ptr(out), B, N, K)
+
+
+def linear(x, weight, out, bias=None, residual=None, activation=None, gated=False):
+    """out[m, n] = act(sum_k x[m, k] weight[n, k] + bias[n]) + residual[m, n].
+
+    x [M, K], residual and out [M, N] (rows packed, any distance apart); weight
+    [N, K] and bias [N] contiguous.  activation: None, "relu", "silu", "gelu" or
+    "gelu_tanh".  gated: weight [2N, K] and bias [2N] hold the gate rows, then
+    the up rows, and out = act(gate) * up + residual.  residual may be out
+    itself; out must not overlap another input.  float16 or bfloat16; sums and
+    epilogue in float32."""
+    _check_cuda(x, weight, out, bias, residual)
+    code, device = _dtype_code(x), x.device
+    if weight.dim() != 2 or x.dim() != 2 or out.dim() != 2:
+        raise ValueError("tecoops.linear: x [M, K], weight [N, K], out [M, N]")
+    rows, K = weight.shape
+    M, N = out.shape
+    if x.shape[0] != M or rows != (2 * N if gated else N):
+        raise ValueError(f"tecoops.linear: weight must be [{2 * N if gated else N}, {x.shape[1]}] "
+                         f"and x [{M}, K] for out [{M}, {N}]")
+    _check_contiguous(weight=weight, bias=bias)
+    _check_device(device, weight=weight, out=out, bias=bias, residual=residual)
+    for name, t in (("weight", weight), ("out", out), ("bias", bias), ("residual", residual)):
+        _check_dtype(t, name, x.dtype)
+    if bias is not None and bias.numel() != rows:
+        raise ValueError(f"tecoops.linear: bias must hold {rows} elements")
+    xs, os_ = _check_rows(x, "x", K), _check_rows(out, "out", N)
+    rs = 0
+    if residual is not None:
+        rs = _check_rows(residual, "residual", N)
+        if residual.shape[0] != M:
+            raise ValueError(f"tecoops.linear: residual must be [{M}, {N}]")
+    act = _choice(_lib.ACTIVATIONS, activation, "activation")
+    if M == 0:
+        return
+    space = _workspace(device, "tecoopsGetLinearWorkspaceSize", M, N, K, int(bool(gated)))
+    _call_on(device, "tecoopsLinear", _handle(device), _ptr(x), xs, _ptr(weight), _ptr(bias),
+             _ptr(residual), rs, _ptr(out), os_, M, N, K, act, int(bool(gated)), _ptr(space),
+             0 if space is None else space.numel(), code)
+
+
+def _workspace(device, size, *args):
+    """A workspace of the bytes that the C function `size` asks for, from
+    torch's allocator (stream-ordered, and of a graph's own pool under capture),
+    or None."""
+    n = ctypes.c_size_t()
+    _call_on(device, size, *args, ctypes.byref(n))
+    return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+
+
+def _axes_args(name, positions, query, key, head_size, sections, cos_sin_cache, base, rot_dim,
+               layout):
+    """Checks shared by the rotary functions of several axes; the C arguments
+    before and after the pointers.  None: no tokens."""
+    _check_cuda(positions, query, key, cos_sin_cache)
+    device = query.device
+    _check_device(device, positions=positions, key=key, cos_sin_cache=cos_sin_cache)
+    sections = [int(n) for n in sections]
+    if positions.dtype != torch.int64:
+        raise TypeError(f"tecoops.{name}: positions must be int64")
+    if positions.dim() != 2 or positions.shape[0] != len(sections):
+        raise ValueError(f"tecoops.{name}: positions must be [axes, tokens], one axis per section")
+    T = positions.shape[1]
+    if T > 1 and positions.stride(1) != 1:
+        raise ValueError(f"tecoops.{name}: the tokens of an axis of positions must be adjacent")
+    heads, strides = [], []
+    for what, t in (("query", query), ("key", key)):
+        if t is None:
+            heads.append(0)
+            strides.append(0)
+            continue
+        _check_dtype(t, what, query.dtype)
+        row = t.numel() // T if T else head_size
+        if t.dim() not in (2, 3) or t.shape[0] != T or row == 0 or row % head_size:
+            raise ValueError(f"tecoops.{name}: {what} must be [tokens, heads * head_size] or "
+                             "[tokens, heads, head_size]")
+        if t.dim() == 3 and t.shape[1] > 1 and t.stride(1) != t.shape[2] or \
+                t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"tecoops.{name}: the heads of a token of {what} must be adjacent")
+        heads.append(row // head_size)
+        strides.append(t.stride(0) if T > 1 else row)
+    if cos_sin_cache is not None:
+        _check_dtype(cos_sin_cache, "cos_sin_cache", torch.float32)
+        _check_contiguous(cos_sin_cache=cos_sin_cache)
+        if cos_sin_cache.dim() != 2 or rot_dim not in (None, cos_sin_cache.shape[1]):
+            raise ValueError(f"tecoops.{name}: cos_sin_cache must be [positions, rot_dim]")
+        rot_dim = cos_sin_cache.shape[1]
+    elif rot_dim is None:
+        rot_dim = head_size
+    lay = _choice(_lib.ROTARY_LAYOUTS, layout, "layout")
+    before = (_ptr(positions), positions.stride(0) if len(sections) > 1 else T, len(sections),
+              (ctypes.c_int * len(sections))(*sections), lay)
+    sizes = (T, heads[0], heads[1], int(head_size), int(rot_dim), strides[0], strides[1])
+    table = (_ptr(cos_sin_cache), cos_sin_cache.shape[0] if cos_sin_cache is not None else 0,
+             float(base))
+    return device, before, sizes, table, _dtype_code(query)
+
+
+def rotary_embedding_axes(positions, query, key, head_size, sections, cos_sin_cache=None,
+                          is_neox=True, base=10000.0, rot_dim=None, layout="contiguous"):
+    """Rotary positions of several axes (time, height, width of images and
+    video), in place on query [T, H*D or H, D] and key likewise (or None; the
+    rows may be slices of a wider product's).
+
+    positions int64 [axes, T]; sections: the number of frequencies of each axis,
+    rot_dim / 2 together.  layout: "contiguous" gives each axis a range of the
+    frequencies, "interleaved" frequency i to axis i % axes while that axis has
+    any left (else to the first), "per_axis" ranges with frequencies of their
+    own, base^(-j / n) for the j-th of an axis' n.  With a cos_sin_cache
+    (float32 [positions, rot_dim]) a token with a position outside it is left as
+    it is; without, angles are computed in 64 bits."""
+    device, before, sizes, table, code = _axes_args("rotary_embedding_axes", positions, query, key,
+                                                    head_size, sections, cos_sin_cache, base,
+                                                    rot_dim, layout)
+    if sizes[0] == 0:
+        return
+    _call_on(device, "tecoopsRotaryEmbeddingAxes", _handle(device), *before, _ptr(query), _ptr(key),
+             *sizes, *table, int(bool(is_neox)), code)
+
+
+def rotary_axes_reshape_and_cache(positions, query, key, value, slot_mapping, key_cache,
+                                  value_cache, head_size, sections, cos_sin_cache=None,
+                                  is_neox=True, base=10000.0, rot_dim=None, layout="contiguous",
+                                  write_key=False):
+    """rotary_embedding_axes on query (in place) and key, and the rotated key and
+    value stored into the paged caches [num_blocks, Hkv, block_size, head_size]
+    at slot_mapping (int64; slots outside the cache are not stored); key is
+    updated in place only when write_key."""
+    name = "rotary_axes_reshape_and_cache"
+    if key is None:
+        raise ValueError(f"tecoops.{name}: key must be given")
+    _check_cuda(value, slot_mapping, key_cache, value_cache)
+    device, before, sizes, table, code = _axes_args(name, positions, query, key, head_size,
+                                                    sections, cos_sin_cache, base, rot_dim, layout)
+    T, _, Hkv, D = sizes[:4]
+    _check_device(device, value=value, slot_mapping=slot_mapping, key_cache=key_cache,
+                  value_cache=value_cache)
+    _check_dtype(slot_mapping, "slot_mapping", torch.int64)
+    for what, t in (("value", value), ("key_cache", key_cache), ("value_cache", value_cache)):
+        _check_dtype(t, what, query.dtype)
+    _check_contiguous(slot_mapping=slot_mapping, key_cache=key_cache, value_cache=value_cache)
+    if slot_mapping.numel() != T:
+        raise ValueError(f"tecoops.{name}: slot_mapping must hold {T} slots")
+    if key_cache.dim() != 4 or key_cache.shape[1] != Hkv or key_cache.shape[3] != D or \
+            value_cache.shape != key_cache.shape:
+        raise ValueError(f"tecoops.{name}: caches must be [num_blocks, {Hkv}, block_size, {D}]")
+    if value.dim() not in (2, 3) or value.shape[0] != T or value.numel() != T * Hkv * D:
+        raise ValueError(f"tecoops.{name}: value must match key")
+    if value.dim() == 3 and value.shape[1] > 1 and value.stride(1) != value.shape[2] or \
+            value.shape[-1] > 1 and value.stride(-1) != 1:
+        raise ValueError(f"tecoops.{name}: the heads of a token of value must be adjacent")
+    if T == 0:
+        return
+    _call_on(device, "tecoopsRotaryAxesReshapeAndCache", _handle(device), *before, _ptr(query),
+             _ptr(key), _ptr(value), _ptr(slot_mapping), _ptr(key_cache), _ptr(value_cache), *sizes,
+             value.stride(0) if T > 1 else Hkv * D, *table, int(bool(is_neox)), key_cache.shape[0],
+             key_cache.shape[2], int(bool(write_key)), code)
 
 
 def memset(t, value):

@@ -27,6 +27,12 @@ DATA_INT64 = 5
 DATA_BFLOAT16 = 9
 
 
+# tecoopsActivation_t
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+# tecoopsRotaryLayout_t
+ROTARY_LAYOUTS = {"contiguous": 0, "interleaved": 1, "per_axis": 2}
+
+
 class TecoopsError(RuntimeError):
     def __init__(self, status, what=""):
         self.status = status
@@ -73,6 +79,12 @@ SIGNATURES = {
                                          F, I, I, I, I, I]),
     "tecoopsGemv": (I, [P, P, P, P, I, I, I, I]),
     "tecoopsGemvInt8": (I, [P, P, P, P, P, I, I, I]),
+    "tecoopsLinear": (I, [P, P, LL, P, P, P, LL, P, LL, I, I, I, I, I, P, SZ, I]),
+    "tecoopsGetLinearWorkspaceSize": (I, [I, I, I, I, P]),
+    "tecoopsRotaryEmbeddingAxes": (I, [P, P, LL, I, P, I, P, P, I, I, I, I, I, LL, LL, P, I, F, I,
+                                       I]),
+    "tecoopsRotaryAxesReshapeAndCache": (I, [P, P, LL, I, P, I, P, P, P, P, P, P, I, I, I, I, I, LL,
+                                             LL, LL, P, I, F, I, I, I, I, I]),
 }
 
 _LIB = None

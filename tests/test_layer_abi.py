@@ -1,0 +1,131 @@
+"""Host checks of the decoder-layer operators' C entry points: bad arguments come
+back as statuses before any device work, and how a product is cut into tiles."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+from tecoops import _lib
+
+BAD, NOT_INIT, NOT_SUP, OK = _lib.BAD_PARAM, _lib.NOT_INITIALIZED, _lib.NOT_SUPPORTED, _lib.SUCCESS
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "teco-ops_amd", "csrc")
+P = 0x1000  # never dereferenced: the checks come first
+
+
+@pytest.fixture
+def handle():
+    h = ctypes.c_void_p()
+    assert _lib.lib().tecoopsCreate(ctypes.byref(h)) == OK
+    yield h
+    assert _lib.lib().tecoopsDestroy(h) == OK
+
+
+def test_linear_refusals(handle):
+    f = _lib.lib().tecoopsLinear
+    good = dict(h=handle, x=P, xs=64, w=P, b=P, r=P, rs=32, o=P, os=32, m=4, n=32, k=64, act=0,
+                gated=0, ws=None, wb=0, dt=1)
+
+    def call(**kw):
+        a = {**good, **kw}
+        return f(*(a[k] for k in good))
+
+    assert call(h=None) == NOT_INIT
+    for kw in (dict(x=None), dict(w=None), dict(o=None), dict(m=-1), dict(n=0), dict(n=-4),
+               dict(k=0), dict(xs=63), dict(os=31), dict(rs=31), dict(act=5), dict(act=-1),
+               dict(dt=0), dict(dt=2), dict(x=P + 1), dict(w=P + 1), dict(b=P + 1), dict(r=P + 1),
+               dict(o=P + 1)):
+        assert call(**kw) == BAD, kw
+    assert call(k=(1 << 21) + 8, xs=(1 << 21) + 8) == NOT_SUP
+    assert call(xs=(1 << 21) + 8) == NOT_SUP
+    assert call(n=(1 << 30) + 4, os=1 << 31, rs=1 << 31) == NOT_SUP
+    assert call(m=0) == OK  # no launch
+    size = ctypes.c_size_t(1)
+    g = _lib.lib().tecoopsGetLinearWorkspaceSize
+    assert g(4, 4, 4, 0, None) == BAD and g(-1, 4, 4, 0, ctypes.byref(size)) == BAD
+    assert g(4, 0, 4, 0, ctypes.byref(size)) == BAD and g(4, 4, 0, 0, ctypes.byref(size)) == BAD
+    assert g(0, 4, 4, 0, ctypes.byref(size)) == OK and size.value == 0
+
+
+def test_rotary_axes_refusals(handle):
+    L = _lib.lib()
+
+    def axes(sections, layout=0, n=None, half=32, **kw):
+        s = (ctypes.c_int * 8)(*sections)
+        a = dict(h=handle, pos=P, stride=5, q=P, k=P, T=5, H=2, Hkv=1, D=64, rot=2 * half, qs=128,
+                 ks=64, table=None, most=0, base=1e4, neox=1, dt=1)
+        a.update(kw)
+        front = (a["h"], a["pos"], a["stride"], len(sections) if n is None else n,
+                 s if kw.get("sec", True) else None, layout, a["q"], a["k"])
+        size = (a["T"], a["H"], a["Hkv"], a["D"], a["rot"], a["qs"], a["ks"])
+        tail = (a["table"], a["most"], a["base"], a["neox"])
+        plain = L.tecoopsRotaryEmbeddingAxes(*front, *size, *tail, a["dt"])
+        fused = L.tecoopsRotaryAxesReshapeAndCache(*front, P, P, P, P, *size, 64, *tail, 4, 16, 0,
+                                                   a["dt"])
+        assert plain == fused
+        return plain
+
+    assert axes([32], h=None) == NOT_INIT
+    for sections, layout in (([16, 15], 0), ([16, 17], 0), ([33, -1], 0), ([4, 14, 14], 1),
+                             ([10, 11, 11], 1), ([32], 3), ([32], -1), ([8, 8, 8, 4, 4], 0)):
+        assert axes(sections, layout) == BAD, (sections, layout)
+    assert axes([32], n=0) == BAD and axes([32], sec=False) == BAD
+    for kw in (dict(stride=4), dict(pos=None), dict(q=None), dict(T=0), dict(T=-1), dict(H=0),
+               dict(Hkv=0), dict(D=0), dict(D=63), dict(half=0), dict(qs=127), dict(ks=63),
+               dict(table=P, most=0), dict(base=0.0), dict(base=float("nan")), dict(dt=0)):
+        assert axes([16, 16] if kw.get("half", 1) else [0, 0], **kw) == BAD, kw
+    s = (ctypes.c_int * 1)(32)
+    fused = L.tecoopsRotaryAxesReshapeAndCache
+    for none in (7, 8, 9, 10, 11):  # key, value, slots, caches
+        a = [handle, P, 5, 1, s, 0, P, P, P, P, P, P, 5, 2, 1, 64, 64, 128, 64, 64, None, 0, 1e4, 1,
+             4, 16, 0, 1]
+        a[none] = None
+        assert fused(*a) == BAD, none
+    for at, bad in ((24, 0), (25, 0), (19, 63)):  # blocks, block size, value stride
+        a = [handle, P, 5, 1, s, 0, P, P, P, P, P, P, 5, 2, 1, 64, 64, 128, 64, 64, None, 0, 1e4, 1,
+             4, 16, 0, 1]
+        a[at] = bad
+        assert fused(*a) == BAD, at
+    a[19], a[24], a[25] = 64, 1 << 20, 1 << 20
+    assert fused(*a) == NOT_SUP
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    d = tmp_path_factory.mktemp("plan")
+    (d / "plan.cpp").write_text("""#include "linear.h"
+extern "C" void plan(int m, int n, int k, int gated, int copy, unsigned long long ws, long long *o) {
+    const auto p = tecoops::linear_plan(m, n, k, gated != 0, copy != 0, ws, 256);
+    o[0] = p.bm; o[1] = p.bn; o[2] = p.tiles_m; o[3] = p.tiles_n;
+    o[4] = p.splits; o[5] = p.stages; o[6] = static_cast<long long>(p.bytes);
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-fPIC", "-shared", "-I", CSRC, str(d / "plan.cpp"), "-o",
+                    str(d / "plan.so")], check=True)
+    lib = ctypes.CDLL(str(d / "plan.so"))
+    lib.plan.argtypes = [ctypes.c_int] * 5 + [ctypes.c_ulonglong, ctypes.c_void_p]
+
+    def run(m, n, k, gated=0, copy=1, ws=(1 << 63)):
+        o = (ctypes.c_longlong * 7)()
+        lib.plan(m, n, k, gated, copy, ws, o)
+        return list(o)
+    return run
+
+
+@pytest.mark.parametrize("copy", [0, 1])
+@pytest.mark.parametrize("gated", [0, 1])
+def test_plan_covers_the_product(plan, gated, copy):
+    """Tiles cover the rows and outputs, splits cover K with none empty, and the
+    workspace holds every split's sums of every row of W."""
+    for m in (1, 64, 65, 127, 128, 129, 333, 1000, 8192, 70000):
+        for n in (1, 63, 64, 65, 300, 4096, 14336, 100000):
+            for k in (1, 8, 64, 65, 512, 588, 4096, 14336, 100000):
+                for ws in (0, 1 << 20, 1 << 63):
+                    bm, bn, tm, tn, splits, stages, need = plan(m, n, k, gated, copy, ws)
+                    out = bn // 2 if gated else bn
+                    assert (tm - 1) * bm < m <= tm * bm and (tn - 1) * out < n <= tn * out
+                    total = -(-k // 64)
+                    assert splits >= 1 and (splits - 1) * stages < total <= splits * stages
+                    assert need == (splits * m * n * (2 if gated else 1) * 4 if splits > 1 else 0)
+                    assert need <= ws
+                    assert copy or bm == 128
