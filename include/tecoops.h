@@ -382,6 +382,34 @@ tecoopsStatus_t tecoopsLinear(tecoopsHandle_t handle, const void *x, long long x
                               tecoopsDataType_t dataType);
 tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, int gated, size_t *bytes);
 
+/* Mixture-of-experts layer.  Per token t with p = softmax(router_logits[t]):
+ *   the top_k experts e_j of the largest logits (ties to the lowest index; -inf
+ *   and NaN are never chosen, so a masked token may have fewer or none),
+ *   w_j = p[e_j], divided by their sum when renormalize != 0,
+ *   h_j = act(x[t] Wg[e_j]^T) * (x[t] Wu[e_j]^T), rounded to dataType,
+ *   out[t] = sum_j w_j (h_j W_out[e_j]^T), fp32 sums, one rounding.
+ * x [tokens, hidden] with row stride x_stride (elements); w_in [experts,
+ * 2 inter, hidden] packed, the inter gate rows Wg of an expert before its up
+ * rows Wu; w_out [experts, hidden, inter] packed; router_logits [tokens,
+ * experts] packed, logitsType FLOAT or dataType; out [tokens, hidden] packed,
+ * zero for a token without experts; out must not overlap an input.  topk_ids
+ * int32 and topk_weights float [tokens, top_k] are written unless NULL, best
+ * first, -1 and 0 where there is none.  Every expert's weights are read once
+ * for all of its tokens (of each 512 tokens, up to 64 at a time).  Up to 1024
+ * experts, top_k 32, hidden and inter 2^20; hidden, inter and x_stride
+ * multiples of 8 and 16-byte aligned tensors are fast.
+ * workspace: tecoopsGetMoeLayerWorkspaceSize() bytes, 16-byte aligned; NULL
+ * uses the handle's scratch (NOT_SUPPORTED on a stream under capture). */
+tecoopsStatus_t tecoopsMoeLayer(tecoopsHandle_t handle, const void *x, long long x_stride,
+                                const void *w_in, const void *w_out, const void *router_logits,
+                                tecoopsDataType_t logitsType, void *out, int *topk_ids,
+                                float *topk_weights, int tokens, int hidden, int inter,
+                                int experts, int top_k, int renormalize,
+                                tecoopsActivation_t activation, void *workspace,
+                                size_t workspace_bytes, tecoopsDataType_t dataType);
+tecoopsStatus_t tecoopsGetMoeLayerWorkspaceSize(int tokens, int hidden, int inter, int experts,
+                                                int top_k, size_t *bytes);
+
 /* Rotary positions of several axes (time, height, width of images and video).
  * As tecoopsRotaryEmbedding, but positions is int64 [axes, num_tokens] (rows
  * position_stride elements apart, at least num_tokens) and pair i of a head

@@ -41,6 +41,7 @@ SOURCES = [
     "gemv.hip",
     "gemv_batch.hip",
     "linear.hip",
+    "moe.hip",
     "flash_attention.hip",
     "fa_split.hip",
     "fa_noalloc.hip",
@@ -70,11 +71,12 @@ EXTRA_FLAGS = {
 # The count is right only if those loads stay between the copies and the
 # wait, which the compiler does not promise for loads of read-only memory,
 # so the device assembly of these sources is checked on every build.
-# flash_attention.hip and gemv_batch.hip wait for their copies by counting only
-# younger copies (inline assembly, which the compiler keeps in order) and
-# linear.hip for all of its copies at once, so only their use of M0 is checked.
+# flash_attention.hip, gemv_batch.hip and moe.hip wait for their copies by
+# counting only younger copies (inline assembly, which the compiler keeps in
+# order) and linear.hip for all of its copies at once, so only their use of M0 is
+# checked.
 COPY_WAIT_CHECKED = {"gemv.hip": True, "gemv_batch.hip": False, "linear.hip": False,
-                     "flash_attention.hip": False, "fa_split.hip": False}
+                     "moe.hip": False, "flash_attention.hip": False, "fa_split.hip": False}
 
 
 def check_copy_waits(asm_text, src="", waits=True):

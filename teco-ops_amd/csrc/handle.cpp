@@ -338,9 +338,9 @@ tecoopsStatus_t handle_scratch(tecoopsHandle_t handle, size_t bytes, void **out)
     // takes it over), leaving the graph writing freed memory.  Under capture
     // the caller passes a workspace or uses the allocation-free entry point.
     if (stream_captured(handle->stream)) {
-        TECO_ERROR("the handle's split-KV scratch cannot be used while its stream is captured: "
-                   "pass a workspace (tecoopsFlashAttentionEx) or call "
-                   "tecoopsFlashAttentionNoAlloc");
+        TECO_ERROR("the handle's scratch cannot be used while its stream is captured: pass a "
+                   "workspace (for attention, tecoopsFlashAttentionEx, or call "
+                   "tecoopsFlashAttentionNoAlloc)");
         return TECOOPS_STATUS_NOT_SUPPORTED;
     }
     return scratch_slot(handle, bytes, out);

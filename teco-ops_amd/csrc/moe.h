@@ -1,0 +1,80 @@
+// moe.h — how moe.hip cuts a mixture-of-experts layer into work items and where
+// they lie in its workspace: host code, shared with the tests.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <initializer_list>
+
+namespace tecoops {
+
+constexpr int kMoeMaxExperts = 1024;
+constexpr int kMoeMaxTopK = 32;
+constexpr int kMoeSlice = 512;  // tokens routed together; more run slice by slice
+
+// Rows of x staged for an item: the tokens of an expert go through in chunks of
+// this many, and W is read again for each.  Few tokens never need a second one;
+// many take the size that an even spread over the experts fills about half, so
+// that few experts overflow it.
+inline int moe_rows(int tokens, int top_k, int experts) {
+    if (tokens <= 4) return 4;
+    if (tokens <= 8) return 8;
+    if (tokens <= 16) return 16;
+    const int even = (tokens * top_k + experts - 1) / experts;
+    return even <= 8 ? 16 : even <= 20 ? 32 : 64;
+}
+
+struct MoeSpace {
+    int pairs, items;      // most (token, expert) pairs and items of a slice
+    int rows;              // of x per item
+    long long h_stride;    // elements between the rows of h
+    size_t items_at, ids_at, token_at, slot_at, weight_at, h_at, part_at;  // bytes
+    size_t bytes;
+};
+
+inline MoeSpace moe_space(int tokens, int hidden, int inter, int experts, int top_k) {
+    MoeSpace s{};
+    const int slice = tokens < kMoeSlice ? tokens : kMoeSlice;
+    s.pairs = slice * top_k;
+    s.rows = moe_rows(slice, top_k, experts);
+    s.items = experts + s.pairs / s.rows;
+    if (s.items > s.pairs) s.items = s.pairs;
+    s.h_stride = (inter + 7) / 8 * 8LL;
+    size_t at = 256;  // the number of items
+    const auto take = [&](size_t bytes) {
+        const size_t from = at;
+        at = (at + bytes + 255) / 256 * 256;
+        return from;
+    };
+    s.items_at = take(16 * static_cast<size_t>(s.items));
+    s.ids_at = take(4 * static_cast<size_t>(s.pairs));
+    s.token_at = take(4 * static_cast<size_t>(s.pairs));
+    s.slot_at = take(4 * static_cast<size_t>(s.pairs));
+    s.weight_at = take(4 * static_cast<size_t>(s.pairs));
+    s.h_at = take(2 * static_cast<size_t>(s.pairs) * s.h_stride);
+    s.part_at = take(4 * static_cast<size_t>(s.pairs) * hidden);
+    s.bytes = at;
+    return s;
+}
+
+// Rows of W per workgroup: the size whose busiest CU copies the fewest bytes of
+// W and x, with as many items as tokens spread evenly would make.
+inline int moe_wrows(int wrows, int tokens, int top_k, int experts, int rows, int cus) {
+    double items = experts;  // those that `tokens` random choices of top_k reach
+    double missed = 1.0;
+    for (int t = 0; t < tokens && missed > 1e-3; ++t) missed *= 1.0 - static_cast<double>(top_k) / experts;
+    items *= 1.0 - missed;
+    int best = 0;
+    double least = 0;
+    for (int r : {128, 64, 32, 16}) {
+        const long long wgs = static_cast<long long>(items + 0.5) * ((wrows + r - 1) / r);
+        const double bytes = static_cast<double>((wgs + cus - 1) / cus) * (2.0 * r + 2.0 * rows);
+        if (best == 0 || bytes < least) {
+            least = bytes;
+            best = r;
+        }
+    }
+    return best;
+}
+
+}  // namespace tecoops

@@ -1,0 +1,428 @@
+// moe.hip — a mixture-of-experts layer for a few tokens (a decode batch).
+//
+//   p = softmax(router_logits[t]);  e_0 .. e_{k-1}: the top k experts
+//   w_j = p[e_j]  (/ sum_j p[e_j] when renormalised)
+//   h_j = act(x W_in[e_j][:I]^T) * (x W_in[e_j][I:]^T)       rounded to T
+//   out[t] = T( sum_j w_j (h_j W_out[e_j]^T) )
+//
+// What bounds it is reading the chosen experts' weights, 3 H I values each.
+// Tokens are therefore grouped by expert: every weight is read from HBM once for
+// all tokens of its expert (gemv_stream.h), not once per token.
+//   route    softmax, top k and the groups: per expert a list of its (token, j)
+//            pairs, cut into items of up to XR pairs
+//   in       per item and block of rows of W_in: h of its pairs
+//   out      per item and block of rows of W_out: w_j (h_j W_out^T) in fp32
+//   combine  the k parts of each token, added in the order of j
+// No sum depends on the order in which workgroups run: a pair's place in its
+// group decides only which column of an MFMA it is.
+#include "moe.h"
+
+#include "common.h"
+#include "epilogue.h"
+#include "gemv_stream.h"
+
+namespace {
+
+using namespace tecoops::stream;
+using tecoops::MoeSpace;
+
+struct MoeArgs {
+    const char *x, *w_in, *w_out;
+    const void *logits;
+    uint16_t *out;
+    int *topk_ids;         // or null
+    float *topk_weights;   // or null
+    long long x_stride;    // bytes
+    int tokens, hidden, inter, experts, top_k;
+    int logits16, renorm, act;
+    int rows;              // of x per item
+    int units;             // blocks of rows of W per item
+    // workspace
+    int *n_items;
+    int4 *items;           // expert, first pair, pairs
+    int *ids;              // [tokens, top_k], -1: none
+    int *token, *slot;     // of a pair in the experts' order: its row of x, t * top_k + j
+    float *weight;
+    uint16_t *h;           // [pairs, h_stride]
+    long long h_stride;
+    float *part;           // [tokens, top_k, hidden]
+};
+
+// ------------------------------------------------------------------- routing
+
+// One workgroup: a wave takes a token at a time, E / 64 logits per lane.  The
+// best logit left is a maximum over the wave, its expert the lowest one that
+// holds it; -inf and NaN are never chosen, so a token may have fewer than k.
+template <typename T>
+__global__ void __launch_bounds__(1024) moe_route_kernel(MoeArgs a) {
+    __shared__ int count[tecoops::kMoeMaxExperts], first[tecoops::kMoeMaxExperts];
+    __shared__ int chunk_first[tecoops::kMoeMaxExperts];
+    __shared__ int wave_pairs[16], wave_chunks[16];
+    constexpr int R = tecoops::kMoeMaxExperts / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int nr = (a.experts + 63) / 64;
+    count[threadIdx.x] = 0;
+    for (int t = wave; t < a.tokens; t += 16) {
+        float v[R];
+        float local = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            v[r] = -INFINITY;
+            if (r >= nr) continue;
+            const int e = 64 * r + lane;
+            if (e < a.experts) {
+                const long long at = static_cast<long long>(t) * a.experts + e;
+                v[r] = a.logits16 ? Cvt<T>::to(static_cast<const uint16_t *>(a.logits)[at])
+                                  : static_cast<const float *>(a.logits)[at];
+                if (!(v[r] > -INFINITY)) v[r] = -INFINITY;  // NaN
+                v[r] += 0.0f;                               // -0 ties with 0
+            }
+            local = fmaxf(local, v[r]);
+        }
+        const float top = wave_max(local);
+        float sum = 0.0f, mine = 0.0f;  // lane j: exp(logit - top) of choice j
+        int id = -1;
+        if (!a.renorm) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (r < nr && v[r] > -INFINITY) sum += v[r] == top ? 1.0f : expf(v[r] - top);
+            sum = wave_sum(sum);
+        }
+        for (int j = 0; j < a.top_k; ++j) {
+            float best = -INFINITY;
+            int at = 0;
+#pragma unroll
+            for (int r = R - 1; r >= 0; --r)
+                if (r < nr && v[r] >= best) {
+                    best = v[r];
+                    at = r;
+                }
+            const float m = wave_max(best);
+            if (!(m > -INFINITY)) break;
+            const float e = -wave_max(best == m ? -static_cast<float>(64 * at + lane) : -INFINITY);
+            if (best == m && 64 * at + lane == static_cast<int>(e)) {
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (r == at) v[r] = -INFINITY;
+            }
+            if (lane == j) {
+                id = static_cast<int>(e);
+                mine = m == top ? 1.0f : expf(m - top);
+            }
+        }
+        if (a.renorm) sum = wave_sum(mine);
+        if (lane < a.top_k) {
+            const float w = id >= 0 ? mine / sum : 0.0f;
+            const int p = t * a.top_k + lane;
+            a.ids[p] = id;
+            if (a.topk_ids != nullptr) a.topk_ids[p] = id;
+            // kept for the lists below, in the pair's own place
+            a.part[p] = w;
+            if (a.topk_weights != nullptr) a.topk_weights[p] = w;
+        }
+    }
+    __syncthreads();
+    const int pairs = a.tokens * a.top_k;
+    for (int p = threadIdx.x; p < pairs; p += 1024) {
+        const int e = a.ids[p];
+        if (e >= 0) atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+    // first pair and first item of each expert: prefix sums over the experts
+    const int c = static_cast<int>(threadIdx.x) < a.experts ? count[threadIdx.x] : 0;
+    const int chunks = (c + a.rows - 1) / a.rows;
+    int sc = c, sk = chunks;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int oc = __shfl_up(sc, d), ok = __shfl_up(sk, d);
+        if (lane >= d) {
+            sc += oc;
+            sk += ok;
+        }
+    }
+    if (lane == 63) {
+        wave_pairs[wave] = sc;
+        wave_chunks[wave] = sk;
+    }
+    __syncthreads();
+    int bc = 0, bk = 0, total = 0;
+    for (int w = 0; w < 16; ++w) {
+        if (w < wave) {
+            bc += wave_pairs[w];
+            bk += wave_chunks[w];
+        }
+        total += wave_chunks[w];
+    }
+    first[threadIdx.x] = bc + sc - c;
+    chunk_first[threadIdx.x] = bk + sk - chunks;
+    for (int i = 0; i < chunks; ++i)
+        a.items[bk + sk - chunks + i] =
+            make_int4(threadIdx.x, bc + sc - c + i * a.rows, min(a.rows, c - i * a.rows), 0);
+    if (threadIdx.x == 0) *a.n_items = total;
+    count[threadIdx.x] = 0;
+    __syncthreads();
+    for (int p = threadIdx.x; p < pairs; p += 1024) {
+        const int e = a.ids[p];
+        if (e < 0) continue;
+        const int at = first[e] + atomicAdd(&count[e], 1);
+        a.token[at] = p / a.top_k;
+        a.slot[at] = p;
+        a.weight[at] = a.part[p];
+    }
+}
+
+// ------------------------------------------------------------------ products
+
+// IN: rows of W_in, 8 gate rows and the 8 up rows of the same outputs in each
+// tile of 16; OUT: rows of W_out.
+template <typename T, int XR, int WR, int RS, int KS, bool OUT>
+__global__ void __launch_bounds__(RS * KS * 64) moe_product_kernel(MoeArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int item = blockIdx.x / a.units, unit = blockIdx.x - item * a.units;
+    if (item >= *a.n_items) return;
+    const int4 it = a.items[item];
+    const int expert = it.x, first = it.y, count = it.z;
+    const int g = (threadIdx.x & 63) >> 4;
+    const int K = OUT ? a.inter : a.hidden, N = OUT ? a.hidden : a.inter;
+    const char *w = (OUT ? a.w_out : a.w_in) +
+                    static_cast<long long>(expert) * (OUT ? 2 : 4) * a.hidden * a.inter;
+    const int n0 = unit * RS * WR / (OUT ? 1 : 2);
+    const auto w_row = [&](int r) {
+        const int from = OUT ? min(n0 + r, N - 1)
+                             : min(n0 + (r >> 4) * 8 + (r & 7), N - 1) + ((r & 8) ? N : 0);
+        return w + static_cast<long long>(from) * K * 2;
+    };
+    const auto x_row = [&](int r) {
+        const int p = first + min(r, count - 1);
+        return OUT ? reinterpret_cast<const char *>(a.h + p * a.h_stride)
+                   : a.x + a.token[p] * a.x_stride;
+    };
+    const auto put = [&](int r, int col, f32x4_t s) {
+        if constexpr (OUT) {
+            const int n = n0 + r;
+            if (col >= count || n >= N) return;  // N % 8 == 0: four at a time
+            const float wt = a.weight[first + col];
+            *reinterpret_cast<f32x4_t *>(a.part + static_cast<long long>(a.slot[first + col]) * N + n) =
+                f32x4_t{wt * s[0], wt * s[1], wt * s[2], wt * s[3]};
+        } else {
+            f32x4_t u;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) u[v] = from_upper_half(s[v]);
+            const int n = n0 + (r >> 4) * 8 + (r & 7);
+            if (col >= count || g >= 2 || n >= N) return;
+            // h is rounded to T, the second product's operand type
+            *reinterpret_cast<uint2 *>(a.h + (first + col) * a.h_stride + n) =
+                make_uint2(pack<T>(activate(s[0], a.act) * u[0], activate(s[1], a.act) * u[1]),
+                           pack<T>(activate(s[2], a.act) * u[2], activate(s[3], a.act) * u[3]));
+        }
+    };
+    product<T, false, XR, WR, RS, KS>(lds, K, unit, w_row, x_row, put);
+}
+
+// Widths that are not in whole 16-byte words, or tensors that are not aligned: a
+// wave per pair and row of the product.
+template <typename T, bool OUT>
+__global__ void __launch_bounds__(256) moe_scalar_kernel(MoeArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int N = OUT ? a.hidden : a.inter, K = OUT ? a.inter : a.hidden;
+    const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int item = blockIdx.y;
+    if (n >= N || item >= *a.n_items) return;
+    const int4 it = a.items[item];
+    const uint16_t *w = reinterpret_cast<const uint16_t *>(OUT ? a.w_out : a.w_in) +
+                        static_cast<long long>(it.x) * (OUT ? 1 : 2) * a.hidden * a.inter +
+                        static_cast<long long>(n) * K;
+    for (int p = it.y; p < it.y + it.z; ++p) {
+        const uint16_t *x = OUT ? a.h + p * a.h_stride
+                                : reinterpret_cast<const uint16_t *>(a.x + a.token[p] * a.x_stride);
+        float s = 0.0f, u = 0.0f;
+        for (int k = lane; k < K; k += 64) {
+            const float xv = Cvt<T>::to(x[k]);
+            s += Cvt<T>::to(w[k]) * xv;
+            if (!OUT) u += Cvt<T>::to(w[static_cast<long long>(N) * K + k]) * xv;
+        }
+        s = wave_sum(s);
+        if (!OUT) u = wave_sum(u);
+        if (lane != 0) continue;
+        if (OUT)
+            a.part[static_cast<long long>(a.slot[p]) * N + n] = a.weight[p] * s;
+        else
+            a.h[p * a.h_stride + n] = Cvt<T>::from(activate(s, a.act) * u);
+    }
+}
+
+// out[t] from the parts of its pairs, in the order of j; zero where it has none.
+template <typename T>
+__global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a) {
+    const int t = blockIdx.y;
+    const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (n >= a.hidden) return;
+    const bool whole = a.hidden % 4 == 0;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < a.top_k; ++j) {
+        const int p = t * a.top_k + j;
+        if (a.ids[p] < 0) break;  // the choices come first
+        const float *src = a.part + static_cast<long long>(p) * a.hidden + n;
+        if (whole) {
+            const f32x4_t v = *reinterpret_cast<const f32x4_t *>(src);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < a.hidden) s[i] += src[i];
+        }
+    }
+    uint16_t *dst = a.out + static_cast<long long>(t) * a.hidden + n;
+    if (whole && tecoops::aligned(dst, 8)) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<T>(s[0], s[1]), pack<T>(s[2], s[3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < a.hidden) dst[i] = Cvt<T>::from(s[i]);
+    }
+}
+
+template <typename T, int XR, int WR, int RS, int KS, bool OUT>
+bool launch(MoeArgs a, int items, hipStream_t s) {
+    using S = Shape<false, XR, WR, RS, KS>;
+    static_assert(S::D >= 2, "two stages fit in LDS");
+    auto *kern = &moe_product_kernel<T, XR, WR, RS, KS, OUT>;
+    if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), S::LDS)) return false;
+    a.units = static_cast<int>(tecoops::ceil_div(OUT ? a.hidden : 2LL * a.inter, RS * WR));
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(a.units) * items), dim3(S::NW * 64), S::LDS, s, a);
+    return true;
+}
+
+template <typename T, int XR, bool OUT>
+bool launch_wrows(const MoeArgs &a, int items, hipStream_t s) {
+    switch (tecoops::moe_wrows(OUT ? a.hidden : 2 * a.inter, a.tokens, a.top_k, a.experts, XR,
+                               tecoops::device_cus())) {
+        case 16: return launch<T, XR, 16, 1, 4, OUT>(a, items, s);
+        case 32: return launch<T, XR, 16, 2, 2, OUT>(a, items, s);
+        case 64: return launch<T, XR, 32, 2, 2, OUT>(a, items, s);
+        default: return launch<T, XR, 16, 8, 1, OUT>(a, items, s);
+    }
+}
+
+template <typename T, bool OUT>
+bool launch_product(const MoeArgs &a, int items, bool copy, hipStream_t s) {
+    if (!copy) {
+        hipLaunchKernelGGL((moe_scalar_kernel<T, OUT>),
+                           dim3(tecoops::ceil_div(OUT ? a.hidden : a.inter, 4), items), dim3(256), 0,
+                           s, a);
+        return true;
+    }
+    switch (a.rows) {
+        case 4: return launch_wrows<T, 4, OUT>(a, items, s);
+        case 8: return launch_wrows<T, 8, OUT>(a, items, s);
+        case 16: return launch_wrows<T, 16, OUT>(a, items, s);
+        case 32: return launch_wrows<T, 32, OUT>(a, items, s);
+        default: return launch_wrows<T, 64, OUT>(a, items, s);
+    }
+}
+
+template <typename T>
+tecoopsStatus_t run_slice(const MoeArgs &a, int items, bool copy, hipStream_t s) {
+    hipLaunchKernelGGL((moe_route_kernel<T>), dim3(1), dim3(1024), 0, s, a);
+    TECO_CHECK_LAUNCH("moe_layer");
+    if (!launch_product<T, false>(a, items, copy, s)) return TECOOPS_STATUS_INTERNAL_ERROR;
+    TECO_CHECK_LAUNCH("moe_layer");
+    if (!launch_product<T, true>(a, items, copy, s)) return TECOOPS_STATUS_INTERNAL_ERROR;
+    TECO_CHECK_LAUNCH("moe_layer");
+    hipLaunchKernelGGL((moe_combine_kernel<T>), dim3(tecoops::ceil_div(a.hidden, 1024), a.tokens),
+                       dim3(256), 0, s, a);
+    TECO_CHECK_LAUNCH("moe_layer");
+    return TECOOPS_STATUS_SUCCESS;
+}
+
+tecoopsStatus_t check_sizes(int tokens, int hidden, int inter, int experts, int top_k) {
+    if (tokens < 0 || hidden <= 0 || inter <= 0 || experts <= 0 || top_k <= 0 || top_k > experts)
+        return TECOOPS_STATUS_BAD_PARAM;
+    if (experts > tecoops::kMoeMaxExperts || top_k > tecoops::kMoeMaxTopK ||
+        hidden > (1 << 20) || inter > (1 << 20))
+        return TECOOPS_STATUS_NOT_SUPPORTED;
+    return TECOOPS_STATUS_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" tecoopsStatus_t tecoopsGetMoeLayerWorkspaceSize(int tokens, int hidden, int inter,
+                                                           int experts, int top_k, size_t *bytes) {
+    if (bytes == nullptr) return TECOOPS_STATUS_BAD_PARAM;
+    const tecoopsStatus_t st = check_sizes(tokens, hidden, inter, experts, top_k);
+    if (st != TECOOPS_STATUS_SUCCESS) return st;
+    *bytes = tokens == 0 ? 0 : tecoops::moe_space(tokens, hidden, inter, experts, top_k).bytes;
+    return TECOOPS_STATUS_SUCCESS;
+}
+
+extern "C" tecoopsStatus_t tecoopsMoeLayer(tecoopsHandle_t handle, const void *x, long long x_stride,
+                                           const void *w_in, const void *w_out,
+                                           const void *router_logits, tecoopsDataType_t logitsType,
+                                           void *out, int *topk_ids, float *topk_weights, int tokens,
+                                           int hidden, int inter, int experts, int top_k,
+                                           int renormalize, tecoopsActivation_t activation,
+                                           void *workspace, size_t workspace_bytes,
+                                           tecoopsDataType_t dataType) {
+    if (handle == nullptr) return TECOOPS_STATUS_NOT_INITIALIZED;
+    if (x == nullptr || w_in == nullptr || w_out == nullptr || router_logits == nullptr ||
+        out == nullptr)
+        return TECOOPS_STATUS_BAD_PARAM;
+    const tecoopsStatus_t st = check_sizes(tokens, hidden, inter, experts, top_k);
+    if (st != TECOOPS_STATUS_SUCCESS) return st;
+    if (x_stride < hidden || !tecoops::epilogue_act_ok(activation) ||
+        !tecoops::is_16bit_float(dataType))
+        return TECOOPS_STATUS_BAD_PARAM;
+    if (logitsType != TECOOPS_DATA_FLOAT && logitsType != dataType) return TECOOPS_STATUS_BAD_PARAM;
+    const size_t logit = logitsType == TECOOPS_DATA_FLOAT ? 4 : 2;
+    if (!tecoops::aligned(x, 2) || !tecoops::aligned(w_in, 2) || !tecoops::aligned(w_out, 2) ||
+        !tecoops::aligned(out, 2) || !tecoops::aligned(router_logits, logit) ||
+        !tecoops::aligned(topk_ids, 4) || !tecoops::aligned(topk_weights, 4))
+        return TECOOPS_STATUS_BAD_PARAM;
+    if (tokens == 0) return TECOOPS_STATUS_SUCCESS;
+    const MoeSpace sp = tecoops::moe_space(tokens, hidden, inter, experts, top_k);
+    if (workspace == nullptr) {
+        const tecoopsStatus_t got = tecoops::handle_scratch(handle, sp.bytes, &workspace);
+        if (got != TECOOPS_STATUS_SUCCESS) return got;
+    } else if (workspace_bytes < sp.bytes || !tecoops::aligned(workspace, 16)) {
+        return TECOOPS_STATUS_BAD_PARAM;
+    }
+    char *ws = static_cast<char *>(workspace);
+    MoeArgs a{};
+    a.w_in = static_cast<const char *>(w_in);
+    a.w_out = static_cast<const char *>(w_out);
+    a.x_stride = x_stride * 2;
+    a.hidden = hidden;
+    a.inter = inter;
+    a.experts = experts;
+    a.top_k = top_k;
+    a.logits16 = logit == 2;
+    a.renorm = renormalize != 0;
+    a.act = activation;
+    a.rows = sp.rows;
+    a.n_items = reinterpret_cast<int *>(ws);
+    a.items = reinterpret_cast<int4 *>(ws + sp.items_at);
+    a.ids = reinterpret_cast<int *>(ws + sp.ids_at);
+    a.token = reinterpret_cast<int *>(ws + sp.token_at);
+    a.slot = reinterpret_cast<int *>(ws + sp.slot_at);
+    a.weight = reinterpret_cast<float *>(ws + sp.weight_at);
+    a.h = reinterpret_cast<uint16_t *>(ws + sp.h_at);
+    a.h_stride = sp.h_stride;
+    a.part = reinterpret_cast<float *>(ws + sp.part_at);
+    const bool copy = hidden % 8 == 0 && inter % 8 == 0 && x_stride % 8 == 0 &&
+                      tecoops::aligned(x, 16) && tecoops::aligned(w_in, 16) &&
+                      tecoops::aligned(w_out, 16);
+    for (int t0 = 0; t0 < tokens; t0 += tecoops::kMoeSlice) {
+        a.tokens = tokens - t0 < tecoops::kMoeSlice ? tokens - t0 : tecoops::kMoeSlice;
+        a.x = static_cast<const char *>(x) + t0 * a.x_stride;
+        a.logits = static_cast<const char *>(router_logits) + static_cast<long long>(t0) * experts * logit;
+        a.out = static_cast<uint16_t *>(out) + static_cast<long long>(t0) * hidden;
+        a.topk_ids = topk_ids ? topk_ids + static_cast<long long>(t0) * top_k : nullptr;
+        a.topk_weights = topk_weights ? topk_weights + static_cast<long long>(t0) * top_k : nullptr;
+        const tecoopsStatus_t done = dataType == TECOOPS_DATA_HALF
+                                         ? run_slice<f16>(a, sp.items, copy, handle->stream)
+                                         : run_slice<bf16>(a, sp.items, copy, handle->stream);
+        if (done != TECOOPS_STATUS_SUCCESS) return done;
+    }
+    return TECOOPS_STATUS_SUCCESS;
+}

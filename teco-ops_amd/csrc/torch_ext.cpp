@@ -372,6 +372,49 @@ void linear(const Tensor &x, const Tensor &weight, Tensor &out, const c10::optio
           "linear");
 }
 
+void moe_layer(const Tensor &x, const Tensor &w_in, const Tensor &w_out, const Tensor &router_logits,
+               int64_t top_k, Tensor &out, bool renormalize, c10::string_view activation,
+               const c10::optional<Tensor> &topk_ids, const c10::optional<Tensor> &topk_weights) {
+    const Tensor *ids = given(topk_ids), *weights = given(topk_weights);
+    need_cuda({&x, &w_in, &w_out, &router_logits, &out, ids, weights});
+    same_device(x, {&w_in, &w_out, &router_logits, &out, ids, weights});
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    const tecoopsDataType_t dt = dtype_of(x);
+    TORCH_CHECK(x.dim() == 2 && w_in.dim() == 3 && w_out.dim() == 3 && router_logits.dim() == 2,
+                "moe_layer: x [T, H], w_in [E, 2I, H], w_out [E, H, I], router_logits [T, E]");
+    const int t = fits_int(x.size(0), "T"), e = fits_int(w_out.size(0), "E"),
+              h = fits_int(w_out.size(1), "H"), i = fits_int(w_out.size(2), "I"),
+              k = fits_int(top_k, "top_k");
+    TORCH_CHECK(w_in.size(0) == e && w_in.size(1) == 2LL * i && w_in.size(2) == h &&
+                    router_logits.size(0) == t && router_logits.size(1) == e && out.dim() == 2 &&
+                    out.size(0) == t && out.size(1) == h,
+                "moe_layer: x [T, H], w_in [E, 2I, H], w_out [E, H, I], router_logits [T, E], out [T, H]");
+    need_contiguous({&w_in, &w_out, &router_logits, &out, ids, weights});
+    need_dtype(w_in, x.scalar_type(), "w_in");
+    need_dtype(w_out, x.scalar_type(), "w_out");
+    need_dtype(out, x.scalar_type(), "out");
+    const bool wide = router_logits.scalar_type() == at::kFloat;
+    if (!wide) need_dtype(router_logits, x.scalar_type(), "router_logits");
+    for (const Tensor *o : {ids, weights})
+        if (o)
+            TORCH_CHECK(o->dim() == 2 && o->size(0) == t && o->size(1) == k,
+                        "moe_layer: topk_ids and topk_weights must be [T, top_k]");
+    if (ids) need_dtype(*ids, at::kInt, "topk_ids");
+    if (weights) need_dtype(*weights, at::kFloat, "topk_weights");
+    const int64_t xs = row_stride(x, t, h, "x");
+    const tecoopsActivation_t act = activation_of(activation);
+    if (t == 0) return;
+    size_t bytes = 0;
+    check(tecoopsGetMoeLayerWorkspaceSize(t, h, i, e, k, &bytes), "moe_layer");
+    const Tensor ws = workspace_of(bytes, x);
+    check(tecoopsMoeLayer(handle_for(x), x.data_ptr(), xs, w_in.data_ptr(), w_out.data_ptr(),
+                          router_logits.data_ptr(), wide ? TECOOPS_DATA_FLOAT : dt, out.data_ptr(),
+                          ids ? ids->data_ptr<int>() : nullptr,
+                          weights ? weights->data_ptr<float>() : nullptr, t, h, i, e, k, renormalize,
+                          act, ws.data_ptr(), bytes, dt),
+          "moe_layer");
+}
+
 // The arguments of the rotary functions of several axes, checked.
 struct AxesArgs {
     std::vector<int> sections;
@@ -514,6 +557,9 @@ TORCH_LIBRARY(tecoops, m) {
     m.def("gemv_int8(Tensor weight, Tensor scales, Tensor x, Tensor(a!) out) -> ()");
     m.def("linear(Tensor x, Tensor weight, Tensor(a!) out, Tensor? bias, Tensor? residual, "
           "str activation, bool gated) -> ()");
+    m.def("moe_layer(Tensor x, Tensor w_in, Tensor w_out, Tensor router_logits, int top_k, "
+          "Tensor(a!) out, bool renormalize, str activation, Tensor(b!)? topk_ids, "
+          "Tensor(c!)? topk_weights) -> ()");
     m.def("rotary_embedding_axes(Tensor positions, Tensor(a!) query, Tensor(b!)? key, "
           "int head_size, int[] sections, Tensor? cos_sin_cache, bool is_neox, float base, "
           "int rot_dim, str layout) -> ()");
@@ -535,6 +581,7 @@ TORCH_LIBRARY_IMPL(tecoops, CUDA, m) {
     m.impl("gemv", &gemv);
     m.impl("gemv_int8", &gemv_int8);
     m.impl("linear", &linear);
+    m.impl("moe_layer", &moe_layer);
     m.impl("rotary_embedding_axes", &rotary_embedding_axes);
     m.impl("rotary_axes_reshape_and_cache", &rotary_axes_reshape_and_cache);
     m.impl("memset", &memset_);

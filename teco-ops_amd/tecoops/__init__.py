@@ -41,7 +41,7 @@ __all__ = [
     "flash_attn_varlen_func", "causal_conv1d_fn_torch",
     # extensions
     "rotary_embedding", "rotary_reshape_and_cache", "gemv", "gemv_int8", "causal_conv1d",
-    "memset", "linear", "rotary_embedding_axes", "rotary_axes_reshape_and_cache", "ops",
+    "memset", "linear", "moe_layer", "rotary_embedding_axes", "rotary_axes_reshape_and_cache", "ops",
 ]
 
 _tls = threading.local()   # per thread: {device index: _Handle}
@@ -417,6 +417,51 @@ def linear(x, weight, out, bias=None, residual=None, activation=None, gated=Fals
     _call_on(device, "tecoopsLinear", _handle(device), _ptr(x), xs, _ptr(weight), _ptr(bias),
              _ptr(residual), rs, _ptr(out), os_, M, N, K, act, int(bool(gated)), _ptr(space),
              0 if space is None else space.numel(), code)
+
+
+def moe_layer(x, w_in, w_out, router_logits, top_k, out, renormalize=True, activation="silu",
+              topk_ids=None, topk_weights=None):
+    """Mixture-of-experts layer for a decode batch: softmax over router_logits
+    [T, E] (float32 or x's type), each token's top_k experts (ties to the lowest
+    index; -inf and NaN never chosen), and the sum of their outputs
+    (act(x Wg^T) * (x Wu^T)) W_out^T with the routing weights, renormalised over
+    the chosen or not.
+
+    x [T, H] (rows packed, any distance apart); w_in [E, 2I, H], an expert's gate
+    rows before its up rows; w_out [E, H, I]; out [T, H], zero for a token all of
+    whose logits are -inf.  topk_ids int32 and topk_weights float32 [T, top_k]
+    are written when given, best first, -1 and 0 where there is none."""
+    _check_cuda(x, w_in, w_out, router_logits, out, topk_ids, topk_weights)
+    code, device = _dtype_code(x), x.device
+    if w_in.dim() != 3 or w_out.dim() != 3 or x.dim() != 2 or router_logits.dim() != 2:
+        raise ValueError("tecoops.moe_layer: x [T, H], w_in [E, 2I, H], w_out [E, H, I], "
+                         "router_logits [T, E]")
+    (E, H, I), T = w_out.shape, x.shape[0]
+    if w_in.shape != (E, 2 * I, H) or router_logits.shape != (T, E) or out.shape != (T, H):
+        raise ValueError(f"tecoops.moe_layer: w_in must be [{E}, {2 * I}, {H}], router_logits "
+                         f"[{T}, {E}] and out [{T}, {H}]")
+    _check_contiguous(w_in=w_in, w_out=w_out, router_logits=router_logits, out=out,
+                      topk_ids=topk_ids, topk_weights=topk_weights)
+    _check_device(device, w_in=w_in, w_out=w_out, router_logits=router_logits, out=out,
+                  topk_ids=topk_ids, topk_weights=topk_weights)
+    for name, t in (("w_in", w_in), ("w_out", w_out), ("out", out)):
+        _check_dtype(t, name, x.dtype)
+    _check_dtype(router_logits, "router_logits", torch.float32, x.dtype)
+    _check_dtype(topk_ids, "topk_ids", torch.int32)
+    _check_dtype(topk_weights, "topk_weights", torch.float32)
+    top_k = int(top_k)
+    for name, t in (("topk_ids", topk_ids), ("topk_weights", topk_weights)):
+        if t is not None and t.shape != (T, top_k):
+            raise ValueError(f"tecoops.moe_layer: {name} must be [{T}, {top_k}]")
+    xs = _check_rows(x, "x", H)
+    act = _choice(_lib.ACTIVATIONS, activation, "activation")
+    if T == 0:
+        return
+    space = _workspace(device, "tecoopsGetMoeLayerWorkspaceSize", T, H, I, E, top_k)
+    _call_on(device, "tecoopsMoeLayer", _handle(device), _ptr(x), xs, _ptr(w_in), _ptr(w_out),
+             _ptr(router_logits), _lib.DATA_FLOAT if router_logits.dtype == torch.float32 else code,
+             _ptr(out), _ptr(topk_ids), _ptr(topk_weights), T, H, I, E, top_k,
+             int(bool(renormalize)), act, _ptr(space), space.numel(), code)
 
 
 def _workspace(device, size, *args):

@@ -81,6 +81,8 @@ SIGNATURES = {
     "tecoopsGemvInt8": (I, [P, P, P, P, P, I, I, I]),
     "tecoopsLinear": (I, [P, P, LL, P, P, P, LL, P, LL, I, I, I, I, I, P, SZ, I]),
     "tecoopsGetLinearWorkspaceSize": (I, [I, I, I, I, P]),
+    "tecoopsMoeLayer": (I, [P, P, LL, P, P, P, I, P, P, P, I, I, I, I, I, I, I, P, SZ, I]),
+    "tecoopsGetMoeLayerWorkspaceSize": (I, [I, I, I, I, I, P]),
     "tecoopsRotaryEmbeddingAxes": (I, [P, P, LL, I, P, I, P, P, I, I, I, I, I, LL, LL, P, I, F, I,
                                        I]),
     "tecoopsRotaryAxesReshapeAndCache": (I, [P, P, LL, I, P, I, P, P, P, P, P, P, I, I, I, I, I, LL,

@@ -129,3 +129,88 @@ def test_plan_covers_the_product(plan, gated, copy):
                     assert need == (splits * m * n * (2 if gated else 1) * 4 if splits > 1 else 0)
                     assert need <= ws
                     assert copy or bm == 128
+
+
+def test_moe_refusals(handle):
+    f = _lib.lib().tecoopsMoeLayer
+    good = dict(h=handle, x=P, xs=64, wi=P, wo=P, lg=P, lt=0, o=P, ids=None, w=None, T=2, H=64, I=32,
+                E=8, k=2, rn=1, act=2, ws=P, wb=1 << 40, dt=1)
+
+    def call(**kw):
+        a = {**good, **kw}
+        return f(*(a[k] for k in good))
+
+    assert call(h=None) == NOT_INIT
+    for kw in (dict(x=None), dict(wi=None), dict(wo=None), dict(lg=None), dict(o=None), dict(T=-1),
+               dict(H=0), dict(I=0), dict(E=0), dict(k=0), dict(k=9), dict(xs=63), dict(act=5),
+               dict(act=-1), dict(dt=0), dict(lt=9), dict(lt=4), dict(x=P + 1), dict(wi=P + 1),
+               dict(wo=P + 1), dict(o=P + 1), dict(lg=P + 2), dict(ids=P + 2), dict(w=P + 2),
+               dict(wb=100), dict(wb=0), dict(ws=P + 8)):
+        assert call(**kw) == BAD, kw
+    assert call(E=1025) == NOT_SUP and call(E=64, k=33) == NOT_SUP
+    assert call(H=(1 << 20) + 8, xs=1 << 21) == NOT_SUP and call(I=(1 << 20) + 8) == NOT_SUP
+    assert call(T=0) == OK  # no launch
+    g = _lib.lib().tecoopsGetMoeLayerWorkspaceSize
+    size = ctypes.c_size_t(1)
+    assert g(2, 64, 32, 8, 2, None) == BAD and g(2, 64, 32, 8, 9, ctypes.byref(size)) == BAD
+    assert g(2, 64, 32, 2000, 9, ctypes.byref(size)) == NOT_SUP
+    assert g(0, 64, 32, 8, 2, ctypes.byref(size)) == OK and size.value == 0
+
+
+@pytest.fixture(scope="module")
+def space(tmp_path_factory):
+    d = tmp_path_factory.mktemp("space")
+    (d / "space.cpp").write_text("""#include "moe.h"
+extern "C" void space(int t, int h, int i, int e, int k, long long *o) {
+    const auto s = tecoops::moe_space(t, h, i, e, k);
+    const long long v[] = {s.pairs, s.items, s.rows, s.h_stride, (long long)s.items_at,
+                           (long long)s.ids_at, (long long)s.token_at, (long long)s.slot_at,
+                           (long long)s.weight_at, (long long)s.h_at, (long long)s.part_at,
+                           (long long)s.bytes};
+    for (int j = 0; j < 12; ++j) o[j] = v[j];
+}
+extern "C" int wrows(int n, int t, int k, int e, int rows) {
+    return tecoops::moe_wrows(n, t, k, e, rows, 256);
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-fPIC", "-shared", "-I", CSRC, str(d / "space.cpp"), "-o",
+                    str(d / "space.so")], check=True)
+    return ctypes.CDLL(str(d / "space.so"))
+
+
+def test_moe_workspace_holds_any_routing(space):
+    """Parts of the workspace do not overlap; the items are enough for every
+    spread of the pairs over the experts."""
+    import random
+    r = random.Random(1)
+    for _ in range(600):
+        E = r.choice([1, 2, 5, 8, 64, 128, 1000])
+        k, T = r.randint(1, min(E, 32)), r.choice([1, 2, 4, 5, 9, 16, 17, 100, 511, 512, 513, 2000])
+        H, I = r.choice([1, 8, 70, 4096]), r.choice([1, 8, 33, 14336])
+        o = (ctypes.c_longlong * 12)()
+        space.space(T, H, I, E, k, o)
+        pairs, items, rows, stride, *at, total = list(o)
+        assert pairs == min(T, 512) * k and stride % 8 == 0 and I <= stride < I + 8
+        sizes = [16 * items, 4 * pairs, 4 * pairs, 4 * pairs, 4 * pairs, 2 * pairs * stride,
+                 4 * pairs * H]
+        assert at[0] >= 4
+        for a, s, nxt in zip(at, sizes, at[1:] + [total]):
+            assert a % 256 == 0 and a + s <= nxt
+        # the spread with the most items: one pair over a multiple of `rows` in as
+        # many experts as possible
+        t = min(T, 512)
+        counts, left = [0] * E, pairs
+        for e in range(E):
+            counts[e] = min(1, left)
+            left -= counts[e]
+        for e in range(E):
+            more = min(left, (t - counts[e]) // rows * rows)
+            counts[e] += more
+            left -= more
+        for e in range(E):
+            more = min(left, t - counts[e])
+            counts[e] += more
+            left -= more
+        assert left == 0 and sum(-(-c // rows) for c in counts) <= items
+        assert T > 4 or rows >= T
+        assert space.wrows(2 * I, t, k, E, rows) in (16, 32, 64, 128)
