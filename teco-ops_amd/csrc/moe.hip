@@ -50,125 +50,192 @@ struct MoeArgs {
 
 // ------------------------------------------------------------------- routing
 
-// One workgroup: a wave takes a token at a time, E / 64 logits per lane.  The
-// best logit left is a maximum over the wave, its expert the lowest one that
-// holds it; -inf and NaN are never chosen, so a token may have fewer than k.
-template <typename T>
-__global__ void __launch_bounds__(1024) moe_route_kernel(MoeArgs a) {
-    __shared__ int count[tecoops::kMoeMaxExperts], first[tecoops::kMoeMaxExperts];
-    __shared__ int chunk_first[tecoops::kMoeMaxExperts];
-    __shared__ int wave_pairs[16], wave_chunks[16];
-    constexpr int R = tecoops::kMoeMaxExperts / 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int nr = (a.experts + 63) / 64;
-    count[threadIdx.x] = 0;
-    for (int t = wave; t < a.tokens; t += 16) {
-        float v[R];
-        float local = -INFINITY;
+// Softmax and top k of token t by one wave, R logits per lane (of expert 64 r +
+// lane).  The best logit left is a maximum over the wave, its expert the lowest
+// one that holds it; -inf and NaN are never chosen, so a token may have fewer
+// than k.  Lane j ends with choice j: its expert or -1, and its weight.
+template <typename T, int R>
+__device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane, int &id, float &weight) {
+    float v[R];
+    float local = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            v[r] = -INFINITY;
-            if (r >= nr) continue;
-            const int e = 64 * r + lane;
-            if (e < a.experts) {
-                const long long at = static_cast<long long>(t) * a.experts + e;
-                v[r] = a.logits16 ? Cvt<T>::to(static_cast<const uint16_t *>(a.logits)[at])
-                                  : static_cast<const float *>(a.logits)[at];
-                if (!(v[r] > -INFINITY)) v[r] = -INFINITY;  // NaN
-                v[r] += 0.0f;                               // -0 ties with 0
-            }
-            local = fmaxf(local, v[r]);
-        }
-        const float top = wave_max(local);
-        float sum = 0.0f, mine = 0.0f;  // lane j: exp(logit - top) of choice j
-        int id = -1;
-        if (!a.renorm) {
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-                if (r < nr && v[r] > -INFINITY) sum += v[r] == top ? 1.0f : expf(v[r] - top);
-            sum = wave_sum(sum);
-        }
-        for (int j = 0; j < a.top_k; ++j) {
-            float best = -INFINITY;
-            int at = 0;
-#pragma unroll
-            for (int r = R - 1; r >= 0; --r)
-                if (r < nr && v[r] >= best) {
-                    best = v[r];
-                    at = r;
-                }
-            const float m = wave_max(best);
-            if (!(m > -INFINITY)) break;
-            const float e = -wave_max(best == m ? -static_cast<float>(64 * at + lane) : -INFINITY);
-            if (best == m && 64 * at + lane == static_cast<int>(e)) {
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-                    if (r == at) v[r] = -INFINITY;
-            }
-            if (lane == j) {
-                id = static_cast<int>(e);
-                mine = m == top ? 1.0f : expf(m - top);
-            }
-        }
-        if (a.renorm) sum = wave_sum(mine);
-        if (lane < a.top_k) {
-            const float w = id >= 0 ? mine / sum : 0.0f;
-            const int p = t * a.top_k + lane;
-            a.ids[p] = id;
-            if (a.topk_ids != nullptr) a.topk_ids[p] = id;
-            // kept for the lists below, in the pair's own place
-            a.part[p] = w;
-            if (a.topk_weights != nullptr) a.topk_weights[p] = w;
+    for (int r = 0; r < R; ++r) {
+        const int e = 64 * r + lane;
+        v[r] = -INFINITY;
+        if (e < a.experts) {
+            const long long at = static_cast<long long>(t) * a.experts + e;
+            v[r] = a.logits16 ? Cvt<T>::to(static_cast<const uint16_t *>(a.logits)[at])
+                              : static_cast<const float *>(a.logits)[at];
         }
     }
-    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (!(v[r] > -INFINITY)) v[r] = -INFINITY;  // NaN
+        v[r] += 0.0f;                               // -0 ties with 0
+        local = fmaxf(local, v[r]);
+    }
+    const float top = wave_max(local);
+    float sum = 0.0f, mine = 0.0f;  // mine: exp(logit - top) of choice `lane`
+    id = -1;
+    if (!a.renorm) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float p = v[r] == top ? 1.0f : expf(v[r] - top);
+            sum += v[r] > -INFINITY ? p : 0.0f;
+        }
+        sum = wave_sum(sum);
+    }
+    for (int j = 0; j < a.top_k; ++j) {
+        float best = v[R - 1];
+        int e = 64 * (R - 1) + lane;
+#pragma unroll
+        for (int r = R - 2; r >= 0; --r)
+            if (v[r] >= best) {
+                best = v[r];
+                e = 64 * r + lane;
+            }
+        const float m = j == 0 ? top : wave_max(best);
+        if (!(m > -INFINITY)) break;
+        const int won = static_cast<int>(-wave_max(best == m ? -static_cast<float>(e) : -INFINITY));
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (won == 64 * r + lane) v[r] = -INFINITY;
+        if (lane == j) {
+            id = won;
+            mine = m;
+        }
+    }
+    mine = id < 0 ? 0.0f : mine == top ? 1.0f : expf(mine - top);
+    if (a.renorm) sum = wave_sum(mine);
+    weight = id < 0 ? 0.0f : mine / sum;
+}
+
+__device__ __forceinline__ void store_choice(const MoeArgs &a, int p, int id, float weight) {
+    a.ids[p] = id;
+    if (a.topk_ids != nullptr) a.topk_ids[p] = id;
+    if (a.topk_weights != nullptr) a.topk_weights[p] = weight;
+}
+
+// Groups the pairs by expert and cuts the groups into items, by a workgroup of
+// 1024: pair(p, e, w) gives pair p's expert and weight.  A pair's place in its
+// group follows the order of the atomics; it decides which column of an MFMA
+// the pair is, and no result depends on it.
+template <typename Pair>
+__device__ __forceinline__ void group(const MoeArgs &a, Pair &&pair) {
+    __shared__ int count[tecoops::kMoeMaxExperts], first[tecoops::kMoeMaxExperts];
+    __shared__ int wave_pairs[16], wave_items[16];
+    const int me = threadIdx.x, lane = me & 63, wave = me >> 6;
     const int pairs = a.tokens * a.top_k;
-    for (int p = threadIdx.x; p < pairs; p += 1024) {
-        const int e = a.ids[p];
+    count[me] = 0;
+    __syncthreads();
+    for (int p = me; p < pairs; p += 1024) {
+        int e;
+        float w;
+        pair(p, e, w);
         if (e >= 0) atomicAdd(&count[e], 1);
     }
     __syncthreads();
-    // first pair and first item of each expert: prefix sums over the experts
-    const int c = static_cast<int>(threadIdx.x) < a.experts ? count[threadIdx.x] : 0;
-    const int chunks = (c + a.rows - 1) / a.rows;
-    int sc = c, sk = chunks;
+    // first pair and first item of expert `me`: prefix sums over the experts
+    const int c = count[me];
+    const int items = (c + a.rows - 1) / a.rows;
+    int sc = c, si = items;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-        const int oc = __shfl_up(sc, d), ok = __shfl_up(sk, d);
+        const int oc = __shfl_up(sc, d), oi = __shfl_up(si, d);
         if (lane >= d) {
             sc += oc;
-            sk += ok;
+            si += oi;
         }
     }
     if (lane == 63) {
         wave_pairs[wave] = sc;
-        wave_chunks[wave] = sk;
+        wave_items[wave] = si;
     }
     __syncthreads();
-    int bc = 0, bk = 0, total = 0;
+    int bc = 0, bi = 0, total = 0;
     for (int w = 0; w < 16; ++w) {
         if (w < wave) {
             bc += wave_pairs[w];
-            bk += wave_chunks[w];
+            bi += wave_items[w];
         }
-        total += wave_chunks[w];
+        total += wave_items[w];
     }
-    first[threadIdx.x] = bc + sc - c;
-    chunk_first[threadIdx.x] = bk + sk - chunks;
-    for (int i = 0; i < chunks; ++i)
-        a.items[bk + sk - chunks + i] =
-            make_int4(threadIdx.x, bc + sc - c + i * a.rows, min(a.rows, c - i * a.rows), 0);
-    if (threadIdx.x == 0) *a.n_items = total;
-    count[threadIdx.x] = 0;
+    bc += sc - c;
+    bi += si - items;
+    for (int i = 0; i < items; ++i)
+        a.items[bi + i] = make_int4(me, bc + i * a.rows, min(a.rows, c - i * a.rows), 0);
+    if (me == 0) *a.n_items = total;
+    first[me] = bc;
+    count[me] = 0;
     __syncthreads();
-    for (int p = threadIdx.x; p < pairs; p += 1024) {
-        const int e = a.ids[p];
+    for (int p = me; p < pairs; p += 1024) {
+        int e;
+        float w;
+        pair(p, e, w);
         if (e < 0) continue;
         const int at = first[e] + atomicAdd(&count[e], 1);
         a.token[at] = p / a.top_k;
         a.slot[at] = p;
-        a.weight[at] = a.part[p];
+        a.weight[at] = w;
     }
+}
+
+// Up to 16 tokens: a wave each, and the groups in the same launch.
+constexpr int kRouteFew = 16;
+
+template <typename T, int R>
+__global__ void __launch_bounds__(1024) moe_route_kernel(MoeArgs a) {
+    __shared__ int id[kRouteFew * tecoops::kMoeMaxTopK];
+    __shared__ float weight[kRouteFew * tecoops::kMoeMaxTopK];
+    const int lane = threadIdx.x & 63, t = threadIdx.x >> 6;
+    if (t < a.tokens) {
+        int e;
+        float w;
+        choose<T, R>(a, t, lane, e, w);
+        if (lane < a.top_k) {
+            const int p = t * a.top_k + lane;
+            id[p] = e;
+            weight[p] = w;
+            store_choice(a, p, e, w);
+        }
+    }
+    __syncthreads();
+    group(a, [&](int p, int &e, float &w) {
+        e = id[p];
+        w = weight[p];
+    });
+}
+
+// More tokens: a wave each over the chip, then one workgroup for the groups.
+template <typename T, int R>
+__global__ void __launch_bounds__(256) moe_choose_kernel(MoeArgs a) {
+    const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (t >= a.tokens) return;
+    int e;
+    float w;
+    choose<T, R>(a, t, lane, e, w);
+    if (lane < a.top_k) {
+        const int p = t * a.top_k + lane;
+        store_choice(a, p, e, w);
+        a.part[p] = w;  // free until the second product
+    }
+}
+
+__global__ void __launch_bounds__(1024) moe_group_kernel(MoeArgs a) {
+    group(a, [&](int p, int &e, float &w) {
+        e = a.ids[p];
+        w = a.part[p];
+    });
+}
+
+template <typename T, int R>
+void launch_route(const MoeArgs &a, hipStream_t s) {
+    if (a.tokens <= kRouteFew) {
+        hipLaunchKernelGGL((moe_route_kernel<T, R>), dim3(1), dim3(1024), 0, s, a);
+        return;
+    }
+    hipLaunchKernelGGL((moe_choose_kernel<T, R>), dim3(tecoops::ceil_div(a.tokens, 4)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(moe_group_kernel, dim3(1), dim3(1024), 0, s, a);
 }
 
 // ------------------------------------------------------------------ products
@@ -256,22 +323,27 @@ template <typename T>
 __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a) {
     const int t = blockIdx.y;
     const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
-    if (n >= a.hidden) return;
     const bool whole = a.hidden % 4 == 0;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j = 0; j < a.top_k; ++j) {
-        const int p = t * a.top_k + j;
-        if (a.ids[p] < 0) break;  // the choices come first
-        const float *src = a.part + static_cast<long long>(p) * a.hidden + n;
-        if (whole) {
-            const f32x4_t v = *reinterpret_cast<const f32x4_t *>(src);
+    // a token's choices come first, so their number is that of its ids >= 0; the
+    // parts are then loaded without a wait between them
+    const int lane = threadIdx.x & 63;
+    const int id = lane < a.top_k ? a.ids[t * a.top_k + lane] : -1;
+    const int chosen = __builtin_popcountll(__ballot(id >= 0));
+    if (n >= a.hidden) return;
+    const float *src = a.part + static_cast<long long>(t) * a.top_k * a.hidden + n;
+    if (whole) {
+#pragma unroll 8
+        for (int j = 0; j < chosen; ++j) {
+            const f32x4_t v = *reinterpret_cast<const f32x4_t *>(src + static_cast<long long>(j) * a.hidden);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] += v[i];
-        } else {
+        }
+    } else {
+        for (int j = 0; j < chosen; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (n + i < a.hidden) s[i] += src[i];
-        }
+                if (n + i < a.hidden) s[i] += src[static_cast<long long>(j) * a.hidden + i];
     }
     uint16_t *dst = a.out + static_cast<long long>(t) * a.hidden + n;
     if (whole && tecoops::aligned(dst, 8)) {
@@ -324,7 +396,10 @@ bool launch_product(const MoeArgs &a, int items, bool copy, hipStream_t s) {
 
 template <typename T>
 tecoopsStatus_t run_slice(const MoeArgs &a, int items, bool copy, hipStream_t s) {
-    hipLaunchKernelGGL((moe_route_kernel<T>), dim3(1), dim3(1024), 0, s, a);
+    if (a.experts <= 64) launch_route<T, 1>(a, s);
+    else if (a.experts <= 128) launch_route<T, 2>(a, s);
+    else if (a.experts <= 256) launch_route<T, 4>(a, s);
+    else launch_route<T, tecoops::kMoeMaxExperts / 64>(a, s);
     TECO_CHECK_LAUNCH("moe_layer");
     if (!launch_product<T, false>(a, items, copy, s)) return TECOOPS_STATUS_INTERNAL_ERROR;
     TECO_CHECK_LAUNCH("moe_layer");

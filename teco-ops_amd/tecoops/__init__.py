@@ -380,6 +380,20 @@ def gemv_int8(weight, scales, x, out):
               _ptr(out), B, N, K)
 
 
+def _fast(name):
+    """The torch op `name` of libtecoops_torch.so, or None when it is not built.
+    Its C++ checks and launch take about a third of the host time of a ctypes call
+    behind Python ones (12.7 us for the latter, which a product of one row with a
+    [4096, 4096] weight does not hide).  What it refuses is put to the Python
+    checks and the C ABI again, for their errors."""
+    return None if ops is None else getattr(ops, name).default
+
+
+_linear, _moe_layer = _fast("linear"), _fast("moe_layer")
+_rotary_axes, _rotary_axes_cache = (_fast("rotary_embedding_axes"),
+                                    _fast("rotary_axes_reshape_and_cache"))
+
+
 def linear(x, weight, out, bias=None, residual=None, activation=None, gated=False):
     """out[m, n] = act(sum_k x[m, k] weight[n, k] + bias[n]) + residual[m, n].
 
@@ -389,6 +403,11 @@ def linear(x, weight, out, bias=None, residual=None, activation=None, gated=Fals
     the up rows, and out = act(gate) * up + residual.  residual may be out
     itself; out must not overlap another input.  float16 or bfloat16; sums and
     epilogue in float32."""
+    if _linear is not None:
+        try:
+            return _linear(x, weight, out, bias, residual, "none" if activation is None else activation, gated)
+        except (RuntimeError, TypeError, ValueError):
+            pass
     _check_cuda(x, weight, out, bias, residual)
     code, device = _dtype_code(x), x.device
     if weight.dim() != 2 or x.dim() != 2 or out.dim() != 2:
@@ -431,6 +450,13 @@ def moe_layer(x, w_in, w_out, router_logits, top_k, out, renormalize=True, activ
     rows before its up rows; w_out [E, H, I]; out [T, H], zero for a token all of
     whose logits are -inf.  topk_ids int32 and topk_weights float32 [T, top_k]
     are written when given, best first, -1 and 0 where there is none."""
+    if _moe_layer is not None:
+        try:
+            return _moe_layer(x, w_in, w_out, router_logits, top_k, out, renormalize,
+                              "none" if activation is None else activation, topk_ids,
+                              topk_weights)
+        except (RuntimeError, TypeError, ValueError):
+            pass
     _check_cuda(x, w_in, w_out, router_logits, out, topk_ids, topk_weights)
     code, device = _dtype_code(x), x.device
     if w_in.dim() != 3 or w_out.dim() != 3 or x.dim() != 2 or router_logits.dim() != 2:
@@ -534,6 +560,12 @@ def rotary_embedding_axes(positions, query, key, head_size, sections, cos_sin_ca
     own, base^(-j / n) for the j-th of an axis' n.  With a cos_sin_cache
     (float32 [positions, rot_dim]) a token with a position outside it is left as
     it is; without, angles are computed in 64 bits."""
+    if _rotary_axes is not None and (rot_dim is None or rot_dim > 0):
+        try:
+            return _rotary_axes(positions, query, key, head_size, sections, cos_sin_cache, is_neox,
+                                base, rot_dim or 0, layout)
+        except (RuntimeError, TypeError, ValueError):
+            pass
     device, before, sizes, table, code = _axes_args("rotary_embedding_axes", positions, query, key,
                                                     head_size, sections, cos_sin_cache, base,
                                                     rot_dim, layout)
@@ -551,6 +583,13 @@ def rotary_axes_reshape_and_cache(positions, query, key, value, slot_mapping, ke
     value stored into the paged caches [num_blocks, Hkv, block_size, head_size]
     at slot_mapping (int64; slots outside the cache are not stored); key is
     updated in place only when write_key."""
+    if _rotary_axes_cache is not None and (rot_dim is None or rot_dim > 0):
+        try:
+            return _rotary_axes_cache(positions, query, key, value, slot_mapping, key_cache,
+                                      value_cache, head_size, sections, cos_sin_cache, is_neox,
+                                      base, rot_dim or 0, layout, write_key)
+        except (RuntimeError, TypeError, ValueError):
+            pass
     name = "rotary_axes_reshape_and_cache"
     if key is None:
         raise ValueError(f"tecoops.{name}: key must be given")
