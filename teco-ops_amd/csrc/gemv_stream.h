@@ -5,7 +5,7 @@
 // W and x go from memory straight into LDS (global_load_lds_dwordx4, no
 // registers) in stages of 256 bytes per row of W, D stages in a ring, and the
 // MFMA operands are 16-byte LDS reads.  The 16-byte chunk c of row r sits at
-// chunk c ^ (r % 8) of its LDS row, so that the 16 rows a fragment read touches
+// chunk c ^ (r % 16) of its LDS row, so that the 16 rows a fragment read touches
 // fall on distinct banks; the copy's source address carries the permutation.
 // Chunks past K are copied from a zero constant, for W and x alike, so any K in
 // whole chunks works.
@@ -138,7 +138,7 @@ __device__ __forceinline__ void product(char *lds, int K, int unit, WRow &&w_row
     for (int m = 0; m < WC; ++m) {
         const int row = 4 * m + (lane >> 4);
         wsrc[m] = w_row(rs * WR + row);
-        wch[m] = kp * nst * 16 + ((lane & 15) ^ (row & 7));
+        wch[m] = kp * nst * 16 + ((lane & 15) ^ (row & 15));
     }
     // x copy q: rows (1024 / XROW) q + lane / XCH, slot lane % XCH; a K part's
     // copies are dealt to its RS waves (the last ones repeated to fill up)
@@ -149,7 +149,7 @@ __device__ __forceinline__ void product(char *lds, int K, int unit, WRow &&w_row
         const int q = (rs + m * RS) % S::XN;
         const int row = (1024 / S::XROW) * q + lane / XCH;
         xsrc[m] = x_row(row);
-        xch[m] = kp * nst * XCH + ((lane % XCH) ^ (row & 7));
+        xch[m] = kp * nst * XCH + ((lane % XCH) ^ (row & 15));
         xdst[m] = q * 1024;
     }
     f32x4_t acc[RT][CT];
@@ -189,7 +189,7 @@ __device__ __forceinline__ void product(char *lds, int K, int unit, WRow &&w_row
     // tile (in a tile of fewer rows the lanes past them repeat its rows, and
     // what they produce is never stored)
     const int wc = WR < 16 ? c & 7 : c, xc = XR < 16 ? c & (XR - 1) : c;
-    const int wsw = wc & 7, xsw = xc & 7;
+    const int wsw = wc, xsw = xc;
     const char *wl = wbuf + wc * 256, *xl = xbuf + xc * S::XROW;
 #pragma unroll
     for (int d = 0; d < D - 1; ++d)

@@ -2,52 +2,98 @@
 // the tests.
 #pragma once
 
+#include "gemv_batch.h"
+
 #include <cstddef>
 
 namespace tecoops {
 
-// Rows of x up to which gemv_batch.hip streams W past them.
+// Rows of x up to which gemv_batch.hip can stream W past them.
 constexpr int kLinearStreamRows = 64;
 // Longest row (of x or W, in elements): 256 rows of it stay within the 32-bit
 // offsets of a tile's copies.
 constexpr int kLinearMaxRow = 1 << 21;
 
+// The tiles built: rows of x and of W, stages in the ring, workgroups that fit a
+// CU, and the microseconds of a workgroup on 256 CUs: per stage of 64 of K at
+// full CUs, per stage at least (its copies' way), and besides its stages.  Fitted
+// to the times of all tiles and splits over 127 products (m 65..8000, n
+// 256..14336, k 256..14336, bf16), on which the size and split of the least
+// estimate take 1.3 % longer than the best in the mean, 21 % at most.  One tile
+// for all is worse by up to: 256 x 256 3.1 times, 64 x 64 2.4 times.
+struct LinearTile {
+    int bm, bn, depth, occupancy;
+    float stage, latency, besides;
+};
+constexpr LinearTile kLinearTiles[] = {
+    {256, 256, 2, 1, 0.097f, 1.405f, 8.4f},
+    {128, 256, 3, 1, 0.057f, 0.809f, 5.0f},
+    {128, 128, 3, 1, 0.033f, 0.507f, 4.0f},
+    {64, 128, 3, 2, 0.353f, 0.008f, 3.0f},
+    {64, 64, 3, 3, 0.225f, 0.267f, 3.1f},
+};
+constexpr int kLinearTileCount = sizeof(kLinearTiles) / sizeof(kLinearTiles[0]);
+// Tiles whose rows can also be loaded through registers (the larger ones have no
+// registers left to hold a stage).
+constexpr int kLinearFirstLoaded = 2;
+
 struct LinearPlan {
-    int bm, bn;            // rows of x and of W per tile
+    bool stream;           // gemv_batch.hip takes it
+    int tile;              // of kLinearTiles
     int tiles_m, tiles_n;
     int splits, stages;    // workgroups along K, stages of 64 in each
     size_t bytes;          // of workspace
 };
 
+// copy: rows in whole 16-byte words.  workspace: bytes there are for the sums of
+// a split K.
 inline LinearPlan linear_plan(int m, int n, int k, bool gated, bool copy, size_t workspace, int cus) {
-    const auto up = [](long long a, long long b) { return static_cast<int>((a + b - 1) / b); };
+    const auto up = [](long long a, long long b) { return (a + b - 1) / b; };
     const long long wrows = gated ? 2LL * n : n;
-    LinearPlan p{};
-    p.bm = p.bn = 256;
-    const auto cut = [&] {
-        p.tiles_m = up(m, p.bm);
-        p.tiles_n = gated ? up(n, p.bn / 2) : up(n, p.bn);
-    };
-    cut();
-    if (!copy || static_cast<long long>(p.tiles_m) * p.tiles_n < cus) {
-        p.bm = p.bn = 128;
-        cut();
-    }
-    p.splits = 1;
-    p.stages = up(k, 64);
-    const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
-    if (p.bm == 128 && tiles < cus) {
-        int want = static_cast<int>(2 * cus / tiles);  // two workgroups to a CU
-        if (want > p.stages / 8) want = p.stages / 8;  // 512 of K each or more
-        while (want > 1 && static_cast<size_t>(want) * m * wrows * 4 > workspace) --want;
-        if (want > 1) {
-            const int per = up(p.stages, want);
-            p.splits = up(p.stages, per);
-            p.stages = per;
+    const long long all = up(k, 64);
+    LinearPlan best{};
+    double least = 0;
+    for (int t = copy ? 0 : kLinearFirstLoaded; t < kLinearTileCount; ++t) {
+        const LinearTile &c = kLinearTiles[t];
+        const long long tm = up(m, c.bm), tn = up(n, gated ? c.bn / 2 : c.bn);
+        for (const int want : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16}) {
+            // a split of 256 of K or more, with workspace for its sums
+            const long long per = up(all, want), splits = up(all, per);
+            const size_t bytes = splits > 1 ? static_cast<size_t>(splits) * m * wrows * 4 : 0;
+            if (want > 1 && (splits != want || per < 4 || bytes > workspace)) continue;
+            const long long each = up(tm * tn * splits, cus);  // workgroups of a CU
+            const long long rounds = up(each, c.occupancy);
+            const double busy = each * per * static_cast<double>(c.stage);
+            const double wait = rounds * per * static_cast<double>(c.latency);
+            double time = 2.2 + rounds * static_cast<double>(c.besides) + (busy > wait ? busy : wait);
+            if (splits > 1) time += 1.4 + splits * 8.0 * m * wrows / 7e6;  // written and read again
+            if (least == 0 || time < least) {
+                least = time;
+                best.tile = t;
+                best.tiles_m = static_cast<int>(tm);
+                best.tiles_n = static_cast<int>(tn);
+                best.splits = static_cast<int>(splits);
+                best.stages = static_cast<int>(per);
+                best.bytes = bytes;
+            }
         }
     }
-    p.bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * m * wrows * 4 : 0;
-    return p;
+    if (copy && m <= kLinearStreamRows) {
+        // Streamed: HBM's rate for W, or a CU's for the rows of W and x it copies;
+        // in tiles W is read at 5.5 TB/s at best.  Few rows of W with a long K leave
+        // the copies of x, which every workgroup makes: [1024, 14336], 64 rows,
+        // 32.2 us streamed, 15.7 in tiles; [14336, 4096], 32 rows, 21.5 and 27.8.
+        // Over 96 products (m 8..64) the choice is 0.7 % slower than the better in
+        // the mean, 11 % at most.
+        const int rows = gemv_batch_rows(static_cast<int>(wrows), k, m, false, cus, gated ? 16 : 8);
+        const double hbm = 2.0 * wrows * k / 6.6e6;
+        const double lds = static_cast<double>(gemv_batch_bytes(wrows, rows, gemv_batch_staged(m), false, cus)) *
+                           k / 65e3;
+        const double tiles = 6.2 + 2.0 * wrows * k / 5.5e6;
+        best.stream = 3.2 + (hbm > lds ? hbm : lds) <= (least > tiles ? least : tiles);
+        if (best.stream) best.bytes = 0;
+    }
+    return best;
 }
 
 }  // namespace tecoops

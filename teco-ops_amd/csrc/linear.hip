@@ -4,19 +4,20 @@
 //   gated: W holds n gate rows, then n up rows;
 //   out[m, n] = T( act(gate[m, n]) * up[m, n] + residual[m, n] )
 //
-// Up to 64 rows of x stream W through gemv_batch.hip.  More rows run here, a
-// tile of out per workgroup on v_mfma_f32_32x32x16_{f16,bf16} with W as the
+// Up to 64 rows of x mostly stream W through gemv_batch.hip.  Other products run
+// here, a tile of out per workgroup on v_mfma_f32_32x32x16_{f16,bf16} with W as the
 // first operand, so that a lane ends with 4 neighbouring outputs of a row.
 //
-// A stage is 64 of K: 128 bytes of each row of W and x of the tile, copied
-// into LDS with no registers (global_load_lds_dwordx4), two stages deep.  The
-// 16-byte chunk c of row r sits at chunk c ^ (r % 8) of its LDS row, so that 8
-// rows read at one chunk fall on distinct banks; the copy's source address
-// carries the permutation.  A wave reads the second half of stage i while it
-// multiplies the first, and the first half of stage i + 1 while it multiplies
-// the second, so the matrix cores wait for LDS at neither; one barrier per
-// stage, in between, says that stage i + 1 has landed and that the slot of
-// stage i is free for stage i + 2.
+// A stage is 64 of K: 128 bytes of each row of W and x of the tile, copied into
+// LDS with no registers (global_load_lds_dwordx4), D stages in a ring.  The
+// 16-byte chunk c of row r sits at chunk c ^ (r / 2 % 8) of its LDS row, so that
+// 16 rows read at one chunk fall on distinct banks (two rows to the 256 bytes of
+// all banks); the copy's source address carries the permutation.  A wave reads the
+// second half of stage i while it multiplies the first, and the first half of
+// stage i + 1 while it multiplies the second, the reads and copies dealt between
+// its matrix instructions, so that the matrix cores wait for LDS at neither.  One
+// barrier per stage, in between, says that stage i + 1 has landed and that the
+// slot of stage i is free for stage i + D.
 //
 // Rows that are not in whole 16-byte words (odd K, views) cannot be copied that
 // way: the same kernel then loads chunks to registers, zero past K, and writes
@@ -30,6 +31,8 @@
 #include "device.h"
 #include "epilogue.h"
 #include "gemv_batch.h"
+
+#include <type_traits>
 
 namespace {
 
@@ -81,6 +84,7 @@ struct TileArgs {
     int wrows;
     long long x_stride;  // bytes
     int tiles_m, tiles_n, splits, stages_per_split;
+    int wide8;          // 8 outputs of a row in one 16-byte word
     Epilogue e;
 };
 
@@ -92,7 +96,127 @@ __device__ __forceinline__ int tile_output(const TileArgs &a, int n0, int r) {
     return min(a.e.gated ? (r >> 6) * 32 + (r & 31) : r, a.n - 1 - n0);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool COPY, bool SPLIT>
+// Four sums of row r of a wave's part of LDS, from its row 4 q of W on.
+__device__ __forceinline__ float4_t sums4(const char *mine, int r, int q) {
+    return *reinterpret_cast<const float4_t *>(mine + r * 256 + ((q ^ r) & 15) * 16);
+}
+
+// Rows of outputs n .. from 64 rows of W in a wave's part of LDS, finished and
+// stored.  A lane has 8 neighbouring outputs of a row (two rows of 4 sums, and
+// their up sums 32 rows of W on) and keeps them for all of its rows.
+template <typename T, int ACT, bool GATED>
+__device__ __forceinline__ void store_rows_as(const TileArgs &a, const char *mine, int lane, long long m,
+                                              int rows, int n) {
+    constexpr int PER = GATED ? 4 : 8;  // lanes of a row
+    const int q = 2 * (lane % PER);
+    n += 4 * q;
+    if (n >= a.n) return;
+    const int last = a.n - 1 - n;
+    float b[8], bu[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int c = n + (i < last ? i : last);
+        b[i] = a.e.bias != nullptr ? Cvt<T>::to(a.e.bias[c]) : 0.0f;
+        bu[i] = GATED && a.e.bias != nullptr ? Cvt<T>::to(a.e.bias[a.n + c]) : 0.0f;
+    }
+    const auto row = [&](int r, const uint4 &res) {
+        float v[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const float4_t s = sums4(mine, r, q + half);
+            float4_t u = s;
+            if (GATED) u = sums4(mine, r, q + half + 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int o = 4 * half + i;
+                v[o] = activate(s[i] + b[o], ACT);
+                if (GATED) v[o] *= u[i] + bu[o];
+            }
+        }
+        uint16_t *dst = a.out + (m + r) * a.e.out_stride + n;
+        if (a.wide8) {
+            const uint32_t w[4] = {res.x, res.y, res.z, res.w};
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (a.e.residual != nullptr) {
+                    v[2 * i] += lo<T>(w[i]);
+                    v[2 * i + 1] += hi<T>(w[i]);
+                }
+                o[i] = pack<T>(v[2 * i], v[2 * i + 1]);
+            }
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+            const uint16_t *rp = a.e.residual + (m + r) * a.e.res_stride + n;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i <= last) dst[i] = Cvt<T>::from(a.e.residual != nullptr ? v[i] + Cvt<T>::to(rp[i]) : v[i]);
+        }
+    };
+    // several rows at once, so that their LDS reads and residuals overlap
+    constexpr int STEP = 64 / PER, B = 4;
+    for (int r = lane / PER; r < rows; r += STEP * B) {
+        uint4 res[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if (a.wide8 && a.e.residual != nullptr && r + STEP * i < rows)
+                res[i] = *reinterpret_cast<const uint4 *>(a.e.residual + (m + r + STEP * i) * a.e.res_stride + n);
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if (r + STEP * i < rows) row(r + STEP * i, res[i]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_rows(const TileArgs &a, const char *mine, int lane, long long m, int rows,
+                                           int n) {
+#define TECO_STORE(ACT)                                                        \
+    case ACT:                                                                  \
+        if (a.e.gated) store_rows_as<T, ACT, true>(a, mine, lane, m, rows, n); \
+        else store_rows_as<T, ACT, false>(a, mine, lane, m, rows, n);          \
+        break
+    switch (a.e.act) {
+        TECO_STORE(TECOOPS_ACTIVATION_RELU);
+        TECO_STORE(TECOOPS_ACTIVATION_SILU);
+        TECO_STORE(TECOOPS_ACTIVATION_GELU);
+        TECO_STORE(TECOOPS_ACTIVATION_GELU_TANH);
+        default: TECO_STORE(TECOOPS_ACTIVATION_NONE);
+    }
+#undef TECO_STORE
+}
+
+// The same for a part of K: the sums themselves, at their rows of W.
+__device__ __forceinline__ void store_part(const TileArgs &a, int split, const char *mine, int lane, long long m,
+                                           int rows, int n0, int r0) {
+    const int q = lane & 15, r4 = r0 + 4 * q;  // 4 rows of W of the tile
+    const int o = a.e.gated ? n0 + (r4 >> 6) * 32 + (r4 & 31) : n0 + r4;
+    if (o >= a.n) return;
+    float *p = a.part + (split * static_cast<long long>(a.m) + m) * a.wrows + (a.e.gated && (r4 & 32) ? a.n : 0) + o;
+#pragma unroll 4
+    for (int r = lane >> 4; r < rows; r += 4) {
+        const float4_t s = sums4(mine, r, q);
+        float *dst = p + static_cast<long long>(r) * a.wrows;
+        if (a.n % 4 == 0) {
+            *reinterpret_cast<float4_t *>(dst) = s;
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (o + t < a.n) dst[t] = s[t];
+        }
+    }
+}
+
+// Waits until this wave has at most N younger copies in flight (no other vector
+// memory operation of its is younger than the copies it waits for) and its LDS
+// reads and writes are done, then for the other waves.
+template <int N>
+__device__ __forceinline__ void settle() {
+    static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+    __builtin_amdgcn_s_waitcnt(((N >> 4) << 14) | 0x0070 | (N & 15));
+    asm volatile("s_barrier" ::: "memory");
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int D, bool COPY, bool SPLIT>
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 linear_tile_kernel(TileArgs a) {
     constexpr int NW = WM * WN;
@@ -100,7 +224,8 @@ linear_tile_kernel(TileArgs a) {
     constexpr int STAGE = (BM + BN) * 128;
     constexpr int CW = BN / 8 / NW, CX = BM / 8 / NW;  // copies of a wave and stage
     static_assert(CW * 8 * NW == BN && CX * 8 * NW == BM, "whole copies");
-    static_assert(NT % 2 == 0 && NW * MT * 32 * 256 <= 2 * STAGE, "the epilogue's part of LDS");
+    static_assert(NT % 2 == 0 && NW * MT * 32 * 256 <= D * STAGE, "the epilogue's part of LDS");
+    static_assert(D >= 2, "a stage to read and one to copy to");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -132,7 +257,8 @@ linear_tile_kernel(TileArgs a) {
 
     // copy c of this wave: rows 8 (wave + NW c) + lane / 8, LDS chunk lane % 8
     const int lrow = lane >> 3;
-    const int cof = ((lane & 7) ^ lrow) * 16;  // byte in the stage's row
+    static_assert(NW % 2 == 0, "rows 8 (wave + NW c) swap chunks alike for every c");
+    const int cof = ((lane & 7) ^ ((8 * wave + lrow) >> 1 & 7)) * 16;  // byte in the stage's row
     const char *const gate = a.w + static_cast<long long>(n0) * kbytes;
     const char *const up = a.e.gated ? gate + static_cast<long long>(a.n) * kbytes : gate;
     const auto wbase = [&](int c) { return (wave + NW * c) & 4 ? up : gate; };
@@ -165,31 +291,30 @@ linear_tile_kernel(TileArgs a) {
     const auto fetch = [&](int i) {  // registers <- stage i
         if constexpr (!COPY) {
             const int b = (st0 + i) * 128 + cof;
+            if ((st0 + i) * 128 + 128 <= kbytes) {  // the whole stage within the rows
 #pragma unroll
-            for (int c = 0; c < CW; ++c) hold[c] = chunk(wbase(c) + woff[c], b);
+                for (int c = 0; c < CW; ++c) __builtin_memcpy(&hold[c], wbase(c) + woff[c] + b, 16);
 #pragma unroll
-            for (int c = 0; c < CX; ++c) hold[CW + c] = chunk(xbase + xoff[c], b);
+                for (int c = 0; c < CX; ++c) __builtin_memcpy(&hold[CW + c], xbase + xoff[c] + b, 16);
+            } else {
+#pragma unroll
+                for (int c = 0; c < CW; ++c) hold[c] = chunk(wbase(c) + woff[c], b);
+#pragma unroll
+                for (int c = 0; c < CX; ++c) hold[CW + c] = chunk(xbase + xoff[c], b);
+            }
         }
     };
-    // LDS <- stage i.  Copies past a row's end take its last chunk: stages past
-    // the last are never read, and the last masks what is past K.
-    const auto commit = [&](int i) {
-        char *dst = lds + (i & 1) * STAGE;
+    // LDS <- stage i, in CW + CX pieces.  Copies past a row's end take its last
+    // chunk: stages past the last are never read, and the last masks what is past
+    // K.
+    const auto commit = [&](int i, int slot, int c) {
+        char *dst = lds + slot + (c < CW ? 0 : BN * 128) + (wave + NW * (c < CW ? c : c - CW)) * 1024;
         if constexpr (COPY) {
             const uint32_t b = min((st0 + i) * 128 + cof, kbytes - 16);
-#pragma unroll
-            for (int c = 0; c < CW; ++c) dma16(wbase(c), woff[c] + b, dst + (wave + NW * c) * 1024);
-#pragma unroll
-            for (int c = 0; c < CX; ++c)
-                dma16(xbase, xoff[c] + b, dst + BN * 128 + (wave + NW * c) * 1024);
+            if (c < CW) dma16(wbase(c), woff[c < CW ? c : 0] + b, dst);
+            else dma16(xbase, xoff[c < CW ? 0 : c - CW] + b, dst);
         } else {
-#pragma unroll
-            for (int c = 0; c < CW; ++c)
-                *reinterpret_cast<u32x4_t *>(dst + (wave + NW * c) * 1024 + lane * 16) = hold[c];
-#pragma unroll
-            for (int c = 0; c < CX; ++c)
-                *reinterpret_cast<u32x4_t *>(dst + BN * 128 + (wave + NW * c) * 1024 + lane * 16) =
-                    hold[CW + c];
+            *reinterpret_cast<u32x4_t *>(dst + lane * 16) = hold[c];
         }
     };
 
@@ -208,26 +333,20 @@ linear_tile_kernel(TileArgs a) {
     };
     const char *wl = lds + (wn * NT * 32 + fr) * 128;
     const char *xl = lds + BN * 128 + (wm * MT * 32 + fr) * 128;
-    const auto read = [&](Frags &f, int slot, int half) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int c = ((4 * half + 2 * s + fg) ^ (fr & 7)) * 16 + slot * STAGE;
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-                f.w[s][i] = *reinterpret_cast<const u32x4_t *>(wl + i * 4096 + c);
-#pragma unroll
-            for (int j = 0; j < MT; ++j)
-                f.x[s][j] = *reinterpret_cast<const u32x4_t *>(xl + j * 4096 + c);
-        }
+    // Fragment number q of a half stage, in the order of their use: of each 16 of
+    // K the x fragments and then those of W.
+    constexpr int NF = 2 * (MT + NT);
+    const auto read = [&](Frags &f, int slot, int half, int q) {
+        const int s = q / (MT + NT), r = q % (MT + NT);
+        const int c = ((4 * half + 2 * s + fg) ^ (fr >> 1 & 7)) * 16 + slot;
+        if (r < MT) f.x[s][r] = *reinterpret_cast<const u32x4_t *>(xl + r * 4096 + c);
+        else f.w[s][r - MT] = *reinterpret_cast<const u32x4_t *>(wl + (r - MT) * 4096 + c);
     };
-    const auto multiply = [&](const Frags &f) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int j = 0; j < MT; ++j) acc[i][j] = Mma32<T>::run(f.w[s][i], f.x[s][j], acc[i][j]);
+    const auto multiply = [&](const Frags &f, int p) {  // product p of 2 NT MT
+        const int s = p / (NT * MT), i = p / MT % NT, j = p % MT;
+        acc[i][j] = Mma32<T>::run(f.w[s][i], f.x[s][j], acc[i][j]);
     };
+    constexpr int NP = 2 * NT * MT;
     // Both operands are cleared past K: the bits there are some other chunk's,
     // which may hold inf or NaN.
     const auto mask = [&](Frags &f, int half) {
@@ -247,78 +366,87 @@ linear_tile_kernel(TileArgs a) {
             }
         }
     };
-    // this wave's copies have landed and its LDS reads and writes are done
-    const auto settle = [&] {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __syncthreads();
+    // The products of one half stage with the reads of the next half (and, with
+    // `copies`, the copies of stage i into `to`) dealt between them in this order:
+    // left to itself the compiler moves the reads to right before their use.
+    const auto phase = [&](const Frags &f, Frags &next, int from, int half, auto copies, int i, int to) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            multiply(f, p);
+#pragma unroll
+            for (int q = p * NF / NP; q < (p + 1) * NF / NP; ++q) read(next, from, half, q);
+            if constexpr (decltype(copies)::value) {
+#pragma unroll
+                for (int c = p * (CW + CX) / NP; c < (p + 1) * (CW + CX) / NP; ++c) commit(i, to, c);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
-
-    fetch(0);
-    commit(0);
-    settle();
-    Frags f0, f1;
-    read(f0, 0, 0);
-    fetch(1);
-    commit(1);
-    for (int i = 0; i + 1 < nst; ++i) {
-        fetch(i + 2);
-        read(f1, i & 1, 1);
-        multiply(f0);
-        settle();
-        commit(i + 2);
-        read(f0, (i + 1) & 1, 0);
-        multiply(f1);
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+        if (!COPY && d == D - 1) break;
+        fetch(d);
+#pragma unroll
+        for (int c = 0; c < CW + CX; ++c) commit(d, d * STAGE, c);
     }
-    read(f1, (nst - 1) & 1, 1);
+    fetch(D - 1);
+    settle<COPY ? (D - 1) * (CW + CX) : 63>();
+    Frags f0, f1;
+#pragma unroll
+    for (int q = 0; q < NF; ++q) read(f0, 0, 0, q);
+    int slot = 0;  // of stage i
+    for (int i = 0; i + 1 < nst; ++i) {
+        const int from = slot + STAGE == D * STAGE ? 0 : slot + STAGE;
+        if constexpr (!COPY) {
+            // written a whole stage after it was loaded, to the slot of stage i - 1
+            const int to = slot == 0 ? (D - 1) * STAGE : slot - STAGE;
+#pragma unroll
+            for (int c = 0; c < CW + CX; ++c) commit(i + D - 1, to, c);
+            fetch(i + D);
+        }
+        phase(f0, f1, slot, 1, std::false_type{}, 0, 0);
+        settle<COPY ? (D - 2) * (CW + CX) : 63>();
+        phase(f1, f0, from, 0, std::integral_constant<bool, COPY>{}, i + D, slot);
+        slot = from;
+    }
+#pragma unroll
+    for (int q = 0; q < NF; ++q) read(f1, slot, 1, q);
     mask(f0, 0);
-    multiply(f0);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) multiply(f0, p);
     mask(f1, 1);
-    multiply(f1);
-    settle();  // the last copies land in LDS before the workgroup's end
+#pragma unroll
+    for (int p = 0; p < NP; ++p) multiply(f1, p);
+    settle<0>();  // the last copies have landed, and everyone has read
 
     // A wave's sums pass through its own part of LDS, 64 rows of W at a time, so
-    // that 16 lanes (8 when gated) end up with neighbouring outputs of one row
-    // and the stores fill whole lines.  Lane l of an accumulator holds row
-    // l % 32 of x and 4 rows of W, from 8 v + 4 (l / 32) on: a 16-byte chunk,
-    // at chunk q ^ (row % 16) of the row's 256 bytes.
+    // that 8 lanes (4 when gated) end up with neighbouring outputs of one row and
+    // the stores fill whole lines.  Lane l of an accumulator holds row l % 32 of x
+    // and 4 rows of W, from 8 v + 4 (l / 32) on: a 16-byte chunk, at chunk
+    // q ^ (row % 16) of the row's 256 bytes.
     char *mine = lds + wave * (MT * 32 * 256);
-    const int per = a.e.gated ? 8 : 16;  // lanes per row
-#pragma unroll
+#pragma unroll 1
     for (int h = 0; h < NT / 2; ++h) {
 #pragma unroll
-        for (int j = 0; j < MT; ++j)
+        for (int hh = 0; hh < NT / 2; ++hh) {
+            if (hh != h) continue;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < MT; ++j)
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const f32x16_t &t = acc[2 * h + i][j];
-                    *reinterpret_cast<float4_t *>(mine + (j * 32 + fr) * 256 +
-                                                  ((8 * i + 2 * v + fg) ^ (fr & 15)) * 16) =
-                        float4_t{t[4 * v], t[4 * v + 1], t[4 * v + 2], t[4 * v + 3]};
-                }
-        wave_lds_fence();
-        const int q = lane & (per - 1);
-        const int r0 = (wn * NT + 2 * h) * 32;  // the tile's rows of W from here on
-        const int n = n0 + (a.e.gated ? r0 / 2 : r0) + 4 * q;
-#pragma unroll 1
-        for (int r = lane / per; r < MT * 32; r += 64 / per) {
-            const long long m = m0 + wm * MT * 32 + r;
-            if (m >= a.m) break;
-            const float4_t s = *reinterpret_cast<const float4_t *>(mine + r * 256 + (q ^ (r & 15)) * 16);
-            const float4_t u = *reinterpret_cast<const float4_t *>(mine + r * 256 + (((q + 8) & 15) ^ (r & 15)) * 16);
-            const float sv[4] = {s[0], s[1], s[2], s[3]}, uv[4] = {u[0], u[1], u[2], u[3]};
-            if constexpr (SPLIT) {
-                float *p = a.part + (static_cast<long long>(split) * a.m + m) * a.wrows + n;
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    if (n + t < a.n) {
-                        p[t] = sv[t];
-                        if (a.e.gated) p[a.n + t] = uv[t];
+                    for (int v = 0; v < 4; ++v) {
+                        const f32x16_t &t = acc[2 * hh + i][j];
+                        *reinterpret_cast<float4_t *>(mine + (j * 32 + fr) * 256 +
+                                                      ((8 * i + 2 * v + fg) ^ (fr & 15)) * 16) =
+                            float4_t{t[4 * v], t[4 * v + 1], t[4 * v + 2], t[4 * v + 3]};
                     }
-            } else {
-                finish4<T>(a.e, a.out, m, n, a.n, sv, uv);
-            }
         }
+        wave_lds_fence();
+        const int r0 = (wn * NT + 2 * h) * 32;  // the tile's rows of W from here on
+        const int mw = m0 + wm * MT * 32, rows = min(MT * 32, a.m - mw);
+        if constexpr (SPLIT) store_part(a, split, mine, lane, mw, rows, n0, r0);
+        else store_rows<T>(a, mine, lane, mw, rows, n0 + (a.e.gated ? r0 / 2 : r0));
         wave_lds_fence();
     }
 }
@@ -332,38 +460,60 @@ __global__ void __launch_bounds__(256) linear_finish_kernel(TileArgs a) {
     if (m >= a.m) return;
     const int n = static_cast<int>(id - m * quads) * 4;
     float s[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
-    for (int p = 0; p < a.splits; ++p) {
-        const float *src = a.part + (static_cast<long long>(p) * a.m + m) * a.wrows + n;
+    const float *src = a.part + m * a.wrows + n;
+    const long long next = static_cast<long long>(a.m) * a.wrows;
+    if (a.n % 4 == 0) {
+#pragma unroll 4
+        for (int p = 0; p < a.splits; ++p, src += next) {
+            const float4_t g = *reinterpret_cast<const float4_t *>(src);
+            const float4_t h = *reinterpret_cast<const float4_t *>(src + (a.e.gated ? a.n : 0));
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (n + t >= a.n) break;
-            s[t] += src[t];
-            if (a.e.gated) u[t] += src[a.n + t];
+            for (int t = 0; t < 4; ++t) {
+                s[t] += g[t];
+                u[t] += h[t];
+            }
         }
+    } else {
+        for (int p = 0; p < a.splits; ++p, src += next)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (n + t < a.n) {
+                    s[t] += src[t];
+                    if (a.e.gated) u[t] += src[a.n + t];
+                }
     }
     finish4<T>(a.e, a.out, m, n, a.n, s, u);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool COPY, bool SPLIT>
+template <typename T, int BM, int BN, int WM, int WN, int D, bool COPY, bool SPLIT>
 bool launch_tile(const TileArgs &a, hipStream_t s) {
-    auto *kern = &linear_tile_kernel<T, BM, BN, WM, WN, COPY, SPLIT>;
-    constexpr size_t lds = 2 * (BM + BN) * 128;
+    auto *kern = &linear_tile_kernel<T, BM, BN, WM, WN, D, COPY, SPLIT>;
+    constexpr size_t lds = D * (BM + BN) * 128;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), lds)) return false;
     hipLaunchKernelGGL(kern, dim3(a.tiles_m * a.tiles_n * a.splits), dim3(WM * WN * 64), lds, s, a);
     return true;
 }
 
+template <typename T, int TILE, int WM, int WN>
+bool launch_as(const TileArgs &a, bool copy, hipStream_t s) {
+    constexpr tecoops::LinearTile t = tecoops::kLinearTiles[TILE];
+    if constexpr (TILE >= tecoops::kLinearFirstLoaded)
+        if (!copy)
+            return a.splits > 1 ? launch_tile<T, t.bm, t.bn, WM, WN, t.depth, false, true>(a, s)
+                                : launch_tile<T, t.bm, t.bn, WM, WN, t.depth, false, false>(a, s);
+    return a.splits > 1 ? launch_tile<T, t.bm, t.bn, WM, WN, t.depth, true, true>(a, s)
+                        : launch_tile<T, t.bm, t.bn, WM, WN, t.depth, true, false>(a, s);
+}
+
+// The waves of each tile along its rows of x and of W.
 template <typename T>
-tecoopsStatus_t run_tiles(TileArgs a, const tecoops::LinearPlan &p, bool copy, hipStream_t s) {
-    bool ok;
-    if (p.bm == 256)
-        ok = launch_tile<T, 256, 256, 4, 2, true, false>(a, s);
-    else if (copy)
-        ok = p.splits > 1 ? launch_tile<T, 128, 128, 2, 2, true, true>(a, s)
-                          : launch_tile<T, 128, 128, 2, 2, true, false>(a, s);
-    else
-        ok = p.splits > 1 ? launch_tile<T, 128, 128, 2, 2, false, true>(a, s)
-                          : launch_tile<T, 128, 128, 2, 2, false, false>(a, s);
+tecoopsStatus_t run_tiles(const TileArgs &a, const tecoops::LinearPlan &p, bool copy, hipStream_t s) {
+    static_assert(tecoops::kLinearTileCount == 5, "a launch for every tile");
+    const bool ok = p.tile == 0   ? launch_as<T, 0, 4, 2>(a, copy, s)
+                    : p.tile == 1 ? launch_as<T, 1, 2, 4>(a, copy, s)
+                    : p.tile == 2 ? launch_as<T, 2, 2, 2>(a, copy, s)
+                    : p.tile == 3 ? launch_as<T, 3, 2, 2>(a, copy, s)
+                                  : launch_as<T, 4, 2, 1>(a, copy, s);
     if (!ok) return TECOOPS_STATUS_INTERNAL_ERROR;
     TECO_CHECK_LAUNCH("linear");
     if (p.splits > 1) {
@@ -375,6 +525,10 @@ tecoopsStatus_t run_tiles(TileArgs a, const tecoops::LinearPlan &p, bool copy, h
     return TECOOPS_STATUS_SUCCESS;
 }
 
+// More workspace than this is not asked for: products that would split further
+// write and read sums for longer than the split saves.
+constexpr size_t kMostWorkspace = size_t{512} << 20;
+
 }  // namespace
 
 extern "C" tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, int gated,
@@ -382,9 +536,8 @@ extern "C" tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, in
     if (bytes == nullptr || m < 0 || n <= 0 || k <= 0) return TECOOPS_STATUS_BAD_PARAM;
     *bytes = 0;
     if (m == 0) return TECOOPS_STATUS_SUCCESS;
-    const bool copy = k % 8 == 0;
-    if (copy && m <= tecoops::kLinearStreamRows) return TECOOPS_STATUS_SUCCESS;
-    *bytes = tecoops::linear_plan(m, n, k, gated != 0, copy, ~size_t{0}, tecoops::device_cus()).bytes;
+    *bytes = tecoops::linear_plan(m, n, k, gated != 0, k % 8 == 0, kMostWorkspace, tecoops::device_cus())
+                 .bytes;
     return TECOOPS_STATUS_SUCCESS;
 }
 
@@ -419,12 +572,12 @@ extern "C" tecoopsStatus_t tecoopsLinear(tecoopsHandle_t handle, const void *x, 
     e.gated = gated != 0;
     e.wide = n % 4 == 0 && out_stride % 4 == 0 && tecoops::aligned(out, 8) &&
              (residual == nullptr || (residual_stride % 4 == 0 && tecoops::aligned(residual, 8)));
-    if (copy && m <= tecoops::kLinearStreamRows)
-        return tecoops::gemv_batch_epilogue(handle->stream, weight, x, x_stride, out, m, wrows, k,
-                                            dataType, e);
-    if (workspace == nullptr || !tecoops::aligned(workspace, 4)) workspace_bytes = 0;
+    if (workspace == nullptr || !tecoops::aligned(workspace, 16)) workspace_bytes = 0;
     const tecoops::LinearPlan p =
         tecoops::linear_plan(m, n, k, gated != 0, copy, workspace_bytes, tecoops::device_cus());
+    if (p.stream)
+        return tecoops::gemv_batch_epilogue(handle->stream, weight, x, x_stride, out, m, wrows, k,
+                                            dataType, e);
     if (static_cast<long long>(p.tiles_m) * p.tiles_n * p.splits > 0x7fffffffll)
         return TECOOPS_STATUS_NOT_SUPPORTED;
     TileArgs a{};
@@ -442,6 +595,8 @@ extern "C" tecoopsStatus_t tecoopsLinear(tecoopsHandle_t handle, const void *x, 
     a.splits = p.splits;
     a.stages_per_split = p.stages;
     a.e = e;
+    a.wide8 = n % 8 == 0 && out_stride % 8 == 0 && tecoops::aligned(out, 16) &&
+              (residual == nullptr || (residual_stride % 8 == 0 && tecoops::aligned(residual, 16)));
     return dataType == TECOOPS_DATA_HALF ? run_tiles<f16>(a, p, copy, handle->stream)
                                          : run_tiles<bf16>(a, p, copy, handle->stream);
 }

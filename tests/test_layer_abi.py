@@ -9,7 +9,8 @@ import pytest
 from tecoops import _lib
 
 BAD, NOT_INIT, NOT_SUP, OK = _lib.BAD_PARAM, _lib.NOT_INITIALIZED, _lib.NOT_SUPPORTED, _lib.SUCCESS
-CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "teco-ops_amd", "csrc")
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(REPO, "teco-ops_amd", "csrc")
 P = 0x1000  # never dereferenced: the checks come first
 
 
@@ -96,19 +97,23 @@ def plan(tmp_path_factory):
     (d / "plan.cpp").write_text("""#include "linear.h"
 extern "C" void plan(int m, int n, int k, int gated, int copy, unsigned long long ws, long long *o) {
     const auto p = tecoops::linear_plan(m, n, k, gated != 0, copy != 0, ws, 256);
-    o[0] = p.bm; o[1] = p.bn; o[2] = p.tiles_m; o[3] = p.tiles_n;
-    o[4] = p.splits; o[5] = p.stages; o[6] = static_cast<long long>(p.bytes);
+    o[0] = tecoops::kLinearTiles[p.tile].bm; o[1] = tecoops::kLinearTiles[p.tile].bn;
+    o[2] = p.tiles_m; o[3] = p.tiles_n; o[4] = p.splits; o[5] = p.stages;
+    o[6] = static_cast<long long>(p.bytes); o[7] = p.stream; o[8] = p.tile;
 }
+extern "C" int first_loaded() { return tecoops::kLinearFirstLoaded; }
 """)
-    subprocess.run(["g++", "-std=c++17", "-fPIC", "-shared", "-I", CSRC, str(d / "plan.cpp"), "-o",
-                    str(d / "plan.so")], check=True)
+    subprocess.run(["g++", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-I", CSRC,
+                    "-I", os.path.join(REPO, "include"), "-I", "/opt/rocm/include",
+                    str(d / "plan.cpp"), "-o", str(d / "plan.so")], check=True)
     lib = ctypes.CDLL(str(d / "plan.so"))
     lib.plan.argtypes = [ctypes.c_int] * 5 + [ctypes.c_ulonglong, ctypes.c_void_p]
 
     def run(m, n, k, gated=0, copy=1, ws=(1 << 63)):
-        o = (ctypes.c_longlong * 7)()
+        o = (ctypes.c_longlong * 9)()
         lib.plan(m, n, k, gated, copy, ws, o)
         return list(o)
+    run.first_loaded = lib.first_loaded()
     return run
 
 
@@ -117,18 +122,30 @@ extern "C" void plan(int m, int n, int k, int gated, int copy, unsigned long lon
 def test_plan_covers_the_product(plan, gated, copy):
     """Tiles cover the rows and outputs, splits cover K with none empty, and the
     workspace holds every split's sums of every row of W."""
-    for m in (1, 64, 65, 127, 128, 129, 333, 1000, 8192, 70000):
+    for m in (1, 8, 33, 64, 65, 127, 128, 129, 333, 1000, 8192, 70000):
         for n in (1, 63, 64, 65, 300, 4096, 14336, 100000):
             for k in (1, 8, 64, 65, 512, 588, 4096, 14336, 100000):
                 for ws in (0, 1 << 20, 1 << 63):
-                    bm, bn, tm, tn, splits, stages, need = plan(m, n, k, gated, copy, ws)
+                    bm, bn, tm, tn, splits, stages, need, stream, tile = plan(m, n, k, gated, copy, ws)
                     out = bn // 2 if gated else bn
                     assert (tm - 1) * bm < m <= tm * bm and (tn - 1) * out < n <= tn * out
                     total = -(-k // 64)
                     assert splits >= 1 and (splits - 1) * stages < total <= splits * stages
+                    if stream:
+                        assert copy and m <= 64 and need == 0
+                        continue
                     assert need == (splits * m * n * (2 if gated else 1) * 4 if splits > 1 else 0)
                     assert need <= ws
-                    assert copy or bm == 128
+                    assert copy or tile >= plan.first_loaded
+
+
+def test_plan_by_size(plan):
+    """Wide products of few rows stream W, few rows of W with a long K do not;
+    large products take the largest tile, unsplit."""
+    assert plan(1, 4096, 4096)[7] and plan(32, 14336, 4096)[7] and plan(24, 14336, 4096, gated=1)[7]
+    assert not plan(64, 1024, 14336)[7] and plan(64, 1024, 14336)[4] > 1
+    assert plan(8192, 14336, 4096, gated=1)[:2] == [256, 256] and plan(8192, 14336, 4096)[4] == 1
+    assert plan(512, 512, 512)[:2] == [64, 64]
 
 
 def test_moe_refusals(handle):
