@@ -28,6 +28,15 @@ inline bool epilogue_act_ok(int act) {
 
 namespace dev {
 
+// Two results rounded to T (to nearest even; one instruction on gfx950).
+template <typename T>
+__device__ __forceinline__ uint32_t round2(float a, float b) {
+    if constexpr (__is_same(T, f16))
+        return __builtin_bit_cast(uint32_t, half2_t{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+    else
+        return __builtin_bit_cast(uint32_t, bf162_t{static_cast<__bf16>(a), static_cast<__bf16>(b)});
+}
+
 // The exponentials are of the hardware's base-2 one: a relative error of about
 // |v| 2^-24, far below half a step of the 16-bit result.  The sigmoid forms
 // overflow to inf in the denominator for very negative v and give -0, their
@@ -70,12 +79,15 @@ __device__ __forceinline__ void finish4(const Epilogue &e, uint16_t *out, long l
             v[2] += lo<T>(r.y);
             v[3] += hi<T>(r.y);
         }
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]));
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(round2<T>(v[0], v[1]), round2<T>(v[2], v[3]));
         return;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (i <= last) dst[i] = Cvt<T>::from(e.residual != nullptr ? v[i] + Cvt<T>::to(res[i]) : v[i]);
+        if (i <= last) {
+            const float f = e.residual != nullptr ? v[i] + Cvt<T>::to(res[i]) : v[i];
+            dst[i] = static_cast<uint16_t>(round2<T>(f, f));
+        }
 }
 
 }  // namespace dev

@@ -38,7 +38,7 @@ constexpr int kLinearTileCount = sizeof(kLinearTiles) / sizeof(kLinearTiles[0]);
 constexpr int kLinearFirstLoaded = 2;
 
 struct LinearPlan {
-    bool stream;           // gemv_batch.hip takes it
+    bool stream;           // gemv_batch.hip takes it (the rest is 0)
     int tile;              // of kLinearTiles
     int tiles_m, tiles_n;
     int splits, stages;    // workgroups along K, stages of 64 in each
@@ -48,50 +48,60 @@ struct LinearPlan {
 // copy: rows in whole 16-byte words.  workspace: bytes there are for the sums of
 // a split K.
 inline LinearPlan linear_plan(int m, int n, int k, bool gated, bool copy, size_t workspace, int cus) {
-    const auto up = [](long long a, long long b) { return (a + b - 1) / b; };
+    const auto up = [](int a, int b) { return (a - 1) / b + 1; };
     const long long wrows = gated ? 2LL * n : n;
-    const long long all = up(k, 64);
     LinearPlan best{};
-    double least = 0;
-    for (int t = copy ? 0 : kLinearFirstLoaded; t < kLinearTileCount; ++t) {
-        const LinearTile &c = kLinearTiles[t];
-        const long long tm = up(m, c.bm), tn = up(n, gated ? c.bn / 2 : c.bn);
-        for (const int want : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16}) {
-            // a split of 256 of K or more, with workspace for its sums
-            const long long per = up(all, want), splits = up(all, per);
-            const size_t bytes = splits > 1 ? static_cast<size_t>(splits) * m * wrows * 4 : 0;
-            if (want > 1 && (splits != want || per < 4 || bytes > workspace)) continue;
-            const long long each = up(tm * tn * splits, cus);  // workgroups of a CU
-            const long long rounds = up(each, c.occupancy);
-            const double busy = each * per * static_cast<double>(c.stage);
-            const double wait = rounds * per * static_cast<double>(c.latency);
-            double time = 2.2 + rounds * static_cast<double>(c.besides) + (busy > wait ? busy : wait);
-            if (splits > 1) time += 1.4 + splits * 8.0 * m * wrows / 7e6;  // written and read again
-            if (least == 0 || time < least) {
-                least = time;
-                best.tile = t;
-                best.tiles_m = static_cast<int>(tm);
-                best.tiles_n = static_cast<int>(tn);
-                best.splits = static_cast<int>(splits);
-                best.stages = static_cast<int>(per);
-                best.bytes = bytes;
-            }
-        }
-    }
+    // Streamed: HBM's rate for W, or a CU's for the rows of W and x it copies; in
+    // tiles W is read at 5.5 TB/s at best.  Few rows of W with a long K leave the
+    // copies of x, which every workgroup makes: [1024, 14336], 64 rows, 32.2 us
+    // streamed, 15.7 in tiles; [14336, 4096], 32 rows, 21.5 and 27.8.  Over 96
+    // products (m 8..64) the choice is 0.7 % slower than the better in the mean,
+    // 11 % at most.
+    double streamed = -1;
     if (copy && m <= kLinearStreamRows) {
-        // Streamed: HBM's rate for W, or a CU's for the rows of W and x it copies;
-        // in tiles W is read at 5.5 TB/s at best.  Few rows of W with a long K leave
-        // the copies of x, which every workgroup makes: [1024, 14336], 64 rows,
-        // 32.2 us streamed, 15.7 in tiles; [14336, 4096], 32 rows, 21.5 and 27.8.
-        // Over 96 products (m 8..64) the choice is 0.7 % slower than the better in
-        // the mean, 11 % at most.
         const int rows = gemv_batch_rows(static_cast<int>(wrows), k, m, false, cus, gated ? 16 : 8);
         const double hbm = 2.0 * wrows * k / 6.6e6;
         const double lds = static_cast<double>(gemv_batch_bytes(wrows, rows, gemv_batch_staged(m), false, cus)) *
                            k / 65e3;
-        const double tiles = 6.2 + 2.0 * wrows * k / 5.5e6;
-        best.stream = 3.2 + (hbm > lds ? hbm : lds) <= (least > tiles ? least : tiles);
-        if (best.stream) best.bytes = 0;
+        streamed = 3.2 + (hbm > lds ? hbm : lds);
+        best.stream = streamed <= 6.2 + 2.0 * wrows * k / 5.5e6;
+        if (best.stream) return best;
+    }
+    const int all = up(k, 64);
+    double least = 0;
+    for (int t = copy ? 0 : kLinearFirstLoaded; t < kLinearTileCount; ++t) {
+        const LinearTile &c = kLinearTiles[t];
+        const int tm = up(m, c.bm), tn = up(n, gated ? c.bn / 2 : c.bn);
+        const long long tiles = static_cast<long long>(tm) * tn;
+        for (const int want : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16}) {
+            // a split of 256 of K or more, where tiles alone do not fill the CUs
+            // and with workspace for its sums
+            if (want > 1 && (tiles * (want - 1) >= static_cast<long long>(cus) * c.occupancy || all < 4 * want)) break;
+            const int per = up(all, want), splits = up(all, per);
+            const size_t bytes = splits > 1 ? static_cast<size_t>(splits) * m * wrows * 4 : 0;
+            if (bytes > workspace) break;
+            if (splits != want) continue;
+            const long long wgs = tiles * splits;
+            const int each = wgs > 0x7fffffff ? 0x7fffffff : up(static_cast<int>(wgs), cus);  // of a CU
+            const int rounds = up(each, c.occupancy);
+            const double busy = static_cast<double>(each) * per * c.stage;
+            const double wait = static_cast<double>(rounds) * per * c.latency;
+            double time = 2.2 + static_cast<double>(rounds) * c.besides + (busy > wait ? busy : wait);
+            if (splits > 1) time += 1.4 + splits * 8.0 * m * wrows / 7e6;  // written and read again
+            if (least == 0 || time < least) {
+                least = time;
+                best.tile = t;
+                best.tiles_m = tm;
+                best.tiles_n = tn;
+                best.splits = splits;
+                best.stages = per;
+                best.bytes = bytes;
+            }
+        }
+    }
+    if (streamed >= 0 && streamed <= least) {
+        best.stream = true;
+        best.bytes = 0;
     }
     return best;
 }

@@ -101,6 +101,11 @@ __device__ __forceinline__ float4_t sums4(const char *mine, int r, int q) {
     return *reinterpret_cast<const float4_t *>(mine + r * 256 + ((q ^ r) & 15) * 16);
 }
 
+// The sum of row r and its row c of W.
+__device__ __forceinline__ float sum1(const char *mine, int r, int c) {
+    return *reinterpret_cast<const float *>(mine + r * 256 + ((c / 4 ^ r) & 15) * 16 + c % 4 * 4);
+}
+
 // Rows of outputs n .. from 64 rows of W in a wave's part of LDS, finished and
 // stored.  A lane has 8 neighbouring outputs of a row (two rows of 4 sums, and
 // their up sums 32 rows of W on) and keeps them for all of its rows.
@@ -110,14 +115,12 @@ __device__ __forceinline__ void store_rows_as(const TileArgs &a, const char *min
     constexpr int PER = GATED ? 4 : 8;  // lanes of a row
     const int q = 2 * (lane % PER);
     n += 4 * q;
-    if (n >= a.n) return;
-    const int last = a.n - 1 - n;
+    if (n >= a.n) return;  // n is a multiple of 8, and so is a.n
     float b[8], bu[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int c = n + (i < last ? i : last);
-        b[i] = a.e.bias != nullptr ? Cvt<T>::to(a.e.bias[c]) : 0.0f;
-        bu[i] = GATED && a.e.bias != nullptr ? Cvt<T>::to(a.e.bias[a.n + c]) : 0.0f;
+        b[i] = a.e.bias != nullptr ? Cvt<T>::to(a.e.bias[n + i]) : 0.0f;
+        bu[i] = GATED && a.e.bias != nullptr ? Cvt<T>::to(a.e.bias[a.n + n + i]) : 0.0f;
     }
     const auto row = [&](int r, const uint4 &res) {
         float v[8];
@@ -133,33 +136,25 @@ __device__ __forceinline__ void store_rows_as(const TileArgs &a, const char *min
                 if (GATED) v[o] *= u[i] + bu[o];
             }
         }
-        uint16_t *dst = a.out + (m + r) * a.e.out_stride + n;
-        if (a.wide8) {
-            const uint32_t w[4] = {res.x, res.y, res.z, res.w};
-            uint32_t o[4];
+        const uint32_t w[4] = {res.x, res.y, res.z, res.w};
+        uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (a.e.residual != nullptr) {
-                    v[2 * i] += lo<T>(w[i]);
-                    v[2 * i + 1] += hi<T>(w[i]);
-                }
-                o[i] = pack<T>(v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) {
+            if (a.e.residual != nullptr) {
+                v[2 * i] += lo<T>(w[i]);
+                v[2 * i + 1] += hi<T>(w[i]);
             }
-            *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-        } else {
-            const uint16_t *rp = a.e.residual + (m + r) * a.e.res_stride + n;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i <= last) dst[i] = Cvt<T>::from(a.e.residual != nullptr ? v[i] + Cvt<T>::to(rp[i]) : v[i]);
+            o[i] = round2<T>(v[2 * i], v[2 * i + 1]);
         }
+        *reinterpret_cast<uint4 *>(a.out + (m + r) * a.e.out_stride + n) = make_uint4(o[0], o[1], o[2], o[3]);
     };
     // several rows at once, so that their LDS reads and residuals overlap
-    constexpr int STEP = 64 / PER, B = 4;
+    constexpr int STEP = 64 / PER, B = 2;
     for (int r = lane / PER; r < rows; r += STEP * B) {
         uint4 res[B];
 #pragma unroll
         for (int i = 0; i < B; ++i)
-            if (a.wide8 && a.e.residual != nullptr && r + STEP * i < rows)
+            if (a.e.residual != nullptr && r + STEP * i < rows)
                 res[i] = *reinterpret_cast<const uint4 *>(a.e.residual + (m + r + STEP * i) * a.e.res_stride + n);
 #pragma unroll
         for (int i = 0; i < B; ++i)
@@ -167,9 +162,33 @@ __device__ __forceinline__ void store_rows_as(const TileArgs &a, const char *min
     }
 }
 
+// Rows that are not in whole 16-byte words: a lane per output, so that a store
+// still covers 128 neighbouring bytes (64 when gated).  [14337, 588] times 3000
+// rows took 236 us with 8 outputs to a lane stored one by one.
+template <typename T>
+__device__ __forceinline__ void store_rows_narrow(const TileArgs &a, const char *mine, int lane, long long m,
+                                                  int rows, int n) {
+    const int per = a.e.gated ? 32 : 64;
+    const int c = lane & (per - 1);
+    n += c;
+    if (n >= a.n) return;
+    const float b = a.e.bias != nullptr ? Cvt<T>::to(a.e.bias[n]) : 0.0f;
+    const float bu = a.e.gated && a.e.bias != nullptr ? Cvt<T>::to(a.e.bias[a.n + n]) : 0.0f;
+    const uint16_t *res = a.e.residual + m * a.e.res_stride + n;
+    uint16_t *dst = a.out + m * a.e.out_stride + n;
+#pragma unroll 2
+    for (int r = lane / per; r < rows; r += 64 / per) {
+        float v = activate(sum1(mine, r, c) + b, a.e.act);
+        if (a.e.gated) v *= sum1(mine, r, c + 32) + bu;
+        if (a.e.residual != nullptr) v += Cvt<T>::to(res[r * a.e.res_stride]);
+        dst[r * a.e.out_stride] = static_cast<uint16_t>(round2<T>(v, v));
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ void store_rows(const TileArgs &a, const char *mine, int lane, long long m, int rows,
                                            int n) {
+    if (!a.wide8) return store_rows_narrow<T>(a, mine, lane, m, rows, n);
 #define TECO_STORE(ACT)                                                        \
     case ACT:                                                                  \
         if (a.e.gated) store_rows_as<T, ACT, true>(a, mine, lane, m, rows, n); \
@@ -273,48 +292,49 @@ linear_tile_kernel(TileArgs a) {
         xoff[c] = static_cast<uint32_t>(min(8 * (wave + NW * c) + lrow, a.m - 1 - m0)) *
                   static_cast<uint32_t>(a.x_stride);
 
-    u32x4_t hold[COPY ? 1 : CW + CX];
-    // chunk of a row at byte b of its kbytes (any alignment of 2), zero past K
+    struct Hold {
+        u32x4_t c[COPY ? 1 : CW + CX];
+    };
+    // The chunk at byte b of a row, zero past its kbytes: 2 bytes at a time, none
+    // past the end, all loaded before the first is used.
     const auto chunk = [&](const char *row, int b) {
-        u32x4_t v = {0u, 0u, 0u, 0u};
-        if (b + 16 <= kbytes) {
-            __builtin_memcpy(&v, row + b, 16);
-        } else {
+        uint32_t h[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (b + 2 * i < kbytes)
-                    v[i >> 1] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(row + b + 2 * i))
-                                 << (16 * (i & 1));
-        }
+        for (int i = 0; i < 8; ++i)
+            h[i] = *reinterpret_cast<const uint16_t *>(row + min(b + 2 * i, kbytes - 2));
+        u32x4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = (b + 4 * i < kbytes ? h[2 * i] : 0u) | (b + 4 * i + 2 < kbytes ? h[2 * i + 1] << 16 : 0u);
         return v;
     };
-    const auto fetch = [&](int i) {  // registers <- stage i
+    const auto fetch = [&](Hold &hold, int i) {  // registers <- stage i
         if constexpr (!COPY) {
             const int b = (st0 + i) * 128 + cof;
             if ((st0 + i) * 128 + 128 <= kbytes) {  // the whole stage within the rows
 #pragma unroll
-                for (int c = 0; c < CW; ++c) __builtin_memcpy(&hold[c], wbase(c) + woff[c] + b, 16);
+                for (int c = 0; c < CW; ++c) __builtin_memcpy(&hold.c[c], wbase(c) + woff[c] + b, 16);
 #pragma unroll
-                for (int c = 0; c < CX; ++c) __builtin_memcpy(&hold[CW + c], xbase + xoff[c] + b, 16);
-            } else {
+                for (int c = 0; c < CX; ++c) __builtin_memcpy(&hold.c[CW + c], xbase + xoff[c] + b, 16);
+            } else if ((st0 + i) * 128 < kbytes) {  // stages past the last are never read
 #pragma unroll
-                for (int c = 0; c < CW; ++c) hold[c] = chunk(wbase(c) + woff[c], b);
+                for (int c = 0; c < CW; ++c) hold.c[c] = chunk(wbase(c) + woff[c], b);
 #pragma unroll
-                for (int c = 0; c < CX; ++c) hold[CW + c] = chunk(xbase + xoff[c], b);
+                for (int c = 0; c < CX; ++c) hold.c[CW + c] = chunk(xbase + xoff[c], b);
             }
         }
     };
     // LDS <- stage i, in CW + CX pieces.  Copies past a row's end take its last
     // chunk: stages past the last are never read, and the last masks what is past
     // K.
-    const auto commit = [&](int i, int slot, int c) {
+    const auto commit = [&](const Hold &hold, int i, int slot, int c) {
         char *dst = lds + slot + (c < CW ? 0 : BN * 128) + (wave + NW * (c < CW ? c : c - CW)) * 1024;
         if constexpr (COPY) {
             const uint32_t b = min((st0 + i) * 128 + cof, kbytes - 16);
             if (c < CW) dma16(wbase(c), woff[c < CW ? c : 0] + b, dst);
             else dma16(xbase, xoff[c < CW ? 0 : c - CW] + b, dst);
         } else {
-            *reinterpret_cast<u32x4_t *>(dst + lane * 16) = hold[c];
+            *reinterpret_cast<u32x4_t *>(dst + lane * 16) = hold.c[c];
         }
     };
 
@@ -377,38 +397,47 @@ linear_tile_kernel(TileArgs a) {
             for (int q = p * NF / NP; q < (p + 1) * NF / NP; ++q) read(next, from, half, q);
             if constexpr (decltype(copies)::value) {
 #pragma unroll
-                for (int c = p * (CW + CX) / NP; c < (p + 1) * (CW + CX) / NP; ++c) commit(i, to, c);
+                for (int c = p * (CW + CX) / NP; c < (p + 1) * (CW + CX) / NP; ++c) commit(Hold{}, i, to, c);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    // Rows loaded through registers: stages 0 .. D - 2 go to LDS, D - 1 and D wait
+    // in registers, all loaded at once.
+    Hold hold[COPY ? 1 : D + 1];
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-        if (!COPY && d == D - 1) break;
-        fetch(d);
+    for (int d = 0; d < (COPY ? 0 : D + 1); ++d) fetch(hold[d], d);
 #pragma unroll
-        for (int c = 0; c < CW + CX; ++c) commit(d, d * STAGE, c);
-    }
-    fetch(D - 1);
+    for (int d = 0; d < (COPY ? D : D - 1); ++d)
+#pragma unroll
+        for (int c = 0; c < CW + CX; ++c) commit(hold[COPY ? 0 : d], d, d * STAGE, c);
     settle<COPY ? (D - 1) * (CW + CX) : 63>();
     Frags f0, f1;
 #pragma unroll
     for (int q = 0; q < NF; ++q) read(f0, 0, 0, q);
     int slot = 0;  // of stage i
-    for (int i = 0; i + 1 < nst; ++i) {
+    const auto stage = [&](int i, Hold &h) {
         const int from = slot + STAGE == D * STAGE ? 0 : slot + STAGE;
         if constexpr (!COPY) {
-            // written a whole stage after it was loaded, to the slot of stage i - 1
+            // written two stages after it was loaded, to the slot of stage i - 1
             const int to = slot == 0 ? (D - 1) * STAGE : slot - STAGE;
 #pragma unroll
-            for (int c = 0; c < CW + CX; ++c) commit(i + D - 1, to, c);
-            fetch(i + D);
+            for (int c = 0; c < CW + CX; ++c) commit(h, i + D - 1, to, c);
+            fetch(h, i + D + 1);
         }
         phase(f0, f1, slot, 1, std::false_type{}, 0, 0);
         settle<COPY ? (D - 2) * (CW + CX) : 63>();
         phase(f1, f0, from, 0, std::integral_constant<bool, COPY>{}, i + D, slot);
         slot = from;
+    };
+    int i = 0;
+    if constexpr (!COPY) {
+        for (; i + 2 < nst; i += 2) {
+            stage(i, hold[D - 1]);
+            stage(i + 1, hold[D]);
+        }
     }
+    for (; i + 1 < nst; ++i) stage(i, hold[COPY ? 0 : D - 1]);
 #pragma unroll
     for (int q = 0; q < NF; ++q) read(f1, slot, 1, q);
     mask(f0, 0);
