@@ -10,6 +10,7 @@ namespace tecoops {
 
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeMaxTopK = 32;
+constexpr int kMoeFew = 8;       // tokens whose second product sums over the experts
 constexpr int kMoeSlice = 512;  // tokens routed together; more run slice by slice
 
 // Rows of x staged for an item: the tokens of an expert go through in chunks of
@@ -28,7 +29,7 @@ struct MoeSpace {
     int pairs, items;      // most (token, expert) pairs and items of a slice
     int rows;              // of x per item
     long long h_stride;    // elements between the rows of h
-    size_t items_at, ids_at, token_at, slot_at, weight_at, h_at, part_at;  // bytes
+    size_t items_at, ids_at, token_at, slot_at, weight_at, cols_at, h_at, part_at;  // bytes
     size_t bytes;
 };
 
@@ -51,19 +52,37 @@ inline MoeSpace moe_space(int tokens, int hidden, int inter, int experts, int to
     s.token_at = take(4 * static_cast<size_t>(s.pairs));
     s.slot_at = take(4 * static_cast<size_t>(s.pairs));
     s.weight_at = take(4 * static_cast<size_t>(s.pairs));
+    s.cols_at = take(slice <= kMoeFew || tokens % kMoeSlice != 0
+                         ? 8 * static_cast<size_t>(s.items) * kMoeFew : 0);
     s.h_at = take(2 * static_cast<size_t>(s.pairs) * s.h_stride);
     s.part_at = take(4 * static_cast<size_t>(s.pairs) * hidden);
     s.bytes = at;
     return s;
 }
 
+// Experts that `tokens` random choices of top_k reach, expected.
+inline double moe_reached(int tokens, int top_k, int experts) {
+    double missed = 1.0;
+    for (int t = 0; t < tokens && missed > 1e-3; ++t) missed *= 1.0 - static_cast<double>(top_k) / experts;
+    return experts * (1.0 - missed);
+}
+
+// Whether few tokens sum over the experts within the second product.  It spares
+// the parts, their sum and a launch, about 5 us, but has a workgroup per 8 (or
+// 16) rows of the result only, which leave part of the chip's bandwidth when they
+// are few (6 tokens, 6 of 60 experts of [640, 9920]: 307 us, 223 in parts; 1 token,
+// 3 of 4 of [1024, 896]: 16.5 and 21 us).
+inline bool moe_out_few(int tokens, int hidden, int inter, int experts, int top_k, int cus) {
+    if (tokens > kMoeFew) return false;
+    const double bytes = 2.0 * hidden * inter * moe_reached(tokens, top_k, experts);
+    const double share = (hidden + 7) / 8 / (0.875 * cus);
+    return bytes / (5.8e6 * (share < 1 ? share : 1)) <= bytes / 5.5e6 + 5;
+}
+
 // Rows of W per workgroup: the size whose busiest CU copies the fewest bytes of
 // W and x, with as many items as tokens spread evenly would make.
 inline int moe_wrows(int wrows, int tokens, int top_k, int experts, int rows, int cus) {
-    double items = experts;  // those that `tokens` random choices of top_k reach
-    double missed = 1.0;
-    for (int t = 0; t < tokens && missed > 1e-3; ++t) missed *= 1.0 - static_cast<double>(top_k) / experts;
-    items *= 1.0 - missed;
+    const double items = moe_reached(tokens, top_k, experts);
     int best = 0;
     double least = 0;
     for (int r : {128, 64, 32, 16}) {

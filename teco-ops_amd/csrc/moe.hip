@@ -46,6 +46,9 @@ struct MoeArgs {
     uint16_t *h;           // [pairs, h_stride]
     long long h_stride;
     float *part;           // [tokens, top_k, hidden]
+    // few tokens: of item i and token t, the pair or -1 and its weight
+    int *col_pair;         // [items, kMoeFew]
+    float *col_weight;
 };
 
 // ------------------------------------------------------------------- routing
@@ -180,14 +183,16 @@ __device__ __forceinline__ void group(const MoeArgs &a, Pair &&pair) {
     }
 }
 
-// Up to 16 tokens: a wave each, and the groups in the same launch.
-constexpr int kRouteFew = 16;
+// Few tokens: a wave each, and the groups in the same launch.  An expert is one
+// item, as no token has it twice: pair p's place is the number of pairs before it
+// in the order of experts, then of pairs, counted over all of them.
+constexpr int kFewPairs = tecoops::kMoeFew * tecoops::kMoeMaxTopK;
 
 template <typename T, int R>
-__global__ void __launch_bounds__(1024) moe_route_kernel(MoeArgs a) {
-    __shared__ int id[kRouteFew * tecoops::kMoeMaxTopK];
-    __shared__ float weight[kRouteFew * tecoops::kMoeMaxTopK];
-    const int lane = threadIdx.x & 63, t = threadIdx.x >> 6;
+__global__ void __launch_bounds__(tecoops::kMoeFew * 64) moe_route_kernel(MoeArgs a) {
+    __shared__ int id[kFewPairs], fresh[kFewPairs], col_pair[kFewPairs * tecoops::kMoeFew];
+    __shared__ float weight[kFewPairs], col_weight[kFewPairs * tecoops::kMoeFew];
+    const int me = threadIdx.x, lane = me & 63, t = me >> 6;
     if (t < a.tokens) {
         int e;
         float w;
@@ -200,10 +205,41 @@ __global__ void __launch_bounds__(1024) moe_route_kernel(MoeArgs a) {
         }
     }
     __syncthreads();
-    group(a, [&](int p, int &e, float &w) {
-        e = id[p];
-        w = weight[p];
-    });
+    const int pairs = a.tokens * a.top_k;
+    const int e = me < pairs ? id[me] : -1;
+    int before = 0, same = 0, count = 0;
+#pragma unroll 8
+    for (int q = 0; q < pairs; ++q) {
+        const int o = id[q];
+        before += o >= 0 && o < e;
+        same += o == e && q < me;
+        count += o == e;
+    }
+    if (me < pairs) fresh[me] = e >= 0 && same == 0 ? e : -1;
+    for (int i = me; i < pairs * tecoops::kMoeFew; i += tecoops::kMoeFew * 64) col_pair[i] = -1;
+    __syncthreads();
+    int item = 0, total = 0;  // experts below e, and all
+#pragma unroll 8
+    for (int q = 0; q < pairs; ++q) {
+        const int o = fresh[q];
+        item += o >= 0 && o < e;
+        total += o >= 0;
+    }
+    if (e >= 0) {
+        const int at = before + same, token = me / a.top_k;
+        a.token[at] = token;
+        a.slot[at] = me;
+        a.weight[at] = weight[me];
+        if (same == 0) a.items[item] = make_int4(e, before, count, 0);
+        col_pair[item * tecoops::kMoeFew + token] = at;
+        col_weight[item * tecoops::kMoeFew + token] = weight[me];
+    }
+    if (me == 0) *a.n_items = total;
+    __syncthreads();
+    for (int i = me; i < total * tecoops::kMoeFew; i += tecoops::kMoeFew * 64) {
+        a.col_pair[i] = col_pair[i];
+        a.col_weight[i] = col_pair[i] >= 0 ? col_weight[i] : 0.0f;
+    }
 }
 
 // More tokens: a wave each over the chip, then one workgroup for the groups.
@@ -230,8 +266,8 @@ __global__ void __launch_bounds__(1024) moe_group_kernel(MoeArgs a) {
 
 template <typename T, int R>
 void launch_route(const MoeArgs &a, hipStream_t s) {
-    if (a.tokens <= kRouteFew) {
-        hipLaunchKernelGGL((moe_route_kernel<T, R>), dim3(1), dim3(1024), 0, s, a);
+    if (a.tokens <= tecoops::kMoeFew) {
+        hipLaunchKernelGGL((moe_route_kernel<T, R>), dim3(1), dim3(tecoops::kMoeFew * 64), 0, s, a);
         return;
     }
     hipLaunchKernelGGL((moe_choose_kernel<T, R>), dim3(tecoops::ceil_div(a.tokens, 4)), dim3(256), 0, s, a);
@@ -284,6 +320,137 @@ __global__ void __launch_bounds__(RS * KS * 64) moe_product_kernel(MoeArgs a) {
         }
     };
     product<T, false, XR, WR, RS, KS>(lds, K, unit, w_row, x_row, put);
+}
+
+// Few tokens: the second product with the sum over the experts in it, straight to
+// out.  A workgroup has WR rows of every expert's W_out; its 8 waves share the
+// items' stages of K out evenly, one item after the other, in a ring of D stages
+// each.  The columns are the tokens; at the end of an item (or of a wave's share
+// of it) a column adds its sums with its routing weight, or nothing where the
+// token has not chosen the expert, whatever was multiplied there.
+template <typename T, int XR, int WR, int D>
+__global__ void __launch_bounds__(512) moe_out_few_kernel(MoeArgs a) {
+    constexpr int KS = 8, RT = (WR + 15) / 16, WC = WR / 4, XC = XR / 4, PER = WC + XC;
+    constexpr int SB = (WR + XR) * 256;
+    static_assert(RT == 1 && D >= 3 && (D - 2) * PER < 64, "one row tile, vmcnt");
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int expert[kFewPairs];
+    __shared__ uint16_t col_pair[kFewPairs * XR];
+    __shared__ float col_weight[kFewPairs * XR];  // -1: the token has not chosen the expert
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    const int n0 = blockIdx.x * WR;
+    const int items = *a.n_items;
+    for (int i = threadIdx.x; i < items; i += 512) expert[i] = a.items[i].x;
+    for (int i = threadIdx.x; i < items * XR; i += 512) {
+        const int at = i / XR * tecoops::kMoeFew + i % XR;
+        const int p = a.col_pair[at];
+        col_pair[i] = static_cast<uint16_t>(max(p, 0));  // any pair's row of h
+        col_weight[i] = p >= 0 ? a.col_weight[at] : -1.0f;
+    }
+    __syncthreads();
+    const int kw = a.inter / 8;          // chunks of a row
+    const int spi = (kw + 15) / 16;      // stages of an item
+    const int stages = items * spi;
+    const int s0 = static_cast<int>(static_cast<long long>(stages) * wave / KS);
+    const int s1 = static_cast<int>(static_cast<long long>(stages) * (wave + 1) / KS);
+    char *ring = lds + wave * D * SB;
+    const int row = lane >> 4;
+    // load of the next stage: li, lst its item and stage in it
+    int li = s0 / spi, lst = s0 - li * spi, lslot = 0;
+    const auto load = [&] {
+        const int e = __builtin_amdgcn_readfirstlane(expert[li]);
+        const char *w = a.w_out + static_cast<long long>(e) * a.hidden * a.inter * 2;
+        char *dst = ring + lslot * SB;
+#pragma unroll
+        for (int m = 0; m < XC; ++m) {
+            const int q = 16 * lst + ((lane & 15) ^ (4 * m + row));
+            const int p = col_pair[li * XR + 4 * m + row];
+            dma16<false>(q < kw ? static_cast<const void *>(reinterpret_cast<const char *>(a.h + p * a.h_stride) + 16 * q)
+                                : static_cast<const void *>(kZero16),
+                         dst + WR * 256 + m * 1024);
+        }
+#pragma unroll
+        for (int m = 0; m < WC; ++m) {
+            const int q = 16 * lst + ((lane & 15) ^ (4 * m + row));
+            const long long r = min(n0 + 4 * m + row, a.hidden - 1);
+            dma16<true>(q < kw ? static_cast<const void *>(w + r * a.inter * 2 + 16 * q)
+                               : static_cast<const void *>(kZero16),
+                        dst + m * 1024);
+        }
+        if (++lst == spi) {
+            lst = 0;
+            ++li;
+        }
+        lslot = lslot + 1 == D ? 0 : lslot + 1;
+    };
+    const int wc = WR < 16 ? c & 7 : c, xc = c & (XR - 1);
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f}, tot = {0.0f, 0.0f, 0.0f, 0.0f};
+    int ui = li, ust = lst, slot = 0;
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d)
+        if (s0 + d < s1) load();
+    for (int s = s0; s < s1; ++s) {
+        // stages s + 1 .. min(s + D - 2, s1 - 1) may still be in flight
+        if (D > 3 && s + 2 < s1) wait_copies<(D > 3 ? 2 : 1) * PER>();
+        else if (s + 1 < s1) wait_copies<PER>();
+        else wait_copies<0>();
+        if (s + D - 1 < s1) load();
+        const char *wl = ring + slot * SB + wc * 256, *xl = ring + slot * SB + WR * 256 + xc * 256;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            acc = Mma16<T>::run(*reinterpret_cast<const u32x4_t *>(wl + 16 * ((4 * u + g) ^ wc)),
+                                *reinterpret_cast<const u32x4_t *>(xl + 16 * ((4 * u + g) ^ xc)), acc);
+        slot = slot + 1 == D ? 0 : slot + 1;
+        if (++ust == spi || s + 1 == s1) {
+            const float wt = col_weight[ui * XR + xc];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) tot[v] += wt >= 0.0f ? wt * acc[v] : 0.0f;
+            acc = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            ust = 0;
+            ++ui;
+        }
+        // the reads of stage s are done before its slot is copied over
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    __syncthreads();
+    float4_t *red = reinterpret_cast<float4_t *>(lds);
+    red[wave * 64 + lane] = float4_t{tot[0], tot[1], tot[2], tot[3]};
+    __syncthreads();
+    if (wave != 0) return;
+    float4_t sum = red[lane];
+#pragma unroll
+    for (int w = 1; w < KS; ++w) sum += red[w * 64 + lane];
+    const int n = n0 + 4 * g;
+    if (c >= a.tokens || g >= WR / 4 || n >= a.hidden) return;  // hidden % 8 == 0: four at a time
+    uint16_t *dst = a.out + static_cast<long long>(c) * a.hidden + n;
+    const uint32_t lo2 = tecoops::dev::round2<T>(sum[0], sum[1]), hi2 = tecoops::dev::round2<T>(sum[2], sum[3]);
+    if (tecoops::aligned(dst, 8)) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(lo2, hi2);
+    } else {
+        dst[0] = static_cast<uint16_t>(lo2);
+        dst[1] = static_cast<uint16_t>(lo2 >> 16);
+        dst[2] = static_cast<uint16_t>(hi2);
+        dst[3] = static_cast<uint16_t>(hi2 >> 16);
+    }
+}
+
+template <typename T, int XR, int WR, int D>
+bool launch_out_few(const MoeArgs &a, hipStream_t s) {
+    auto *kern = &moe_out_few_kernel<T, XR, WR, D>;
+    constexpr size_t lds = 8 * D * (WR + XR) * 256;
+    if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), lds)) return false;
+    hipLaunchKernelGGL(kern, dim3(tecoops::ceil_div(a.hidden, WR)), dim3(512), lds, s, a);
+    return true;
+}
+
+// 16 rows of W_out to a workgroup where that leaves every CU one, else 8.
+template <typename T>
+bool run_out_few(const MoeArgs &a, hipStream_t s) {
+    const bool wide = a.hidden >= 16 * tecoops::device_cus();
+    if (a.rows == 4) return wide ? launch_out_few<T, 4, 16, 3>(a, s) : launch_out_few<T, 4, 8, 4>(a, s);
+    return wide ? launch_out_few<T, 8, 16, 3>(a, s) : launch_out_few<T, 8, 8, 4>(a, s);
 }
 
 // Widths that are not in whole 16-byte words, or tensors that are not aligned: a
@@ -403,6 +570,11 @@ tecoopsStatus_t run_slice(const MoeArgs &a, int items, bool copy, hipStream_t s)
     TECO_CHECK_LAUNCH("moe_layer");
     if (!launch_product<T, false>(a, items, copy, s)) return TECOOPS_STATUS_INTERNAL_ERROR;
     TECO_CHECK_LAUNCH("moe_layer");
+    if (copy && tecoops::moe_out_few(a.tokens, a.hidden, a.inter, a.experts, a.top_k, tecoops::device_cus())) {
+        if (!run_out_few<T>(a, s)) return TECOOPS_STATUS_INTERNAL_ERROR;
+        TECO_CHECK_LAUNCH("moe_layer");
+        return TECOOPS_STATUS_SUCCESS;
+    }
     if (!launch_product<T, true>(a, items, copy, s)) return TECOOPS_STATUS_INTERNAL_ERROR;
     TECO_CHECK_LAUNCH("moe_layer");
     hipLaunchKernelGGL((moe_combine_kernel<T>), dim3(tecoops::ceil_div(a.hidden, 1024), a.tokens),
@@ -484,6 +656,8 @@ extern "C" tecoopsStatus_t tecoopsMoeLayer(tecoopsHandle_t handle, const void *x
     a.h = reinterpret_cast<uint16_t *>(ws + sp.h_at);
     a.h_stride = sp.h_stride;
     a.part = reinterpret_cast<float *>(ws + sp.part_at);
+    a.col_pair = reinterpret_cast<int *>(ws + sp.cols_at);
+    a.col_weight = reinterpret_cast<float *>(ws + sp.cols_at) + sp.items * tecoops::kMoeFew;
     const bool copy = hidden % 8 == 0 && inter % 8 == 0 && x_stride % 8 == 0 &&
                       tecoops::aligned(x, 16) && tecoops::aligned(w_in, 16) &&
                       tecoops::aligned(w_out, 16);
