@@ -22,6 +22,8 @@
 #include "common.h"
 #include "device.h"
 
+#include <type_traits>
+
 namespace {
 
 using namespace tecoops::dev;
@@ -43,6 +45,7 @@ struct OnePosition {
     // tokens outside the table turn by nothing in the fused kernel: pairs with
     // an infinity become NaN there
     static constexpr bool kCopySkipped = false;
+    static constexpr bool kEarlyLoads = false;
 
     __device__ __forceinline__ float2 angle(int t, int i) const {
         const int half = rot_dim >> 1;
@@ -80,6 +83,11 @@ struct AxisPositions {
     double log2_base;
 
     static constexpr bool kCopySkipped = true;  // as they are, whatever they hold
+    // The 64-bit angles take a good part of a microsecond: a workgroup's first loads
+    // of q, k and v are under way meanwhile, and few tasks take 128 threads (q and k
+    // [16380, 16, 128] fp16 in rows of 12288 bytes 49.7 us without, 46.0 with; with
+    // the store, 4 tokens 4.2 and 3.8 us, 8191 tokens 40 us either way).
+    static constexpr bool kEarlyLoads = true;
 
     __device__ __forceinline__ float2 angle(int t, int i) const {
         const int half = rot_dim >> 1;
@@ -211,6 +219,44 @@ rotary_kernel(Angles angles, uint16_t *__restrict__ query, uint16_t *__restrict_
     __shared__ int skip[kTokensPerBlock];
     const int half = rot_dim >> 1;
     const int tbase = blockIdx.x * kTokensPerBlock;
+    if constexpr (Angles::kEarlyLoads && NEOX && VW == 2) {
+        static_assert(kTokensPerBlock == 1, "the workgroup's token");
+        const int threads = blockDim.x, per_head = half / 8, nq = num_heads * per_head;
+        const int total = (num_heads + (key ? num_kv_heads : 0)) * per_head;
+        uint16_t *const q = query + tbase * q_stride;
+        uint16_t *const k = key + tbase * k_stride;
+        uint4 xa[kRotBatch], xb[kRotBatch];
+        uint16_t *rp[kRotBatch];
+        int i0[kRotBatch];
+        const auto load = [&](int base) {
+#pragma unroll
+            for (int u = 0; u < kRotBatch; ++u) {
+                const int task = min(base + threads * u, total - 1);
+                const int local = task < nq ? task : task - nq;
+                const int h = local / per_head;
+                i0[u] = (local - h * per_head) * 8;
+                rp[u] = (task < nq ? q : k) + h * head_size + i0[u];
+                xa[u] = ld_stream(reinterpret_cast<const uint4 *>(rp[u]));
+                xb[u] = ld_stream(reinterpret_cast<const uint4 *>(rp[u] + half));
+            }
+        };
+        load(threadIdx.x);
+        if (angles.skipped(tbase)) return;
+        for (int i = threadIdx.x; i < half; i += threads) cs[0][i] = angles.angle(tbase, i);
+        __syncthreads();
+        for (int base = threadIdx.x; base < total; base += threads * kRotBatch) {
+            if (base != static_cast<int>(threadIdx.x)) load(base);
+#pragma unroll
+            for (int u = 0; u < kRotBatch; ++u) {
+                if (base + threads * u >= total) continue;
+                uint4 oa, ob;
+                rot_neox8<T>(xa[u], xb[u], &cs[0][i0[u]], oa, ob);
+                st_stream(reinterpret_cast<uint4 *>(rp[u]), oa);
+                st_stream(reinterpret_cast<uint4 *>(rp[u] + half), ob);
+            }
+        }
+        return;
+    }
     for (int e = threadIdx.x; e < kTokensPerBlock * half; e += blockDim.x) {
         const int tt = e / half, i = e - tt * half;
         const int t = tbase + tt;
@@ -304,6 +350,50 @@ rotary_kernel(Angles angles, uint16_t *__restrict__ query, uint16_t *__restrict_
     }
 }
 
+// NeoX halves that are not whole 128-byte lines (heads of 64, 80, 96): the two
+// loads of a pair would each fetch the lines they share.  A token's rows go
+// through LDS instead, loaded and stored in the order of memory (q and k [16380,
+// 16, 80] fp16 in rows of 7680 bytes: 42.4 us in pairs of loads, 31.6 so, 5.3 TB/s;
+// heads of 64 32.7 and 26.2, of 96 44.7 and 36.7).
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+rotary_rows_kernel(AxisPositions angles, uint16_t *__restrict__ query, uint16_t *__restrict__ key,
+                   int num_heads, int num_kv_heads, int head_size, long long q_stride, long long k_stride) {
+    extern __shared__ uint4 rows[];
+    __shared__ float2 cs[kMaxHalf];
+    const int half = head_size >> 1, threads = blockDim.x;
+    const int nq = num_heads * head_size / 8, n = nq + num_kv_heads * head_size / 8;  // 16-byte words
+    uint4 *const q = reinterpret_cast<uint4 *>(query + blockIdx.x * q_stride);
+    uint4 *const k = reinterpret_cast<uint4 *>(key + blockIdx.x * k_stride) - nq;
+    constexpr int B = 4;
+    uint4 x[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+        const int c = min(static_cast<int>(threadIdx.x) + threads * u, n - 1);
+        x[u] = ld_stream((c < nq ? q : k) + c);
+    }
+    if (angles.skipped(blockIdx.x)) return;
+    for (int i = threadIdx.x; i < half; i += threads) cs[i] = angles.angle(blockIdx.x, i);
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+        const int c = threadIdx.x + threads * u;
+        if (c < n) rows[c] = x[u];
+    }
+    for (int c = threadIdx.x + threads * B; c < n; c += threads) rows[c] = ld_stream((c < nq ? q : k) + c);
+    __syncthreads();
+    const int per = half / 8, tasks = (num_heads + num_kv_heads) * per;
+    for (int t = threadIdx.x; t < tasks; t += threads) {
+        const int h = t / per, i = t - h * per;
+        uint4 *const a = rows + h * 2 * per + i;
+        uint4 oa, ob;
+        rot_neox8<T>(a[0], a[per], &cs[8 * i], oa, ob);
+        a[0] = oa;
+        a[per] = ob;
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < n; c += threads) st_stream((c < nq ? q : k) + c, rows[c]);
+}
+
 // Fused decode-step kernel: rotary on query (in place) and key, rotated key
 // and value written straight into the paged caches [num_blocks, Hkv,
 // block_size, D] at slot_mapping[t] (key also written back in place when
@@ -333,6 +423,71 @@ __global__ void __launch_bounds__(kThreads) rotary_cache_kernel(Angles angles, F
     const int half = a.rot_dim >> 1;
     const int D = a.head_size;
     const int tbase = blockIdx.x * kTokensPerBlock;
+    if constexpr (Angles::kEarlyLoads && NEOX && VW == 2) {
+        if (a.rot_dim == D) {
+            const int threads = blockDim.x, per_head = half / 8, per_copy = D / 8;
+            const int nq = a.num_heads * per_head, nk = a.num_kv_heads * per_head;
+            const int total = nq + nk + a.num_kv_heads * per_copy;
+            uint16_t *const q = a.query + tbase * a.q_stride;
+            uint16_t *const k = a.key + tbase * a.k_stride;
+            const uint16_t *const v = a.value + tbase * a.v_stride;
+            uint4 xa[kFusedBatch], xb[kFusedBatch];
+            int head[kFusedBatch], elem[kFusedBatch];  // of the task: its head and first element
+            const auto load = [&](int base) {
+#pragma unroll
+                for (int u = 0; u < kFusedBatch; ++u) {
+                    const int task = min(base + threads * u, total - 1);
+                    const bool copy = task >= nq + nk;
+                    const int local = copy ? task - nq - nk : task < nq ? task : task - nq;
+                    const int per = copy ? per_copy : per_head;
+                    head[u] = local / per;
+                    elem[u] = (local - head[u] * per) * 8;
+                    const uint16_t *row = (copy ? v : task < nq ? q : k) + head[u] * D + elem[u];
+                    xa[u] = ld_stream(reinterpret_cast<const uint4 *>(row));
+                    xb[u] = ld_stream(reinterpret_cast<const uint4 *>(copy ? row : row + half));
+                }
+            };
+            load(threadIdx.x);
+            const bool skip = angles.skipped(tbase);
+            const int64_t slot = a.slots[tbase];
+            long long at = -1;  // first element of the token's cache row
+            if (slot >= 0 && slot < a.capacity) {
+                const int s32 = static_cast<int>(slot);
+                const int blk = a.lbs >= 0 ? s32 >> a.lbs : s32 / a.block_size;
+                at = (static_cast<long long>(blk) * a.num_kv_heads * a.block_size + (s32 - blk * a.block_size)) * D;
+            }
+            if (!skip)
+                for (int i = threadIdx.x; i < half; i += threads) cs[0][i] = angles.angle(tbase, i);
+            __syncthreads();
+            const long long step = static_cast<long long>(a.block_size) * D;  // cache, per kv head
+            for (int base = threadIdx.x; base < total; base += threads * kFusedBatch) {
+                if (base != static_cast<int>(threadIdx.x)) load(base);
+#pragma unroll
+                for (int u = 0; u < kFusedBatch; ++u) {
+                    const int task = base + threads * u;
+                    if (task >= total) continue;
+                    if (task >= nq + nk) {
+                        if (at >= 0)
+                            st_stream(reinterpret_cast<uint4 *>(a.vcache + at + head[u] * step + elem[u]), xa[u]);
+                        continue;
+                    }
+                    uint4 oa = xa[u], ob = xb[u];
+                    if (!skip) rot_neox8<T>(xa[u], xb[u], &cs[0][elem[u]], oa, ob);
+                    if (task < nq || a.write_key) {
+                        uint16_t *row = (task < nq ? q : k) + head[u] * D + elem[u];
+                        st_stream(reinterpret_cast<uint4 *>(row), oa);
+                        st_stream(reinterpret_cast<uint4 *>(row + half), ob);
+                    }
+                    if (task >= nq && at >= 0) {
+                        uint16_t *row = a.kcache + at + head[u] * step + elem[u];
+                        st_stream(reinterpret_cast<uint4 *>(row), oa);
+                        st_stream(reinterpret_cast<uint4 *>(row + half), ob);
+                    }
+                }
+            }
+            return;
+        }
+    }
     for (int e = threadIdx.x; e < kTokensPerBlock * half; e += blockDim.x) {
         const int tt = e / half, i = e - tt * half;
         const int t = tbase + tt;
@@ -588,7 +743,19 @@ struct Rows {
 template <typename T, bool NEOX, int VW, typename Angles>
 void launch_vw(const Angles &an, const Rows &r, hipStream_t s) {
     const unsigned grid = tecoops::ceil_div(r.num_tokens, kTokensPerBlock);
-    hipLaunchKernelGGL((rotary_kernel<T, NEOX, VW, Angles>), dim3(grid), dim3(kThreads), 0, s, an,
+    if constexpr (std::is_same<Angles, AxisPositions>::value && NEOX && VW == 2) {
+        const size_t lds = static_cast<size_t>(r.num_heads + r.num_kv_heads) * r.head_size * 2;
+        if (r.rot_dim == r.head_size && r.rot_dim % 128 != 0 && lds <= 32 * 1024) {
+            hipLaunchKernelGGL((rotary_rows_kernel<T>), dim3(grid), dim3(lds <= 8 * 1024 ? 128 : 256), lds, s, an,
+                               static_cast<uint16_t *>(r.query), static_cast<uint16_t *>(r.key), r.num_heads,
+                               r.num_kv_heads, r.head_size, r.query_stride, r.key_stride);
+            return;
+        }
+    }
+    // threads with two tasks each fill the last round best
+    const int tasks = (r.num_heads + r.num_kv_heads) * (r.rot_dim / 16);
+    const int threads = Angles::kEarlyLoads && NEOX && VW == 2 && tasks <= kThreads ? kThreads / 2 : kThreads;
+    hipLaunchKernelGGL((rotary_kernel<T, NEOX, VW, Angles>), dim3(grid), dim3(threads), 0, s, an,
                        static_cast<uint16_t *>(r.query), static_cast<uint16_t *>(r.key),
                        r.num_tokens, r.num_heads, r.num_kv_heads, r.head_size, r.rot_dim,
                        r.query_stride, r.key_stride);
