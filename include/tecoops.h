@@ -349,8 +349,7 @@ tecoopsStatus_t tecoopsGemvInt8(tecoopsHandle_t handle, const int8_t *weight,
                                 const void *scales, const void *x, void *y,
                                 int batch, int n, int k);
 
-/* ---- operators of a decoder layer around attention.  Work on no rows (m or
- *      num_tokens 0) is done without a launch. ---- */
+/* ---- operators of a decoder layer around attention ---- */
 
 typedef enum {
     TECOOPS_ACTIVATION_NONE = 0,
@@ -369,7 +368,7 @@ typedef enum {
  * residual may be out itself (same pointer and stride); other overlaps of out
  * with an input are not allowed.  dataType HALF or BFLOAT16, any sizes (rows
  * of x and W in whole, aligned 16-byte words are fastest) up to k and x_stride
- * 2^21 and n 2^30.
+ * 2^21, n 2^23 and 2^23 tiles of out; m = 0 is done without a launch.
  * workspace: tecoopsGetLinearWorkspaceSize() bytes for the same sizes let few
  * tiles be split along k; with less, or NULL, the call runs with fewer splits
  * (slower, the same result up to fp32 rounding).  Nothing is allocated. */
@@ -386,7 +385,8 @@ tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, int gated, si
  *   the top_k experts e_j of the largest logits (ties to the lowest index; -inf
  *   and NaN are never chosen, so a masked token may have fewer or none),
  *   w_j = p[e_j], divided by their sum when renormalize != 0,
- *   h_j = act(x[t] Wg[e_j]^T) * (x[t] Wu[e_j]^T), rounded to dataType,
+ *   h_j = act(x[t] Wg[e_j]^T) * (x[t] Wu[e_j]^T), rounded to dataType (fp16:
+ *         infinite from 65520 on),
  *   out[t] = sum_j w_j (h_j W_out[e_j]^T), fp32 sums, one rounding.
  * x [tokens, hidden] with row stride x_stride (elements); w_in [experts,
  * 2 inter, hidden] packed, the inter gate rows Wg of an expert before its up
@@ -396,8 +396,9 @@ tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, int gated, si
  * int32 and topk_weights float [tokens, top_k] are written unless NULL, best
  * first, -1 and 0 where there is none.  Every expert's weights are read once
  * for all of its tokens (of each 512 tokens, up to 64 at a time).  Up to 1024
- * experts, top_k 32, hidden and inter 2^20; hidden, inter and x_stride
- * multiples of 8 and 16-byte aligned tensors are fast.
+ * experts, top_k 32, hidden and inter 2^16; hidden, inter and x_stride
+ * multiples of 8 and 16-byte aligned tensors are fast; tokens = 0 is done
+ * without a launch.
  * workspace: tecoopsGetMoeLayerWorkspaceSize() bytes, 16-byte aligned; NULL
  * uses the handle's scratch (NOT_SUPPORTED on a stream under capture). */
 tecoopsStatus_t tecoopsMoeLayer(tecoopsHandle_t handle, const void *x, long long x_stride,

@@ -13,6 +13,7 @@ constexpr int kLinearStreamRows = 64;
 // Longest row (of x or W, in elements): 256 rows of it stay within the 32-bit
 // offsets of a tile's copies.
 constexpr int kLinearMaxRow = 1 << 21;
+constexpr int kLinearMaxOutputs = 1 << 23;
 
 // The tiles built: rows of x and of W, stages in the ring, workgroups that fit a
 // CU, and the microseconds of a workgroup on 256 CUs: per stage of 64 of K at

@@ -585,8 +585,8 @@ extern "C" tecoopsStatus_t tecoopsLinear(tecoopsHandle_t handle, const void *x, 
     if (!tecoops::is_16bit_float(dataType)) return TECOOPS_STATUS_BAD_PARAM;
     for (const void *p : {x, weight, bias, residual, const_cast<const void *>(out)})
         if (!tecoops::aligned(p, 2)) return TECOOPS_STATUS_BAD_PARAM;
-    // a tile's offsets into x and W and the rows of W are 32-bit
-    if (x_stride > tecoops::kLinearMaxRow || k > tecoops::kLinearMaxRow || n > (1 << 30))
+    // a tile's offsets into x and W are 32-bit, and so is a grid's number of threads
+    if (x_stride > tecoops::kLinearMaxRow || k > tecoops::kLinearMaxRow || n > tecoops::kLinearMaxOutputs)
         return TECOOPS_STATUS_NOT_SUPPORTED;
     if (m == 0) return TECOOPS_STATUS_SUCCESS;
     const int wrows = gated ? 2 * n : n;
@@ -607,7 +607,7 @@ extern "C" tecoopsStatus_t tecoopsLinear(tecoopsHandle_t handle, const void *x, 
     if (p.stream)
         return tecoops::gemv_batch_epilogue(handle->stream, weight, x, x_stride, out, m, wrows, k,
                                             dataType, e);
-    if (static_cast<long long>(p.tiles_m) * p.tiles_n * p.splits > 0x7fffffffll)
+    if (static_cast<long long>(p.tiles_m) * p.tiles_n * p.splits > 0x7fffff)
         return TECOOPS_STATUS_NOT_SUPPORTED;
     TileArgs a{};
     a.w = static_cast<const char *>(weight);

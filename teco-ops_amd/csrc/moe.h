@@ -10,6 +10,7 @@ namespace tecoops {
 
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeMaxTopK = 32;
+constexpr int kMoeMaxWidth = 1 << 16;  // the threads of every grid stay below 2^32
 constexpr int kMoeFew = 8;       // tokens whose second product sums over the experts
 constexpr int kMoeSlice = 512;  // tokens routed together; more run slice by slice
 

@@ -285,6 +285,54 @@ def test_torch_op():
     assert torch.equal(out15, linear64(x, w.clamp(-1, 1), None, None, None, True).to(dt))
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 40, 128), (100, 70, 512), (90, 33, 77)])
+def test_without_the_torch_library(m, n, k, monkeypatch):
+    """The Python function through the C ABI alone gives the same bits; so do
+    parameters that require a gradient."""
+    dt = torch.float16
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x, w, b = whole(g, m, k, dtype=dt), whole(g, 2 * n, k, dtype=dt, most=1), whole(g, 2 * n, dtype=dt)
+    r, out = whole(g, m, n, dtype=dt), torch.empty(m, n, dtype=dt, device="cuda")
+    kw = dict(bias=b, residual=r, activation="silu", gated=True)
+    tecoops.linear(x, w, out, **kw)
+    with_grad = torch.empty_like(out)
+    tecoops.linear(x, torch.nn.Parameter(w.clone()), with_grad, **kw)
+    assert torch.equal(out, with_grad) and not with_grad.requires_grad
+    monkeypatch.setattr(tecoops, "_linear", None)
+    again = torch.empty_like(out)
+    tecoops.linear(x, w, again, **kw)
+    assert torch.equal(out, again)
+
+
+def test_past_32_bits():
+    """Weights of more than 2^32 bytes and rows of x, residual and out far apart:
+    the last rows and outputs come from where they are."""
+    dt, k = torch.bfloat16, 8192
+    n = (1 << 32) // (2 * k) + 300
+    w = torch.zeros(n, k, dtype=dt, device="cuda")
+    w[-1, -1], w[n - 2, 5], w[3, 7] = 2, 3, 4
+    for m in (2, 70, 300):
+        x = torch.zeros(m, k, dtype=dt, device="cuda")
+        x[m - 1] = 1
+        out = torch.full((m, n), 9.0, dtype=dt, device="cuda")
+        tecoops.linear(x, w, out)
+        assert (out[:m - 1] == 0).all()
+        last = out[m - 1]
+        assert (last[n - 1], last[n - 2], last[3]) == (2, 3, 4) and last.count_nonzero() == 3
+    del w, out
+    m, n, k, apart = 1100, 96, 64, 1 << 21
+    wide = torch.empty(m * apart, dtype=dt, device="cuda")
+    x = wide.view(m, apart)[:, :k]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x.copy_(whole(g, m, k, dtype=dt))
+    res = wide.view(m, apart)[:, 1000:1000 + n]
+    res.copy_(whole(g, m, n, dtype=dt))
+    out = wide.view(m, apart)[:, 2000:2000 + n]
+    w = whole(g, n, k, dtype=dt)
+    tecoops.linear(x, w, out, residual=res)
+    assert torch.equal(out, linear64(x, w, None, res, None, False).to(dt))
+
+
 def test_no_rows_and_refusals():
     dt = torch.float16
     x, w = torch.zeros(4, 16, dtype=dt, device="cuda"), torch.zeros(6, 16, dtype=dt, device="cuda")

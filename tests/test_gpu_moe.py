@@ -344,6 +344,37 @@ def test_torch_op():
     assert torch.equal(out, o2)
 
 
+@pytest.mark.parametrize("T,H,I", [(3, 64, 32), (40, 64, 32), (3, 33, 31)])
+def test_without_the_torch_library(T, H, I, monkeypatch):
+    dt, E, k = torch.bfloat16, 8, 2
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = whole(g, T, H, dtype=dt, most=2)
+    w_in, w_out = sparse_rows(g, E, 2 * I, H, dtype=dt), whole(g, E, H, I, dtype=dt)
+    logits = torch.randn(T, E, generator=g, device="cuda")
+    first = run(x, w_in, w_out, logits, k)
+    second = run(x, torch.nn.Parameter(w_in), w_out, logits, k)
+    monkeypatch.setattr(tecoops, "_moe_layer", None)
+    for a, b, c in zip(first, second, run(x, w_in, w_out, logits, k)):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("T", [2, 20])
+def test_past_32_bits(T):
+    """Experts whose weights lie past 2^32 bytes."""
+    dt, E, H, I = torch.bfloat16, 48, 4096, 12288
+    w_in = torch.zeros(E, 2 * I, H, dtype=dt, device="cuda")
+    w_out = torch.zeros(E, H, I, dtype=dt, device="cuda")
+    w_in[E - 1, I - 1, 0], w_in[E - 1, 2 * I - 1, 1] = 1, 1  # the last gate and up rows
+    w_out[E - 1, H - 1, I - 1], w_out[E - 1, 0, I - 1] = 1, 2
+    x = torch.zeros(T, H, dtype=dt, device="cuda")
+    x[:, 0], x[:, 1] = 2, 3
+    logits = torch.zeros(T, E, device="cuda")
+    logits[:, E - 1] = 1
+    out, ids, _ = run(x, w_in, w_out, logits, 1, act="relu")
+    assert (ids == E - 1).all()
+    assert (out[:, H - 1] == 6).all() and (out[:, 0] == 12).all() and out.count_nonzero() == 2 * T
+
+
 def test_no_tokens_and_refusals():
     dt, T, H, I, E = torch.float16, 4, 16, 8, 4
     x, out = (torch.zeros(T, H, dtype=dt, device="cuda") for _ in range(2))

@@ -229,6 +229,48 @@ def test_torch_ops():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_without_the_torch_library(D, monkeypatch):
+    T, H, Hkv, dt, half = 11, 4, 2, torch.bfloat16, D // 2
+    _, (q, k, v) = make(4, T, H, Hkv, D, dt)
+    pos, slots = positions(6, 2, T, 500).cuda(), torch.arange(T, device="cuda")
+    got = []
+    for _ in range(2):
+        q1, k1, q2, k2 = q.clone(), k.clone(), q.clone(), k.clone()
+        kc, vc = (torch.zeros(2, Hkv, 16, D, dtype=dt, device="cuda") for _ in range(2))
+        sec = [half - 10, 10]
+        tecoops.rotary_embedding_axes(pos, q1, k1, D, sec)
+        tecoops.rotary_axes_reshape_and_cache(pos, q2, k2, v, slots, kc, vc, D, sec, write_key=True)
+        assert torch.equal(q1, q2) and torch.equal(k1, k2)
+        got.append((q1, k1, kc, vc))
+        monkeypatch.setattr(tecoops, "_rotary_axes", None)
+        monkeypatch.setattr(tecoops, "_rotary_axes_cache", None)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_past_32_bits():
+    """Cache rows and rows of q and k past 2^32 bytes."""
+    T, H, Hkv, D, bs, dt = 3, 2, 2, 128, 16, torch.float16
+    nb = (1 << 32) // (2 * Hkv * D * bs) + 8
+    kc, vc = (torch.zeros(nb, Hkv, bs, D, dtype=dt, device="cuda") for _ in range(2))
+    apart = 1 << 30
+    wide = torch.zeros(T * apart, dtype=dt, device="cuda").view(T, apart)
+    _, (q0, k0, v0) = make(2, T, H, Hkv, D, dt)
+    q, k, v = wide[:, :H * D], wide[:, 1000:1000 + Hkv * D], wide[:, 2000:2000 + Hkv * D]
+    for row, was in ((q, q0), (k, k0), (v, v0)):
+        row.copy_(was.flatten(1))
+    pos = positions(1, 3, T, 1000)
+    slots = torch.tensor([nb * bs - 1, 5, nb * bs - 20], device="cuda")
+    tecoops.rotary_axes_reshape_and_cache(pos.cuda(), q, k, v, slots, kc, vc, D, [24, 20, 20],
+                                          layout="interleaved", write_key=True)
+    check(q.unflatten(1, (H, D)), q0, pos.numpy(), [24, 20, 20], D, 10000.0, "interleaved", True)
+    check(k.unflatten(1, (Hkv, D)), k0, pos.numpy(), [24, 20, 20], D, 10000.0, "interleaved", True)
+    page, row = slots // bs, slots % bs
+    assert torch.equal(kc[page, :, row].flatten(1), k) and torch.equal(vc[page, :, row].flatten(1), v)
+    assert kc.count_nonzero() <= T * Hkv * D
+    tecoops.rotary_embedding_axes(pos.cuda(), q, None, D, [24, 20, 20], layout="interleaved")
+
+
 def test_no_tokens_and_refusals():
     T, H, D, dt = 6, 2, 64, torch.float16
     q, k = (torch.zeros(T, H, D, dtype=dt, device="cuda") for _ in range(2))

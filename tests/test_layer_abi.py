@@ -39,7 +39,8 @@ def test_linear_refusals(handle):
         assert call(**kw) == BAD, kw
     assert call(k=(1 << 21) + 8, xs=(1 << 21) + 8) == NOT_SUP
     assert call(xs=(1 << 21) + 8) == NOT_SUP
-    assert call(n=(1 << 30) + 4, os=1 << 31, rs=1 << 31) == NOT_SUP
+    assert call(n=(1 << 23) + 4, os=1 << 31, rs=1 << 31) == NOT_SUP
+    assert call(m=(1 << 31) - 1, n=2000, os=2000, rs=2000) == NOT_SUP  # too many tiles
     assert call(m=0) == OK  # no launch
     size = ctypes.c_size_t(1)
     g = _lib.lib().tecoopsGetLinearWorkspaceSize
@@ -165,7 +166,7 @@ def test_moe_refusals(handle):
                dict(wb=100), dict(wb=0), dict(ws=P + 8)):
         assert call(**kw) == BAD, kw
     assert call(E=1025) == NOT_SUP and call(E=64, k=33) == NOT_SUP
-    assert call(H=(1 << 20) + 8, xs=1 << 21) == NOT_SUP and call(I=(1 << 20) + 8) == NOT_SUP
+    assert call(H=(1 << 16) + 8, xs=1 << 21) == NOT_SUP and call(I=(1 << 16) + 8) == NOT_SUP
     assert call(T=0) == OK  # no launch
     g = _lib.lib().tecoopsGetMoeLayerWorkspaceSize
     size = ctypes.c_size_t(1)
