@@ -5,8 +5,10 @@
 //   out[m, n] = T( act(gate[m, n]) * up[m, n] + residual[m, n] )
 //
 // Up to 64 rows of x mostly stream W through gemv_batch.hip.  Other products run
-// here, a tile of out per workgroup on v_mfma_f32_32x32x16_{f16,bf16} with W as the
-// first operand, so that a lane ends with 4 neighbouring outputs of a row.
+// here, a tile of out per workgroup on v_mfma_f32_16x16x32_{f16,bf16} with W as the
+// first operand, so that a lane ends with 4 neighbouring outputs of a row.  (With
+// 32x32x16 the same kernel is slower: 8192 x 28672 x 4096 bf16 gated 1577 us for
+// 1523, 4096^3 115 for 108.5, 333 x 4096 x 14336 60 for 55.6.)
 //
 // A stage is 64 of K: 128 bytes of each row of W and x of the tile, copied into
 // LDS with no registers (global_load_lds_dwordx4), D stages in a ring.  The
@@ -42,18 +44,17 @@ using tecoops::Epilogue;
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
-template <typename T> struct Mma32;
-template <> struct Mma32<f16> {
-    static __device__ __forceinline__ f32x16_t run(u32x4_t a, u32x4_t b, f32x16_t c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+template <typename T> struct Mma;
+template <> struct Mma<f16> {
+    static __device__ __forceinline__ float4_t run(u32x4_t a, u32x4_t b, float4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
                                                       __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
     }
 };
-template <> struct Mma32<bf16> {
-    static __device__ __forceinline__ f32x16_t run(u32x4_t a, u32x4_t b, f32x16_t c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+template <> struct Mma<bf16> {
+    static __device__ __forceinline__ float4_t run(u32x4_t a, u32x4_t b, float4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                        __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     }
 };
@@ -239,7 +240,7 @@ template <typename T, int BM, int BN, int WM, int WN, int D, bool COPY, bool SPL
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 linear_tile_kernel(TileArgs a) {
     constexpr int NW = WM * WN;
-    constexpr int MT = BM / WM / 32, NT = BN / WN / 32;  // 32 x 32 tiles of a wave
+    constexpr int MT = BM / WM / 32, NT = BN / WN / 32;  // blocks of 32 rows of a wave
     constexpr int STAGE = (BM + BN) * 128;
     constexpr int CW = BN / 8 / NW, CX = BM / 8 / NW;  // copies of a wave and stage
     static_assert(CW * 8 * NW == BN && CX * 8 * NW == BM, "whole copies");
@@ -338,52 +339,44 @@ linear_tile_kernel(TileArgs a) {
         }
     };
 
-    f32x16_t acc[NT][MT];
+    float4_t acc[2 * NT][2 * MT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < 2 * NT; ++i)
 #pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+        for (int j = 0; j < 2 * MT; ++j) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // fragments: row lane % 32 of a 32-row block, 8 of K at 8 (lane / 32)
-    const int fr = lane & 31, fg = lane >> 5;
+    // fragments: row lane % 16 of a 16-row block, 8 of K at 8 (lane / 16)
+    const int fr = lane & 15, fg = lane >> 4;
     struct Frags {
-        u32x4_t w[2][NT], x[2][MT];
+        u32x4_t w[2 * NT], x[2 * MT];
     };
     const char *wl = lds + (wn * NT * 32 + fr) * 128;
     const char *xl = lds + BN * 128 + (wm * MT * 32 + fr) * 128;
-    // Fragment number q of a half stage, in the order of their use: of each 16 of
-    // K the x fragments and then those of W.
+    // Fragment number q of a half stage, in the order of their use.
     constexpr int NF = 2 * (MT + NT);
     const auto read = [&](Frags &f, int slot, int half, int q) {
-        const int s = q / (MT + NT), r = q % (MT + NT);
-        const int c = ((4 * half + 2 * s + fg) ^ (fr >> 1 & 7)) * 16 + slot;
-        if (r < MT) f.x[s][r] = *reinterpret_cast<const u32x4_t *>(xl + r * 4096 + c);
-        else f.w[s][r - MT] = *reinterpret_cast<const u32x4_t *>(wl + (r - MT) * 4096 + c);
+        const int c = ((4 * half + fg) ^ (fr >> 1 & 7)) * 16 + slot;
+        if (q < 2 * MT) f.x[q] = *reinterpret_cast<const u32x4_t *>(xl + q * 2048 + c);
+        else f.w[q - 2 * MT] = *reinterpret_cast<const u32x4_t *>(wl + (q - 2 * MT) * 2048 + c);
     };
-    const auto multiply = [&](const Frags &f, int p) {  // product p of 2 NT MT
-        const int s = p / (NT * MT), i = p / MT % NT, j = p % MT;
-        acc[i][j] = Mma32<T>::run(f.w[s][i], f.x[s][j], acc[i][j]);
+    const auto multiply = [&](const Frags &f, int p) {  // product p of 4 NT MT
+        const int i = p / (2 * MT), j = p % (2 * MT);
+        acc[i][j] = Mma<T>::run(f.w[i], f.x[j], acc[i][j]);
     };
-    constexpr int NP = 2 * NT * MT;
+    constexpr int NP = 4 * NT * MT;
     // Both operands are cleared past K: the bits there are some other chunk's,
     // which may hold inf or NaN.
     const auto mask = [&](Frags &f, int half) {
         const int left = a.k - (st0 + nst - 1) * 64;
         if (left >= 64) return;
+        const int k0 = 32 * half + 8 * fg;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int k0 = 32 * half + 16 * s + 8 * fg;
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t keep = (k0 + 2 * e < left ? 0xffffu : 0u) | (k0 + 2 * e + 1 < left ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t keep = (k0 + 2 * e < left ? 0xffffu : 0u) |
-                                      (k0 + 2 * e + 1 < left ? 0xffff0000u : 0u);
+            for (int i = 0; i < 2 * NT; ++i) f.w[i][e] &= keep;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) f.w[s][i][e] &= keep;
-#pragma unroll
-                for (int j = 0; j < MT; ++j) f.x[s][j][e] &= keep;
-            }
+            for (int j = 0; j < 2 * MT; ++j) f.x[j][e] &= keep;
         }
     };
     // The products of one half stage with the reads of the next half (and, with
@@ -450,8 +443,8 @@ linear_tile_kernel(TileArgs a) {
 
     // A wave's sums pass through its own part of LDS, 64 rows of W at a time, so
     // that 8 lanes (4 when gated) end up with neighbouring outputs of one row and
-    // the stores fill whole lines.  Lane l of an accumulator holds row l % 32 of x
-    // and 4 rows of W, from 8 v + 4 (l / 32) on: a 16-byte chunk, at chunk
+    // the stores fill whole lines.  Lane l of an accumulator holds row l % 16 of its
+    // 16 rows of x and 4 rows of W, from 4 (l / 16) on: a 16-byte chunk, at chunk
     // q ^ (row % 16) of the row's 256 bytes.
     char *mine = lds + wave * (MT * 32 * 256);
 #pragma unroll 1
@@ -460,16 +453,11 @@ linear_tile_kernel(TileArgs a) {
         for (int hh = 0; hh < NT / 2; ++hh) {
             if (hh != h) continue;
 #pragma unroll
-            for (int j = 0; j < MT; ++j)
+            for (int j = 0; j < 2 * MT; ++j)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        const f32x16_t &t = acc[2 * hh + i][j];
-                        *reinterpret_cast<float4_t *>(mine + (j * 32 + fr) * 256 +
-                                                      ((8 * i + 2 * v + fg) ^ (fr & 15)) * 16) =
-                            float4_t{t[4 * v], t[4 * v + 1], t[4 * v + 2], t[4 * v + 3]};
-                    }
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<float4_t *>(mine + (j * 16 + fr) * 256 + ((4 * i + fg) ^ fr) * 16) =
+                        acc[4 * hh + i][j];
         }
         wave_lds_fence();
         const int r0 = (wn * NT + 2 * h) * 32;  // the tile's rows of W from here on
