@@ -11,7 +11,7 @@ namespace tecoops {
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeMaxTopK = 32;
 constexpr int kMoeMaxWidth = 1 << 16;  // the threads of every grid stay below 2^32
-constexpr int kMoeFew = 8;       // tokens whose second product sums over the experts
+constexpr int kMoeFew = 8;  // tokens that route, and sum over the experts, within the products
 constexpr int kMoeSlice = 512;  // tokens routed together; more run slice by slice
 
 // Rows of x staged for an item: the tokens of an expert go through in chunks of
@@ -53,8 +53,7 @@ inline MoeSpace moe_space(int tokens, int hidden, int inter, int experts, int to
     s.token_at = take(4 * static_cast<size_t>(s.pairs));
     s.slot_at = take(4 * static_cast<size_t>(s.pairs));
     s.weight_at = take(4 * static_cast<size_t>(s.pairs));
-    s.cols_at = take(slice <= kMoeFew || tokens % kMoeSlice != 0
-                         ? 8 * static_cast<size_t>(s.items) * kMoeFew : 0);
+    s.cols_at = take(slice <= kMoeFew ? 8 * static_cast<size_t>(s.items) * kMoeFew : 0);
     s.h_at = take(2 * static_cast<size_t>(s.pairs) * s.h_stride);
     s.part_at = take(4 * static_cast<size_t>(s.pairs) * hidden);
     s.bytes = at;

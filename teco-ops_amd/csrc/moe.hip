@@ -183,17 +183,26 @@ __device__ __forceinline__ void group(const MoeArgs &a, Pair &&pair) {
     }
 }
 
-// Few tokens: a wave each, and the groups in the same launch.  An expert is one
-// item, as no token has it twice: pair p's place is the number of pairs before it
-// in the order of experts, then of pairs, counted over all of them.
+// Few tokens: groups without atomics, in one workgroup of their own or in every
+// workgroup of the first product, whose first one then also writes what the later
+// kernels read.  An expert is one item, as no token has it twice: pair p's place is
+// the number of pairs before it in the order of experts, then of pairs, counted
+// over all of them.
 constexpr int kFewPairs = tecoops::kMoeFew * tecoops::kMoeMaxTopK;
 
+struct FewItem {
+    int items, expert, first, count;
+    int token[tecoops::kMoeFew];  // of its pairs
+};
+
+// Fills `out` (shared) for `item`; `lds` is scratch, free again at the return.
 template <typename T, int R>
-__global__ void __launch_bounds__(tecoops::kMoeFew * 64) moe_route_kernel(MoeArgs a) {
-    __shared__ int id[kFewPairs], fresh[kFewPairs], col_pair[kFewPairs * tecoops::kMoeFew];
-    __shared__ float weight[kFewPairs], col_weight[kFewPairs * tecoops::kMoeFew];
-    const int me = threadIdx.x, lane = me & 63, t = me >> 6;
-    if (t < a.tokens) {
+__device__ __forceinline__ void route_few(const MoeArgs &a, char *lds, int item, FewItem *out) {
+    int *const id = reinterpret_cast<int *>(lds), *const fresh = id + kFewPairs;
+    float *const weight = reinterpret_cast<float *>(fresh + kFewPairs);
+    const int me = threadIdx.x, lane = me & 63;
+    const bool store = blockIdx.x == 0;
+    for (int t = me >> 6; t < a.tokens; t += blockDim.x >> 6) {
         int e;
         float w;
         choose<T, R>(a, t, lane, e, w);
@@ -201,11 +210,11 @@ __global__ void __launch_bounds__(tecoops::kMoeFew * 64) moe_route_kernel(MoeArg
             const int p = t * a.top_k + lane;
             id[p] = e;
             weight[p] = w;
-            store_choice(a, p, e, w);
+            if (store) store_choice(a, p, e, w);
         }
     }
     __syncthreads();
-    const int pairs = a.tokens * a.top_k;
+    const int pairs = a.tokens * a.top_k;  // at most blockDim.x
     const int e = me < pairs ? id[me] : -1;
     int before = 0, same = 0, count = 0;
 #pragma unroll 8
@@ -216,30 +225,45 @@ __global__ void __launch_bounds__(tecoops::kMoeFew * 64) moe_route_kernel(MoeArg
         count += o == e;
     }
     if (me < pairs) fresh[me] = e >= 0 && same == 0 ? e : -1;
-    for (int i = me; i < pairs * tecoops::kMoeFew; i += tecoops::kMoeFew * 64) col_pair[i] = -1;
     __syncthreads();
-    int item = 0, total = 0;  // experts below e, and all
+    int mine = 0, total = 0;  // experts below e, and all
 #pragma unroll 8
     for (int q = 0; q < pairs; ++q) {
         const int o = fresh[q];
-        item += o >= 0 && o < e;
+        mine += o >= 0 && o < e;
         total += o >= 0;
     }
-    if (e >= 0) {
-        const int at = before + same, token = me / a.top_k;
-        a.token[at] = token;
-        a.slot[at] = me;
-        a.weight[at] = weight[me];
-        if (same == 0) a.items[item] = make_int4(e, before, count, 0);
-        col_pair[item * tecoops::kMoeFew + token] = at;
-        col_weight[item * tecoops::kMoeFew + token] = weight[me];
+    if (me == 0) out->items = total;
+    if (e >= 0 && mine == item) {
+        out->token[same] = me / a.top_k;
+        if (same == 0) {
+            out->expert = e;
+            out->first = before;
+            out->count = count;
+        }
     }
-    if (me == 0) *a.n_items = total;
+    if (store) {
+        if (me == 0) *a.n_items = total;
+        for (int i = me; i < total * tecoops::kMoeFew; i += blockDim.x) a.col_pair[i] = -1;
+        __syncthreads();
+        if (e >= 0) {
+            const int at = before + same, token = me / a.top_k;
+            a.token[at] = token;
+            a.slot[at] = me;
+            a.weight[at] = weight[me];
+            if (same == 0) a.items[mine] = make_int4(e, before, count, 0);
+            a.col_pair[mine * tecoops::kMoeFew + token] = at;
+            a.col_weight[mine * tecoops::kMoeFew + token] = weight[me];
+        }
+    }
     __syncthreads();
-    for (int i = me; i < total * tecoops::kMoeFew; i += tecoops::kMoeFew * 64) {
-        a.col_pair[i] = col_pair[i];
-        a.col_weight[i] = col_pair[i] >= 0 ? col_weight[i] : 0.0f;
-    }
+}
+
+template <typename T, int R>
+__global__ void __launch_bounds__(tecoops::kMoeFew * 64) moe_route_kernel(MoeArgs a) {
+    __shared__ int scratch[3 * kFewPairs];
+    __shared__ FewItem none;
+    route_few<T, R>(a, reinterpret_cast<char *>(scratch), -1, &none);
 }
 
 // More tokens: a wave each over the chip, then one workgroup for the groups.
@@ -264,13 +288,24 @@ __global__ void __launch_bounds__(1024) moe_group_kernel(MoeArgs a) {
     });
 }
 
-template <typename T, int R>
-void launch_route(const MoeArgs &a, hipStream_t s) {
-    if (a.tokens <= tecoops::kMoeFew) {
-        hipLaunchKernelGGL((moe_route_kernel<T, R>), dim3(1), dim3(tecoops::kMoeFew * 64), 0, s, a);
+// Whether there is a table of the tokens' pairs: few tokens, rows in whole words.
+bool few_tokens(const MoeArgs &a, bool copy) { return copy && a.tokens <= tecoops::kMoeFew && a.rows <= 8; }
+
+template <typename T>
+void launch_route(const MoeArgs &a, bool copy, hipStream_t s) {
+    if (few_tokens(a, copy)) {
+        if (a.experts <= 128)
+            hipLaunchKernelGGL((moe_route_kernel<T, 2>), dim3(1), dim3(tecoops::kMoeFew * 64), 0, s, a);
+        else
+            hipLaunchKernelGGL((moe_route_kernel<T, tecoops::kMoeMaxExperts / 64>), dim3(1),
+                               dim3(tecoops::kMoeFew * 64), 0, s, a);
         return;
     }
-    hipLaunchKernelGGL((moe_choose_kernel<T, R>), dim3(tecoops::ceil_div(a.tokens, 4)), dim3(256), 0, s, a);
+    const dim3 grid(tecoops::ceil_div(a.tokens, 4));
+    if (a.experts <= 64) hipLaunchKernelGGL((moe_choose_kernel<T, 1>), grid, dim3(256), 0, s, a);
+    else if (a.experts <= 128) hipLaunchKernelGGL((moe_choose_kernel<T, 2>), grid, dim3(256), 0, s, a);
+    else if (a.experts <= 256) hipLaunchKernelGGL((moe_choose_kernel<T, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((moe_choose_kernel<T, tecoops::kMoeMaxExperts / 64>), grid, dim3(256), 0, s, a);
     hipLaunchKernelGGL(moe_group_kernel, dim3(1), dim3(1024), 0, s, a);
 }
 
@@ -278,13 +313,20 @@ void launch_route(const MoeArgs &a, hipStream_t s) {
 
 // IN: rows of W_in, 8 gate rows and the 8 up rows of the same outputs in each
 // tile of 16; OUT: rows of W_out.
-template <typename T, int XR, int WR, int RS, int KS, bool OUT>
+// R > 0: few tokens, routed here (R logits per lane).
+template <typename T, int XR, int WR, int RS, int KS, bool OUT, int R>
 __global__ void __launch_bounds__(RS * KS * 64) moe_product_kernel(MoeArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ FewItem few;
     const int item = blockIdx.x / a.units, unit = blockIdx.x - item * a.units;
-    if (item >= *a.n_items) return;
-    const int4 it = a.items[item];
-    const int expert = it.x, first = it.y, count = it.z;
+    if constexpr (R > 0) {
+        static_assert(RS * KS * 64 >= kFewPairs, "a thread per pair");
+        route_few<T, R>(a, lds, item, &few);
+    }
+    if (item >= (R > 0 ? few.items : *a.n_items)) return;
+    const int4 it = R > 0 ? make_int4(few.expert, few.first, few.count, 0) : a.items[item];
+    const int expert = __builtin_amdgcn_readfirstlane(it.x), first = __builtin_amdgcn_readfirstlane(it.y);
+    const int count = __builtin_amdgcn_readfirstlane(it.z);
     const int g = (threadIdx.x & 63) >> 4;
     const int K = OUT ? a.inter : a.hidden, N = OUT ? a.hidden : a.inter;
     const char *w = (OUT ? a.w_out : a.w_in) +
@@ -296,9 +338,9 @@ __global__ void __launch_bounds__(RS * KS * 64) moe_product_kernel(MoeArgs a) {
         return w + static_cast<long long>(from) * K * 2;
     };
     const auto x_row = [&](int r) {
-        const int p = first + min(r, count - 1);
-        return OUT ? reinterpret_cast<const char *>(a.h + p * a.h_stride)
-                   : a.x + a.token[p] * a.x_stride;
+        const int i = min(r, count - 1);
+        return OUT ? reinterpret_cast<const char *>(a.h + (first + i) * a.h_stride)
+                   : a.x + (R > 0 ? few.token[i] : a.token[first + i]) * a.x_stride;
     };
     const auto put = [&](int r, int col, f32x4_t s) {
         if constexpr (OUT) {
@@ -522,15 +564,36 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a) {
     }
 }
 
-template <typename T, int XR, int WR, int RS, int KS, bool OUT>
-bool launch(MoeArgs a, int items, hipStream_t s) {
+template <typename T, int XR, int WR, int RS, int KS, bool OUT, int R>
+bool launch_as(MoeArgs a, int items, hipStream_t s) {
     using S = Shape<false, XR, WR, RS, KS>;
     static_assert(S::D >= 2, "two stages fit in LDS");
-    auto *kern = &moe_product_kernel<T, XR, WR, RS, KS, OUT>;
+    auto *kern = &moe_product_kernel<T, XR, WR, RS, KS, OUT, R>;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), S::LDS)) return false;
     a.units = static_cast<int>(tecoops::ceil_div(OUT ? a.hidden : 2LL * a.inter, RS * WR));
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(a.units) * items), dim3(S::NW * 64), S::LDS, s, a);
     return true;
+}
+
+// Whether the tokens are routed within the first product: it spares a launch and
+// its wait, 6 us, for 2 to 5 us at the start of every workgroup, so only where each
+// CU has one of them (2 tokens, 1 of 128 experts of [1792, 672]: 16.7 us with a
+// launch, 13.5 within; 6 tokens, 6 of 60 of [640, 9920], many to a CU: 219 and 397).
+bool routes_within(const MoeArgs &a, int items, bool copy) {
+    const int cus = tecoops::device_cus();
+    return few_tokens(a, copy) &&
+           static_cast<long long>(items) * tecoops::ceil_div(2LL * a.inter,
+               tecoops::moe_wrows(2 * a.inter, a.tokens, a.top_k, a.experts, a.rows, cus)) <= cus;
+}
+
+template <typename T, int XR, int WR, int RS, int KS, bool OUT>
+bool launch(const MoeArgs &a, int items, hipStream_t s) {
+    if constexpr (!OUT && XR <= 8)
+        if (routes_within(a, items, true))
+            return a.experts <= 128
+                       ? launch_as<T, XR, WR, RS, KS, OUT, 2>(a, items, s)
+                       : launch_as<T, XR, WR, RS, KS, OUT, tecoops::kMoeMaxExperts / 64>(a, items, s);
+    return launch_as<T, XR, WR, RS, KS, OUT, 0>(a, items, s);
 }
 
 template <typename T, int XR, bool OUT>
@@ -563,14 +626,13 @@ bool launch_product(const MoeArgs &a, int items, bool copy, hipStream_t s) {
 
 template <typename T>
 tecoopsStatus_t run_slice(const MoeArgs &a, int items, bool copy, hipStream_t s) {
-    if (a.experts <= 64) launch_route<T, 1>(a, s);
-    else if (a.experts <= 128) launch_route<T, 2>(a, s);
-    else if (a.experts <= 256) launch_route<T, 4>(a, s);
-    else launch_route<T, tecoops::kMoeMaxExperts / 64>(a, s);
-    TECO_CHECK_LAUNCH("moe_layer");
+    if (!routes_within(a, items, copy)) {
+        launch_route<T>(a, copy, s);
+        TECO_CHECK_LAUNCH("moe_layer");
+    }
     if (!launch_product<T, false>(a, items, copy, s)) return TECOOPS_STATUS_INTERNAL_ERROR;
     TECO_CHECK_LAUNCH("moe_layer");
-    if (copy && tecoops::moe_out_few(a.tokens, a.hidden, a.inter, a.experts, a.top_k, tecoops::device_cus())) {
+    if (few_tokens(a, copy) && tecoops::moe_out_few(a.tokens, a.hidden, a.inter, a.experts, a.top_k, tecoops::device_cus())) {
         if (!run_out_few<T>(a, s)) return TECOOPS_STATUS_INTERNAL_ERROR;
         TECO_CHECK_LAUNCH("moe_layer");
         return TECOOPS_STATUS_SUCCESS;

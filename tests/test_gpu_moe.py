@@ -104,7 +104,9 @@ SHAPES = [(1, 64, 32, 4, 2, 0), (1, 8, 8, 1, 1, 0), (1, 512, 1000, 8, 8, 0), (3,
           (40, 128, 64, 64, 8, 5), (64, 520, 264, 8, 2, 0), (100, 256, 128, 4, 4, 0),
           (300, 64, 96, 16, 8, 7), (512, 32, 16, 2, 1, 0), (513, 48, 24, 8, 2, 0),
           (1100, 16, 40, 5, 1, 30), (2, 70, 33, 5, 2, 0), (30, 9, 7, 3, 2, 1), (600, 24, 17, 4, 1, 0),
-          (64, 8, 8, 1, 1, 0), (1, 4096, 16, 4, 1, 0), (20, 16, 4096, 160, 8, 0)]
+          (64, 8, 8, 1, 1, 0), (1, 4096, 16, 4, 1, 0), (20, 16, 4096, 160, 8, 0),
+          (4, 64, 32, 200, 8, 1), (8, 256, 2048, 1000, 8, 0), (2, 2048, 264, 160, 4, 0),
+          (6, 32, 3000, 64, 8, 1), (8, 40, 64, 40, 32, 0), (7, 4104, 136, 9, 4, 0)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
