@@ -576,8 +576,8 @@ bool launch_as(MoeArgs a, int items, hipStream_t s) {
 }
 
 // Whether the tokens are routed within the first product: it spares a launch and
-// its wait, 6 us, for 2 to 5 us at the start of every workgroup, so only where each
-// CU has one of them (2 tokens, 1 of 128 experts of [1792, 672]: 16.7 us with a
+// its wait, but every workgroup does it again at its start, so only where each CU
+// has one of them (2 tokens, 1 of 128 experts of [1792, 672]: 16.7 us with a
 // launch, 13.5 within; 6 tokens, 6 of 60 of [640, 9920], many to a CU: 219 and 397).
 bool routes_within(const MoeArgs &a, int items, bool copy) {
     const int cus = tecoops::device_cus();
