@@ -395,9 +395,9 @@ tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, int gated, si
  * zero for a token without experts; out must not overlap an input.  topk_ids
  * int32 and topk_weights float [tokens, top_k] are written unless NULL, best
  * first, -1 and 0 where there is none.  Every expert's weights are read once
- * for all of its tokens (of each 512 tokens, up to 64 at a time).  Up to 1024
- * experts, top_k 32, hidden and inter 2^16; hidden, inter and x_stride
- * multiples of 8 and 16-byte aligned tensors are fast; tokens = 0 is done
+ * for all of its tokens (of each 512 tokens, up to 64 at a time).  Up to 2^30
+ * tokens, 1024 experts, top_k 32, hidden and inter 2^16; hidden, inter and
+ * x_stride multiples of 8 and 16-byte aligned tensors are fast; tokens = 0 is done
  * without a launch.
  * workspace: tecoopsGetMoeLayerWorkspaceSize() bytes, 16-byte aligned; NULL
  * uses the handle's scratch (NOT_SUPPORTED on a stream under capture). */

@@ -10,6 +10,7 @@ namespace tecoops {
 
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeMaxTopK = 32;
+constexpr int kMoeMaxTokens = 1 << 30;  // slices are counted in 32 bits
 constexpr int kMoeMaxWidth = 1 << 16;  // the threads of every grid stay below 2^32
 constexpr int kMoeFew = 8;  // tokens that route, and sum over the experts, within the products
 constexpr int kMoeSlice = 512;  // tokens routed together; more run slice by slice

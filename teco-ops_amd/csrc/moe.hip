@@ -648,7 +648,7 @@ tecoopsStatus_t run_slice(const MoeArgs &a, int items, bool copy, hipStream_t s)
 tecoopsStatus_t check_sizes(int tokens, int hidden, int inter, int experts, int top_k) {
     if (tokens < 0 || hidden <= 0 || inter <= 0 || experts <= 0 || top_k <= 0 || top_k > experts)
         return TECOOPS_STATUS_BAD_PARAM;
-    if (experts > tecoops::kMoeMaxExperts || top_k > tecoops::kMoeMaxTopK ||
+    if (tokens > tecoops::kMoeMaxTokens || experts > tecoops::kMoeMaxExperts || top_k > tecoops::kMoeMaxTopK ||
         hidden > tecoops::kMoeMaxWidth || inter > tecoops::kMoeMaxWidth)
         return TECOOPS_STATUS_NOT_SUPPORTED;
     return TECOOPS_STATUS_SUCCESS;

@@ -168,6 +168,8 @@ def test_moe_refusals(handle):
     assert call(E=1025) == NOT_SUP and call(E=64, k=33) == NOT_SUP
     assert call(H=(1 << 16) + 8, xs=1 << 21) == NOT_SUP and call(I=(1 << 16) + 8) == NOT_SUP
     assert call(T=0) == OK  # no launch
+    # the next slice's first token would pass 2^31
+    assert call(T=(1 << 31) - 1, H=1, I=1, E=1, k=1) == NOT_SUP and call(T=(1 << 30) + 1) == NOT_SUP
     g = _lib.lib().tecoopsGetMoeLayerWorkspaceSize
     size = ctypes.c_size_t(1)
     assert g(2, 64, 32, 8, 2, None) == BAD and g(2, 64, 32, 8, 9, ctypes.byref(size)) == BAD
