@@ -385,8 +385,8 @@ tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, int gated, si
  *   the top_k experts e_j of the largest logits (ties to the lowest index; -inf
  *   and NaN are never chosen, so a masked token may have fewer or none),
  *   w_j = p[e_j], divided by their sum when renormalize != 0,
- *   h_j = act(x[t] Wg[e_j]^T) * (x[t] Wu[e_j]^T), rounded to dataType (fp16:
- *         infinite from 65520 on),
+ *   h_j = act(x[t] Wg[e_j]^T) * (x[t] Wu[e_j]^T), held to 16 bits or more of
+ *         its mantissa (fp16 22; there infinite from 65520 * 256 on),
  *   out[t] = sum_j w_j (h_j W_out[e_j]^T), fp32 sums, one rounding.
  * x [tokens, hidden] with row stride x_stride (elements); w_in [experts,
  * 2 inter, hidden] packed, the inter gate rows Wg of an expert before its up

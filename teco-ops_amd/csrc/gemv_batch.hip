@@ -80,7 +80,7 @@ gemv_batch_kernel(const char *__restrict__ W, const uint16_t *__restrict__ scale
                 if (n + v < N) dst[v] = Cvt<T>::from(s[v]);
         }
     };
-    tecoops::stream::product<T, I8, XR, WR, RS, KS>(lds, K, blockIdx.x, w_row, x_row, put);
+    tecoops::stream::product<T, I8 ? kInt8 : kPlain, XR, WR, RS, KS>(lds, K, blockIdx.x, w_row, x_row, put);
 }
 
 // A product's operands; N counts the rows of W.
@@ -95,7 +95,7 @@ struct Product {
 
 template <typename T, bool I8, int XR, int WR, int RS, int KS, bool EPI>
 bool launch(const Product &p, int B) {
-    using S = Shape<I8, XR, WR, RS, KS>;
+    using S = Shape<I8 ? kInt8 : kPlain, XR, WR, RS, KS>;
     static_assert(S::D >= 2, "two stages fit in LDS");
     auto *kern = &gemv_batch_kernel<T, I8, XR, WR, RS, KS, EPI>;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), S::LDS)) return false;

@@ -84,15 +84,24 @@ __device__ __forceinline__ void widen_i8x16(u32x4_t q, u32x4_t &lo8, u32x4_t &hi
     }
 }
 
+// What W and x hold: both 16-bit values; int8 W, widened to fp16; or 16-bit W and
+// x as sums of two 16-bit terms, hi + kLow * lo, whose row holds 8 his, then the 8
+// los of the same values, and so on.
+enum Operands { kPlain, kInt8, kTwoTerms };
+
+// What the second term counts.  In fp16 it is kept 2^11 times its size, so that it
+// loses no bits to the type's small exponents.
+template <typename T> constexpr float kLow = __is_same(T, f16) ? 0x1p-11f : 1.0f;
+
 // Sizes of a workgroup's stages.  XR: rows of x staged; WR: rows of W per wave.
-template <bool I8, int XR, int WR, int RS, int KS>
+template <Operands OP, int XR, int WR, int RS, int KS>
 struct Shape {
     static constexpr int NW = RS * KS;
     static constexpr int CT = (XR + 15) / 16;      // column tiles of 16
     static constexpr int RT = (WR + 15) / 16;      // row tiles of 16
     static constexpr int WB = WR * 256;            // W bytes of a wave's stage
     static constexpr int WC = WR / 4;              // W copies of a wave and stage
-    static constexpr int XROW = I8 ? 512 : 256;    // x bytes of a row and stage
+    static constexpr int XROW = OP == kPlain ? 256 : 512;  // x bytes of a row and stage
     static constexpr int XB = XR * XROW;           // x bytes of a K part's stage
     static constexpr int SB = NW * WB + KS * XB;   // bytes of a stage
     static constexpr int XN = XB / 1024;           // x copies of a K part and stage
@@ -118,18 +127,19 @@ struct Shape {
 // With RS > 1 one barrier per stage publishes the x copies of the other waves
 // and, since every wave passes it after reading stage i - 1, frees the slot
 // the next copies go to.  With RS = 1 a wave reads only what it copied.
-template <typename T, bool I8, int XR, int WR, int RS, int KS, typename WRow, typename XRow,
+template <typename T, Operands OP, int XR, int WR, int RS, int KS, typename WRow, typename XRow,
           typename Put>
 __device__ __forceinline__ void product(char *lds, int K, int unit, WRow &&w_row, XRow &&x_row,
                                         Put &&put) {
-    using S = Shape<I8, XR, WR, RS, KS>;
+    using S = Shape<OP, XR, WR, RS, KS>;
+    constexpr bool I8 = OP == kInt8, TWO = OP == kTwoTerms;
     constexpr int NW = S::NW, CT = S::CT, RT = S::RT, D = S::D, WC = S::WC, XC = S::XC, PER = S::PER;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rs = wave % RS, kp = wave / RS;
     const int g = lane >> 4, c = lane & 15;
-    const int kw = I8 ? K / 16 : K / 8, kx = K / 8;  // 16-byte chunks of a row of W / x
-    constexpr int XCH = I8 ? 32 : 16;                // x chunks of a row and stage
+    const int kw = I8 ? K / 16 : K / 8, kx = TWO ? K / 4 : K / 8;  // 16-byte chunks of a row of W / x
+    constexpr int XCH = S::XROW / 16;                // x chunks of a row and stage
     const int nst = ((kw + 15) / 16 + KS - 1) / KS;  // stages of a K part
     // W copy m: rows 4m + lane / 16, chunk slot lane % 16
     const char *wsrc[WC];
@@ -152,11 +162,14 @@ __device__ __forceinline__ void product(char *lds, int K, int unit, WRow &&w_row
         xch[m] = kp * nst * XCH + ((lane % XCH) ^ (row & 15));
         xdst[m] = q * 1024;
     }
-    f32x4_t acc[RT][CT];
+    f32x4_t acc[RT][CT], low[TWO ? RT : 1][TWO ? CT : 1];  // low: of the second terms
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int t = 0; t < CT; ++t) acc[r][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < CT; ++t) {
+            acc[r][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (TWO) low[r][t] = acc[r][t];
+        }
     // Workgroups start their sweep of K at different stages, so that the
     // requests in flight spread over the HBM channels (rows a power of two
     // bytes apart start on the same one).  The step is odd: nst mostly is a
@@ -208,7 +221,7 @@ __device__ __forceinline__ void product(char *lds, int K, int unit, WRow &&w_row
 #pragma unroll
             for (int r = 0; r < RT; ++r)
                 a[r] = *reinterpret_cast<const u32x4_t *>(wl + so + r * 4096 + 16 * ((4 * u + g) ^ wsw));
-            if constexpr (I8) {
+            if constexpr (OP != kPlain) {
                 u32x4_t b0[CT], b1[CT];
 #pragma unroll
                 for (int t = 0; t < CT; ++t) {
@@ -218,12 +231,13 @@ __device__ __forceinline__ void product(char *lds, int K, int unit, WRow &&w_row
                 }
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    u32x4_t a0, a1;
-                    widen_i8x16(a[r], a0, a1);
+                    u32x4_t a0 = a[r], a1;
+                    if constexpr (I8) widen_i8x16(a[r], a0, a1);
 #pragma unroll
                     for (int t = 0; t < CT; ++t) {
                         acc[r][t] = Mma16<T>::run(a0, b0[t], acc[r][t]);
-                        acc[r][t] = Mma16<T>::run(a1, b1[t], acc[r][t]);
+                        if constexpr (TWO) low[r][t] = Mma16<T>::run(a0, b1[t], low[r][t]);
+                        else acc[r][t] = Mma16<T>::run(a1, b1[t], acc[r][t]);
                     }
                 }
             } else {
@@ -241,6 +255,13 @@ __device__ __forceinline__ void product(char *lds, int K, int unit, WRow &&w_row
         // the reads of stage i are done before its slot is copied over
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
+    if constexpr (TWO)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) acc[r][t][v] = fmaf(kLow<T>, low[r][t][v], acc[r][t][v]);
     if constexpr (KS > 1) {
         __syncthreads();  // every wave is done with the ring
         float *red = reinterpret_cast<float *>(lds);

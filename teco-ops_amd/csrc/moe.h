@@ -30,7 +30,7 @@ inline int moe_rows(int tokens, int top_k, int experts) {
 struct MoeSpace {
     int pairs, items;      // most (token, expert) pairs and items of a slice
     int rows;              // of x per item
-    long long h_stride;    // elements between the rows of h
+    long long h_stride;    // values between the rows of h, 4 bytes each
     size_t items_at, ids_at, token_at, slot_at, weight_at, cols_at, h_at, part_at;  // bytes
     size_t bytes;
 };
@@ -55,7 +55,7 @@ inline MoeSpace moe_space(int tokens, int hidden, int inter, int experts, int to
     s.slot_at = take(4 * static_cast<size_t>(s.pairs));
     s.weight_at = take(4 * static_cast<size_t>(s.pairs));
     s.cols_at = take(slice <= kMoeFew ? 8 * static_cast<size_t>(s.items) * kMoeFew : 0);
-    s.h_at = take(2 * static_cast<size_t>(s.pairs) * s.h_stride);
+    s.h_at = take(4 * static_cast<size_t>(s.pairs) * s.h_stride);
     s.part_at = take(4 * static_cast<size_t>(s.pairs) * hidden);
     s.bytes = at;
     return s;
@@ -81,7 +81,8 @@ inline bool moe_out_few(int tokens, int hidden, int inter, int experts, int top_
 }
 
 // Rows of W per workgroup: the size whose busiest CU copies the fewest bytes of
-// W and x, with as many items as tokens spread evenly would make.
+// W and x (`rows` rows of 16-bit values, or twice as many of two-term ones), with as
+// many items as tokens spread evenly would make.
 inline int moe_wrows(int wrows, int tokens, int top_k, int experts, int rows, int cus) {
     const double items = moe_reached(tokens, top_k, experts);
     int best = 0;

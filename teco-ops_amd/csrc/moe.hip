@@ -2,7 +2,7 @@
 //
 //   p = softmax(router_logits[t]);  e_0 .. e_{k-1}: the top k experts
 //   w_j = p[e_j]  (/ sum_j p[e_j] when renormalised)
-//   h_j = act(x W_in[e_j][:I]^T) * (x W_in[e_j][I:]^T)       rounded to T
+//   h_j = act(x W_in[e_j][:I]^T) * (x W_in[e_j][I:]^T)
 //   out[t] = T( sum_j w_j (h_j W_out[e_j]^T) )
 //
 // What bounds it is reading the chosen experts' weights, 3 H I values each.
@@ -13,6 +13,13 @@
 //   in       per item and block of rows of W_in: h of its pairs
 //   out      per item and block of rows of W_out: w_j (h_j W_out^T) in fp32
 //   combine  the k parts of each token, added in the order of j
+// h is a matrix operand of the second product, where one 16-bit value in its place
+// would cost as much as the result's own rounding (rms against 64 bits 0.0023 in
+// bf16 and 0.0003 in fp16, for 0.0016 and 0.0002).  It is therefore the sum of two
+// (`two_terms`), which the product takes in turn: 4 bytes a value instead of 2, and
+// twice the matrix instructions, of which the stream of W leaves enough (256 tokens, 8
+// of 128 experts of [4096, 1024] bf16: 559 us with one value, 574 with two; 1 token, 2
+// of 8 of [4096, 14336] 111 either way).
 // No sum depends on the order in which workgroups run: a pair's place in its
 // group decides only which column of an MFMA it is.
 #include "moe.h"
@@ -43,8 +50,8 @@ struct MoeArgs {
     int *ids;              // [tokens, top_k], -1: none
     int *token, *slot;     // of a pair in the experts' order: its row of x, t * top_k + j
     float *weight;
-    uint16_t *h;           // [pairs, h_stride]
-    long long h_stride;
+    uint16_t *h;           // [pairs, h_stride] in two terms; fp32 for the scalar kernels
+    long long h_stride;    // values
     float *part;           // [tokens, top_k, hidden]
     // few tokens: of item i and token t, the pair or -1 and its weight
     int *col_pair;         // [items, kMoeFew]
@@ -311,6 +318,21 @@ void launch_route(const MoeArgs &a, bool copy, hipStream_t s) {
 
 // ------------------------------------------------------------------ products
 
+// h = kUnit (hi + kLow lo), with 16 bits of it in bf16 and 22 in fp16.  kUnit moves
+// fp16's range to 65520 * 256 (beyond, hi is infinite and lo is 0) and its smallest
+// step, that of lo, to 2^-27.  (An infinite weight gives NaN where lo is 0.)
+template <typename T> constexpr float kUnit = __is_same(T, f16) ? 256.0f : 1.0f;
+
+template <typename T>
+__device__ __forceinline__ void two_terms(float v0, float v1, uint32_t &hi2, uint32_t &lo2) {
+    v0 *= 1.0f / kUnit<T>;
+    v1 *= 1.0f / kUnit<T>;
+    hi2 = round2<T>(v0, v1);
+    const float h0 = lo<T>(hi2), h1 = hi<T>(hi2);
+    lo2 = round2<T>(fabsf(h0) < INFINITY ? (v0 - h0) * (1.0f / kLow<T>) : 0.0f,
+                    fabsf(h1) < INFINITY ? (v1 - h1) * (1.0f / kLow<T>) : 0.0f);
+}
+
 // IN: rows of W_in, 8 gate rows and the 8 up rows of the same outputs in each
 // tile of 16; OUT: rows of W_out.
 // R > 0: few tokens, routed here (R logits per lane).
@@ -339,14 +361,14 @@ __global__ void __launch_bounds__(RS * KS * 64) moe_product_kernel(MoeArgs a) {
     };
     const auto x_row = [&](int r) {
         const int i = min(r, count - 1);
-        return OUT ? reinterpret_cast<const char *>(a.h + (first + i) * a.h_stride)
+        return OUT ? reinterpret_cast<const char *>(a.h) + (first + i) * a.h_stride * 4
                    : a.x + (R > 0 ? few.token[i] : a.token[first + i]) * a.x_stride;
     };
     const auto put = [&](int r, int col, f32x4_t s) {
         if constexpr (OUT) {
             const int n = n0 + r;
             if (col >= count || n >= N) return;  // N % 8 == 0: four at a time
-            const float wt = a.weight[first + col];
+            const float wt = kUnit<T> * a.weight[first + col];
             *reinterpret_cast<f32x4_t *>(a.part + static_cast<long long>(a.slot[first + col]) * N + n) =
                 f32x4_t{wt * s[0], wt * s[1], wt * s[2], wt * s[3]};
         } else {
@@ -355,26 +377,28 @@ __global__ void __launch_bounds__(RS * KS * 64) moe_product_kernel(MoeArgs a) {
             for (int v = 0; v < 4; ++v) u[v] = from_upper_half(s[v]);
             const int n = n0 + (r >> 4) * 8 + (r & 7);
             if (col >= count || g >= 2 || n >= N) return;
-            // h is rounded to T, the second product's operand type
-            *reinterpret_cast<uint2 *>(a.h + (first + col) * a.h_stride + n) =
-                make_uint2(pack<T>(activate(s[0], a.act) * u[0], activate(s[1], a.act) * u[1]),
-                           pack<T>(activate(s[2], a.act) * u[2], activate(s[3], a.act) * u[3]));
+            uint2 high, low;
+            two_terms<T>(activate(s[0], a.act) * u[0], activate(s[1], a.act) * u[1], high.x, low.x);
+            two_terms<T>(activate(s[2], a.act) * u[2], activate(s[3], a.act) * u[3], high.y, low.y);
+            uint16_t *dst = a.h + (first + col) * a.h_stride * 2 + n / 8 * 16 + n % 8;
+            *reinterpret_cast<uint2 *>(dst) = high;
+            *reinterpret_cast<uint2 *>(dst + 8) = low;
         }
     };
-    product<T, false, XR, WR, RS, KS>(lds, K, unit, w_row, x_row, put);
+    product<T, OUT ? kTwoTerms : kPlain, XR, WR, RS, KS>(lds, K, unit, w_row, x_row, put);
 }
 
 // Few tokens: the second product with the sum over the experts in it, straight to
-// out.  A workgroup has WR rows of every expert's W_out; its 8 waves share the
+// out.  A workgroup has WR rows of every expert's W_out; its KS waves share the
 // items' stages of K out evenly, one item after the other, in a ring of D stages
 // each.  The columns are the tokens; at the end of an item (or of a wave's share
 // of it) a column adds its sums with its routing weight, or nothing where the
 // token has not chosen the expert, whatever was multiplied there.
-template <typename T, int XR, int WR, int D>
-__global__ void __launch_bounds__(512) moe_out_few_kernel(MoeArgs a) {
-    constexpr int KS = 8, RT = (WR + 15) / 16, WC = WR / 4, XC = XR / 4, PER = WC + XC;
-    constexpr int SB = (WR + XR) * 256;
-    static_assert(RT == 1 && D >= 3 && (D - 2) * PER < 64, "one row tile, vmcnt");
+template <typename T, int XR, int WR, int KS, int D>
+__global__ void __launch_bounds__(KS * 64) moe_out_few_kernel(MoeArgs a) {
+    constexpr int RT = (WR + 15) / 16, WC = WR / 4, XC = XR / 2, PER = WC + XC;
+    constexpr int SB = WR * 256 + XR * 512;
+    static_assert(RT == 1 && D <= 4 && D >= 3 && (D - 2) * PER < 64, "one row tile, vmcnt");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int expert[kFewPairs];
     __shared__ uint16_t col_pair[kFewPairs * XR];
@@ -384,8 +408,8 @@ __global__ void __launch_bounds__(512) moe_out_few_kernel(MoeArgs a) {
     const int g = lane >> 4, c = lane & 15;
     const int n0 = blockIdx.x * WR;
     const int items = *a.n_items;
-    for (int i = threadIdx.x; i < items; i += 512) expert[i] = a.items[i].x;
-    for (int i = threadIdx.x; i < items * XR; i += 512) {
+    for (int i = threadIdx.x; i < items; i += KS * 64) expert[i] = a.items[i].x;
+    for (int i = threadIdx.x; i < items * XR; i += KS * 64) {
         const int at = i / XR * tecoops::kMoeFew + i % XR;
         const int p = a.col_pair[at];
         col_pair[i] = static_cast<uint16_t>(max(p, 0));  // any pair's row of h
@@ -407,10 +431,11 @@ __global__ void __launch_bounds__(512) moe_out_few_kernel(MoeArgs a) {
         char *dst = ring + lslot * SB;
 #pragma unroll
         for (int m = 0; m < XC; ++m) {
-            const int q = 16 * lst + ((lane & 15) ^ (4 * m + row));
-            const int p = col_pair[li * XR + 4 * m + row];
-            dma16<false>(q < kw ? static_cast<const void *>(reinterpret_cast<const char *>(a.h + p * a.h_stride) + 16 * q)
-                                : static_cast<const void *>(kZero16),
+            const int xr = 2 * m + (lane >> 5), q = 32 * lst + ((lane & 31) ^ xr);
+            const int p = col_pair[li * XR + xr];
+            dma16<false>(q < 2 * kw ? static_cast<const void *>(reinterpret_cast<const char *>(a.h) +
+                                                                p * a.h_stride * 4 + 16 * q)
+                                    : static_cast<const void *>(kZero16),
                          dst + WR * 256 + m * 1024);
         }
 #pragma unroll
@@ -428,7 +453,7 @@ __global__ void __launch_bounds__(512) moe_out_few_kernel(MoeArgs a) {
         lslot = lslot + 1 == D ? 0 : lslot + 1;
     };
     const int wc = WR < 16 ? c & 7 : c, xc = c & (XR - 1);
-    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f}, tot = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f}, low = acc, tot = acc;
     int ui = li, ust = lst, slot = 0;
 #pragma unroll
     for (int d = 0; d < D - 1; ++d)
@@ -439,17 +464,19 @@ __global__ void __launch_bounds__(512) moe_out_few_kernel(MoeArgs a) {
         else if (s + 1 < s1) wait_copies<PER>();
         else wait_copies<0>();
         if (s + D - 1 < s1) load();
-        const char *wl = ring + slot * SB + wc * 256, *xl = ring + slot * SB + WR * 256 + xc * 256;
+        const char *wl = ring + slot * SB + wc * 256, *xl = ring + slot * SB + WR * 256 + xc * 512;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            acc = Mma16<T>::run(*reinterpret_cast<const u32x4_t *>(wl + 16 * ((4 * u + g) ^ wc)),
-                                *reinterpret_cast<const u32x4_t *>(xl + 16 * ((4 * u + g) ^ xc)), acc);
+        for (int u = 0; u < 4; ++u) {
+            const u32x4_t w = *reinterpret_cast<const u32x4_t *>(wl + 16 * ((4 * u + g) ^ wc));
+            acc = Mma16<T>::run(w, *reinterpret_cast<const u32x4_t *>(xl + 16 * ((8 * u + 2 * g) ^ xc)), acc);
+            low = Mma16<T>::run(w, *reinterpret_cast<const u32x4_t *>(xl + 16 * ((8 * u + 2 * g + 1) ^ xc)), low);
+        }
         slot = slot + 1 == D ? 0 : slot + 1;
         if (++ust == spi || s + 1 == s1) {
-            const float wt = col_weight[ui * XR + xc];
+            const float wt = kUnit<T> * col_weight[ui * XR + xc];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) tot[v] += wt >= 0.0f ? wt * acc[v] : 0.0f;
-            acc = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int v = 0; v < 4; ++v) tot[v] += wt >= 0.0f ? wt * fmaf(kLow<T>, low[v], acc[v]) : 0.0f;
+            acc = low = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
             ust = 0;
             ++ui;
         }
@@ -478,12 +505,12 @@ __global__ void __launch_bounds__(512) moe_out_few_kernel(MoeArgs a) {
     }
 }
 
-template <typename T, int XR, int WR, int D>
+template <typename T, int XR, int WR, int KS, int D>
 bool launch_out_few(const MoeArgs &a, hipStream_t s) {
-    auto *kern = &moe_out_few_kernel<T, XR, WR, D>;
-    constexpr size_t lds = 8 * D * (WR + XR) * 256;
+    auto *kern = &moe_out_few_kernel<T, XR, WR, KS, D>;
+    constexpr size_t lds = KS * D * (WR * 256 + XR * 512);
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), lds)) return false;
-    hipLaunchKernelGGL(kern, dim3(tecoops::ceil_div(a.hidden, WR)), dim3(512), lds, s, a);
+    hipLaunchKernelGGL(kern, dim3(tecoops::ceil_div(a.hidden, WR)), dim3(KS * 64), lds, s, a);
     return true;
 }
 
@@ -491,8 +518,8 @@ bool launch_out_few(const MoeArgs &a, hipStream_t s) {
 template <typename T>
 bool run_out_few(const MoeArgs &a, hipStream_t s) {
     const bool wide = a.hidden >= 16 * tecoops::device_cus();
-    if (a.rows == 4) return wide ? launch_out_few<T, 4, 16, 3>(a, s) : launch_out_few<T, 4, 8, 4>(a, s);
-    return wide ? launch_out_few<T, 8, 16, 3>(a, s) : launch_out_few<T, 8, 8, 4>(a, s);
+    if (a.rows == 4) return wide ? launch_out_few<T, 4, 16, 8, 3>(a, s) : launch_out_few<T, 4, 8, 8, 4>(a, s);
+    return wide ? launch_out_few<T, 8, 16, 4, 4>(a, s) : launch_out_few<T, 8, 8, 8, 3>(a, s);
 }
 
 // Widths that are not in whole 16-byte words, or tensors that are not aligned: a
@@ -509,11 +536,11 @@ __global__ void __launch_bounds__(256) moe_scalar_kernel(MoeArgs a) {
                         static_cast<long long>(it.x) * (OUT ? 1 : 2) * a.hidden * a.inter +
                         static_cast<long long>(n) * K;
     for (int p = it.y; p < it.y + it.z; ++p) {
-        const uint16_t *x = OUT ? a.h + p * a.h_stride
-                                : reinterpret_cast<const uint16_t *>(a.x + a.token[p] * a.x_stride);
+        float *const h = reinterpret_cast<float *>(a.h) + p * a.h_stride;
+        const uint16_t *x = reinterpret_cast<const uint16_t *>(a.x + a.token[p] * a.x_stride);
         float s = 0.0f, u = 0.0f;
         for (int k = lane; k < K; k += 64) {
-            const float xv = Cvt<T>::to(x[k]);
+            const float xv = OUT ? h[k] : Cvt<T>::to(x[k]);
             s += Cvt<T>::to(w[k]) * xv;
             if (!OUT) u += Cvt<T>::to(w[static_cast<long long>(N) * K + k]) * xv;
         }
@@ -523,7 +550,7 @@ __global__ void __launch_bounds__(256) moe_scalar_kernel(MoeArgs a) {
         if (OUT)
             a.part[static_cast<long long>(a.slot[p]) * N + n] = a.weight[p] * s;
         else
-            a.h[p * a.h_stride + n] = Cvt<T>::from(activate(s, a.act) * u);
+            h[n] = activate(s, a.act) * u;
     }
 }
 
@@ -566,7 +593,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a) {
 
 template <typename T, int XR, int WR, int RS, int KS, bool OUT, int R>
 bool launch_as(MoeArgs a, int items, hipStream_t s) {
-    using S = Shape<false, XR, WR, RS, KS>;
+    using S = Shape<OUT ? kTwoTerms : kPlain, XR, WR, RS, KS>;
     static_assert(S::D >= 2, "two stages fit in LDS");
     auto *kern = &moe_product_kernel<T, XR, WR, RS, KS, OUT, R>;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), S::LDS)) return false;
@@ -598,11 +625,15 @@ bool launch(const MoeArgs &a, int items, hipStream_t s) {
 
 template <typename T, int XR, bool OUT>
 bool launch_wrows(const MoeArgs &a, int items, hipStream_t s) {
-    switch (tecoops::moe_wrows(OUT ? a.hidden : 2 * a.inter, a.tokens, a.top_k, a.experts, XR,
+    // 64 rows of two-term x leave two stages in LDS from 32 rows of W on
+    constexpr bool kLong = OUT && XR > 32;
+    switch (tecoops::moe_wrows(OUT ? a.hidden : 2 * a.inter, a.tokens, a.top_k, a.experts, OUT ? 2 * XR : XR,
                                tecoops::device_cus())) {
-        case 16: return launch<T, XR, 16, 1, 4, OUT>(a, items, s);
+        case 16:
+            if constexpr (!kLong) return launch<T, XR, 16, 1, 4, OUT>(a, items, s);
+            [[fallthrough]];
         case 32: return launch<T, XR, 16, 2, 2, OUT>(a, items, s);
-        case 64: return launch<T, XR, 32, 2, 2, OUT>(a, items, s);
+        case 64: return launch<T, XR, kLong ? 16 : 32, kLong ? 4 : 2, kLong ? 1 : 2, OUT>(a, items, s);
         default: return launch<T, XR, 16, 8, 1, OUT>(a, items, s);
     }
 }
