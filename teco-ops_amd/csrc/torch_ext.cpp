@@ -384,7 +384,7 @@ void moe_layer(const Tensor &x, const Tensor &w_in, const Tensor &w_out, const T
                 "moe_layer: x [T, H], w_in [E, 2I, H], w_out [E, H, I], router_logits [T, E]");
     const int t = fits_int(x.size(0), "T"), e = fits_int(w_out.size(0), "E"),
               h = fits_int(w_out.size(1), "H"), i = fits_int(w_out.size(2), "I"),
-              k = fits_int(top_k, "top_k");
+              k = static_cast<int>(std::min<int64_t>(std::max<int64_t>(top_k, -1), 1 << 20));
     TORCH_CHECK(w_in.size(0) == e && w_in.size(1) == 2LL * i && w_in.size(2) == h &&
                     router_logits.size(0) == t && router_logits.size(1) == e && out.dim() == 2 &&
                     out.size(0) == t && out.size(1) == h,

@@ -384,9 +384,17 @@ def _fast(name):
     """The torch op `name` of libtecoops_torch.so, or None when it is not built.
     Its C++ checks and launch take about a third of the host time of a ctypes call
     behind Python ones (12.7 us for the latter, which a product of one row with a
-    [4096, 4096] weight does not hide).  What it refuses is put to the Python
-    checks and the C ABI again, for their errors."""
+    [4096, 4096] weight does not hide).  When it raises, the Python checks say what
+    was wrong with the arguments; what they let pass is raised by _raise.  It is not
+    called again: it may have launched, and some of the outputs are inputs too."""
     return None if ops is None else getattr(ops, name).default
+
+
+def _raise(error, name):
+    """An error of the torch op for arguments that the Python checks accept: the
+    TecoopsError of the C function's status when it ended in one, else itself."""
+    status = _lib.status_of(str(error))
+    raise error if status is None else TecoopsError(status, name) from error
 
 
 _linear, _moe_layer = _fast("linear"), _fast("moe_layer")
@@ -403,11 +411,13 @@ def linear(x, weight, out, bias=None, residual=None, activation=None, gated=Fals
     the up rows, and out = act(gate) * up + residual.  residual may be out
     itself; out must not overlap another input.  float16 or bfloat16; sums and
     epilogue in float32."""
+    refused = None
     if _linear is not None:
         try:
-            return _linear(x, weight, out, bias, residual, "none" if activation is None else activation, gated)
-        except (RuntimeError, TypeError, ValueError):
-            pass
+            return _linear(x, weight, out, bias, residual, "none" if activation is None else activation,
+                           bool(gated))
+        except (RuntimeError, TypeError, ValueError) as e:
+            refused = e
     _check_cuda(x, weight, out, bias, residual)
     code, device = _dtype_code(x), x.device
     if weight.dim() != 2 or x.dim() != 2 or out.dim() != 2:
@@ -430,6 +440,8 @@ def linear(x, weight, out, bias=None, residual=None, activation=None, gated=Fals
         if residual.shape[0] != M:
             raise ValueError(f"tecoops.linear: residual must be [{M}, {N}]")
     act = _choice(_lib.ACTIVATIONS, activation, "activation")
+    if refused is not None:
+        _raise(refused, "tecoopsLinear")
     if M == 0:
         return
     space = _workspace(device, "tecoopsGetLinearWorkspaceSize", M, N, K, int(bool(gated)))
@@ -450,13 +462,14 @@ def moe_layer(x, w_in, w_out, router_logits, top_k, out, renormalize=True, activ
     rows before its up rows; w_out [E, H, I]; out [T, H], zero for a token all of
     whose logits are -inf.  topk_ids int32 and topk_weights float32 [T, top_k]
     are written when given, best first, -1 and 0 where there is none."""
+    refused = None
     if _moe_layer is not None:
         try:
-            return _moe_layer(x, w_in, w_out, router_logits, top_k, out, renormalize,
+            return _moe_layer(x, w_in, w_out, router_logits, int(top_k), out, bool(renormalize),
                               "none" if activation is None else activation, topk_ids,
                               topk_weights)
-        except (RuntimeError, TypeError, ValueError):
-            pass
+        except (RuntimeError, TypeError, ValueError) as e:
+            refused = e
     _check_cuda(x, w_in, w_out, router_logits, out, topk_ids, topk_weights)
     code, device = _dtype_code(x), x.device
     if w_in.dim() != 3 or w_out.dim() != 3 or x.dim() != 2 or router_logits.dim() != 2:
@@ -481,6 +494,8 @@ def moe_layer(x, w_in, w_out, router_logits, top_k, out, renormalize=True, activ
             raise ValueError(f"tecoops.moe_layer: {name} must be [{T}, {top_k}]")
     xs = _check_rows(x, "x", H)
     act = _choice(_lib.ACTIVATIONS, activation, "activation")
+    if refused is not None:
+        _raise(refused, "tecoopsMoeLayer")
     if T == 0:
         return
     space = _workspace(device, "tecoopsGetMoeLayerWorkspaceSize", T, H, I, E, top_k)
@@ -506,7 +521,9 @@ def _axes_args(name, positions, query, key, head_size, sections, cos_sin_cache, 
     _check_cuda(positions, query, key, cos_sin_cache)
     device = query.device
     _check_device(device, positions=positions, key=key, cos_sin_cache=cos_sin_cache)
-    sections = [int(n) for n in sections]
+    sections, head_size = [int(n) for n in sections], int(head_size)
+    if head_size <= 0:
+        raise ValueError(f"tecoops.{name}: head_size must be positive")
     if positions.dtype != torch.int64:
         raise TypeError(f"tecoops.{name}: positions must be int64")
     if positions.dim() != 2 or positions.shape[0] != len(sections):
@@ -560,15 +577,18 @@ def rotary_embedding_axes(positions, query, key, head_size, sections, cos_sin_ca
     own, base^(-j / n) for the j-th of an axis' n.  With a cos_sin_cache
     (float32 [positions, rot_dim]) a token with a position outside it is left as
     it is; without, angles are computed in 64 bits."""
+    refused = None
     if _rotary_axes is not None and (rot_dim is None or rot_dim > 0):
         try:
-            return _rotary_axes(positions, query, key, head_size, sections, cos_sin_cache, is_neox,
-                                base, rot_dim or 0, layout)
-        except (RuntimeError, TypeError, ValueError):
-            pass
+            return _rotary_axes(positions, query, key, int(head_size), [int(n) for n in sections],
+                                cos_sin_cache, bool(is_neox), float(base), int(rot_dim or 0), layout)
+        except (RuntimeError, TypeError, ValueError) as e:
+            refused = e
     device, before, sizes, table, code = _axes_args("rotary_embedding_axes", positions, query, key,
                                                     head_size, sections, cos_sin_cache, base,
                                                     rot_dim, layout)
+    if refused is not None:
+        _raise(refused, "tecoopsRotaryEmbeddingAxes")
     if sizes[0] == 0:
         return
     _call_on(device, "tecoopsRotaryEmbeddingAxes", _handle(device), *before, _ptr(query), _ptr(key),
@@ -583,13 +603,15 @@ def rotary_axes_reshape_and_cache(positions, query, key, value, slot_mapping, ke
     value stored into the paged caches [num_blocks, Hkv, block_size, head_size]
     at slot_mapping (int64; slots outside the cache are not stored); key is
     updated in place only when write_key."""
+    refused = None
     if _rotary_axes_cache is not None and (rot_dim is None or rot_dim > 0):
         try:
             return _rotary_axes_cache(positions, query, key, value, slot_mapping, key_cache,
-                                      value_cache, head_size, sections, cos_sin_cache, is_neox,
-                                      base, rot_dim or 0, layout, write_key)
-        except (RuntimeError, TypeError, ValueError):
-            pass
+                                      value_cache, int(head_size), [int(n) for n in sections],
+                                      cos_sin_cache, bool(is_neox), float(base), int(rot_dim or 0),
+                                      layout, bool(write_key))
+        except (RuntimeError, TypeError, ValueError) as e:
+            refused = e
     name = "rotary_axes_reshape_and_cache"
     if key is None:
         raise ValueError(f"tecoops.{name}: key must be given")
@@ -613,6 +635,8 @@ def rotary_axes_reshape_and_cache(positions, query, key, value, slot_mapping, ke
     if value.dim() == 3 and value.shape[1] > 1 and value.stride(1) != value.shape[2] or \
             value.shape[-1] > 1 and value.stride(-1) != 1:
         raise ValueError(f"tecoops.{name}: the heads of a token of value must be adjacent")
+    if refused is not None:
+        _raise(refused, "tecoopsRotaryAxesReshapeAndCache")
     if T == 0:
         return
     _call_on(device, "tecoopsRotaryAxesReshapeAndCache", _handle(device), *before, _ptr(query),

@@ -108,6 +108,14 @@ def lib():
     return _LIB
 
 
+def status_of(message):
+    """The status that a torch op's error message names, or None."""
+    for status in range(NOT_INITIALIZED, NOT_SUPPORTED + 1):
+        if lib().tecoopsGetErrorString(status).decode() in message:
+            return status
+    return None
+
+
 def check(status, what=""):
     if status != SUCCESS:
         raise TecoopsError(status, what)

@@ -1,0 +1,52 @@
+"""A decoder-layer operator whose torch op raises after its launch has changed its
+in-place tensors once, and the error comes out."""
+import pytest
+import torch
+
+import tecoops
+from tecoops import TecoopsError
+
+pytestmark = pytest.mark.gpu
+
+
+def after_launch(monkeypatch, name):
+    real = getattr(tecoops, name)
+
+    def op(*args):
+        real(*args)
+        raise RuntimeError("op: TECOOPS_STATUS_INTERNAL_ERROR")
+    monkeypatch.setattr(tecoops, name, op)
+
+
+@pytest.mark.parametrize("m", [1, 100])
+def test_linear_into_its_residual(m, monkeypatch):
+    x, w = torch.ones(m, 64, dtype=torch.float16, device="cuda"), torch.ones(32, 64, dtype=torch.float16,
+                                                                             device="cuda")
+    out = torch.ones(m, 32, dtype=torch.float16, device="cuda")
+    after_launch(monkeypatch, "_linear")
+    with pytest.raises(TecoopsError):
+        tecoops.linear(x, w, out, residual=out)
+    assert (out == 65).all()
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_rotary_in_place(fused, monkeypatch):
+    T, H, D, dt = 5, 2, 64, torch.float16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(T, H * D, generator=g, device="cuda").to(dt) for _ in range(3))
+    pos = torch.arange(3 * T, device="cuda").view(3, T)
+    kc, vc = (torch.zeros(2, H, 16, D, dtype=dt, device="cuda") for _ in range(2))
+
+    def call(q, k):
+        if fused:
+            tecoops.rotary_axes_reshape_and_cache(pos, q, k, v, torch.arange(T, device="cuda"), kc, vc, D,
+                                                  [12, 10, 10], write_key=True)
+        else:
+            tecoops.rotary_embedding_axes(pos, q, k, D, [12, 10, 10])
+
+    once = q.clone(), k.clone()
+    call(*once)
+    after_launch(monkeypatch, "_rotary_axes_cache" if fused else "_rotary_axes")
+    with pytest.raises(TecoopsError):
+        call(q, k)
+    assert torch.equal(q, once[0]) and torch.equal(k, once[1])
