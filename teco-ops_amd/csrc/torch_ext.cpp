@@ -461,9 +461,8 @@ struct AxesArgs {
     int rows(const Tensor &t, const Tensor &query, int64_t head_size, const char *name,
              int64_t *stride) const {
         need_dtype(t, query.scalar_type(), name);
-        const int64_t row = tokens ? t.numel() / tokens : head_size;
-        TORCH_CHECK((t.dim() == 2 || t.dim() == 3) && t.size(0) == tokens && row > 0 &&
-                        row % head_size == 0,
+        const int64_t row = t.dim() == 2 ? t.size(1) : t.dim() == 3 ? t.size(1) * t.size(2) : 0;
+        TORCH_CHECK(row > 0 && t.size(0) == tokens && row % head_size == 0,
                     "tecoops: ", name, " must be [tokens, heads * head_size] or [tokens, heads, head_size]");
         TORCH_CHECK((t.dim() == 2 || t.size(1) <= 1 || t.stride(1) == t.size(2)) &&
                         (t.size(-1) <= 1 || t.stride(-1) == 1),

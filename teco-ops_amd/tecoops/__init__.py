@@ -17,6 +17,7 @@ Differences from the reference wrappers, all toward its documented intent:
     transposing x and out (torch_ext.cpp:186-205).
 """
 import ctypes
+import math
 import os
 import sys
 import threading
@@ -538,7 +539,7 @@ def _axes_args(name, positions, query, key, head_size, sections, cos_sin_cache, 
             strides.append(0)
             continue
         _check_dtype(t, what, query.dtype)
-        row = t.numel() // T if T else head_size
+        row = math.prod(t.shape[1:])
         if t.dim() not in (2, 3) or t.shape[0] != T or row == 0 or row % head_size:
             raise ValueError(f"tecoops.{name}: {what} must be [tokens, heads * head_size] or "
                              "[tokens, heads, head_size]")
@@ -630,7 +631,7 @@ def rotary_axes_reshape_and_cache(positions, query, key, value, slot_mapping, ke
     if key_cache.dim() != 4 or key_cache.shape[1] != Hkv or key_cache.shape[3] != D or \
             value_cache.shape != key_cache.shape:
         raise ValueError(f"tecoops.{name}: caches must be [num_blocks, {Hkv}, block_size, {D}]")
-    if value.dim() not in (2, 3) or value.shape[0] != T or value.numel() != T * Hkv * D:
+    if value.dim() not in (2, 3) or value.shape[0] != T or math.prod(value.shape[1:]) != Hkv * D:
         raise ValueError(f"tecoops.{name}: value must match key")
     if value.dim() == 3 and value.shape[1] > 1 and value.stride(1) != value.shape[2] or \
             value.shape[-1] > 1 and value.stride(-1) != 1:

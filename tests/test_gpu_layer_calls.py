@@ -1,5 +1,5 @@
-"""A decoder-layer operator whose torch op raises after its launch has changed its
-in-place tensors once, and the error comes out."""
+"""The calls of the decoder-layer operators at their edges: an op that raises after its
+launch has changed its in-place tensors once, and the error comes out; empty batches."""
 import pytest
 import torch
 
@@ -50,3 +50,22 @@ def test_rotary_in_place(fused, monkeypatch):
     with pytest.raises(TecoopsError):
         call(q, k)
     assert torch.equal(q, once[0]) and torch.equal(k, once[1])
+
+
+@pytest.mark.parametrize("kv_heads", [1, 2, 5])
+@pytest.mark.parametrize("fused", [False, True])
+def test_rotary_of_no_tokens(fused, kv_heads):
+    """An empty batch, through the Python functions and the torch ops alike."""
+    D, dt, sec = 64, torch.float16, [12, 10, 10]
+    q, k = (torch.zeros(0, h, D, dtype=dt, device="cuda") for h in (5, kv_heads))
+    pos = torch.zeros(3, 0, dtype=torch.int64, device="cuda")
+    kc = torch.ones(2, kv_heads, 16, D, dtype=dt, device="cuda")
+    if fused:
+        args = pos, q, k, k, pos[0], kc, kc, D, sec
+        tecoops.rotary_axes_reshape_and_cache(*args)
+        torch.ops.tecoops.rotary_axes_reshape_and_cache(*args, None, True, 1e4, D, "contiguous", False)
+    else:
+        tecoops.rotary_embedding_axes(pos, q, k, D, sec)
+        torch.ops.tecoops.rotary_embedding_axes(pos, q, k, D, sec, None, True, 1e4, D, "contiguous")
+    torch.cuda.synchronize()
+    assert (kc == 1).all()

@@ -71,7 +71,7 @@ def test_other_errors_stay_what_they_are(name, error, stub):
     assert e.value is error and launched == ["op"]
 
 
-@pytest.mark.parametrize("name", NAMES[:3])
+@pytest.mark.parametrize("name", NAMES)
 def test_no_tokens(name, stub):
     """An error without any work to do is still one."""
     t = tensors()
@@ -82,6 +82,22 @@ def test_no_tokens(name, stub):
     with pytest.raises(RuntimeError):
         calls(t)[name]()
     assert launched == ["op"]
+
+
+@pytest.mark.parametrize("heads", [(H * D,), (H, D)])
+def test_empty_batch_of_several_heads(heads, stub, monkeypatch):
+    """No tokens, any number of heads: nothing to do (the checks alone, without the op)."""
+    launched = stub("_rotary_axes", RuntimeError("not called"))
+    t = tensors()
+    q = torch.zeros(0, *heads, dtype=F16)
+    monkeypatch.setattr(tecoops, "_rotary_axes", None)
+    monkeypatch.setattr(tecoops, "_rotary_axes_cache", None)
+    tecoops.rotary_embedding_axes(t["pos"][:, :0], q, q, D, [12, 10, 10])
+    args = (t["slots"][:0], t["kc"], t["vc"], D, [12, 10, 10])
+    tecoops.rotary_axes_reshape_and_cache(t["pos"][:, :0], q, q, q, *args)
+    assert launched == []
+    with pytest.raises(ValueError):  # one kv head of value, two of key
+        tecoops.rotary_axes_reshape_and_cache(t["pos"][:, :0], q, q, torch.zeros(0, D, dtype=F16), *args)
 
 
 def test_refused_arguments_keep_their_errors(stub):
