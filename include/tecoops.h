@@ -413,8 +413,9 @@ tecoopsStatus_t tecoopsGetMoeLayerWorkspaceSize(int tokens, int hidden, int inte
 
 /* Rotary positions of several axes (time, height, width of images and video).
  * As tecoopsRotaryEmbedding, but positions is int64 [axes, num_tokens] (rows
- * position_stride elements apart, at least num_tokens) and pair i of a head
- * turns by the position of one axis.  sections (host, [axes]) are the axes'
+ * position_stride elements apart, at least num_tokens, or 0: all axes at the same
+ * positions, as in plain text) and pair i of a head turns by the position of one
+ * axis.  sections (host, [axes]) are the axes'
  * numbers of frequencies; their sum has to be rot_dim / 2.
  *   CONTIGUOUS   the first sections[0] pairs to axis 0, the next to axis 1, ...;
  *                pair i at base^(-2i/rot_dim)

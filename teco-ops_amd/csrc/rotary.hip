@@ -920,7 +920,9 @@ tecoopsStatus_t axis_positions(AxisPositions *out, const int64_t *positions,
         return TECOOPS_STATUS_BAD_PARAM;
     if (layout < TECOOPS_ROTARY_CONTIGUOUS || layout > TECOOPS_ROTARY_PER_AXIS)
         return TECOOPS_STATUS_BAD_PARAM;
-    if (axes > 1 && position_stride < r.num_tokens) return TECOOPS_STATUS_BAD_PARAM;
+    // positions are only read: all axes may share one row of them (stride 0)
+    if (axes > 1 && position_stride != 0 && position_stride < r.num_tokens)
+        return TECOOPS_STATUS_BAD_PARAM;
     const int half = r.rot_dim / 2;
     int sum = 0;
     for (int a = 0; a < TECOOPS_ROTARY_MAX_AXES; ++a) {

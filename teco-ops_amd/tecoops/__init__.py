@@ -571,11 +571,11 @@ def rotary_embedding_axes(positions, query, key, head_size, sections, cos_sin_ca
     video), in place on query [T, H*D or H, D] and key likewise (or None; the
     rows may be slices of a wider product's).
 
-    positions int64 [axes, T]; sections: the number of frequencies of each axis,
-    rot_dim / 2 together.  layout: "contiguous" gives each axis a range of the
-    frequencies, "interleaved" frequency i to axis i % axes while that axis has
-    any left (else to the first), "per_axis" ranges with frequencies of their
-    own, base^(-j / n) for the j-th of an axis' n.  With a cos_sin_cache
+    positions int64 [axes, T] (for plain text, [1, T] expanded); sections: the
+    number of frequencies of each axis, rot_dim / 2 together.  layout:
+    "contiguous" gives each axis a range of the frequencies, "interleaved"
+    frequency i to axis i % axes while that axis has any left (else to the
+    first), "per_axis" ranges with frequencies of their own, base^(-j / n) for the j-th of an axis' n.  With a cos_sin_cache
     (float32 [positions, rot_dim]) a token with a position outside it is left as
     it is; without, angles are computed in 64 bits."""
     refused = None

@@ -69,3 +69,38 @@ def test_rotary_of_no_tokens(fused, kv_heads):
         torch.ops.tecoops.rotary_embedding_axes(pos, q, k, D, sec, None, True, 1e4, D, "contiguous")
     torch.cuda.synchronize()
     assert (kc == 1).all()
+
+
+@pytest.mark.parametrize("table", [False, True])
+@pytest.mark.parametrize("op", [True, False])
+@pytest.mark.parametrize("T", [1, 2, 37])
+def test_expanded_positions(T, op, table, monkeypatch):
+    """positions.expand(3, -1), one row for all axes: as its copy, through the torch
+    ops and the C functions, in place and with the cache store."""
+    H, Hkv, D, dt, sec = 4, 2, 128, torch.bfloat16, [24, 20, 20]
+    g = torch.Generator(device="cuda").manual_seed(T)
+    q0, k0, v = (torch.randn(T, h * D, generator=g, device="cuda").to(dt) for h in (H, Hkv, Hkv))
+    row = torch.randint(0, 100, (T,), generator=g, device="cuda")
+    angles = torch.rand(100, D, generator=g, device="cuda") if table else None
+    slots = torch.arange(T, device="cuda")
+    if not op:
+        monkeypatch.setattr(tecoops, "_rotary_axes", None)
+        monkeypatch.setattr(tecoops, "_rotary_axes_cache", None)
+    got = []
+    for pos in (row.expand(3, -1), row[None].expand(3, T), row.expand(3, -1).contiguous()):
+        q, k, q2 = q0.clone(), k0.clone(), q0.clone()
+        kc, vc = (torch.zeros(3, Hkv, 16, D, dtype=dt, device="cuda") for _ in range(2))
+        kw = dict(cos_sin_cache=angles, layout="interleaved")
+        tecoops.rotary_embedding_axes(pos, q, k, D, sec, **kw)
+        tecoops.rotary_axes_reshape_and_cache(pos, q2, k0, v, slots, kc, vc, D, sec, **kw)
+        got.append((q, k, q2, kc, vc))
+    assert not torch.equal(got[0][0], q0)
+    for a in got[:2]:
+        assert all(torch.equal(x, y) for x, y in zip(a, got[2]))
+
+
+def test_overlapping_positions_are_refused():
+    pos = torch.zeros(64, dtype=torch.int64, device="cuda").as_strided((3, 37), (1, 1))
+    q = torch.zeros(37, 512, dtype=torch.float16, device="cuda")
+    with pytest.raises(TecoopsError):
+        tecoops.rotary_embedding_axes(pos, q, None, 128, [24, 20, 20])
