@@ -370,7 +370,7 @@ typedef enum {
  * of x and W in whole, aligned 16-byte words are fastest) up to k and x_stride
  * 2^21, n 2^23 and 2^23 tiles of out; m = 0 is done without a launch.
  * workspace: tecoopsGetLinearWorkspaceSize() bytes for the same sizes let few
- * tiles be split along k; with less, or NULL, the call runs with fewer splits
+ * tiles be split along k, wherever x and weight lie; with less, or NULL, the call runs with fewer splits
  * (slower, the same result up to fp32 rounding).  Nothing is allocated. */
 tecoopsStatus_t tecoopsLinear(tecoopsHandle_t handle, const void *x, long long x_stride,
                               const void *weight, const void *bias,

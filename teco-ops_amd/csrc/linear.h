@@ -5,6 +5,7 @@
 #include "gemv_batch.h"
 
 #include <cstddef>
+#include <cstdint>
 
 namespace tecoops {
 
@@ -106,5 +107,14 @@ inline LinearPlan linear_plan(int m, int n, int k, bool gated, bool copy, size_t
     }
     return best;
 }
+
+// Whether rows of x and W can be copied into LDS: in whole, aligned 16-byte words.
+inline bool linear_copies(int k, long long x_stride, const void *x, const void *weight) {
+    const auto whole = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    return k % 8 == 0 && x_stride % 8 == 0 && whole(x) && whole(weight);
+}
+
+// Bytes of workspace that such a product can use (linear.hip).
+size_t linear_workspace(int m, int n, int k, bool gated, bool copy);
 
 }  // namespace tecoops

@@ -548,13 +548,24 @@ constexpr size_t kMostWorkspace = size_t{512} << 20;
 
 }  // namespace
 
+size_t tecoops::linear_workspace(int m, int n, int k, bool gated, bool copy) {
+    return linear_plan(m, n, k, gated, copy, kMostWorkspace, device_cus()).bytes;
+}
+
 extern "C" tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, int gated,
                                                          size_t *bytes) {
     if (bytes == nullptr || m < 0 || n <= 0 || k <= 0) return TECOOPS_STATUS_BAD_PARAM;
     *bytes = 0;
     if (m == 0) return TECOOPS_STATUS_SUCCESS;
-    *bytes = tecoops::linear_plan(m, n, k, gated != 0, k % 8 == 0, kMostWorkspace, tecoops::device_cus())
-                 .bytes;
+    // enough wherever x and the weight lie: a view off 16 bytes or with another
+    // stride is loaded through registers, by a plan of its own (8 rows of x, [4096,
+    // 14336]: copied they stream W without a workspace, through registers K is split
+    // 8 ways)
+    *bytes = tecoops::linear_workspace(m, n, k, gated != 0, false);
+    if (k % 8 == 0) {
+        const size_t copied = tecoops::linear_workspace(m, n, k, gated != 0, true);
+        if (copied > *bytes) *bytes = copied;
+    }
     return TECOOPS_STATUS_SUCCESS;
 }
 
@@ -578,8 +589,7 @@ extern "C" tecoopsStatus_t tecoopsLinear(tecoopsHandle_t handle, const void *x, 
         return TECOOPS_STATUS_NOT_SUPPORTED;
     if (m == 0) return TECOOPS_STATUS_SUCCESS;
     const int wrows = gated ? 2 * n : n;
-    const bool copy = k % 8 == 0 && x_stride % 8 == 0 && tecoops::aligned(weight, 16) &&
-                      tecoops::aligned(x, 16);
+    const bool copy = tecoops::linear_copies(k, x_stride, x, weight);
     Epilogue e;
     e.bias = static_cast<const uint16_t *>(bias);
     e.residual = static_cast<const uint16_t *>(residual);

@@ -23,6 +23,7 @@
 #include <unordered_map>
 
 #include "flash_attention.h"
+#include "linear.h"
 #include "tecoops.h"
 
 namespace {
@@ -363,8 +364,9 @@ void linear(const Tensor &x, const Tensor &weight, Tensor &out, const c10::optio
     const int64_t rs = r ? row_stride(*r, m, n, "residual") : 0;
     const tecoopsActivation_t act = activation_of(activation);
     if (m == 0) return;
-    size_t bytes = 0;
-    check(tecoopsGetLinearWorkspaceSize(m, n, k, gated, &bytes), "linear");
+    // of these tensors' plan alone: most products of few rows need none
+    const size_t bytes = n > 0 && k > 0 ? tecoops::linear_workspace(m, n, k, gated,
+        tecoops::linear_copies(k, xs, x.data_ptr(), weight.data_ptr())) : 0;
     const Tensor ws = workspace_of(bytes, x);
     check(tecoopsLinear(handle_for(x), x.data_ptr(), xs, weight.data_ptr(), b ? b->data_ptr() : nullptr,
                         r ? r->data_ptr() : nullptr, rs, out.data_ptr(), os, m, n, k, act, gated,
