@@ -190,36 +190,54 @@ tecoopsStatus_t tecoopsMorton3DInvert(tecoopsHandle_t handle, const int *indices
 
 namespace tecoops {
 
-// The largest size set for each kernel so far is kept in a fixed table (no
-// heap allocation, so the allocation-free entry points can use it too): the
-// attribute is set again only when a launch needs more than that (the GEMV
-// kernels' LDS grows with K), and past the table's capacity on every launch.
+// The largest size set for each kernel so far is kept in a fixed hash table (no heap
+// allocation, so the allocation-free entry points can use it too), three times as
+// large as the kernels that ask for LDS here (about 650): the attribute is set again
+// only when a launch needs more than that (the GEMV kernels' LDS grows with K).  A
+// launch that needs no more takes no lock.
+struct LdsSlot {
+    std::atomic<const void *> kernel;
+    std::atomic<size_t> bytes;
+};
+constexpr size_t kLdsSlots = 2048;
+
+// The kernel's slot or the free one that it would take; nullptr when the table is full.
+static LdsSlot *lds_slot(LdsSlot *table, const void *kernel) {
+    const uint64_t h = reinterpret_cast<uintptr_t>(kernel) * 0x9E3779B97F4A7C15ull;
+    for (size_t i = 0; i < kLdsSlots; ++i) {
+        LdsSlot *s = &table[(h / (~0ull / kLdsSlots + 1) + i) % kLdsSlots];
+        const void *k = s->kernel.load(std::memory_order_acquire);
+        if (k == kernel || k == nullptr) return s;
+    }
+    return nullptr;
+}
+
 bool reserve_lds(const void *kernel, size_t bytes) {
     static std::mutex mu;
-    static const void *kern[256];
-    static size_t size[256];
-    static int n = 0;
+    static LdsSlot table[kLdsSlots];
     if (bytes <= kLdsDefault) return true;
     if (bytes > kLdsMax) {
         TECO_ERROR("a kernel asks for %zu bytes of LDS, more than the %zu a workgroup can hold",
                    bytes, kLdsMax);
         return false;
     }
+    const LdsSlot *seen = lds_slot(table, kernel);
+    if (seen != nullptr && seen->kernel.load(std::memory_order_acquire) == kernel &&
+        seen->bytes.load(std::memory_order_relaxed) >= bytes)
+        return true;
     std::lock_guard<std::mutex> lock(mu);
-    int i = 0;
-    while (i < n && kern[i] != kernel) ++i;
-    if (i < n && size[i] >= bytes) return true;
+    LdsSlot *slot = lds_slot(table, kernel);  // another thread may have filled it
+    const bool known = slot != nullptr && slot->kernel.load(std::memory_order_relaxed) == kernel;
+    if (known && slot->bytes.load(std::memory_order_relaxed) >= bytes) return true;
     if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                             static_cast<int>(bytes)) != hipSuccess) {
         (void)hipGetLastError();
         TECO_ERROR("cannot reserve %zu bytes of LDS for a kernel", bytes);
         return false;
     }
-    if (i < n) {
-        size[i] = bytes;
-    } else if (n < 256) {
-        kern[n] = kernel;
-        size[n++] = bytes;
+    if (slot != nullptr) {
+        slot->bytes.store(bytes, std::memory_order_relaxed);
+        slot->kernel.store(kernel, std::memory_order_release);
     }
     return true;
 }
