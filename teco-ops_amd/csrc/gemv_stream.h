@@ -93,6 +93,13 @@ enum Operands { kPlain, kInt8, kTwoTerms };
 // loses no bits to the type's small exponents.
 template <typename T> constexpr float kLow = __is_same(T, f16) ? 0x1p-11f : 1.0f;
 
+// The sum of the terms' sums.  An infinite weight makes that of the second terms
+// infinite or NaN whatever they are (0 or of the other sign, say): the first decides.
+template <typename T>
+__device__ __forceinline__ float both_terms(float high, float low) {
+    return fabsf(low) < INFINITY ? fmaf(kLow<T>, low, high) : high;
+}
+
 // Sizes of a workgroup's stages.  XR: rows of x staged; WR: rows of W per wave.
 template <Operands OP, int XR, int WR, int RS, int KS>
 struct Shape {
@@ -261,7 +268,7 @@ __device__ __forceinline__ void product(char *lds, int K, int unit, WRow &&w_row
 #pragma unroll
             for (int t = 0; t < CT; ++t)
 #pragma unroll
-                for (int v = 0; v < 4; ++v) acc[r][t][v] = fmaf(kLow<T>, low[r][t][v], acc[r][t][v]);
+                for (int v = 0; v < 4; ++v) acc[r][t][v] = both_terms<T>(acc[r][t][v], low[r][t][v]);
     if constexpr (KS > 1) {
         __syncthreads();  // every wave is done with the ring
         float *red = reinterpret_cast<float *>(lds);

@@ -320,7 +320,7 @@ void launch_route(const MoeArgs &a, bool copy, hipStream_t s) {
 
 // h = kUnit (hi + kLow lo), with 16 bits of it in bf16 and 22 in fp16.  kUnit moves
 // fp16's range to 65520 * 256 (beyond, hi is infinite and lo is 0) and its smallest
-// step, that of lo, to 2^-27.  (An infinite weight gives NaN where lo is 0.)
+// step, that of lo, to 2^-27.
 template <typename T> constexpr float kUnit = __is_same(T, f16) ? 256.0f : 1.0f;
 
 template <typename T>
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(KS * 64) moe_out_few_kernel(MoeArgs a) {
         if (++ust == spi || s + 1 == s1) {
             const float wt = kUnit<T> * col_weight[ui * XR + xc];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) tot[v] += wt >= 0.0f ? wt * fmaf(kLow<T>, low[v], acc[v]) : 0.0f;
+            for (int v = 0; v < 4; ++v) tot[v] += wt >= 0.0f ? wt * both_terms<T>(acc[v], low[v]) : 0.0f;
             acc = low = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
             ust = 0;
             ++ui;

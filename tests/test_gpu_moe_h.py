@@ -109,3 +109,21 @@ def test_infinite_h_stays_in_its_token(T, dtype):
     tecoops.moe_layer(x, w_in, w_out, logits.index_fill(0, torch.tensor([T - 1], device="cuda"), -math.inf), 2,
                       out, activation="relu")
     assert torch.equal(out[:T - 1], first[:T - 1]) and (out[T - 1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("I", [64, 35])
+@pytest.mark.parametrize("T", [1, 4, 8, 30, 200])
+def test_infinite_down_weight(T, I, dtype):
+    """An infinite weight gives an infinity of h's sign, not NaN, whatever terms h
+    falls into, and only in its row of the result."""
+    H, E, dt = 72, 2, DT[dtype]
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.rand(T, H, generator=g, device="cuda").to(dt) + 0.5
+    w_in, w_out = (torch.rand(*s, generator=g, device="cuda").to(dt) for s in ((E, 2 * I, H), (E, H, I)))
+    w_out[:, 3, I - 1], w_out[:, 5, 0] = math.inf, -math.inf
+    out = torch.empty_like(x)
+    tecoops.moe_layer(x, w_in / 8, w_out / 8, torch.zeros(T, E, device="cuda"), 2, out)
+    assert (out[:, 3] == math.inf).all() and (out[:, 5] == -math.inf).all()
+    rest = [i for i in range(H) if i not in (3, 5)]
+    assert torch.isfinite(out[:, rest]).all()
