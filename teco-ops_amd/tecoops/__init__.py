@@ -391,11 +391,19 @@ def _fast(name):
     return None if ops is None else getattr(ops, name).default
 
 
-def _raise(error, name):
-    """An error of the torch op for arguments that the Python checks accept: the
-    TecoopsError of the C function's status when it ended in one, else itself."""
-    status = _lib.status_of(str(error))
-    raise error if status is None else TecoopsError(status, name) from error
+def _raise(refused, name):
+    """The error that the torch op raised for arguments which the Python checks accept
+    (the one in the list `refused`): the TecoopsError of the C function's status when it
+    ended in one, else itself.  No frame keeps it, so that the tensors of a failed call
+    live no longer than the caller's."""
+    error = refused.pop()
+    try:
+        status = _lib.status_of(str(error))
+        if status is None:
+            raise error
+        raise TecoopsError(status, name) from error
+    finally:
+        del error
 
 
 _linear, _moe_layer = _fast("linear"), _fast("moe_layer")
@@ -412,13 +420,13 @@ def linear(x, weight, out, bias=None, residual=None, activation=None, gated=Fals
     the up rows, and out = act(gate) * up + residual.  residual may be out
     itself; out must not overlap another input.  float16 or bfloat16; sums and
     epilogue in float32."""
-    refused = None
+    refused = []
     if _linear is not None:
         try:
             return _linear(x, weight, out, bias, residual, "none" if activation is None else activation,
                            bool(gated))
         except (RuntimeError, TypeError, ValueError) as e:
-            refused = e
+            refused.append(e.with_traceback(None))
     _check_cuda(x, weight, out, bias, residual)
     code, device = _dtype_code(x), x.device
     if weight.dim() != 2 or x.dim() != 2 or out.dim() != 2:
@@ -441,7 +449,7 @@ def linear(x, weight, out, bias=None, residual=None, activation=None, gated=Fals
         if residual.shape[0] != M:
             raise ValueError(f"tecoops.linear: residual must be [{M}, {N}]")
     act = _choice(_lib.ACTIVATIONS, activation, "activation")
-    if refused is not None:
+    if refused:
         _raise(refused, "tecoopsLinear")
     if M == 0:
         return
@@ -463,14 +471,14 @@ def moe_layer(x, w_in, w_out, router_logits, top_k, out, renormalize=True, activ
     rows before its up rows; w_out [E, H, I]; out [T, H], zero for a token all of
     whose logits are -inf.  topk_ids int32 and topk_weights float32 [T, top_k]
     are written when given, best first, -1 and 0 where there is none."""
-    refused = None
+    refused = []
     if _moe_layer is not None:
         try:
             return _moe_layer(x, w_in, w_out, router_logits, int(top_k), out, bool(renormalize),
                               "none" if activation is None else activation, topk_ids,
                               topk_weights)
         except (RuntimeError, TypeError, ValueError) as e:
-            refused = e
+            refused.append(e.with_traceback(None))
     _check_cuda(x, w_in, w_out, router_logits, out, topk_ids, topk_weights)
     code, device = _dtype_code(x), x.device
     if w_in.dim() != 3 or w_out.dim() != 3 or x.dim() != 2 or router_logits.dim() != 2:
@@ -495,7 +503,7 @@ def moe_layer(x, w_in, w_out, router_logits, top_k, out, renormalize=True, activ
             raise ValueError(f"tecoops.moe_layer: {name} must be [{T}, {top_k}]")
     xs = _check_rows(x, "x", H)
     act = _choice(_lib.ACTIVATIONS, activation, "activation")
-    if refused is not None:
+    if refused:
         _raise(refused, "tecoopsMoeLayer")
     if T == 0:
         return
@@ -578,17 +586,17 @@ def rotary_embedding_axes(positions, query, key, head_size, sections, cos_sin_ca
     first), "per_axis" ranges with frequencies of their own, base^(-j / n) for the j-th of an axis' n.  With a cos_sin_cache
     (float32 [positions, rot_dim]) a token with a position outside it is left as
     it is; without, angles are computed in 64 bits."""
-    refused = None
+    refused = []
     if _rotary_axes is not None and (rot_dim is None or rot_dim > 0):
         try:
             return _rotary_axes(positions, query, key, int(head_size), [int(n) for n in sections],
                                 cos_sin_cache, bool(is_neox), float(base), int(rot_dim or 0), layout)
         except (RuntimeError, TypeError, ValueError) as e:
-            refused = e
+            refused.append(e.with_traceback(None))
     device, before, sizes, table, code = _axes_args("rotary_embedding_axes", positions, query, key,
                                                     head_size, sections, cos_sin_cache, base,
                                                     rot_dim, layout)
-    if refused is not None:
+    if refused:
         _raise(refused, "tecoopsRotaryEmbeddingAxes")
     if sizes[0] == 0:
         return
@@ -604,7 +612,7 @@ def rotary_axes_reshape_and_cache(positions, query, key, value, slot_mapping, ke
     value stored into the paged caches [num_blocks, Hkv, block_size, head_size]
     at slot_mapping (int64; slots outside the cache are not stored); key is
     updated in place only when write_key."""
-    refused = None
+    refused = []
     if _rotary_axes_cache is not None and (rot_dim is None or rot_dim > 0):
         try:
             return _rotary_axes_cache(positions, query, key, value, slot_mapping, key_cache,
@@ -612,7 +620,7 @@ def rotary_axes_reshape_and_cache(positions, query, key, value, slot_mapping, ke
                                       cos_sin_cache, bool(is_neox), float(base), int(rot_dim or 0),
                                       layout, bool(write_key))
         except (RuntimeError, TypeError, ValueError) as e:
-            refused = e
+            refused.append(e.with_traceback(None))
     name = "rotary_axes_reshape_and_cache"
     if key is None:
         raise ValueError(f"tecoops.{name}: key must be given")
@@ -636,7 +644,7 @@ def rotary_axes_reshape_and_cache(positions, query, key, value, slot_mapping, ke
     if value.dim() == 3 and value.shape[1] > 1 and value.stride(1) != value.shape[2] or \
             value.shape[-1] > 1 and value.stride(-1) != 1:
         raise ValueError(f"tecoops.{name}: the heads of a token of value must be adjacent")
-    if refused is not None:
+    if refused:
         _raise(refused, "tecoopsRotaryAxesReshapeAndCache")
     if T == 0:
         return

@@ -145,3 +145,30 @@ def test_arguments_of_other_types(monkeypatch):
 def test_status_of_a_message():
     assert _lib.status_of("linear: TECOOPS_STATUS_NOT_SUPPORTED\nraised from here") == _lib.NOT_SUPPORTED
     assert _lib.status_of("tensors must be contiguous") is None
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("error", ["no memory", "x: TECOOPS_STATUS_INTERNAL_ERROR"])
+def test_a_failed_call_keeps_no_tensors(name, error, stub, monkeypatch):
+    """A caller that catches the error and lets go of its tensors gets their memory
+    back, without waiting for a collection of cycles."""
+    import gc
+    import weakref
+    t = tensors()
+    held = [weakref.ref(v) for v in t.values()]
+    call = calls(t)[name]
+    stub(name, None)
+
+    def op(*args):
+        raise RuntimeError(error)
+    monkeypatch.setattr(tecoops, name, op)
+    gc.disable()
+    try:
+        try:
+            call()
+        except RuntimeError:
+            pass
+        del call, t
+        assert all(ref() is None for ref in held)
+    finally:
+        gc.enable()
