@@ -394,8 +394,10 @@ tecoopsStatus_t tecoopsGetLinearWorkspaceSize(int m, int n, int k, int gated, si
  * experts] packed, logitsType FLOAT or dataType; out [tokens, hidden] packed,
  * zero for a token without experts; out must not overlap an input.  topk_ids
  * int32 and topk_weights float [tokens, top_k] are written unless NULL, best
- * first, -1 and 0 where there is none.  Every expert's weights are read once
- * for all of its tokens (of each 512 tokens, up to 64 at a time).  Up to 2^30
+ * first, -1 and 0 where there is none.  For decode batches: an expert's weights
+ * are read once for up to 4, 8 or 16 of its tokens (batches of that many), 16, 32 or
+ * 64 (larger ones, by their mean per expert), and again for every 512 tokens of the
+ * batch; a prompt, or most tokens at few experts, reads them many times.  Up to 2^30
  * tokens, 1024 experts, top_k 32, hidden and inter 2^16; hidden, inter and
  * x_stride multiples of 8 and 16-byte aligned tensors are fast; tokens = 0 is done
  * without a launch.
@@ -426,7 +428,7 @@ tecoopsStatus_t tecoopsGetMoeLayerWorkspaceSize(int tokens, int hidden, int inte
  *                base^(-j/n)
  * With a cos_sin_cache (float32 [max_position, rot_dim]) column i of either half
  * is pair i; a token with any position outside it is left as it is.  Without,
- * angles are computed in 64 bits. */
+ * angles are computed in 64 bits from base as given, a float. */
 #define TECOOPS_ROTARY_MAX_AXES 4
 typedef enum {
     TECOOPS_ROTARY_CONTIGUOUS = 0,

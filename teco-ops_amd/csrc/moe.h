@@ -18,7 +18,7 @@ constexpr int kMoeSlice = 512;  // tokens routed together; more run slice by sli
 // Rows of x staged for an item: the tokens of an expert go through in chunks of
 // this many, and W is read again for each.  Few tokens never need a second one;
 // many take the size that an even spread over the experts fills about half, so
-// that few experts overflow it.
+// that few experts overflow it (a skewed routing does, and reads W again).
 inline int moe_rows(int tokens, int top_k, int experts) {
     if (tokens <= 4) return 4;
     if (tokens <= 8) return 8;
@@ -71,8 +71,8 @@ inline double moe_reached(int tokens, int top_k, int experts) {
 // Whether few tokens sum over the experts within the second product.  It spares
 // the parts, their sum and a launch, about 5 us, but has a workgroup per 8 (or
 // 16) rows of the result only, which leave part of the chip's bandwidth when they
-// are few (6 tokens, 6 of 60 experts of [640, 9920]: 307 us, 223 in parts; 1 token,
-// 3 of 4 of [1024, 896]: 16.5 and 21 us).
+// are few (6 tokens, 6 of 60 experts of [640, 9920]: 289 us, 182 in parts; 1 token,
+// 3 of 4 of [1024, 896]: 12.6 and 14.7 us).
 inline bool moe_out_few(int tokens, int hidden, int inter, int experts, int top_k, int cus) {
     if (tokens > kMoeFew) return false;
     const double bytes = 2.0 * hidden * inter * moe_reached(tokens, top_k, experts);

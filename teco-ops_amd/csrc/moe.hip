@@ -6,8 +6,12 @@
 //   out[t] = T( sum_j w_j (h_j W_out[e_j]^T) )
 //
 // What bounds it is reading the chosen experts' weights, 3 H I values each.
-// Tokens are therefore grouped by expert: every weight is read from HBM once for
-// all tokens of its expert (gemv_stream.h), not once per token.
+// Tokens are therefore grouped by expert: a weight is read from HBM once for an item
+// of up to XR tokens of its expert (gemv_stream.h), not once per token.  XR comes of
+// an even spread of the tokens, and the whole of W is swept again for the items past
+// an expert's first: 512 tokens, 1 of 128 experts of [2048, 768], 204 us spread at
+// random (188 to read the weights), 54 all at one expert; 512 tokens, 2 of 8 of [4096,
+// 14336], 1305 us where one pass of the weights would take 447.
 //   route    softmax, top k and the groups: per expert a list of its (token, j)
 //            pairs, cut into items of up to XR pairs
 //   in       per item and block of rows of W_in: h of its pairs
@@ -604,8 +608,8 @@ bool launch_as(MoeArgs a, int items, hipStream_t s) {
 
 // Whether the tokens are routed within the first product: it spares a launch and
 // its wait, but every workgroup does it again at its start, so only where each CU
-// has one of them (2 tokens, 1 of 128 experts of [1792, 672]: 16.7 us with a
-// launch, 13.5 within; 6 tokens, 6 of 60 of [640, 9920], many to a CU: 219 and 397).
+// has one of them (2 tokens, 1 of 128 experts of [1792, 672]: 12.3 us with a
+// launch, 10.5 within; 6 tokens, 6 of 60 of [640, 9920], many to a CU: 182 and 286).
 bool routes_within(const MoeArgs &a, int items, bool copy) {
     const int cus = tecoops::device_cus();
     return few_tokens(a, copy) &&

@@ -465,12 +465,14 @@ def moe_layer(x, w_in, w_out, router_logits, top_k, out, renormalize=True, activ
     [T, E] (float32 or x's type), each token's top_k experts (ties to the lowest
     index; -inf and NaN never chosen), and the sum of their outputs
     (act(x Wg^T) * (x Wu^T)) W_out^T with the routing weights, renormalised over
-    the chosen or not.
+    the chosen or not.  Right for any T, but made for few: every 512 tokens read
+    the experts' weights again.
 
     x [T, H] (rows packed, any distance apart); w_in [E, 2I, H], an expert's gate
     rows before its up rows; w_out [E, H, I]; out [T, H], zero for a token all of
-    whose logits are -inf.  topk_ids int32 and topk_weights float32 [T, top_k]
-    are written when given, best first, -1 and 0 where there is none."""
+    whose logits are -inf; out must not overlap an input.  topk_ids int32 and
+    topk_weights float32 [T, top_k] are written when given, best first, -1 and 0
+    where there is none."""
     refused = []
     if _moe_layer is not None:
         try:
@@ -583,9 +585,10 @@ def rotary_embedding_axes(positions, query, key, head_size, sections, cos_sin_ca
     number of frequencies of each axis, rot_dim / 2 together.  layout:
     "contiguous" gives each axis a range of the frequencies, "interleaved"
     frequency i to axis i % axes while that axis has any left (else to the
-    first), "per_axis" ranges with frequencies of their own, base^(-j / n) for the j-th of an axis' n.  With a cos_sin_cache
-    (float32 [positions, rot_dim]) a token with a position outside it is left as
-    it is; without, angles are computed in 64 bits."""
+    first), "per_axis" ranges with frequencies of their own, base^(-j / n) for
+    the j-th of an axis' n.  With a cos_sin_cache (float32 [positions, rot_dim]) a
+    token with a position outside it is left as it is; without, angles are
+    computed in 64 bits (base is taken in float32)."""
     refused = []
     if _rotary_axes is not None and (rot_dim is None or rot_dim > 0):
         try:
