@@ -463,6 +463,95 @@ tecoopsStatus_t tecoopsRotaryAxesReshapeAndCache(tecoopsHandle_t handle, const i
                                                  int block_size, int write_key,
                                                  tecoopsDataType_t dataType);
 
+/* ---- a decode path held in 4 bits: norms with the rotation, the cache, its
+ *      attention, weight products ---- */
+
+/* The norm of each head of query and key, then the rotation, in one pass, in
+ * place:  y = x / sqrt(mean(x^2) + eps) * w over the head_size elements of a head
+ * (w: query_weight or key_weight, [head_size] of dataType), then y turned as
+ * tecoopsRotaryEmbeddingAxes turns it; fp32 throughout, one rounding.  key may be
+ * NULL, with key_weight.  Positions, sections and layout are those of
+ * tecoopsRotaryEmbeddingAxes; sections may be NULL for one axis.  A token with a
+ * position outside the cos_sin_cache is left as it is, not normalised either.
+ * head_size up to 1024, fewer than 2^24 tokens (head sizes in whole 16-byte words,
+ * aligned, up to 512 are fastest; others up to 2^25 heads of all tokens). */
+tecoopsStatus_t tecoopsQkNormRotary(tecoopsHandle_t handle, const int64_t *positions,
+                                    long long position_stride, int axes, const int *sections,
+                                    tecoopsRotaryLayout_t layout, void *query, void *key,
+                                    const void *query_weight, const void *key_weight, float eps,
+                                    int num_tokens, int num_heads, int num_kv_heads, int head_size,
+                                    int rot_dim, long long query_stride, long long key_stride,
+                                    const float *cos_sin_cache, int max_position, float base,
+                                    int is_neox, tecoopsDataType_t dataType);
+
+/* The same fused with the store into the paged caches, as
+ * tecoopsRotaryReshapeAndCache: the cached values are bit-identical to the two
+ * calls in sequence. */
+tecoopsStatus_t tecoopsQkNormRotaryReshapeAndCache(
+    tecoopsHandle_t handle, const int64_t *positions, long long position_stride, int axes,
+    const int *sections, tecoopsRotaryLayout_t layout, void *query, void *key, const void *value,
+    const void *query_weight, const void *key_weight, float eps, const int64_t *slot_mapping,
+    void *key_cache, void *value_cache, int num_tokens, int num_heads, int num_kv_heads,
+    int head_size, int rot_dim, long long query_stride, long long key_stride,
+    long long value_stride, const float *cos_sin_cache, int max_position, float base, int is_neox,
+    int num_blocks, int block_size, int write_key, tecoopsDataType_t dataType);
+
+/* reshape_and_cache into a cache held in 4 bits.  key / value [num_tokens,
+ * num_kv_heads, head_size] with token strides in elements (heads of a token
+ * adjacent).  A row x of a head is held as codes n of 0..15 and a pair (scale, low)
+ * of dataType that stands for scale * n + low:
+ *   low = min x,  scale = (max x - min x) / 15 in fp32, rounded to dataType,
+ *   n = (x - low) / scale to the nearest integer, ties to even, at most 15
+ *   (0 where scale is 0);
+ * a row with a NaN, or whose range is not finite in fp32, is (NaN, NaN), codes 0.
+ * key_cache / value_cache uint8 [num_blocks, num_kv_heads, block_size, head_size /
+ * 2], element 2j in the low half of byte j; key_scales / value_scales dataType
+ * [num_blocks, num_kv_heads, block_size, 2].  Slots < 0 or past the cache are not
+ * stored; a slot is at most once in a call.  head_size a multiple of 8 up to 512;
+ * fewer than 2^26 (token, head) rows; num_tokens = 0 is done without a launch. */
+tecoopsStatus_t tecoopsReshapeAndCacheInt4(tecoopsHandle_t handle, const void *key,
+                                           const void *value, const int64_t *slot_mapping,
+                                           void *key_cache, void *value_cache, void *key_scales,
+                                           void *value_scales, int num_tokens, int num_kv_heads,
+                                           int head_size, long long key_stride,
+                                           long long value_stride, int num_blocks, int block_size,
+                                           tecoopsDataType_t dataType);
+
+/* Attention over that cache.  Rows, lengths, masks and bounds are those of
+ * tecoopsFlashAttentionEx with cu_seqlens_q (bottom-right causal, rows of no
+ * sequence and rows without a key written as zeros, the bounds shape the launch
+ * alone), but the softmax has no clamp at 0, so that scores of any size are
+ * weighed.  q and out [total_q, num_heads, head_size] packed; block_table int32
+ * [batch, blocks_per_seq], rows block_table_stride apart; head_size in {32, 64,
+ * 96, 128, 160, 192}.  Up to 64 (query row, head) pairs of a kv head read K and V
+ * as they are held; longer queries widen them to fp16 first (one more rounding).
+ * What the cache holds behind a sequence's last key is not used, whatever it is.
+ * workspace: tecoopsGetFlashAttentionInt4WorkspaceSize() bytes for the same sizes
+ * and bounds, 16-byte aligned; with less the keys are cut into fewer splits.  NULL
+ * uses the handle's scratch, and none on a stream under capture (unsplit: slower,
+ * the same result up to rounding). */
+tecoopsStatus_t tecoopsFlashAttentionInt4(
+    tecoopsHandle_t handle, int max_seqlen_q, int max_seqlen_k, const int *cu_seqlens_q,
+    const int *kv_seq_lens, const int *block_table, long long block_table_stride, int batch,
+    int blocks_per_seq, const void *q, const void *key_cache, const void *value_cache,
+    const void *key_scales, const void *value_scales, void *out, int total_q, int num_heads,
+    int num_kv_heads, int head_size, int num_blocks, int block_size, float softmax_scale, int causal,
+    void *workspace, size_t workspace_bytes, tecoopsDataType_t dataType);
+tecoopsStatus_t tecoopsGetFlashAttentionInt4WorkspaceSize(int batch, int total_q, int num_heads,
+                                                          int num_kv_heads, int head_size,
+                                                          int max_seqlen_q, int max_seqlen_k,
+                                                          size_t *bytes);
+
+/* y[b, n] = sum_k W[n, k] x[b, k] with W[n, k] = (code - zero) * scale, fp32
+ * accumulation.  weight uint8 [n, k / 2], 16-byte aligned, code 2j of a row in the
+ * low half of byte j; scales and zeros dataType [n, k / group_size] (zeros NULL: 8
+ * everywhere; they need not be whole); x [batch, k], y [batch, n].  group_size a
+ * multiple of 32 that divides k.  For decode batches; batch = 0 is done without a
+ * launch. */
+tecoopsStatus_t tecoopsGemvInt4(tecoopsHandle_t handle, const void *weight, const void *scales,
+                                const void *zeros, const void *x, void *y, int batch, int n, int k,
+                                int group_size, tecoopsDataType_t dataType);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,16 +35,20 @@ SOURCES = [
     "handle.cpp",
     "memset.hip",
     "reshape_and_cache.hip",
+    "cache_int4.hip",
     "rms_norm.hip",
     "rotary.hip",
+    "qk_norm_rotary.hip",
     "causal_conv1d.hip",
     "gemv.hip",
     "gemv_batch.hip",
     "linear.hip",
     "moe.hip",
+    "gemv_int4.hip",
     "flash_attention.hip",
     "fa_split.hip",
     "fa_noalloc.hip",
+    "fa_int4.hip",
 ]
 
 ARCH = os.environ.get("TECOOPS_OFFLOAD_ARCH", "gfx950")

@@ -19,8 +19,7 @@
 // Positions of several axes (time, height, width of images and video): pair i
 // turns by the position of the axis its frequency belongs to.  Only the angles
 // of a token differ, so the same kernels run with another source of them.
-#include "common.h"
-#include "device.h"
+#include "rotary.h"
 
 #include <type_traits>
 
@@ -29,7 +28,6 @@ namespace {
 using namespace tecoops::dev;
 
 constexpr int kThreads = 256;
-constexpr int kMaxHalf = 256;  // rot_dim <= 512
 
 // Where the angles of token t come from: angle(t, i) is (cos, sin) of pair i,
 // skipped(t) whether the token is left unturned.
@@ -69,70 +67,6 @@ struct OnePosition {
     }
 };
 
-// One position per token and axis, positions[axis * stride + t].  first[a] is
-// the first frequency of axis a in ranges of them, first[a + 1] - first[a] its
-// number of frequencies.  Angles are computed in turns in 64 bits and reduced
-// to half a turn before sin and cos, so that far positions lose nothing: in 32
-// bits an angle of 200000 is off by up to 0.008.
-struct AxisPositions {
-    const int64_t *__restrict__ positions;
-    long long stride;
-    const float *__restrict__ cos_sin_cache;
-    int max_position, rot_dim, axes, layout;
-    int first[TECOOPS_ROTARY_MAX_AXES + 1];
-    double log2_base;
-
-    static constexpr bool kCopySkipped = true;  // as they are, whatever they hold
-    // The 64-bit angles take a good part of a microsecond: a workgroup's first loads
-    // of q, k and v are under way meanwhile, and few tasks take 128 threads (q and k
-    // [16380, 16, 128] fp16 in rows of 12288 bytes 49.7 us without, 46.0 with; with
-    // the store, 4 tokens 4.2 and 3.8 us, 8191 tokens 40 us either way).
-    static constexpr bool kEarlyLoads = true;
-
-    __device__ __forceinline__ float2 angle(int t, int i) const {
-        const int half = rot_dim >> 1;
-        int axis = 0, from = 0, n = first[1];
-        if (layout == TECOOPS_ROTARY_INTERLEAVED) {
-            const int a = i % axes;
-#pragma unroll
-            for (int b = 1; b < TECOOPS_ROTARY_MAX_AXES; ++b)
-                if (a == b && i < axes * (first[b + 1] - first[b])) axis = b;
-        } else {
-#pragma unroll
-            for (int b = 1; b < TECOOPS_ROTARY_MAX_AXES; ++b)
-                if (b < axes && i >= first[b]) {
-                    axis = b;
-                    from = first[b];
-                    n = first[b + 1] - first[b];
-                }
-        }
-        const int64_t pos = positions[axis * stride + t];
-        float c = 1.0f, s = 0.0f;
-        if (cos_sin_cache != nullptr) {
-            if (pos >= 0 && pos < max_position) {
-                c = cos_sin_cache[pos * rot_dim + i];
-                s = cos_sin_cache[pos * rot_dim + half + i];
-            }
-            return make_float2(c, s);
-        }
-        const double power = layout == TECOOPS_ROTARY_PER_AXIS
-                                 ? static_cast<double>(i - from) / n
-                                 : static_cast<double>(i) / half;
-        const double turns = static_cast<double>(pos) * (exp2(-power * log2_base) * 0.15915494309189535);
-        sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-        return make_float2(c, s);
-    }
-    __device__ __forceinline__ bool skipped(int t) const {
-        if (cos_sin_cache == nullptr) return false;
-        bool out = false;
-        for (int a = 0; a < axes; ++a) {
-            const int64_t pos = positions[a * stride + t];
-            out = out || pos < 0 || pos >= max_position;
-        }
-        return out;
-    }
-};
-
 // One token per workgroup, each thread's (at most two) tasks loaded together
 // before any store.  More tokens per workgroup put more of q and k in flight
 // at once, which the memory system serves slower.  q [8192, 32, 128], k
@@ -145,16 +79,6 @@ struct AxisPositions {
 constexpr int kTokensPerBlock = 1;
 constexpr int kRotBatch = 2;  // rotation tasks per thread with loads in flight together
 constexpr int kFusedBatch = 2;  // tasks per thread in flight together, fused kernel
-
-// o1 = x1 cos - x2 sin, o2 = x2 cos + x1 sin with the roundings spelled out
-// (one product, then one fused multiply-add), so every kernel that rotates
-// gets bit-identical results whatever the compiler would contract.
-__device__ __forceinline__ float rot1(float x1, float x2, float c, float s) {
-    return fmaf(x1, c, -(x2 * s));
-}
-__device__ __forceinline__ float rot2(float x1, float x2, float c, float s) {
-    return fmaf(x2, c, x1 * s);
-}
 
 // Rotation of 4 NeoX pairs (x1 = a, x2 = b, 4 elements each, as 8-byte words)
 // with (cos, sin) c[0..3]: o1 = x1 cos - x2 sin, o2 = x2 cos + x1 sin.
@@ -733,13 +657,6 @@ __global__ void __launch_bounds__(kThreads) rotary_cache_kernel(Angles angles, F
     }
 }
 
-// Heads and strides of a call, and the widest words it can be done in.
-struct Rows {
-    void *query, *key;
-    int num_tokens, num_heads, num_kv_heads, head_size, rot_dim;
-    long long query_stride, key_stride;
-};
-
 template <typename T, bool NEOX, int VW, typename Angles>
 void launch_vw(const Angles &an, const Rows &r, hipStream_t s) {
     const unsigned grid = tecoops::ceil_div(r.num_tokens, kTokensPerBlock);
@@ -771,24 +688,6 @@ void launch(int vw, const Angles &an, const Rows &r, hipStream_t s) {
         launch_vw<T, NEOX, 0>(an, r, s);
 }
 
-// Arguments that both kinds of positions share.
-tecoopsStatus_t check_rows(const Rows &r, const void *positions, const float *cos_sin_cache,
-                           int max_position, float base, tecoopsDataType_t dataType) {
-    if (positions == nullptr || r.query == nullptr) return TECOOPS_STATUS_BAD_PARAM;
-    if (r.num_tokens <= 0 || r.num_heads <= 0 || r.head_size <= 0) return TECOOPS_STATUS_BAD_PARAM;
-    if (r.key != nullptr && r.num_kv_heads <= 0) return TECOOPS_STATUS_BAD_PARAM;
-    if (r.rot_dim <= 0 || (r.rot_dim & 1) || r.rot_dim > r.head_size || r.rot_dim / 2 > kMaxHalf)
-        return TECOOPS_STATUS_BAD_PARAM;
-    if (r.query_stride < static_cast<long long>(r.num_heads) * r.head_size)
-        return TECOOPS_STATUS_BAD_PARAM;
-    if (r.key != nullptr && r.key_stride < static_cast<long long>(r.num_kv_heads) * r.head_size)
-        return TECOOPS_STATUS_BAD_PARAM;
-    if (cos_sin_cache != nullptr && max_position <= 0) return TECOOPS_STATUS_BAD_PARAM;
-    if (cos_sin_cache == nullptr && !(base > 0.0f)) return TECOOPS_STATUS_BAD_PARAM;
-    if (!tecoops::is_16bit_float(dataType)) return TECOOPS_STATUS_BAD_PARAM;
-    return TECOOPS_STATUS_SUCCESS;
-}
-
 template <typename Angles>
 tecoopsStatus_t run_rotary(const Angles &an, Rows r, int is_neox, tecoopsDataType_t dataType,
                            hipStream_t s) {
@@ -817,27 +716,6 @@ tecoopsStatus_t run_rotary(const Angles &an, Rows r, int is_neox, tecoopsDataTyp
         else launch<bf16, false>(vw, an, r, s);
     }
     TECO_CHECK_LAUNCH("rotary_embedding");
-    return TECOOPS_STATUS_SUCCESS;
-}
-
-// The paged caches that the fused kernel writes to.
-struct Pages {
-    const void *value;
-    const int64_t *slot_mapping;
-    void *key_cache, *value_cache;
-    long long value_stride;
-    int num_blocks, block_size, write_key;
-};
-
-tecoopsStatus_t check_pages(const Rows &r, const Pages &g) {
-    if (r.key == nullptr || g.value == nullptr || g.slot_mapping == nullptr ||
-        g.key_cache == nullptr || g.value_cache == nullptr)
-        return TECOOPS_STATUS_BAD_PARAM;
-    if (g.num_blocks <= 0 || g.block_size <= 0) return TECOOPS_STATUS_BAD_PARAM;
-    if (g.value_stride < static_cast<long long>(r.num_kv_heads) * r.head_size)
-        return TECOOPS_STATUS_BAD_PARAM;
-    if (static_cast<long long>(g.num_blocks) * g.block_size >= (1ll << 31))
-        return TECOOPS_STATUS_NOT_SUPPORTED;
     return TECOOPS_STATUS_SUCCESS;
 }
 
@@ -907,44 +785,6 @@ tecoopsStatus_t run_fused(const Angles &an, const Rows &r, const Pages &g, int i
 OnePosition one_position(const int64_t *positions, const float *cos_sin_cache, int max_position,
                          int rot_dim, float base) {
     return {positions, cos_sin_cache, max_position, rot_dim, cos_sin_cache ? 0.0f : log2f(base)};
-}
-
-// The axes' frequencies have to fill the rotated half; interleaved, frequency
-// i belongs to axis i % axes while that axis has any left, so every axis but
-// the first has to find its last one inside the half.
-tecoopsStatus_t axis_positions(AxisPositions *out, const int64_t *positions,
-                               long long position_stride, int axes, const int *sections, int layout,
-                               const Rows &r, const float *cos_sin_cache, int max_position,
-                               float base) {
-    if (axes < 1 || axes > TECOOPS_ROTARY_MAX_AXES || sections == nullptr)
-        return TECOOPS_STATUS_BAD_PARAM;
-    if (layout < TECOOPS_ROTARY_CONTIGUOUS || layout > TECOOPS_ROTARY_PER_AXIS)
-        return TECOOPS_STATUS_BAD_PARAM;
-    // positions are only read: all axes may share one row of them (stride 0)
-    if (axes > 1 && position_stride != 0 && position_stride < r.num_tokens)
-        return TECOOPS_STATUS_BAD_PARAM;
-    const int half = r.rot_dim / 2;
-    int sum = 0;
-    for (int a = 0; a < TECOOPS_ROTARY_MAX_AXES; ++a) {
-        out->first[a] = sum;
-        if (a >= axes) continue;
-        if (sections[a] < 0 || sections[a] > half - sum) return TECOOPS_STATUS_BAD_PARAM;
-        if (layout == TECOOPS_ROTARY_INTERLEAVED && a > 0 && sections[a] > 0 &&
-            axes * (sections[a] - 1) + a >= half)
-            return TECOOPS_STATUS_BAD_PARAM;
-        sum += sections[a];
-    }
-    out->first[TECOOPS_ROTARY_MAX_AXES] = sum;
-    if (sum != half) return TECOOPS_STATUS_BAD_PARAM;
-    out->positions = positions;
-    out->stride = position_stride;
-    out->cos_sin_cache = cos_sin_cache;
-    out->max_position = max_position;
-    out->rot_dim = r.rot_dim;
-    out->axes = axes;
-    out->layout = layout;
-    out->log2_base = cos_sin_cache ? 0.0 : log2(static_cast<double>(base));
-    return TECOOPS_STATUS_SUCCESS;
 }
 
 }  // namespace

@@ -525,6 +525,209 @@ void rotary_axes_reshape_and_cache(const Tensor &positions, Tensor &query, Tenso
           "rotary_axes_reshape_and_cache");
 }
 
+// The positions and sections of a call in one or several axes: [tokens] and no
+// sections is one axis that all frequencies turn by.
+struct Axes {
+    Tensor positions;
+    std::vector<int64_t> sections;
+
+    Axes(const Tensor &p, at::IntArrayRef sec, const Tensor *cos_sin_cache, int64_t head_size, int64_t rot)
+        : positions(p.dim() == 1 ? p.unsqueeze(0) : p), sections(sec.vec()) {
+        if (!sections.empty()) return;
+        if (cos_sin_cache && cos_sin_cache->dim() == 2) rot = cos_sin_cache->size(1);
+        sections.push_back((rot > 0 ? rot : head_size) / 2);
+    }
+};
+
+void need_weight(const Tensor *w, const Tensor &query, int64_t head_size, const char *name) {
+    TORCH_CHECK(w && w->dim() == 1 && w->size(0) == head_size, "tecoops: ", name, " must be [head_size]");
+    need_dtype(*w, query.scalar_type(), name);
+    need_contiguous({w});
+}
+
+void qk_norm_rotary(const Tensor &positions, Tensor &query, const c10::optional<Tensor> &key,
+                    const Tensor &query_weight, const c10::optional<Tensor> &key_weight, int64_t head_size,
+                    double eps, at::IntArrayRef sections, const c10::optional<Tensor> &cos_sin_cache,
+                    bool is_neox, double base, int64_t rot_dim, c10::string_view layout) {
+    const Tensor *k = given(key), *table = given(cos_sin_cache), *kw = given(key_weight);
+    need_cuda({&positions, &query, k, &query_weight, kw});
+    same_device(query, {&query_weight, kw});
+    const Axes ax(positions, sections, table, head_size, rot_dim);
+    const AxesArgs a(ax.positions, query, k, head_size, ax.sections, table, rot_dim, layout);
+    need_weight(&query_weight, query, head_size, "query_weight");
+    if (k) need_weight(kw, query, head_size, "key_weight");
+    if (a.tokens == 0) return;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(query.device());
+    check(tecoopsQkNormRotary(
+              handle_for(query), ax.positions.data_ptr<int64_t>(), a.position_stride,
+              static_cast<int>(a.sections.size()), a.sections.data(), a.layout, query.data_ptr(),
+              k ? k->data_ptr() : nullptr, query_weight.data_ptr(), k ? kw->data_ptr() : nullptr,
+              static_cast<float>(eps), a.tokens, a.heads, a.kv_heads, fits_int(head_size, "head_size"), a.rot_dim,
+              a.query_stride, a.key_stride, a.table, a.max_position, static_cast<float>(base), is_neox ? 1 : 0,
+              dtype_of(query)),
+          "qk_norm_rotary");
+}
+
+void qk_norm_rotary_reshape_and_cache(const Tensor &positions, Tensor &query, Tensor &key, const Tensor &value,
+                                      const Tensor &query_weight, const Tensor &key_weight,
+                                      const Tensor &slot_mapping, Tensor &key_cache, Tensor &value_cache,
+                                      int64_t head_size, double eps, at::IntArrayRef sections,
+                                      const c10::optional<Tensor> &cos_sin_cache, bool is_neox, double base,
+                                      int64_t rot_dim, c10::string_view layout, bool write_key) {
+    const Tensor *table = given(cos_sin_cache);
+    need_cuda({&positions, &query, &key, &value, &query_weight, &key_weight, &slot_mapping, &key_cache, &value_cache});
+    same_device(query, {&query_weight, &key_weight, &value, &slot_mapping, &key_cache, &value_cache});
+    const Axes ax(positions, sections, table, head_size, rot_dim);
+    const AxesArgs a(ax.positions, query, &key, head_size, ax.sections, table, rot_dim, layout);
+    need_weight(&query_weight, query, head_size, "query_weight");
+    need_weight(&key_weight, query, head_size, "key_weight");
+    need_contiguous({&slot_mapping, &key_cache, &value_cache});
+    need_dtype(slot_mapping, at::kLong, "slot_mapping");
+    need_dtype(key_cache, query.scalar_type(), "key_cache");
+    need_dtype(value_cache, query.scalar_type(), "value_cache");
+    TORCH_CHECK(slot_mapping.numel() == a.tokens, "tecoops: slot_mapping must hold a slot per token");
+    TORCH_CHECK(key_cache.dim() == 4 && key_cache.size(1) == a.kv_heads && key_cache.size(3) == head_size &&
+                    value_cache.sizes() == key_cache.sizes(),
+                "tecoops: caches must be [num_blocks, kv heads, block_size, head_size]");
+    int64_t value_stride = 0;
+    TORCH_CHECK(a.rows(value, query, head_size, "value", &value_stride) == a.kv_heads,
+                "tecoops: value must match key");
+    if (a.tokens == 0) return;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(query.device());
+    check(tecoopsQkNormRotaryReshapeAndCache(
+              handle_for(query), ax.positions.data_ptr<int64_t>(), a.position_stride,
+              static_cast<int>(a.sections.size()), a.sections.data(), a.layout, query.data_ptr(), key.data_ptr(),
+              value.data_ptr(), query_weight.data_ptr(), key_weight.data_ptr(), static_cast<float>(eps),
+              slot_mapping.data_ptr<int64_t>(), key_cache.data_ptr(), value_cache.data_ptr(), a.tokens, a.heads,
+              a.kv_heads, fits_int(head_size, "head_size"), a.rot_dim, a.query_stride, a.key_stride, value_stride,
+              a.table, a.max_position, static_cast<float>(base), is_neox ? 1 : 0,
+              fits_int(key_cache.size(0), "num_blocks"), fits_int(key_cache.size(2), "block_size"),
+              write_key ? 1 : 0, dtype_of(query)),
+          "qk_norm_rotary_reshape_and_cache");
+}
+
+// The four tensors of a 4-bit cache of `like`'s type, checked.
+void need_cache_int4(const Tensor &key_cache, const Tensor &value_cache, const Tensor &key_scales,
+                     const Tensor &value_scales, const Tensor &like, int64_t head_size) {
+    need_cuda({&key_cache, &value_cache, &key_scales, &value_scales});
+    same_device(like, {&key_cache, &value_cache, &key_scales, &value_scales});
+    need_contiguous({&key_cache, &value_cache, &key_scales, &value_scales});
+    need_dtype(key_cache, at::kByte, "key_cache");
+    need_dtype(value_cache, at::kByte, "value_cache");
+    need_dtype(key_scales, like.scalar_type(), "key_scales");
+    need_dtype(value_scales, like.scalar_type(), "value_scales");
+    TORCH_CHECK(key_cache.dim() == 4 && 2 * key_cache.size(3) == head_size && value_cache.sizes() == key_cache.sizes(),
+                "tecoops: caches must be uint8 [num_blocks, kv heads, block_size, head_size / 2]");
+    TORCH_CHECK(key_scales.dim() == 4 && key_scales.size(0) == key_cache.size(0) &&
+                    key_scales.size(1) == key_cache.size(1) && key_scales.size(2) == key_cache.size(2) &&
+                    key_scales.size(3) == 2 && value_scales.sizes() == key_scales.sizes(),
+                "tecoops: scales must be [num_blocks, kv heads, block_size, 2]");
+}
+
+// [tokens, heads, head_size] with packed heads, tokens any distance apart: the distance.
+int64_t token_stride(const Tensor &t, const char *name) {
+    const int64_t row = t.size(1) * t.size(2);
+    TORCH_CHECK((t.size(2) <= 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) == t.size(2)) &&
+                    (t.size(0) <= 1 || t.stride(0) >= row),
+                "tecoops: the heads of a token of ", name, " must be adjacent");
+    return t.size(0) > 1 ? t.stride(0) : row;
+}
+
+void reshape_and_cache_int4(const Tensor &key, const Tensor &value, const Tensor &slot_mapping, Tensor &key_cache,
+                            Tensor &value_cache, Tensor &key_scales, Tensor &value_scales) {
+    need_cuda({&key, &value, &slot_mapping});
+    same_device(key, {&value, &slot_mapping});
+    const tecoopsDataType_t dt = dtype_of(key);
+    need_dtype(value, key.scalar_type(), "value");
+    need_dtype(slot_mapping, at::kLong, "slot_mapping");
+    need_contiguous({&slot_mapping});
+    TORCH_CHECK(key.dim() == 3 && value.sizes() == key.sizes() && slot_mapping.numel() == key.size(0),
+                "reshape_and_cache_int4: key / value [tokens, kv heads, head_size], slot_mapping [tokens]");
+    need_cache_int4(key_cache, value_cache, key_scales, value_scales, key, key.size(2));
+    TORCH_CHECK(key_cache.size(1) == key.size(1), "reshape_and_cache_int4: the caches' kv heads must be key's");
+    const int64_t ks = token_stride(key, "key"), vs = token_stride(value, "value");
+    if (key.size(0) == 0) return;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(key.device());
+    check(tecoopsReshapeAndCacheInt4(
+              handle_for(key), key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr<int64_t>(), key_cache.data_ptr(),
+              value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), fits_int(key.size(0), "tokens"),
+              fits_int(key.size(1), "kv heads"), fits_int(key.size(2), "head_size"), ks, vs,
+              fits_int(key_cache.size(0), "num_blocks"), fits_int(key_cache.size(2), "block_size"), dt),
+          "reshape_and_cache_int4");
+}
+
+void flash_attn_varlen_int4(const Tensor &q, const Tensor &key_cache, const Tensor &value_cache,
+                            const Tensor &key_scales, const Tensor &value_scales, int64_t max_seqlen_q,
+                            const Tensor &cu_seqlens_q, int64_t max_seqlen_k, const Tensor &seqused_k,
+                            double softmax_scale, bool causal, const Tensor &block_table, Tensor &out) {
+    need_cuda({&q, &cu_seqlens_q, &seqused_k, &block_table, &out});
+    same_device(q, {&cu_seqlens_q, &seqused_k, &block_table, &out});
+    const tecoopsDataType_t dt = dtype_of(q);
+    TORCH_CHECK(q.dim() == 3 && out.sizes() == q.sizes(), "flash_attn_varlen_int4: q and out [rows, heads, head_size]");
+    need_dtype(out, q.scalar_type(), "out");
+    need_contiguous({&q, &out, &cu_seqlens_q, &seqused_k});
+    need_cache_int4(key_cache, value_cache, key_scales, value_scales, q, q.size(2));
+    need_dtype(cu_seqlens_q, at::kInt, "cu_seqlens_q");
+    need_dtype(seqused_k, at::kInt, "seqused_k");
+    need_dtype(block_table, at::kInt, "block_table");
+    const int64_t batch = seqused_k.numel();
+    TORCH_CHECK(batch > 0 && cu_seqlens_q.numel() == batch + 1 && block_table.dim() == 2 &&
+                    block_table.size(0) == batch && (block_table.size(1) <= 1 || block_table.stride(1) == 1),
+                "flash_attn_varlen_int4: cu_seqlens_q [batch + 1], seqused_k [batch], block_table [batch, blocks] "
+                "with adjacent entries in a row");
+    const auto bound = [](int64_t v) { return static_cast<int>(std::min<int64_t>(std::max<int64_t>(v, 0), 0x7fffffff)); };
+    const int total = fits_int(q.size(0), "rows"), heads = fits_int(q.size(1), "heads"),
+              kv_heads = fits_int(key_cache.size(1), "kv heads"), head_size = fits_int(q.size(2), "head_size");
+    const int most_q = bound(max_seqlen_q);
+    // (keys that the table can name bound those of a sequence)
+    const int64_t cap = std::max<int64_t>(1, std::min<int64_t>(block_table.size(1) * key_cache.size(2), 0x7fffffff));
+    const int most_k = static_cast<int>(max_seqlen_k > 0 ? std::min(max_seqlen_k, cap) : cap);
+    if (total == 0) return;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
+    size_t bytes = 0;
+    check(tecoopsGetFlashAttentionInt4WorkspaceSize(static_cast<int>(batch), total, heads, kv_heads, head_size, most_q,
+                                                    most_k, &bytes),
+          "flash_attn_varlen_int4");
+    const Tensor ws = workspace_of(bytes, q);
+    check(tecoopsFlashAttentionInt4(
+              handle_for(q), most_q, most_k, cu_seqlens_q.data_ptr<int>(), seqused_k.data_ptr<int>(),
+              block_table.data_ptr<int>(), block_table.size(0) > 1 ? block_table.stride(0) : block_table.size(1),
+              static_cast<int>(batch), fits_int(block_table.size(1), "blocks"), q.data_ptr(), key_cache.data_ptr(),
+              value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), out.data_ptr(), total, heads,
+              kv_heads, head_size, fits_int(key_cache.size(0), "num_blocks"), fits_int(key_cache.size(2), "block_size"),
+              softmax_scale > 0 ? static_cast<float>(softmax_scale) : -1.0f, causal ? 1 : 0,
+              bytes ? ws.data_ptr() : nullptr, bytes, dt),
+          "flash_attn_varlen_int4");
+}
+
+void gemv_int4(const Tensor &weight, const Tensor &scales, const Tensor &x, Tensor &out,
+               const c10::optional<Tensor> &zeros) {
+    const Tensor *z = given(zeros);
+    need_cuda({&weight, &scales, &x, &out, z});
+    same_device(x, {&weight, &scales, &out, z});
+    need_contiguous({&weight, &scales, &x, &out, z});
+    const tecoopsDataType_t dt = dtype_of(x);
+    need_dtype(weight, at::kByte, "weight");
+    need_dtype(scales, x.scalar_type(), "scales");
+    need_dtype(out, x.scalar_type(), "out");
+    TORCH_CHECK((x.dim() == 1 || x.dim() == 2) && weight.dim() == 2 && scales.dim() == 2,
+                "gemv_int4: weight [N, K / 2], scales [N, K / group], x [B, K] or [K]");
+    const int b = x.dim() == 2 ? fits_int(x.size(0), "B") : 1, n = fits_int(weight.size(0), "N"),
+              k = fits_int(2 * weight.size(1), "K");
+    TORCH_CHECK(x.size(-1) == k && out.numel() == static_cast<int64_t>(b) * n && scales.size(0) == n &&
+                    scales.size(1) > 0 && k > 0 && k % scales.size(1) == 0,
+                "gemv_int4: weight [N, K / 2], scales [N, K / group], x [B, K], out [B, N]");
+    if (z) {
+        need_dtype(*z, x.scalar_type(), "zeros");
+        TORCH_CHECK(z->sizes() == scales.sizes(), "gemv_int4: zeros must match scales");
+    }
+    if (b == 0) return;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    check(tecoopsGemvInt4(handle_for(x), weight.data_ptr(), scales.data_ptr(), z ? z->data_ptr() : nullptr, x.data_ptr(),
+                          out.data_ptr(), b, n, k, static_cast<int>(k / scales.size(1)), dt),
+          "gemv_int4");
+}
+
 void memset_(Tensor &t, int64_t value) {
     need_cuda({&t});
     check(tecoopsMemset(handle_for(t), t.data_ptr(), static_cast<int>(value),
@@ -568,6 +771,22 @@ TORCH_LIBRARY(tecoops, m) {
           "Tensor value, Tensor slot_mapping, Tensor(c!) key_cache, Tensor(d!) value_cache, "
           "int head_size, int[] sections, Tensor? cos_sin_cache, bool is_neox, float base, "
           "int rot_dim, str layout, bool write_key) -> ()");
+    m.def("qk_norm_rotary(Tensor positions, Tensor(a!) query, Tensor(b!)? key, Tensor query_weight, "
+          "Tensor? key_weight, int head_size, float eps, int[] sections, Tensor? cos_sin_cache, "
+          "bool is_neox, float base, int rot_dim, str layout) -> ()");
+    m.def("qk_norm_rotary_reshape_and_cache(Tensor positions, Tensor(a!) query, Tensor(b!) key, "
+          "Tensor value, Tensor query_weight, Tensor key_weight, Tensor slot_mapping, "
+          "Tensor(c!) key_cache, Tensor(d!) value_cache, int head_size, float eps, int[] sections, "
+          "Tensor? cos_sin_cache, bool is_neox, float base, int rot_dim, str layout, "
+          "bool write_key) -> ()");
+    m.def("reshape_and_cache_int4(Tensor key, Tensor value, Tensor slot_mapping, "
+          "Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor(c!) key_scales, "
+          "Tensor(d!) value_scales) -> ()");
+    m.def("flash_attn_varlen_int4(Tensor q, Tensor key_cache, Tensor value_cache, Tensor key_scales, "
+          "Tensor value_scales, int max_seqlen_q, Tensor cu_seqlens_q, int max_seqlen_k, "
+          "Tensor seqused_k, float softmax_scale, bool causal, Tensor block_table, "
+          "Tensor(a!) out) -> ()");
+    m.def("gemv_int4(Tensor weight, Tensor scales, Tensor x, Tensor(a!) out, Tensor? zeros) -> ()");
     m.def("memset(Tensor(a!) t, int value) -> ()");
 }
 
@@ -585,5 +804,10 @@ TORCH_LIBRARY_IMPL(tecoops, CUDA, m) {
     m.impl("moe_layer", &moe_layer);
     m.impl("rotary_embedding_axes", &rotary_embedding_axes);
     m.impl("rotary_axes_reshape_and_cache", &rotary_axes_reshape_and_cache);
+    m.impl("qk_norm_rotary", &qk_norm_rotary);
+    m.impl("qk_norm_rotary_reshape_and_cache", &qk_norm_rotary_reshape_and_cache);
+    m.impl("reshape_and_cache_int4", &reshape_and_cache_int4);
+    m.impl("flash_attn_varlen_int4", &flash_attn_varlen_int4);
+    m.impl("gemv_int4", &gemv_int4);
     m.impl("memset", &memset_);
 }

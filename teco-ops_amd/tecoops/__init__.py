@@ -42,7 +42,9 @@ __all__ = [
     "flash_attn_varlen_func", "causal_conv1d_fn_torch",
     # extensions
     "rotary_embedding", "rotary_reshape_and_cache", "gemv", "gemv_int8", "causal_conv1d",
-    "memset", "linear", "moe_layer", "rotary_embedding_axes", "rotary_axes_reshape_and_cache", "ops",
+    "memset", "linear", "moe_layer", "rotary_embedding_axes", "rotary_axes_reshape_and_cache",
+    "qk_norm_rotary", "qk_norm_rotary_reshape_and_cache", "reshape_and_cache_int4",
+    "flash_attn_varlen_int4", "gemv_int4", "ops",
 ]
 
 _tls = threading.local()   # per thread: {device index: _Handle}
@@ -655,6 +657,278 @@ def rotary_axes_reshape_and_cache(positions, query, key, value, slot_mapping, ke
              _ptr(key), _ptr(value), _ptr(slot_mapping), _ptr(key_cache), _ptr(value_cache), *sizes,
              value.stride(0) if T > 1 else Hkv * D, *table, int(bool(is_neox)), key_cache.shape[0],
              key_cache.shape[2], int(bool(write_key)), code)
+
+
+_qk_norm, _qk_norm_cache = _fast("qk_norm_rotary"), _fast("qk_norm_rotary_reshape_and_cache")
+_cache_int4, _attn_int4, _gemv_int4 = (_fast("reshape_and_cache_int4"),
+                                       _fast("flash_attn_varlen_int4"), _fast("gemv_int4"))
+
+
+def _one_or_more_axes(positions, sections, cos_sin_cache, head_size, rot_dim):
+    """positions as [axes, T] and the sections: [T] and None are one axis."""
+    if positions.dim() == 1:
+        positions = positions.unsqueeze(0)
+    if sections is None:
+        if cos_sin_cache is not None and cos_sin_cache.dim() == 2:
+            rot_dim = cos_sin_cache.shape[1]
+        sections = [(head_size if rot_dim is None else rot_dim) // 2]
+    return positions, sections
+
+
+def _check_weight(t, name, query, head_size):
+    if t is None or t.dim() != 1 or t.shape[0] != head_size:
+        raise ValueError(f"tecoops: {name} must be [{head_size}]")
+    _check_dtype(t, name, query.dtype)
+    _check_contiguous(**{name: t})
+    _check_device(query.device, **{name: t})
+
+
+def _check_caches(name, T, Hkv, D, dtype, device, value, slot_mapping, key_cache, value_cache):
+    _check_cuda(value, slot_mapping, key_cache, value_cache)
+    _check_device(device, value=value, slot_mapping=slot_mapping, key_cache=key_cache,
+                  value_cache=value_cache)
+    _check_dtype(slot_mapping, "slot_mapping", torch.int64)
+    for what, t in (("value", value), ("key_cache", key_cache), ("value_cache", value_cache)):
+        _check_dtype(t, what, dtype)
+    _check_contiguous(slot_mapping=slot_mapping, key_cache=key_cache, value_cache=value_cache)
+    if slot_mapping.numel() != T:
+        raise ValueError(f"tecoops.{name}: slot_mapping must hold {T} slots")
+    if key_cache.dim() != 4 or key_cache.shape[1] != Hkv or key_cache.shape[3] != D or \
+            value_cache.shape != key_cache.shape:
+        raise ValueError(f"tecoops.{name}: caches must be [num_blocks, {Hkv}, block_size, {D}]")
+    if value.dim() not in (2, 3) or value.shape[0] != T or math.prod(value.shape[1:]) != Hkv * D:
+        raise ValueError(f"tecoops.{name}: value must match key")
+    if value.dim() == 3 and value.shape[1] > 1 and value.stride(1) != value.shape[2] or \
+            value.shape[-1] > 1 and value.stride(-1) != 1:
+        raise ValueError(f"tecoops.{name}: the heads of a token of value must be adjacent")
+
+
+def qk_norm_rotary(positions, query, key, query_weight, key_weight, head_size, eps=1e-6,
+                   cos_sin_cache=None, is_neox=True, base=10000.0, rot_dim=None, sections=None,
+                   layout="contiguous"):
+    """The norm of each head of query and key, then the rotation, in one pass, in
+    place on query [T, H*D or H, D] and key likewise (or None, with its weight):
+    x / sqrt(mean(x^2) + eps) * weight over the D = head_size elements of a head,
+    turned by the token's position; float32 throughout, one rounding.
+
+    positions int64 [T], or [axes, T] with sections and layout as in
+    rotary_embedding_axes.  query_weight and key_weight [D] of query's type.  The
+    rows may be slices of a wider product's.  A token with a position outside the
+    cos_sin_cache is left as it is, not normalised either."""
+    refused = []
+    if _qk_norm is not None and (rot_dim is None or rot_dim > 0) and sections != []:
+        try:
+            return _qk_norm(positions, query, key, query_weight, key_weight, int(head_size), float(eps),
+                            [] if sections is None else [int(n) for n in sections], cos_sin_cache,
+                            bool(is_neox), float(base), int(rot_dim or 0), layout)
+        except (RuntimeError, TypeError, ValueError) as e:
+            refused.append(e.with_traceback(None))
+    name = "qk_norm_rotary"
+    positions, sections = _one_or_more_axes(positions, sections, cos_sin_cache, head_size, rot_dim)
+    device, before, sizes, table, code = _axes_args(name, positions, query, key, head_size, sections,
+                                                    cos_sin_cache, base, rot_dim, layout)
+    _check_weight(query_weight, "query_weight", query, head_size)
+    if key is not None:
+        _check_weight(key_weight, "key_weight", query, head_size)
+    if refused:
+        _raise(refused, "tecoopsQkNormRotary")
+    if sizes[0] == 0:
+        return
+    _call_on(device, "tecoopsQkNormRotary", _handle(device), *before, _ptr(query), _ptr(key),
+             _ptr(query_weight), _ptr(key_weight), float(eps), *sizes, *table, int(bool(is_neox)), code)
+
+
+def qk_norm_rotary_reshape_and_cache(positions, query, key, value, query_weight, key_weight,
+                                     slot_mapping, key_cache, value_cache, head_size, eps=1e-6,
+                                     cos_sin_cache=None, is_neox=True, base=10000.0, rot_dim=None,
+                                     sections=None, layout="contiguous", write_key=False):
+    """qk_norm_rotary on query (in place) and key, and the key that comes of it and
+    value stored into the paged caches [num_blocks, Hkv, block_size, head_size] at
+    slot_mapping (int64; slots outside the cache are not stored); key is updated in
+    place only when write_key."""
+    refused = []
+    if _qk_norm_cache is not None and (rot_dim is None or rot_dim > 0) and sections != []:
+        try:
+            return _qk_norm_cache(positions, query, key, value, query_weight, key_weight, slot_mapping,
+                                  key_cache, value_cache, int(head_size), float(eps),
+                                  [] if sections is None else [int(n) for n in sections],
+                                  cos_sin_cache, bool(is_neox), float(base), int(rot_dim or 0), layout,
+                                  bool(write_key))
+        except (RuntimeError, TypeError, ValueError) as e:
+            refused.append(e.with_traceback(None))
+    name = "qk_norm_rotary_reshape_and_cache"
+    if key is None:
+        raise ValueError(f"tecoops.{name}: key must be given")
+    positions, sections = _one_or_more_axes(positions, sections, cos_sin_cache, head_size, rot_dim)
+    device, before, sizes, table, code = _axes_args(name, positions, query, key, head_size, sections,
+                                                    cos_sin_cache, base, rot_dim, layout)
+    _check_weight(query_weight, "query_weight", query, head_size)
+    _check_weight(key_weight, "key_weight", query, head_size)
+    T, _, Hkv, D = sizes[:4]
+    _check_caches(name, T, Hkv, D, query.dtype, device, value, slot_mapping, key_cache, value_cache)
+    if refused:
+        _raise(refused, "tecoopsQkNormRotaryReshapeAndCache")
+    if T == 0:
+        return
+    _call_on(device, "tecoopsQkNormRotaryReshapeAndCache", _handle(device), *before, _ptr(query),
+             _ptr(key), _ptr(value), _ptr(query_weight), _ptr(key_weight), float(eps),
+             _ptr(slot_mapping), _ptr(key_cache), _ptr(value_cache), *sizes,
+             value.stride(0) if T > 1 else Hkv * D, *table, int(bool(is_neox)), key_cache.shape[0],
+             key_cache.shape[2], int(bool(write_key)), code)
+
+
+def _check_cache_int4(name, device, dtype, D, key_cache, value_cache, key_scales, value_scales):
+    _check_cuda(key_cache, value_cache, key_scales, value_scales)
+    held = dict(key_cache=key_cache, value_cache=value_cache, key_scales=key_scales,
+                value_scales=value_scales)
+    _check_device(device, **held)
+    _check_contiguous(**held)
+    for what, t in held.items():
+        _check_dtype(t, what, torch.uint8 if what.endswith("cache") else dtype)
+    if key_cache.dim() != 4 or 2 * key_cache.shape[3] != D or value_cache.shape != key_cache.shape:
+        raise ValueError(f"tecoops.{name}: caches must be uint8 [num_blocks, kv heads, block_size, "
+                         f"{D} / 2]")
+    if key_scales.shape != (*key_cache.shape[:3], 2) or value_scales.shape != key_scales.shape:
+        raise ValueError(f"tecoops.{name}: scales must be [num_blocks, kv heads, block_size, 2]")
+
+
+def reshape_and_cache_int4(key, value, slot_mapping, key_cache, value_cache, key_scales,
+                           value_scales):
+    """key/value [T, Hkv, D] (heads of a token adjacent, tokens any distance apart)
+    stored in 4 bits at slot_mapping (int64 [T]; slots outside the cache are not
+    stored, a slot is at most once in a call): a row x of a head as codes n of 0..15
+    and a pair (scale, low) that stands for scale * n + low, low = min x, scale =
+    (max x - min x) / 15 in key's type, n = (x - low) / scale to the nearest.  A row
+    with a NaN or an infinity reads as NaN.
+
+    key_cache / value_cache uint8 [num_blocks, Hkv, block_size, D / 2], element 2j
+    in the low half of byte j; key_scales / value_scales of key's type [num_blocks,
+    Hkv, block_size, 2].  D a multiple of 8 up to 512."""
+    refused = []
+    if _cache_int4 is not None:
+        try:
+            return _cache_int4(key, value, slot_mapping, key_cache, value_cache, key_scales,
+                               value_scales)
+        except (RuntimeError, TypeError, ValueError) as e:
+            refused.append(e.with_traceback(None))
+    name = "reshape_and_cache_int4"
+    _check_cuda(key, value, slot_mapping)
+    code, device = _dtype_code(key), key.device
+    _check_device(device, value=value, slot_mapping=slot_mapping)
+    _check_dtype(value, "value", key.dtype)
+    _check_dtype(slot_mapping, "slot_mapping", torch.int64)
+    _check_contiguous(slot_mapping=slot_mapping)
+    if key.dim() != 3 or value.shape != key.shape or slot_mapping.numel() != key.shape[0]:
+        raise ValueError(f"tecoops.{name}: key / value [tokens, kv heads, head_size], slot_mapping "
+                         "[tokens]")
+    T, H, D = key.shape
+    _check_cache_int4(name, device, key.dtype, D, key_cache, value_cache, key_scales, value_scales)
+    if key_cache.shape[1] != H:
+        raise ValueError(f"tecoops.{name}: the caches must hold {H} kv heads")
+    for what, t in (("key", key), ("value", value)):
+        if D > 1 and t.stride(2) != 1 or H > 1 and t.stride(1) != D or T > 1 and t.stride(0) < H * D:
+            raise ValueError(f"tecoops.{name}: the heads of a token of {what} must be adjacent")
+    if refused:
+        _raise(refused, "tecoopsReshapeAndCacheInt4")
+    if T == 0:
+        return
+    _call_on(device, "tecoopsReshapeAndCacheInt4", _handle(device), _ptr(key), _ptr(value),
+             _ptr(slot_mapping), _ptr(key_cache), _ptr(value_cache), _ptr(key_scales),
+             _ptr(value_scales), T, H, D, key.stride(0) if T > 1 else H * D,
+             value.stride(0) if T > 1 else H * D, key_cache.shape[0], key_cache.shape[2], code)
+
+
+def flash_attn_varlen_int4(q, key_cache, value_cache, key_scales, value_scales, max_seqlen_q,
+                           cu_seqlens_q, max_seqlen_k, seqused_k, softmax_scale, causal, block_table,
+                           out):
+    """flash_attn_varlen_func over a cache held in 4 bits (reshape_and_cache_int4).
+
+    q, out [sum(L), H, D] contiguous; cu_seqlens_q int32 [B+1]; seqused_k int32 [B];
+    block_table int32 [B, blocks] (rows any distance apart).  softmax_scale None: 1 /
+    sqrt(D).  max_seqlen_q and max_seqlen_k shape the launch only.  Rows of no
+    sequence and rows without a visible key are 0; what the cache holds behind a
+    sequence's last key is not used."""
+    refused = []
+    scale = float(softmax_scale) if softmax_scale is not None and softmax_scale > 0 else -1.0
+    if _attn_int4 is not None:
+        try:
+            return _attn_int4(q, key_cache, value_cache, key_scales, value_scales, int(max_seqlen_q),
+                              cu_seqlens_q, int(max_seqlen_k), seqused_k, scale, bool(causal),
+                              block_table, out)
+        except (RuntimeError, TypeError, ValueError) as e:
+            refused.append(e.with_traceback(None))
+    name = "flash_attn_varlen_int4"
+    _check_cuda(q, cu_seqlens_q, seqused_k, block_table, out)
+    code, device = _dtype_code(q), q.device
+    _check_device(device, cu_seqlens_q=cu_seqlens_q, seqused_k=seqused_k, block_table=block_table,
+                  out=out)
+    if q.dim() != 3 or out.shape != q.shape:
+        raise ValueError(f"tecoops.{name}: q and out must be [rows, heads, head_size]")
+    _check_dtype(out, "out", q.dtype)
+    _check_contiguous(q=q, out=out, cu_seqlens_q=cu_seqlens_q, seqused_k=seqused_k)
+    T, H, D = q.shape
+    _check_cache_int4(name, device, q.dtype, D, key_cache, value_cache, key_scales, value_scales)
+    for what, t in (("cu_seqlens_q", cu_seqlens_q), ("seqused_k", seqused_k),
+                    ("block_table", block_table)):
+        _check_dtype(t, what, torch.int32)
+    B = seqused_k.numel()
+    if B == 0 or cu_seqlens_q.numel() != B + 1 or block_table.dim() != 2 or \
+            block_table.shape[0] != B or block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError(f"tecoops.{name}: cu_seqlens_q must be [batch + 1], seqused_k [batch] and "
+                         "block_table [batch, blocks] with adjacent entries in a row")
+    if refused:
+        _raise(refused, "tecoopsFlashAttentionInt4")
+    if T == 0:
+        return
+    NB, Hkv, BS = key_cache.shape[:3]
+    most_q = min(max(int(max_seqlen_q), 0), 0x7fffffff)
+    cap = max(1, min(block_table.shape[1] * BS, 0x7fffffff))
+    most_k = min(int(max_seqlen_k), cap) if max_seqlen_k > 0 else cap
+    space = _workspace(device, "tecoopsGetFlashAttentionInt4WorkspaceSize", B, T, H, Hkv, D, most_q,
+                       most_k)
+    _call_on(device, "tecoopsFlashAttentionInt4", _handle(device), most_q, most_k, _ptr(cu_seqlens_q),
+             _ptr(seqused_k), _ptr(block_table), block_table.stride(0) if B > 1 else block_table.shape[1],
+             B, block_table.shape[1], _ptr(q), _ptr(key_cache), _ptr(value_cache), _ptr(key_scales),
+             _ptr(value_scales), _ptr(out), T, H, Hkv, D, NB, BS, scale, int(bool(causal)), _ptr(space),
+             0 if space is None else space.numel(), code)
+
+
+def gemv_int4(weight, scales, x, out, zeros=None):
+    """out[b, n] = sum_k W[n, k] x[b, k] with 4-bit weights, W[n, k] = (code - zero) *
+    scale of the group that k is in; float32 sums, one rounding.
+
+    weight uint8 [N, K / 2], code 2j of a row in the low half of byte j; scales and
+    zeros (None: 8) of x's type [N, K / group], group a multiple of 32; x [B, K] or
+    [K], out [B, N].  For decode batches."""
+    refused = []
+    if _gemv_int4 is not None:
+        try:
+            return _gemv_int4(weight, scales, x, out, zeros)
+        except (RuntimeError, TypeError, ValueError) as e:
+            refused.append(e.with_traceback(None))
+    _check_cuda(weight, scales, x, out, zeros)
+    code, device = _dtype_code(x), x.device
+    _check_device(device, weight=weight, scales=scales, out=out, zeros=zeros)
+    _check_contiguous(weight=weight, scales=scales, x=x, out=out, zeros=zeros)
+    _check_dtype(weight, "weight", torch.uint8)
+    for name, t in (("scales", scales), ("out", out), ("zeros", zeros)):
+        _check_dtype(t, name, x.dtype)
+    if x.dim() not in (1, 2) or weight.dim() != 2 or scales.dim() != 2:
+        raise ValueError("tecoops.gemv_int4: weight [N, K / 2], scales [N, K / group], x [B, K] or [K]")
+    N, K = weight.shape[0], 2 * weight.shape[1]
+    B = x.shape[0] if x.dim() == 2 else 1
+    if x.shape[-1] != K or out.numel() != B * N or scales.shape[0] != N or scales.shape[1] == 0 or \
+            K == 0 or K % scales.shape[1]:
+        raise ValueError(f"tecoops.gemv_int4: scales must be [{N}, K / group], x [B, {K}] and out "
+                         f"[B, {N}]")
+    if zeros is not None and zeros.shape != scales.shape:
+        raise ValueError("tecoops.gemv_int4: zeros must match scales")
+    if refused:
+        _raise(refused, "tecoopsGemvInt4")
+    if B == 0:
+        return
+    _call_on(device, "tecoopsGemvInt4", _handle(device), _ptr(weight), _ptr(scales), _ptr(zeros),
+             _ptr(x), _ptr(out), B, N, K, K // scales.shape[1], code)
 
 
 def memset(t, value):

@@ -87,6 +87,15 @@ SIGNATURES = {
                                        I]),
     "tecoopsRotaryAxesReshapeAndCache": (I, [P, P, LL, I, P, I, P, P, P, P, P, P, I, I, I, I, I, LL,
                                              LL, LL, P, I, F, I, I, I, I, I]),
+    "tecoopsQkNormRotary": (I, [P, P, LL, I, P, I, P, P, P, P, F, I, I, I, I, I, LL, LL, P, I, F, I,
+                                I]),
+    "tecoopsQkNormRotaryReshapeAndCache": (I, [P, P, LL, I, P, I, P, P, P, P, P, F, P, P, P, I, I, I,
+                                               I, I, LL, LL, LL, P, I, F, I, I, I, I, I]),
+    "tecoopsReshapeAndCacheInt4": (I, [P, P, P, P, P, P, P, P, I, I, I, LL, LL, I, I, I]),
+    "tecoopsFlashAttentionInt4": (I, [P, I, I, P, P, P, LL, I, I, P, P, P, P, P, P, I, I, I, I, I, I,
+                                      F, I, P, SZ, I]),
+    "tecoopsGetFlashAttentionInt4WorkspaceSize": (I, [I, I, I, I, I, I, I, P]),
+    "tecoopsGemvInt4": (I, [P, P, P, P, P, P, I, I, I, I, I]),
 }
 
 _LIB = None
