@@ -546,11 +546,16 @@ tecoopsStatus_t tecoopsGetFlashAttentionInt4WorkspaceSize(int batch, int total_q
  * accumulation.  weight uint8 [n, k / 2], 16-byte aligned, code 2j of a row in the
  * low half of byte j; scales and zeros dataType [n, k / group_size] (zeros NULL: 8
  * everywhere; they need not be whole); x [batch, k], y [batch, n].  group_size a
- * multiple of 32 that divides k.  For decode batches; batch = 0 is done without a
- * launch. */
+ * multiple of 32 that divides k.  For decode batches: the weights are read again
+ * for every 64 rows of x; batch = 0 is done without a launch.
+ * workspace: tecoopsGetGemvInt4WorkspaceSize() bytes for the same sizes let few rows
+ * of W be split along k; with less, or NULL, there are fewer splits (slower, the
+ * same result up to fp32 rounding).  Nothing is allocated. */
 tecoopsStatus_t tecoopsGemvInt4(tecoopsHandle_t handle, const void *weight, const void *scales,
                                 const void *zeros, const void *x, void *y, int batch, int n, int k,
-                                int group_size, tecoopsDataType_t dataType);
+                                int group_size, void *workspace, size_t workspace_bytes,
+                                tecoopsDataType_t dataType);
+tecoopsStatus_t tecoopsGetGemvInt4WorkspaceSize(int batch, int n, int k, size_t *bytes);
 
 #ifdef __cplusplus
 }

@@ -24,6 +24,9 @@ namespace {
 
 using namespace tecoops::dev;
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 __attribute__((aligned(2))) u32x4_a2;  // (16-byte loads need no alignment)
+
 constexpr int kThreads = 256;
 constexpr int kBatch = 2;  // (token, head) rows a thread has under way
 
@@ -36,7 +39,6 @@ struct Args {
     int heads, head_size, block_size, lbs;
     long long capacity;  // num_blocks * block_size
     long long rows;      // tokens * heads
-    int narrow;          // elements loaded one by one
 };
 
 template <int LANES>
@@ -61,14 +63,13 @@ __device__ __forceinline__ void group_range(float &lo, float &hi) {
 
 // Codes and pair of one row from this lane's chunk of it.
 template <typename T, int LANES>
-__device__ __forceinline__ void quantise(const uint4 &x, uint32_t &codes, uint32_t &pair) {
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+__device__ __forceinline__ void quantise(const u32x4 &x, uint32_t &codes, uint32_t &pair) {
     float f[8], lo_ = INFINITY, hi_ = -INFINITY;
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        f[2 * i] = lo<T>(w[i]);
-        f[2 * i + 1] = hi<T>(w[i]);
+        f[2 * i] = lo<T>(x[i]);
+        f[2 * i + 1] = hi<T>(x[i]);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Args a) {
     constexpr int ROWS = kThreads / LANES;
     const int c = threadIdx.x % LANES, chunks = a.head_size / 8, cc = min(c, chunks - 1);
     const long long row0 = static_cast<long long>(blockIdx.x) * (ROWS * kBatch) + threadIdx.x / LANES;
-    uint4 x[kBatch][2];
+    u32x4 x[kBatch][2];
     int64_t slot[kBatch];
     int head[kBatch];
 #pragma unroll
@@ -113,14 +114,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Args a) {
                                   a.value + t * a.v_stride + head[u] * a.head_size + 8 * cc};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (!a.narrow) {
-                x[u][i] = ld_stream(reinterpret_cast<const uint4 *>(src[i]));
-            } else {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = src[i][2 * e] | (static_cast<uint32_t>(src[i][2 * e + 1]) << 16);
-                x[u][i] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            x[u][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_a2 *>(src[i]));
         }
     }
 #pragma unroll
@@ -196,8 +190,6 @@ extern "C" tecoopsStatus_t tecoopsReshapeAndCacheInt4(
     a.lbs = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
     a.capacity = static_cast<long long>(num_blocks) * block_size;
     a.rows = rows;
-    a.narrow = !(tecoops::aligned(key, 16) && tecoops::aligned(value, 16) && key_stride % 8 == 0 &&
-                 value_stride % 8 == 0);
     if (dataType == TECOOPS_DATA_HALF) launch<f16>(a, handle->stream);
     else launch<bf16>(a, handle->stream);
     TECO_CHECK_LAUNCH("reshape_and_cache_int4");

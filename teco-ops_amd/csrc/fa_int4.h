@@ -7,19 +7,21 @@
 namespace tecoops {
 namespace fa4 {
 
-// The split route serves `cols` (query head of a group, query row) pairs of each
-// sequence and kv head in tiles of 16 * ct columns, over keys cut into splits.
+// Both routes serve the (query row, query head of a group) pairs of each sequence
+// and kv head as columns, in tiles, over keys cut into splits.
 struct Plan {
-    bool split;      // the split route, else query tiles over all their keys
-    int rows;        // the bound on a sequence's query rows
-    int ct, tiles;   // column tiles of 16 in a workgroup, and such workgroups
-    int cols;        // columns of a sequence and kv head in the workspace
+    bool split;      // the split route, else the tile route
+    int ct;          // split route: column tiles of 16 in a workgroup
+    int waves;       // tile route: waves of 32 columns in a workgroup
+    int tiles;       // column tiles of a sequence and kv head
+    int cols;        // its columns
     int split_len, splits;
     size_t bytes;    // workspace: partial states where splits > 1
 };
 
-constexpr int kWaves = 4;              // of a workgroup
+constexpr int kWaves = 4;                 // of a workgroup of the split route
 constexpr int kLeastSplit = 32 * kWaves;  // keys: a block of 32 for each wave
+constexpr int kSplitCols = 64;            // columns that the split route serves
 
 inline size_t state_bytes(int batch, int kv_heads, int splits, int cols, int head_size) {
     return splits <= 1 ? 0
@@ -30,22 +32,34 @@ inline size_t state_bytes(int batch, int kv_heads, int splits, int cols, int hea
 // bytes; cus: compute units.
 inline Plan make_plan(int batch, int heads, int kv_heads, int head_size, int rows, int keys, size_t room, int cus) {
     Plan p{};
-    const long long group = heads / kv_heads;
-    const long long cols = group * rows;
-    p.rows = rows;
-    p.split = cols <= 64;
-    if (!p.split) return p;
+    const long long cols = std::min<long long>(static_cast<long long>(heads / kv_heads) * rows, 0x7fffffff);
     p.cols = static_cast<int>(cols);
-    p.ct = cols <= 16 ? 1 : 2;
-    p.tiles = static_cast<int>((cols + 16 * p.ct - 1) / (16 * p.ct));
-    // as long as the grid has four workgroups a CU, else down to one block a wave
-    const long long units = static_cast<long long>(batch) * kv_heads * p.tiles;
-    long long len = 2048;
-    while (len > kLeastSplit && units * ((keys + len - 1) / len) < 4ll * cus) len /= 2;
+    p.split = cols <= kSplitCols;
+    p.splits = 1;
+    long long len = 0;
     const auto splits = [&](long long l) { return std::max(1ll, (keys + l - 1) / l); };
+    if (p.split) {
+        p.ct = cols <= 16 ? 1 : 2;
+        p.tiles = static_cast<int>((cols + 16 * p.ct - 1) / (16 * p.ct));
+        // as long as the grid has four workgroups a CU, else down to one block a wave
+        const long long units = static_cast<long long>(batch) * kv_heads * p.tiles;
+        len = 2048;
+        while (len > kLeastSplit && units * splits(len) < 4ll * cus) len /= 2;
+    } else {
+        const int wide = head_size <= 128 ? 12 : 8;
+        p.waves = cols <= 128 ? 4 : wide;
+        const long long tile = 32 * p.waves;
+        p.tiles = static_cast<int>((cols + tile - 1) / tile);
+        // where the tiles leave workgroup slots empty, as many splits as fill them,
+        // of 512 keys or more
+        const long long units = static_cast<long long>(batch) * kv_heads * p.tiles;
+        const long long slots = static_cast<long long>(cus) * (p.waves == 4 ? 3 : 1);
+        const long long want = std::min(slots / std::max(units, 1ll), static_cast<long long>(keys) / 512);
+        len = want > 1 ? ((keys + want - 1) / want + 95) / 96 * 96 : std::max(keys, 1);
+    }
     while (splits(len) > 1 && state_bytes(batch, kv_heads, static_cast<int>(splits(len)), p.cols, head_size) > room)
         len *= 2;
-    p.split_len = static_cast<int>(std::min(len, 1ll << 30));
+    p.split_len = static_cast<int>(std::min(len, (1ll << 30) / 384 * 384));
     p.splits = static_cast<int>(splits(len));
     p.bytes = state_bytes(batch, kv_heads, p.splits, p.cols, head_size);
     return p;

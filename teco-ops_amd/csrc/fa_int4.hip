@@ -52,10 +52,10 @@ struct Params {
     int batch, H, Hkv, G, bs, lbs, num_blocks;  // lbs = log2(bs) or -1
     int kv_cap;                                 // keys that a table row can name
     float scale_log2;
-    int causal, bf16;
+    int causal;
     long long total_q;
     float *ws_o, *ws_ml;
-    int rows, cols, tiles, split_len, splits;
+    int cols, tiles, split_len, splits;
 };
 
 typedef unsigned __attribute__((aligned(4))) u32_a4;
@@ -66,13 +66,6 @@ __device__ __forceinline__ f32x4_t mma16(const u32x4 &a, const u32x4 &b, f32x4_t
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
                                                   0, 0, 0);
 }
-
-__device__ __forceinline__ float widen(uint16_t b, int is_bf16) { return is_bf16 ? b2f(b) : h2f(b); }
-__device__ __forceinline__ float low_of(uint32_t w, int is_bf16) { return widen(static_cast<uint16_t>(w), is_bf16); }
-__device__ __forceinline__ float high_of(uint32_t w, int is_bf16) {
-    return widen(static_cast<uint16_t>(w >> 16), is_bf16);
-}
-__device__ __forceinline__ uint16_t narrow(float f, int is_bf16) { return is_bf16 ? f2b(f) : f2h(f); }
 
 // 2^e, e within a float's normal exponents.
 __device__ __forceinline__ float power2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
@@ -107,6 +100,7 @@ __device__ __forceinline__ long long row_of(const Params &p, int kvh, int page, 
 // most twice the reference: P s stays below 2^15.
 constexpr float kTop = 10.0f, kSlack = 4.0f;
 constexpr float kMiddle = 7.5f;  // of the codes
+constexpr int kLeastRef = -90;   // (sums of 2^24 weights stay within fp32)
 constexpr float kNever = -1e30f;  // the running maximum before any key
 
 // Block-size modes: 1 a multiple of 16 (a block of 16 keys lies in one page: its
@@ -119,10 +113,15 @@ struct Block {
     uint32_t k[2][KW];
     uint32_t v[2][4][N128 + N64 + N32];
     u32x4 ks[2], vs[2];
-    int kp[2], vp[2][VP];  // table entries of the next load()
 
-    __device__ __forceinline__ void pages(const Params &p, const int *table, int j0, int limit) {
+    // The block-table entries that a load() needs, fetched one load ahead of it.
+    struct Pages {
+        int kp[2], vp[2][VP];
+    };
+
+    static __device__ __forceinline__ void pages(Pages &g, const Params &p, const int *table, int j0, int limit) {
         const int lane = threadIdx.x & 63;
+        int(&kp)[2] = g.kp, (&vp)[2][VP] = g.vp;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             if constexpr (BSM == 1) {
@@ -141,39 +140,38 @@ struct Block {
         }
     }
 
-    // The 32 keys from j0 on; what lies at `limit` or behind it is some row.
-    __device__ __forceinline__ void load(const Params &p, int kvh, int j0, int limit) {
+    // The 32 keys (load_k) or values (load_v) from j0 on; what lies at `limit` or
+    // behind it is some row.
+    __device__ __forceinline__ void load_k(const Pages &pg, const Params &p, int kvh, int j0, int limit) {
         const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            long long kr, vr[4];
-            if constexpr (BSM == 1) {
-                const int key = j0 + 16 * b < limit ? j0 + 16 * b : 0;
-                const long long first = row_of(p, kvh, kp[b], key, block_at(p, key));
-                kr = first + m;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vr[i] = first + 4 * g + i;
-            } else {
-                int key = j0 + 16 * b + m;
-                key = key < limit ? key : 0;
-                kr = row_of(p, kvh, kp[b], key, block_at(p, key));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (VP == 1 && i > 0) {
-                        vr[i] = vr[0] + i;
-                        continue;
-                    }
-                    int kv = j0 + 16 * b + 4 * g + i;
-                    kv = kv < limit ? kv : 0;
-                    vr[i] = row_of(p, kvh, vp[b][i], kv, block_at(p, kv));
-                }
-            }
+            int key = j0 + 16 * b + (BSM == 1 ? 0 : m);
+            key = key < limit ? key : 0;
+            long long kr = row_of(p, kvh, pg.kp[b], key, block_at(p, key));
+            long long sr = kr + 4 * g;
+            if (BSM == 1) kr += m;
             const u32_a4 *kw = reinterpret_cast<const u32_a4 *>(p.kc + kr * (D / 2)) + g * KW;
 #pragma unroll
             for (int w = 0; w < KW; ++w) k[b][w] = __builtin_nontemporal_load(kw + w);
+            if constexpr (BSM != 1) sr = row4(pg, p, kvh, j0, limit, b, 0);
+            ks[b] = pairs4(pg, p, p.ks, kvh, j0, limit, b, sr);
+        }
+    }
+    __device__ __forceinline__ void load_v(const Pages &pg, const Params &p, int kvh, int j0, int limit) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            long long r0;
+            if constexpr (BSM == 1) {
+                const int key = j0 + 16 * b < limit ? j0 + 16 * b : 0;
+                r0 = row_of(p, kvh, pg.kp[b], key, block_at(p, key)) + 4 * g;
+            } else {
+                r0 = row4(pg, p, kvh, j0, limit, b, 0);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint8_t *row = p.vc + vr[i] * (D / 2);
+                const uint8_t *row = p.vc + (BSM == 0 && i > 0 ? row4(pg, p, kvh, j0, limit, b, i) : r0 + i) * (D / 2);
 #pragma unroll
                 for (int n = 0; n < N128; ++n)
                     v[b][i][n] = __builtin_nontemporal_load(reinterpret_cast<const u32_a4 *>(row + 64 * n) + m);
@@ -181,17 +179,29 @@ struct Block {
                     v[b][i][N128] = *(reinterpret_cast<const uint16_t *>(row + 64 * N128) + m);
                 if constexpr (N32 > 0) v[b][i][N128 + N64] = row[64 * N128 + 32 * N64 + m];
             }
-            if constexpr (BSM == 0) {
+            vs[b] = pairs4(pg, p, p.vs, kvh, j0, limit, b, r0);
+        }
+    }
+
+private:
+    // Row of this lane's key i of its four of half b.
+    static __device__ __forceinline__ long long row4(const Pages &pg, const Params &p, int kvh, int j0, int limit, int b,
+                                                     int i) {
+        int key = j0 + 16 * b + 4 * static_cast<int>(threadIdx.x >> 4 & 3) + i;
+        key = key < limit ? key : 0;
+        return row_of(p, kvh, pg.vp[b][BSM == 0 ? i : 0], key, block_at(p, key));
+    }
+    // The pairs of its four keys, the first in row r0.
+    static __device__ __forceinline__ u32x4 pairs4(const Pages &pg, const Params &p, const uint32_t *pairs, int kvh, int j0,
+                                                   int limit, int b, long long r0) {
+        if constexpr (BSM == 0) {
+            u32x4 x;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    ks[b][i] = p.ks[vr[i]];
-                    vs[b][i] = p.vs[vr[i]];
-                }
-            } else {
-                typedef u32x4 __attribute__((aligned(4))) u32x4_a4;
-                ks[b] = *reinterpret_cast<const u32x4_a4 *>(p.ks + vr[0]);
-                vs[b] = *reinterpret_cast<const u32x4_a4 *>(p.vs + vr[0]);
-            }
+            for (int i = 0; i < 4; ++i) x[i] = pairs[i == 0 ? r0 : row4(pg, p, kvh, j0, limit, b, i)];
+            return x;
+        } else {
+            typedef u32x4 __attribute__((aligned(4))) u32x4_a4;
+            return *reinterpret_cast<const u32x4_a4 *>(pairs + r0);
         }
     }
 };
@@ -205,13 +215,14 @@ __device__ __forceinline__ u32x4 widen8(uint32_t w) {
 
 // State of a wave: per column tile the running maximum (log2 domain), the sums of
 // the weights and of weight * middle of the row over this lane's keys, and the
-// unnormalised sums of weight * scale * code; `ref` is the power of two that scales are taken
-// relative to.
+// unnormalised sums of weight * scale * code, all in units of the power of two `ref`
+// that the scales are taken relative to.
 template <int D, int CT>
 struct State {
     f32x4_t acc[CT][D / 16], w[CT];  // w: sums of the weights * scale as rounded
     float m[CT], l[CT], r[CT];
-    float ref, inv_ref;
+    float twice_ref;
+    int ref;
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -222,8 +233,8 @@ struct State {
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) acc[t][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        ref = power2(-100);
-        inv_ref = power2(100);
+        ref = kLeastRef;
+        twice_ref = power2(kLeastRef + 1);
     }
 };
 
@@ -236,7 +247,7 @@ struct Column {
     int vis;        // keys that it sees
 };
 
-template <int D>
+template <typename T, int D>
 __device__ __forceinline__ void load_column(const Params &p, Column<D> &c, const uint16_t *src, bool there) {
     // this lane's quarter of the head: elements [g D/4, (g + 1) D/4)
     const int g = (threadIdx.x & 63) >> 4;
@@ -252,7 +263,7 @@ __device__ __forceinline__ void load_column(const Params &p, Column<D> &c, const
             most = max(most, max(a & 0xffffu, a >> 16));
         }
     }
-    const float big = row_swap_max(half_swap_max(widen(static_cast<uint16_t>(most), p.bf16)));
+    const float big = row_swap_max(half_swap_max(Cvt<T>::to(static_cast<uint16_t>(most))));
     // the largest element to [2^14, 2^15); infinities and NaN stay what they are
     int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
     e = min(max(e, -100), 120);
@@ -263,8 +274,8 @@ __device__ __forceinline__ void load_column(const Params &p, Column<D> &c, const
         float f[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            f[2 * i] = low_of(raw[w][i], p.bf16) * up;
-            f[2 * i + 1] = high_of(raw[w][i], p.bf16) * up;
+            f[2 * i] = lo<T>(raw[w][i]) * up;
+            f[2 * i + 1] = hi<T>(raw[w][i]) * up;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += f[i];
@@ -279,14 +290,13 @@ __device__ __forceinline__ void load_column(const Params &p, Column<D> &c, const
     c.to_log2 = p.scale_log2 * power2(e - 14) * 0x1p24f;
 }
 
-// The 32 keys from j0 on, held in `b`, into the state.  Keys at `limit` or behind
-// it, and keys that a column does not see, weigh nothing, whatever the cache holds
-// there; `edge`: some are among these.
-template <int D, int CT, int BSM>
-__device__ __forceinline__ void attend(const Params &p, const Block<D, BSM> &b, const Column<D> (&col)[CT],
-                                       State<D, CT> &st, int j0, int limit, bool edge) {
+// Scores of the 32 keys from j0 on, held in `b`, before their factor to_log2.  Keys at
+// `limit` or behind it, and keys that a column does not see, score -inf and have pairs
+// of 0, whatever the cache holds there; `edge`: some are among these.
+template <typename T, int D, int CT, int BSM>
+__device__ __forceinline__ void scores(Block<D, BSM> &b, const Column<D> (&col)[CT], f32x4_t (&s)[CT][2], int j0,
+                                       int limit, bool edge) {
     const int g = (threadIdx.x & 63) >> 4;
-    f32x4_t s[CT][2];
 #pragma unroll
     for (int t = 0; t < CT; ++t)
 #pragma unroll
@@ -299,22 +309,24 @@ __device__ __forceinline__ void attend(const Params &p, const Block<D, BSM> &b, 
 #pragma unroll
             for (int t = 0; t < CT; ++t) s[t][h] = mma16(a, col[t].q[w], s[t][h]);
         }
-    float sv[2][4], av[2][4];
-    float top = 0.0f;
+    if (edge) {
+        asm volatile("");  // (a branch, taken in the last block alone)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (j0 + 16 * h + 4 * g + i >= limit) b.ks[h][i] = 0u;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t kw = b.ks[h][i], vw = b.vs[h][i];
-            if (edge && j0 + 16 * h + 4 * g + i >= limit) kw = vw = 0u;
-            const float sk = low_of(kw, p.bf16), ak = high_of(kw, p.bf16);
-            sv[h][i] = low_of(vw, p.bf16);
-            av[h][i] = fmaf(kMiddle, sv[h][i], high_of(vw, p.bf16));
-            top = fmaxf(top, fabsf(sv[h][i]));
+            const float sk = lo<T>(b.ks[h][i]), ak = hi<T>(b.ks[h][i]);
 #pragma unroll
             for (int t = 0; t < CT; ++t) s[t][h][i] = fmaf(sk, s[t][h][i], ak * col[t].sum);
         }
     if (edge) {
+        asm volatile("");
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
@@ -323,16 +335,43 @@ __device__ __forceinline__ void attend(const Params &p, const Block<D, BSM> &b, 
                 for (int i = 0; i < 4; ++i)
                     if (j0 + 16 * h + 4 * g + i >= min(limit, col[t].vis)) s[t][h][i] = kNegInf;
     }
+}
+
+// Their values, weighted by the softmax of the scores, into the state.
+template <typename T, int D, int CT, int BSM>
+__device__ __forceinline__ void weigh(Block<D, BSM> &b, const Column<D> (&col)[CT], const f32x4_t (&s)[CT][2],
+                                      State<D, CT> &st, int j0, int limit, bool edge) {
+    const int g = (threadIdx.x & 63) >> 4;
+    if (edge) {
+        asm volatile("");
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (j0 + 16 * h + 4 * g + i >= limit) b.vs[h][i] = 0u;
+    }
+    float sv[2][4], av[2][4];
+    float top = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sv[h][i] = lo<T>(b.vs[h][i]);
+            av[h][i] = fmaf(kMiddle, sv[h][i], hi<T>(b.vs[h][i]));
+            top = fmaxf(top, fabsf(sv[h][i]));
+        }
     // scales relative to a power of two that is at least half of the largest seen
-    if (!__all(top <= 2.0f * st.ref)) {
+    if (!__all(top <= st.twice_ref)) {
         top = row_swap_max(half_swap_max(top));
         const int e = min(static_cast<int>(__float_as_uint(top) >> 23) - 127, 100);
-        const float f = power2(e), down = st.ref / f;
-        if (f > st.ref) {
-            st.ref = f;
-            st.inv_ref = power2(-e);
+        if (e > st.ref) {
+            const float down = e - st.ref > 120 ? 0.0f : power2(st.ref - e);
+            st.ref = e;
+            st.twice_ref = power2(e + 1);
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
+                st.l[t] *= down;
+                st.r[t] *= down;
                 st.w[t] *= down;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= down;
@@ -355,7 +394,7 @@ __device__ __forceinline__ void attend(const Params &p, const Block<D, BSM> &b, 
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= f;
         }
-        const float shift = kTop - st.m[t];
+        const float shift = kTop - st.m[t] - static_cast<float>(st.ref);
         float w[2][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -364,7 +403,7 @@ __device__ __forceinline__ void attend(const Params &p, const Block<D, BSM> &b, 
                 const float e = __builtin_amdgcn_exp2f(fmaf(s[t][h][i], col[t].to_log2, shift));
                 st.l[t] += e;
                 st.r[t] = fmaf(e, av[h][i], st.r[t]);
-                w[h][i] = e * (sv[h][i] * st.inv_ref);
+                w[h][i] = e * sv[h][i];
             }
         pw[t] = u32x4{Mma<f16>::pack2(w[0][0], w[0][1]), Mma<f16>::pack2(w[0][2], w[0][3]),
                       Mma<f16>::pack2(w[1][0], w[1][1]), Mma<f16>::pack2(w[1][2], w[1][3])};
@@ -422,7 +461,7 @@ constexpr size_t split_lds() {
 // Columns [c0, c0 + 16 CT) of (sequence, kv head) over the keys [lo, hi): column j
 // is query row j / G, head j % G of the group.  Leaves the waves' states in LDS,
 // after a barrier: maximum, sum and unnormalised output of each column.
-template <int D, int CT, int BSM>
+template <typename T, int D, int CT, int BSM>
 __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, int kvh, long long q_off, int L, int S,
                                            int c0, int lo, int hi) {
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
@@ -438,35 +477,47 @@ __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, i
     for (int t = 0; t < CT; ++t) {
         const int j = min(c0 + 16 * t + n, last);
         const int row = j / p.G, head = j - row * p.G;
-        load_column<D>(p, col[t], p.q + ((q_off + row) * p.H + kvh * p.G + head) * D, c0 + 16 * t + n <= last);
+        load_column<T, D>(p, col[t], p.q + ((q_off + row) * p.H + kvh * p.G + head) * D, c0 + 16 * t + n <= last);
         col[t].vis = p.causal ? q_start + row + 1 : S;
     }
     State<D, CT> st;
     st.clear();
-    Block<D, BSM> next;
+    // The next block's keys are asked for once this one's scores are done, its values
+    // once these are used: one set of registers each, and more waves, whose loads
+    // overlap, in place of a second set.
+    using B = Block<D, BSM>;
+    B blk;
+    typename B::Pages pages, next;
+    constexpr int STEP = 32 * kWaves;
     int j0 = lo + 32 * wave;
     if (j0 < limit) {
-        next.pages(p, table, j0, limit);
-        next.load(p, kvh, j0, limit);
-        next.pages(p, table, j0 + 32 * kWaves, limit);
+        B::pages(pages, p, table, j0, limit);
+        blk.load_k(pages, p, kvh, j0, limit);
+        blk.load_v(pages, p, kvh, j0, limit);
+        if (j0 + STEP < limit) B::pages(next, p, table, j0 + STEP, limit);
     }
-    for (; j0 < limit; j0 += 32 * kWaves) {
-        const Block<D, BSM> now = next;
-        if (j0 + 32 * kWaves < limit) {
-            next.load(p, kvh, j0 + 32 * kWaves, limit);
-            next.pages(p, table, j0 + 64 * kWaves, limit);
+    for (; j0 < limit; j0 += STEP) {
+        const bool edge = j0 + 32 > least, more = j0 + STEP < limit;
+        f32x4_t s[CT][2];
+        scores<T, D, CT, BSM>(blk, col, s, j0, limit, edge);
+        pages = next;
+        if (more) {
+            blk.load_k(pages, p, kvh, j0 + STEP, limit);
+            if (j0 + 2 * STEP < limit) B::pages(next, p, table, j0 + 2 * STEP, limit);
         }
-        attend<D, CT, BSM>(p, now, col, st, j0, limit, j0 + 32 > least);
+        weigh<T, D, CT, BSM>(blk, col, s, st, j0, limit, edge);
+        if (more) blk.load_v(pages, p, kvh, j0 + STEP, limit);
     }
     constexpr int COLS = 16 * CT;
     float *lm = lds, *ll = lm + kWaves * COLS, *lout = ll + kWaves * COLS;
+    const float ref = power2(st.ref);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         const float l = row_swap_sum(half_swap_sum(st.l[t])), r = row_swap_sum(half_swap_sum(st.r[t]));
         const int c = wave * COLS + 16 * t + n;
         if (g == 0) {
             lm[c] = st.m[t];
-            ll[c] = l;
+            ll[c] = l * ref;
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
@@ -474,7 +525,7 @@ __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, i
 #pragma unroll
             for (int v = 0; v < 4; ++v)
                 lout[c * D + channel_of<D>(i, 4 * g + v)] =
-                    fmaf(st.ref, fmaf(st.acc[t][i][v], unit, -kMiddle * st.w[t][v]), r);
+                    ref * (fmaf(st.acc[t][i][v], unit, -kMiddle * st.w[t][v]) + r);
         }
     }
     __syncthreads();
@@ -509,8 +560,8 @@ __device__ __forceinline__ int splits_of(const Params &p, int S) {
 // key past the splits, and rows past the bound that the grid was made for are done
 // by the workgroups of split 0, over all keys, so that the bounds shape the launch
 // alone.
-template <int D, int CT, int BSM>
-__global__ void __launch_bounds__(64 * kWaves, D * CT <= 64 ? 4 : D * CT <= 128 ? 3 : D <= 128 ? 2 : 1) split_kernel(Params p) {
+template <typename T, int D, int CT, int BSM>
+__global__ void __launch_bounds__(64 * kWaves, D * CT <= 64 && CT == 1 ? 4 : D * CT <= 128 ? 3 : D * CT <= 256 ? 2 : 1) split_kernel(Params p) {
     extern __shared__ __attribute__((aligned(16))) float states[];
     if (blockIdx.x == 0 && blockIdx.y == 0) zero_tail(p, D);
     const int tile = blockIdx.x % p.tiles;
@@ -525,14 +576,14 @@ __global__ void __launch_bounds__(64 * kWaves, D * CT <= 64 ? 4 : D * CT <= 128 
         return [&, c0](int c, int d, float out, float, float sum) {
             const int j = c0 + c, row = j / p.G;
             p.o[((q_off + row) * p.H + kvh * p.G + (j - row * p.G)) * D + d] =
-                narrow(sum > 0.0f ? out / sum : 0.0f * sum, p.bf16);
+                Cvt<T>::from(sum > 0.0f ? out / sum : 0.0f * sum);
         };
     };
     int c0 = tile * 16 * CT;
     if (c0 < min(all, p.cols) && split < ns) {
         const int lo = split * p.split_len, hi = split == ns - 1 ? S : lo + p.split_len;
         const int cols = min(16 * CT, min(all, p.cols) - c0);
-        split_pass<D, CT, BSM>(p, states, b, kvh, q_off, L, S, c0, lo, hi);
+        split_pass<T, D, CT, BSM>(p, states, b, kvh, q_off, L, S, c0, lo, hi);
         if (p.splits == 1) {
             merge_states<D, CT>(states, cols, write(c0));
         } else {
@@ -550,13 +601,13 @@ __global__ void __launch_bounds__(64 * kWaves, D * CT <= 64 ? 4 : D * CT <= 128 
     // (p.cols need not be a whole number of tiles: the rest starts at it)
     for (c0 = p.cols + tile * 16 * CT; c0 < all; c0 += p.tiles * 16 * CT) {
         __syncthreads();
-        split_pass<D, CT, BSM>(p, states, b, kvh, q_off, L, S, c0, 0, S);
+        split_pass<T, D, CT, BSM>(p, states, b, kvh, q_off, L, S, c0, 0, S);
         merge_states<D, CT>(states, min(16 * CT, all - c0), write(c0));
     }
 }
 
 // The splits' states of a column into its output row: D / 4 lanes a column.
-template <int D>
+template <typename T, int D>
 __global__ void __launch_bounds__(256) combine_kernel(Params p) {
     constexpr int V = D / 4, COLS = 256 / V, AHEAD = 4;
     const int kvh = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
@@ -595,10 +646,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Params p) {
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f * sum;
     const int row = c / p.G;
     uint16_t *dst = p.o + ((q_off + row) * p.H + kvh * p.G + (c - row * p.G)) * D + 4 * e;
-    uint2 w;
-    w.x = narrow(out.x * inv, p.bf16) | (static_cast<uint32_t>(narrow(out.y * inv, p.bf16)) << 16);
-    w.y = narrow(out.z * inv, p.bf16) | (static_cast<uint32_t>(narrow(out.w * inv, p.bf16)) << 16);
-    *reinterpret_cast<uint2 *>(dst) = w;
+    store_row4<T>(dst, out.x * inv, out.y * inv, out.z * inv, out.w * inv);
 }
 
 // ---------------------------------------------------------------- tile route
@@ -606,7 +654,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Params p) {
 // K and V tiles of TILE keys from the cache into LDS as fp16, both row-major (the
 // layout that wave_attend reads with transposing loads): a thread's tasks are
 // 16-byte words of codes, 32 elements of a row.
-template <int D, int TILE, int NT>
+template <typename T, int D, int TILE, int NT>
 struct Widener {
     static constexpr int KP = D + 8, VR = D + kVRowPad;
     static constexpr int VOFF = TILE * KP, ELEMS = TILE * (KP + VR);
@@ -641,15 +689,15 @@ struct Widener {
             if (!there) pair[i] = 0u;
         }
     }
-    // rows times 2^-ek (keys) and 2^-ev (values)
-    __device__ __forceinline__ void store(const Params &p, uint16_t *buf, float down_k, float down_v) {
+    // rows times down_k (keys) and down_v (values)
+    __device__ __forceinline__ void store(uint16_t *buf, float down_k, float down_v) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int t = static_cast<int>(threadIdx.x) + i * NT;
             if (TASKS % NT != 0 && t >= TASKS) continue;
             const int task = t % HALF, word = task % WORDS, row = task / WORDS;
             const bool is_v = t >= HALF;
-            const float s = low_of(pair[i], p.bf16), a = high_of(pair[i], p.bf16);
+            const float s = lo<T>(pair[i]), a = hi<T>(pair[i]);
             const float most = fmaxf(fabsf(a), fabsf(fmaf(15.0f, s, a)));
             if (is_v) most_v = fmaxf(most_v, most);
             else most_k = fmaxf(most_k, most);
@@ -674,41 +722,42 @@ struct Widener {
     }
 };
 
-template <int D, int TILE, int W, int HW>
+template <int D, int TILE, int W>
 constexpr size_t tile_lds() {
-    using Wd = Widener<D, TILE, W * 64>;
-    constexpr size_t kv = 2ull * Wd::ELEMS, o = static_cast<size_t>(32 * (W / HW)) * o_row<D, HW>();
+    constexpr size_t kv = 2ull * Widener<f16, D, TILE, W * 64>::ELEMS, o = static_cast<size_t>(32 * W) * (D + 8);
     return sizeof(uint16_t) * (kv > o ? kv : o);
 }
 
-// Query rows [q0, q0 + 32 W / HW) of HW heads: wave w serves head w % HW and rows
-// 32 (w / HW) .. + 31.  Ends with a barrier.
-template <int D, int W, int HW, int TILE>
-__device__ __forceinline__ void query_tile(const Params &p, uint16_t *lds, float *meet, int b, int kvh, int hg,
-                                           long long q_off, int L, int S, int q0) {
-    constexpr int NKB = TILE % 64 == 0 ? 2 : 1, KB = 32 * NKB, QT = 32 * (W / HW);
-    using Wd = Widener<D, TILE, W * 64>;
+// Columns [c0, c0 + 32 W) below `all` of (sequence, kv head) over the keys [from, to): wave w
+// serves columns 32 w .. + 31, column j being query row j / G, head j % G of the
+// group, so that heads of any number fill the waves.  Into the output rows, or with
+// `part` into the states [column][D], (maximum, sum) [column].  Ends with a barrier.
+template <typename T, int D, int W, int TILE>
+__device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, float *meet, int b, int kvh, long long q_off,
+                                            int L, int S, int all, int c0, int from, int to, float *part,
+                                            float *part_ml) {
+    constexpr int NKB = TILE % 64 == 0 ? 2 : 1, KB = 32 * NKB, COLS = 32 * W;
+    using Wd = Widener<T, D, TILE, W * 64>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5, r32 = lane & 31;
-    const int h = kvh * p.G + hg * HW + wave % HW;
-    const int qw0 = q0 + wave / HW * 32;
+    const int cw0 = c0 + 32 * wave;
     const int q_start = p.causal ? max(S - L, 0) : 0;
-    const int kv_end = p.causal ? min(S, q_start + min(q0 + QT, L)) : S;
-    const int wave_end = __builtin_amdgcn_readfirstlane(p.causal ? min(S, q_start + min(qw0 + 32, L)) : S);
-    const int wave_least = __builtin_amdgcn_readfirstlane(p.causal ? min(S, q_start + qw0 + 1) : S);
+    const auto seen = [&](int j) { return p.causal ? min(to, q_start + j / p.G + 1) : to; };
+    const int kv_end = seen(min(c0 + COLS, all) - 1);
+    const int wave_end = __builtin_amdgcn_readfirstlane(cw0 < all ? seen(min(cw0 + 32, all) - 1) : from);
+    const int wave_least = __builtin_amdgcn_readfirstlane(seen(min(cw0, all - 1)));
     const int *table = p.bt + b * p.bt_stride;
-    const int row = qw0 + r32;
-    const int vis = p.causal ? min(S, q_start + row + 1) : S;
+    const int j = min(cw0 + r32, all - 1), row = j / p.G;
+    const int vis = seen(j);
 
-    // the wave's queries in fp16, their largest element to [2^14, 2^15) if need be
+    // the wave's queries in fp16, their largest element to [2^8, 2^9)
     u32x4 qf[1][D / 16];
     float q_unit;
     {
-        const uint16_t *src = p.q + ((q_off + min(row, L - 1)) * p.H + h) * D;
+        const uint16_t *src = p.q + ((q_off + row) * p.H + kvh * p.G + (j - row * p.G)) * D;
         uint32_t most = 0;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-            u32x4 x = *reinterpret_cast<const u32x4 *>(src + 16 * ks + 8 * g);
-            if (row >= L) x = u32x4{0u, 0u, 0u, 0u};
+            const u32x4 x = *reinterpret_cast<const u32x4 *>(src + 16 * ks + 8 * g);
             qf[0][ks] = x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -716,7 +765,7 @@ __device__ __forceinline__ void query_tile(const Params &p, uint16_t *lds, float
                 most = max(most, max(a & 0xffffu, a >> 16));
             }
         }
-        const float big = wave_max(widen(static_cast<uint16_t>(most), p.bf16));
+        const float big = wave_max(Cvt<T>::to(static_cast<uint16_t>(most)));
         int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
         e = min(max(e, -100), 120);
         const float up = power2(8 - e);
@@ -725,14 +774,14 @@ __device__ __forceinline__ void query_tile(const Params &p, uint16_t *lds, float
         for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                qf[0][ks][i] = Mma<f16>::pack2(low_of(qf[0][ks][i], p.bf16) * up, high_of(qf[0][ks][i], p.bf16) * up);
+                qf[0][ks][i] = Mma<f16>::pack2(tecoops::dev::lo<T>(qf[0][ks][i]) * up, tecoops::dev::hi<T>(qf[0][ks][i]) * up);
     }
 
     float m[1], lsum[1];
     f32x16_t oacc[1][D / 32];
     Wd wd;
     int ek = 0, ev = 0;
-    const int ntiles = (kv_end + TILE - 1) / TILE;
+    const int ntiles = kv_end > from ? (kv_end - from + TILE - 1) / TILE : 0;
     for (int pass = 0;; ++pass) {
         const float down_k = power2(-ek), down_v = power2(-ev);
         const float scale = p.scale_log2 * q_unit * power2(ek), inv_scale = 1.0f / scale;
@@ -745,28 +794,28 @@ __device__ __forceinline__ void query_tile(const Params &p, uint16_t *lds, float
         wd.most_k = wd.most_v = 0.0f;
         const auto buf = [&](int t) { return lds + __builtin_amdgcn_readfirstlane((t & 1) * Wd::ELEMS); };
         if (ntiles > 0) {
-            wd.pages(p, table, 0, S);
-            wd.load(p, kvh, 0, S);
-            wd.pages(p, table, TILE, S);
-            wd.store(p, buf(0), down_k, down_v);
+            wd.pages(p, table, from, to);
+            wd.load(p, kvh, from, to);
+            wd.pages(p, table, from + TILE, to);
+            wd.store(buf(0), down_k, down_v);
         }
         __syncthreads();
         for (int it = 0; it < ntiles; ++it) {
             const uint16_t *cur = buf(it);
             if (it + 1 < ntiles) {
-                wd.load(p, kvh, (it + 1) * TILE, S);
-                wd.pages(p, table, (it + 2) * TILE, S);
+                wd.load(p, kvh, from + (it + 1) * TILE, to);
+                wd.pages(p, table, from + (it + 2) * TILE, to);
             }
 #pragma unroll
             for (int hb = 0; hb < TILE / KB; ++hb) {
-                const int j0 = it * TILE + KB * hb;
+                const int j0 = from + it * TILE + KB * hb;
                 if (j0 < wave_end) {
                     const int lim[1] = {vis - j0 - 4 * g};
                     wave_attend<f16, D, Wd::KP, 0, Wd::VR, NKB, 1, true>(cur, cur + Wd::VOFF, KB * hb, qf, oacc, m, lsum,
                                                                         lim, scale, inv_scale, j0 + KB > wave_least);
                 }
             }
-            if (it + 1 < ntiles) wd.store(p, buf(it + 1), down_k, down_v);
+            if (it + 1 < ntiles) wd.store(buf(it + 1), down_k, down_v);
             __syncthreads();
         }
         // rows out of fp16's range, or all of them down where it has few bits: once
@@ -793,97 +842,130 @@ __device__ __forceinline__ void query_tile(const Params &p, uint16_t *lds, float
         ek = __builtin_amdgcn_readfirstlane(power(all_k));
         ev = __builtin_amdgcn_readfirstlane(power(all_v));
     }
-
-    // O leaves through LDS, a row at a time
-    constexpr int OROW = o_row<D, HW>(), RCH = HW * D / 8, NOC = (QT * RCH + W * 64 - 1) / (W * 64);
     const float lt = half_swap_sum(lsum[0]);
+    if (part != nullptr) {
+        if (cw0 + r32 < all) {
+            float *dst = part + static_cast<long long>(j) * D;
+            const float unit = power2(ev);
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    *reinterpret_cast<float4_t *>(dst + 32 * db + 8 * u + 4 * g) =
+                        float4_t{oacc[0][db][4 * u] * unit, oacc[0][db][4 * u + 1] * unit, oacc[0][db][4 * u + 2] * unit,
+                                 oacc[0][db][4 * u + 3] * unit};
+            if (g == 0) *reinterpret_cast<float2_t *>(part_ml + static_cast<long long>(j) * 2) = float2_t{m[0], lt};
+        }
+        return;  // (the loop's last barrier has passed)
+    }
+    // O leaves through LDS, a column at a time
+    constexpr int OROW = D + 8, RCH = D / 8, NOC = (COLS * RCH + W * 64 - 1) / (W * 64);
     const float inv = (lt > 0.0f ? 1.0f / lt : 0.0f * lt) * power2(ev);
-    uint16_t *dst = lds + (wave / HW * 32 + r32) * OROW + wave % HW * D;
+    uint16_t *dst = lds + (32 * wave + r32) * OROW;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            float f[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = oacc[0][db][4 * u + i] * inv;
-            if (p.bf16) store_row4<bf16>(dst + 32 * db + 8 * u + 4 * g, f[0], f[1], f[2], f[3]);
-            else store_row4<f16>(dst + 32 * db + 8 * u + 4 * g, f[0], f[1], f[2], f[3]);
-        }
+        for (int u = 0; u < 4; ++u)
+            store_row4<T>(dst + 32 * db + 8 * u + 4 * g, oacc[0][db][4 * u] * inv, oacc[0][db][4 * u + 1] * inv,
+                          oacc[0][db][4 * u + 2] * inv, oacc[0][db][4 * u + 3] * inv);
     __syncthreads();
-    uint16_t *rows = p.o + (q_off * p.H + kvh * p.G + hg * HW) * D;
 #pragma unroll
-    for (int j = 0; j < NOC; ++j) {
-        const int c = static_cast<int>(threadIdx.x) + j * W * 64, rr = c / RCH;
-        if (c < QT * RCH && q0 + rr < L)
-            *reinterpret_cast<u32x4 *>(rows + static_cast<long long>(q0 + rr) * p.H * D + (c - rr * RCH) * 8) =
-                *reinterpret_cast<const u32x4 *>(lds + rr * OROW + (c - rr * RCH) * 8);
+    for (int i = 0; i < NOC; ++i) {
+        const int t = static_cast<int>(threadIdx.x) + i * W * 64, c = t / RCH, jj = c0 + c;
+        if (t >= COLS * RCH || jj >= all) continue;
+        const int r = jj / p.G;
+        *reinterpret_cast<u32x4 *>(p.o + ((q_off + r) * p.H + kvh * p.G + (jj - r * p.G)) * D + (t - c * RCH) * 8) =
+            *reinterpret_cast<const u32x4 *>(lds + c * OROW + (t - c * RCH) * 8);
     }
     __syncthreads();
 }
 
-// Workgroup (sequence, kv head, head group) and query tile, the heaviest first;
-// that of tile 0 goes on to the tiles past the grid, of which there are none where
-// the bound on the rows holds.
-template <int D, int W, int HW, int TILE>
-__global__ void __launch_bounds__(W * 64, W >= 12 || TILE == 32 ? 3 : 2) tile_kernel(Params p) {
+// Workgroup (sequence, kv head) and (column tile, split), the heaviest tiles first;
+// that of tile 0 and split 0 goes on to the columns past the grid, of which there
+// are none where the bound on the rows holds.
+template <typename T, int D, int W, int TILE>
+__global__ void __launch_bounds__(W * 64, W >= 12 ? 3 : D <= 128 && W == 4 ? 3 : 2) tile_kernel(Params p) {
     extern __shared__ __attribute__((aligned(16))) uint16_t tiles_lds[];
     __shared__ float meet[2 * W];
     if (blockIdx.x == 0 && blockIdx.y == 0) zero_tail(p, D);
-    constexpr int QT = 32 * (W / HW);
-    const int groups = p.G / HW;
-    const int hg = blockIdx.x % groups, kvh = blockIdx.x / groups % p.Hkv, b = blockIdx.x / groups / p.Hkv;
+    constexpr int COLS = 32 * W;
+    const int kvh = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
+    const int split = blockIdx.y % p.splits, tile = p.tiles - 1 - blockIdx.y / p.splits;
     long long q_off;
     int L, S;
     sequence(p, b, q_off, L, S);
-    const int first = gridDim.y - 1 - blockIdx.y;
-    const int ntiles = L > 0 ? (L - 1) / QT + 1 : 0, rows = gridDim.y;
-    for (int t = first; t < ntiles; t = t < rows ? (t == 0 ? rows : ntiles) : t + 1)
-        query_tile<D, W, HW, TILE>(p, tiles_lds, meet, b, kvh, hg, q_off, L, S, t * QT);
+    if (L <= 0) return;
+    const int all = p.G * L, bound = min(all, p.cols);
+    int c0 = tile * COLS;
+    if (c0 < bound && p.splits == 1) {
+        column_tile<T, D, W, TILE>(p, tiles_lds, meet, b, kvh, q_off, L, S, bound, c0, 0, S, nullptr, nullptr);
+    } else if (c0 < bound) {
+        const int ns = splits_of(p, S);
+        const long long at = (static_cast<long long>(b) * p.Hkv + kvh) * p.splits + split;
+        if (split < ns)
+            column_tile<T, D, W, TILE>(p, tiles_lds, meet, b, kvh, q_off, L, S, bound, c0, split * p.split_len,
+                                       split == ns - 1 ? S : (split + 1) * p.split_len, p.ws_o + at * p.cols * D,
+                                       p.ws_ml + at * p.cols * 2);
+    }
+    if (tile != 0 || split != 0) return;
+    for (c0 = p.cols; c0 < all; c0 += COLS) {
+        __syncthreads();
+        column_tile<T, D, W, TILE>(p, tiles_lds, meet, b, kvh, q_off, L, S, all, c0, 0, S, nullptr, nullptr);
+    }
 }
 
 // ------------------------------------------------------------------- host
 
-template <int D, int CT>
+template <typename T, int D>
+tecoopsStatus_t launch_combine(const Params &p, const Plan &pl, hipStream_t s) {
+    if (pl.splits <= 1) return TECOOPS_STATUS_SUCCESS;
+    constexpr int COLS = 256 / (D / 4);
+    hipLaunchKernelGGL((combine_kernel<T, D>), dim3(p.batch * p.Hkv, tecoops::ceil_div(pl.cols, COLS)), dim3(256), 0, s, p);
+    TECO_CHECK_LAUNCH("flash_attention_int4 combine");
+    return TECOOPS_STATUS_SUCCESS;
+}
+
+template <typename T, int D, int CT>
 tecoopsStatus_t launch_split(const Params &p, const Plan &pl, hipStream_t s) {
     const size_t lds = split_lds<D, CT>();
-    auto *kern = p.bs % 16 == 0 ? &split_kernel<D, CT, 1> : p.bs % 4 == 0 ? &split_kernel<D, CT, 2> : &split_kernel<D, CT, 0>;
+    auto *kern = p.bs % 16 == 0  ? &split_kernel<T, D, CT, 1>
+                 : p.bs % 4 == 0 ? &split_kernel<T, D, CT, 2>
+                                 : &split_kernel<T, D, CT, 0>;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), lds)) return TECOOPS_STATUS_INTERNAL_ERROR;
     hipLaunchKernelGGL(kern, dim3(p.batch * p.Hkv * pl.tiles, pl.splits), dim3(64 * kWaves), lds, s, p);
     TECO_CHECK_LAUNCH("flash_attention_int4");
-    if (pl.splits > 1) {
-        constexpr int COLS = 256 / (D / 4);
-        hipLaunchKernelGGL((combine_kernel<D>), dim3(p.batch * p.Hkv, tecoops::ceil_div(pl.cols, COLS)), dim3(256), 0, s, p);
-        TECO_CHECK_LAUNCH("flash_attention_int4 combine");
-    }
-    return TECOOPS_STATUS_SUCCESS;
+    return launch_combine<T, D>(p, pl, s);
 }
 
-template <int D, int W, int HW, int TILE>
+template <typename T, int D, int W, int TILE>
 tecoopsStatus_t launch_tiles(const Params &p, const Plan &pl, hipStream_t s) {
-    constexpr int QT = 32 * (W / HW);
-    const size_t lds = tile_lds<D, TILE, W, HW>();
-    static_assert(tile_lds<D, TILE, W, HW>() + 8 * W <= tecoops::kLdsMax, "fits the LDS");
-    auto *kern = &tile_kernel<D, W, HW, TILE>;
+    constexpr size_t lds = tile_lds<D, TILE, W>();
+    static_assert(lds + 8 * W <= tecoops::kLdsMax, "fits the LDS");
+    auto *kern = &tile_kernel<T, D, W, TILE>;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), lds)) return TECOOPS_STATUS_INTERNAL_ERROR;
-    const unsigned tiles = std::min(tecoops::ceil_div(pl.rows, QT), 32768u);
-    hipLaunchKernelGGL(kern, dim3(p.batch * p.Hkv * (p.G / HW), tiles), dim3(W * 64), lds, s, p);
+    hipLaunchKernelGGL(kern, dim3(p.batch * p.Hkv, pl.tiles * pl.splits), dim3(W * 64), lds, s, p);
     TECO_CHECK_LAUNCH("flash_attention_int4");
-    return TECOOPS_STATUS_SUCCESS;
+    return launch_combine<T, D>(p, pl, s);
 }
 
-template <int D, int HW>
-tecoopsStatus_t launch_heads(const Params &p, const Plan &pl, hipStream_t s) {
-    if (pl.rows <= 1024) return launch_tiles<D, 4, HW, 32>(p, pl, s);
-    if constexpr (D <= 128) return launch_tiles<D, 12, HW, 96>(p, pl, s);
-    else return launch_tiles<D, 8, HW, 64>(p, pl, s);
-}
-
-template <int D>
+template <typename T, int D>
 tecoopsStatus_t launch_size(const Params &p, const Plan &pl, hipStream_t s) {
-    if (pl.split) return pl.ct == 1 ? launch_split<D, 1>(p, pl, s) : launch_split<D, 2>(p, pl, s);
-    if (p.G % 4 == 0) return launch_heads<D, 4>(p, pl, s);
-    if (p.G % 2 == 0) return launch_heads<D, 2>(p, pl, s);
-    return launch_heads<D, 1>(p, pl, s);
+    if (pl.split) return pl.ct == 1 ? launch_split<T, D, 1>(p, pl, s) : launch_split<T, D, 2>(p, pl, s);
+    if (pl.waves == 4) return launch_tiles<T, D, 4, 32>(p, pl, s);
+    if constexpr (D <= 128) return launch_tiles<T, D, 12, 96>(p, pl, s);
+    else return launch_tiles<T, D, 8, 64>(p, pl, s);
+}
+
+template <typename T>
+tecoopsStatus_t launch_type(const Params &p, const Plan &pl, int head_size, hipStream_t s) {
+    switch (head_size) {
+        case 32: return launch_size<T, 32>(p, pl, s);
+        case 64: return launch_size<T, 64>(p, pl, s);
+        case 96: return launch_size<T, 96>(p, pl, s);
+        case 128: return launch_size<T, 128>(p, pl, s);
+        case 160: return launch_size<T, 160>(p, pl, s);
+        default: return launch_size<T, 192>(p, pl, s);
+    }
 }
 
 bool head_size_ok(int D) { return D >= 32 && D <= 192 && D % 32 == 0; }
@@ -951,7 +1033,6 @@ extern "C" tecoopsStatus_t tecoopsFlashAttentionInt4(
     const float scale = softmax_scale > 0.0f ? softmax_scale : 1.0f / std::sqrt(static_cast<float>(head_size));
     p.scale_log2 = scale * 1.4426950408889634f;
     p.causal = causal != 0;
-    p.bf16 = dataType == TECOOPS_DATA_BFLOAT16;
     p.total_q = total_q;
     const int rows = std::max(max_seqlen_q, static_cast<int>(tecoops::ceil_div(total_q, batch)));
     const int keys = max_seqlen_k > 0 ? max_seqlen_k : std::max(p.kv_cap, 1);
@@ -962,30 +1043,20 @@ extern "C" tecoopsStatus_t tecoopsFlashAttentionInt4(
         return tecoops::fa4::make_plan(batch, num_heads, num_kv_heads, head_size, rows, keys, room, cus);
     };
     Plan pl = plan(workspace != nullptr ? workspace_bytes : ~size_t{0});
-    if (pl.split && pl.bytes > 0 && workspace == nullptr) {
+    if (pl.bytes > 0 && workspace == nullptr) {
         workspace = tecoops::handle_scratch_if_any(handle, pl.bytes);
         if (workspace == nullptr) pl = plan(0);
     }
     // the grid within 32-bit thread counts
-    const long long wgs = static_cast<long long>(batch) * num_heads * (pl.split ? pl.tiles : 1);
-    if (wgs * std::max(1, pl.split ? pl.splits : 1) >= (1ll << 22) || wgs >= (1ll << 22) || rows > (1 << 25))
-        return TECOOPS_STATUS_NOT_SUPPORTED;
-    p.rows = pl.rows;
+    if (static_cast<long long>(batch) * num_kv_heads * pl.tiles * pl.splits > (1ll << 22)) return TECOOPS_STATUS_NOT_SUPPORTED;
     p.cols = pl.cols;
     p.tiles = pl.tiles;
     p.split_len = pl.split_len;
     p.splits = pl.splits;
-    if (pl.split && pl.splits > 1) {
+    if (pl.splits > 1) {
         p.ws_o = static_cast<float *>(workspace);
         p.ws_ml = p.ws_o + pl.bytes / sizeof(float) / (head_size + 2) * head_size;
     }
     hipStream_t s = handle->stream;
-    switch (head_size) {
-        case 32: return launch_size<32>(p, pl, s);
-        case 64: return launch_size<64>(p, pl, s);
-        case 96: return launch_size<96>(p, pl, s);
-        case 128: return launch_size<128>(p, pl, s);
-        case 160: return launch_size<160>(p, pl, s);
-        default: return launch_size<192>(p, pl, s);
-    }
+    return dataType == TECOOPS_DATA_HALF ? launch_type<f16>(p, pl, head_size, s) : launch_type<bf16>(p, pl, head_size, s);
 }

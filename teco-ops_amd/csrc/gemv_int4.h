@@ -1,0 +1,43 @@
+// gemv_int4.h — how a product with 4-bit weights (gemv_int4.hip) is cut.
+#pragma once
+
+#include <algorithm>
+#include <cstddef>
+
+namespace tecoops {
+
+constexpr int kGemvInt4Stage = 512;  // of K, staged at a time by the matrix-core kernel
+constexpr int kGemvInt4DotK = 4096;  // the longest K of the kernel of one row of x
+constexpr int kGemvInt4Rows = 64;    // rows of W of its workgroups
+
+// Rows of x that a workgroup of it stages.
+inline int gemv_int4_staged(int batch) { return batch <= 8 ? 8 : batch >= 64 ? 64 : (batch + 15) / 16 * 16; }
+
+struct GemvInt4Plan {
+    bool dot;      // the kernel of one row of x
+    int parts;     // parts of K, their sums in the workspace where more than one
+    size_t bytes;  // of it
+};
+
+// room: bytes of workspace.
+inline GemvInt4Plan gemv_int4_plan(int batch, int n, int k, size_t room, int cus) {
+    GemvInt4Plan p{};
+    p.parts = 1;
+    const long long staged = gemv_int4_staged(batch);
+    const long long wgs = (n + kGemvInt4Rows - 1ll) / kGemvInt4Rows * ((batch + staged - 1) / staged);
+    const int stages = (k + kGemvInt4Stage - 1) / kGemvInt4Stage;
+    const size_t part = static_cast<size_t>(batch) * n * sizeof(float);
+    // as many parts as leave a workgroup a CU, two stages each or more
+    const long long most = std::min<long long>(cus / std::max(wgs, 1ll), stages / 2);
+    p.parts = static_cast<int>(std::max(1ll, std::min<long long>(most, static_cast<long long>(room / part))));
+    // one row over a short K takes about as long in either kernel, but two launches
+    // here where K is split (us, dot / this and the sums of its parts: 4096 x 4096
+    // 6.8 / 4.6 + 1.8, 2048 x 2048 5.9 / 4.9 + 2.0; 28672 x 4096 20.7 / 15.5,
+    // 4096 x 14336 18.4 / 10.2 + 2.0)
+    p.dot = batch == 1 && most > 1 && k <= kGemvInt4DotK;
+    if (p.dot) p.parts = 1;
+    p.bytes = p.parts > 1 ? part * p.parts : 0;
+    return p;
+}
+
+}  // namespace tecoops

@@ -723,8 +723,12 @@ void gemv_int4(const Tensor &weight, const Tensor &scales, const Tensor &x, Tens
     }
     if (b == 0) return;
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    size_t bytes = 0;
+    check(tecoopsGetGemvInt4WorkspaceSize(b, n, k, &bytes), "gemv_int4");
+    const Tensor ws = workspace_of(bytes, x);
     check(tecoopsGemvInt4(handle_for(x), weight.data_ptr(), scales.data_ptr(), z ? z->data_ptr() : nullptr, x.data_ptr(),
-                          out.data_ptr(), b, n, k, static_cast<int>(k / scales.size(1)), dt),
+                          out.data_ptr(), b, n, k, static_cast<int>(k / scales.size(1)), bytes ? ws.data_ptr() : nullptr,
+                          bytes, dt),
           "gemv_int4");
 }
 

@@ -927,8 +927,10 @@ def gemv_int4(weight, scales, x, out, zeros=None):
         _raise(refused, "tecoopsGemvInt4")
     if B == 0:
         return
+    space = _workspace(device, "tecoopsGetGemvInt4WorkspaceSize", B, N, K)
     _call_on(device, "tecoopsGemvInt4", _handle(device), _ptr(weight), _ptr(scales), _ptr(zeros),
-             _ptr(x), _ptr(out), B, N, K, K // scales.shape[1], code)
+             _ptr(x), _ptr(out), B, N, K, K // scales.shape[1], _ptr(space),
+             0 if space is None else space.numel(), code)
 
 
 def memset(t, value):

@@ -95,7 +95,8 @@ SIGNATURES = {
     "tecoopsFlashAttentionInt4": (I, [P, I, I, P, P, P, LL, I, I, P, P, P, P, P, P, I, I, I, I, I, I,
                                       F, I, P, SZ, I]),
     "tecoopsGetFlashAttentionInt4WorkspaceSize": (I, [I, I, I, I, I, I, I, P]),
-    "tecoopsGemvInt4": (I, [P, P, P, P, P, P, I, I, I, I, I]),
+    "tecoopsGemvInt4": (I, [P, P, P, P, P, P, I, I, I, I, P, SZ, I]),
+    "tecoopsGetGemvInt4WorkspaceSize": (I, [I, I, I, P]),
 }
 
 _LIB = None

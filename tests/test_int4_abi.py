@@ -102,18 +102,57 @@ def test_attention_refusals(handle):
 
 
 def test_gemv_refusals(handle):
-    good = dict(h=handle, w=P, s=P, z=P, x=P, y=P, B=2, n=32, k=256, g=64, dt=1)
+    good = dict(h=handle, w=P, s=P, z=P, x=P, y=P, B=2, n=32, k=256, g=64, ws=None, wb=0, dt=1)
     call = caller("tecoopsGemvInt4", good)
     assert call(h=None) == NOT_INIT
     for name in ("w", "s", "x", "y"):
         assert call(**{name: None}) == BAD, name
     for kw in (dict(B=-1), dict(n=0), dict(k=0), dict(g=0), dict(g=96), dict(dt=0), dict(w=P + 8), dict(s=P + 1),
-               dict(z=P + 1), dict(x=P + 1), dict(y=P + 1)):
+               dict(z=P + 1), dict(x=P + 1), dict(y=P + 1), dict(ws=P + 2, wb=64)):
         assert call(**kw) == BAD, kw
     assert call(g=16) == NOT_SUP and call(k=48, g=48) == NOT_SUP
     assert call(n=(1 << 26) + 1) == NOT_SUP and call(B=(1 << 16) + 1) == NOT_SUP
     assert call(B=1 << 14, n=1 << 14) == NOT_SUP
     assert call(B=0) == OK  # no launch
+    size = ctypes.c_size_t(1)
+    g = _lib.lib().tecoopsGetGemvInt4WorkspaceSize
+    assert g(2, 32, 256, None) == BAD and g(-1, 32, 256, ctypes.byref(size)) == BAD
+    assert g(2, 0, 256, ctypes.byref(size)) == BAD and g(2, 32, 0, ctypes.byref(size)) == BAD
+    assert g(0, 32, 256, ctypes.byref(size)) == OK and size.value == 0
+
+
+@pytest.fixture(scope="module")
+def parts(tmp_path_factory):
+    d = tmp_path_factory.mktemp("parts")
+    (d / "parts.cpp").write_text("""#include "gemv_int4.h"
+extern "C" void parts(int b, int n, int k, unsigned long long room, long long *o) {
+    const auto p = tecoops::gemv_int4_plan(b, n, k, room, 256);
+    o[0] = p.dot; o[1] = p.parts; o[2] = (long long)p.bytes; o[3] = tecoops::gemv_int4_staged(b);
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-fPIC", "-shared", "-I", CSRC, str(d / "parts.cpp"), "-o",
+                    str(d / "parts.so")], check=True)
+    lib = ctypes.CDLL(str(d / "parts.so"))
+    lib.parts.argtypes = [ctypes.c_int] * 3 + [ctypes.c_ulonglong, ctypes.c_void_p]
+
+    def run(b, n, k, room=(1 << 63)):
+        o = (ctypes.c_longlong * 4)()
+        lib.parts(b, n, k, room, o)
+        return list(o)
+    return run
+
+
+def test_parts_of_k(parts):
+    """No more parts than stages of K, and their sums fit the workspace."""
+    for b in (1, 2, 3, 8, 9, 33, 64, 65, 1000):
+        for n in (1, 64, 65, 1000, 4096, 28672, 1 << 20):
+            for k in (32, 512, 513, 1024, 4096, 14336, 1 << 20):
+                for room in (0, 1 << 20, 1 << 63):
+                    dot, count, need, staged = parts(b, n, k, room)
+                    assert staged >= min(b, 64) and staged in (8, 16, 32, 48, 64)
+                    assert 1 <= count <= max(1, k // 1024) and need <= room
+                    assert need == (b * n * 4 * count if count > 1 else 0)
+                    assert count == 1 or not dot
 
 
 @pytest.fixture(scope="module")
@@ -122,8 +161,8 @@ def plan(tmp_path_factory):
     (d / "plan.cpp").write_text("""#include "fa_int4.h"
 extern "C" void plan(int b, int h, int hkv, int d, int rows, int keys, unsigned long long room, long long *o) {
     const auto p = tecoops::fa4::make_plan(b, h, hkv, d, rows, keys, room, 256);
-    o[0] = p.split; o[1] = p.ct; o[2] = p.tiles; o[3] = p.cols; o[4] = p.split_len; o[5] = p.splits;
-    o[6] = (long long)p.bytes;
+    o[0] = p.split; o[1] = p.split ? p.ct * 16 : p.waves * 32; o[2] = p.tiles; o[3] = p.cols;
+    o[4] = p.split_len; o[5] = p.splits; o[6] = (long long)p.bytes;
 }
 """)
     subprocess.run(["g++", "-std=c++17", "-fPIC", "-shared", "-I", CSRC, str(d / "plan.cpp"), "-o",
@@ -146,12 +185,11 @@ def test_splits_cover_the_keys(plan, room):
         for h, hkv in ((1, 1), (8, 1), (32, 8), (64, 1), (40, 8)):
             for rows in (1, 2, 5, 17, 64, 1000):
                 for keys in (1, 31, 32, 128, 129, 777, 8192, 100000, (1 << 31) - 4097):
-                    split, ct, tiles, cols, length, splits, need = plan(b, h, hkv, 128, rows, keys, room)
-                    if not split:
-                        assert h // hkv * rows > 16 and need == 0
-                        continue
-                    assert cols == h // hkv * rows and (tiles - 1) * 16 * ct < cols <= tiles * 16 * ct
-                    assert length % 128 == 0 and need <= room
+                    split, tile, tiles, cols, length, splits, need = plan(b, h, hkv, 128, rows, keys, room)
+                    assert cols == h // hkv * rows and (tiles - 1) * tile < cols <= tiles * tile
+                    # whole rounds of a workgroup's waves, whole tiles of keys
+                    assert length % (128 if split else 96) == 0 or splits == 1
+                    assert need <= room
                     assert splits >= 1 and (splits - 1) * length < keys
                     assert splits * length >= keys or splits == 1
                     assert need == (0 if splits == 1 else b * hkv * splits * cols * (128 + 2) * 4)
