@@ -74,13 +74,15 @@ EXTRA_FLAGS = {
 # with a fixed vmcnt that leaves the compiler's own younger loads in flight.
 # The count is right only if those loads stay between the copies and the
 # wait, which the compiler does not promise for loads of read-only memory,
-# so the device assembly of these sources is checked on every build.
-# flash_attention.hip, gemv_batch.hip and moe.hip wait for their copies by
+# so the device assembly of these sources is checked on every build (with it
+# the waits behind matrix products).
+# flash_attention.hip, fa_int4.hip, gemv_batch.hip and moe.hip wait for their copies by
 # counting only younger copies (inline assembly, which the compiler keeps in
 # order) and linear.hip for all of its copies at once, so only their use of M0 is
 # checked.
 COPY_WAIT_CHECKED = {"gemv.hip": True, "gemv_batch.hip": False, "linear.hip": False,
-                     "moe.hip": False, "flash_attention.hip": False, "fa_split.hip": False}
+                     "moe.hip": False, "flash_attention.hip": False, "fa_split.hip": False,
+                     "fa_int4.hip": False}
 
 
 def check_copy_waits(asm_text, src="", waits=True):
@@ -101,6 +103,9 @@ def check_copy_waits(asm_text, src="", waits=True):
         lines = [l for l in lines if l and not l.startswith(".")]
         if not any(l.startswith("global_load_lds") for l in lines):
             continue
+        # (a wait state may stand between M0 and its copy)
+        lines = [l for i, l in enumerate(lines)
+                 if not (l.startswith("s_nop") and i and lines[i - 1].startswith("s_mov_b32 m0,"))]
         pending, since = False, 0
         for i, l in enumerate(lines):
             if re.search(r"\bm0\b", l) and not (l.startswith("s_mov_b32 m0,") and i + 1 < len(lines)
@@ -127,6 +132,65 @@ def check_copy_waits(asm_text, src="", waits=True):
     return checked
 
 
+def _vector_registers(text):
+    import re
+    regs = set()
+    for m in re.finditer(r"\bv\[(\d+):(\d+)\]|\bv(\d+)\b", text):
+        regs |= {int(m.group(3))} if m.group(3) else set(range(int(m.group(1)), int(m.group(2)) + 1))
+    return regs
+
+
+def check_matrix_waits(asm_text, src=""):
+    """Checks that on every path of each kernel enough wait states lie between a
+    v_mfma and the first vector or memory instruction that reads its result or
+    overwrites it (for a product of P passes P + 4, of 2 passes 5;
+    those of 4 x 4 results have 2 passes, of 16 x 16 at most 4 here, of 32 x 32 8, or
+    16 with a depth of 8 or less).  The
+    hardware does not wait by itself, and the compiler has left the wait out where a
+    branch lay between the two.  Returns the number of products; raises
+    RuntimeError on a violation."""
+    import re
+    count = 0
+    for k in re.finditer(r"^(_Z\S*):", asm_text, re.M):
+        code, labels = [], {}
+        for l in asm_text[k.end():asm_text.find(".Lfunc_end", k.end())].split("\n"):
+            l = l.split(";")[0].strip()
+            m = re.match(r"(\.L\S+):", l)
+            if m:
+                labels[m.group(1)] = len(code)
+            elif l and not l.startswith("."):
+                op, _, args = l.partition(" ") if " " in l else l.partition("\t")
+                code.append((op, args.strip()))
+        for i, (op, args) in enumerate(code):
+            if not op.startswith("v_mfma"):
+                continue
+            count += 1
+            need = 5 if "_4x4x" in op else 8 if "_16x16x" in op else 12 if "_32x32x16" in op else 20
+            result = _vector_registers(args.split(",")[0])
+            paths, seen = [(i + 1, 0)], set()
+            while paths:
+                j, passed = paths.pop()
+                if j >= len(code) or passed >= need or (j, passed) in seen:
+                    continue
+                seen.add((j, passed))
+                o, a = code[j]
+                if o.startswith("v_mfma"):
+                    used = _vector_registers(",".join(re.findall(r"v\[\d+:\d+\]", a)[1:3]))
+                elif o.startswith(("v_", "ds_", "global_", "buffer_", "flat_", "scratch_")):
+                    used = _vector_registers(a)
+                else:
+                    used = set()
+                if used & result:
+                    raise RuntimeError(f"{src}: {k.group(1)}: {o} {a} only {passed} wait states behind "
+                                       f"{op} {args}")
+                passed += 1 + (int(a) if o == "s_nop" else 0)
+                if o.startswith(("s_branch", "s_cbranch")):
+                    paths.append((labels[a], passed))
+                if o not in ("s_branch", "s_endpgm"):
+                    paths.append((j + 1, passed))
+    return count
+
+
 def _check_copies(src, waits):
     out = os.path.join(BUILD, os.path.splitext(src)[0] + ".s")
     cmd = [HIPCC, *CFLAGS, *EXTRA_FLAGS.get(src, []), "--cuda-device-only", "-S",
@@ -135,7 +199,9 @@ def _check_copies(src, waits):
     if r.returncode != 0:
         raise RuntimeError(f"assembly failed: {src}\n{' '.join(cmd)}\n{r.stderr[-4000:]}")
     with open(out) as f:
-        n = check_copy_waits(f.read(), src, waits)
+        asm = f.read()
+    n = check_copy_waits(asm, src, waits)
+    check_matrix_waits(asm, src)
     os.remove(out)
     if n == 0:
         raise RuntimeError(f"{src}: no LDS copies found to check")

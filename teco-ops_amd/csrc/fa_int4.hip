@@ -22,9 +22,9 @@
 //   * Scores are computed transposed (keys x columns, 16x16x32), so that a lane
 //     holds 8 keys of one column, which are the operand of the second product as
 //     they are: neither P nor the codes go through LDS.
-//   * A wave takes every 4th block of 32 keys; the next block's loads are under
-//     way meanwhile.  Partial states meet in LDS, those of splits in a second
-//     kernel.
+//   * A wave takes every 4th block of 32 keys, copied into a ring in LDS without
+//     registers while it works on the blocks before.  Partial states meet in LDS,
+//     those of splits in a second kernel.
 //
 // Tile route (prefill).  K and V tiles are widened to fp16 once per workgroup, on
 // the way into LDS, and attended as in flash_attention.hip (fa_device.h).  fp16
@@ -50,7 +50,9 @@ struct Params {
     long long bt_stride;
     const int *cu_q, *kv_lens;
     int batch, H, Hkv, G, bs, lbs, num_blocks;  // lbs = log2(bs) or -1
+    uint32_t inv_bs;                            // 2^32 / bs rounded up, or 0
     int kv_cap;                                 // keys that a table row can name
+    long long page_rows;                        // rows of a block: heads * keys
     float scale_log2;
     int causal;
     long long total_q;
@@ -58,7 +60,6 @@ struct Params {
     int cols, tiles, split_len, splits;
 };
 
-typedef unsigned __attribute__((aligned(4))) u32_a4;
 typedef float4_t f32x4_t;
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
@@ -87,7 +88,12 @@ __device__ __forceinline__ void zero_tail(const Params &p, int D) {
         o[c] = u32x4{0u, 0u, 0u, 0u};
 }
 
-__device__ __forceinline__ int block_at(const Params &p, int key) { return p.lbs >= 0 ? key >> p.lbs : key / p.bs; }
+// Cache block of a key: a shift, a product with 2^32 / bs where that is exact for
+// every key that the table can name, or a division.
+__device__ __forceinline__ int block_at(const Params &p, int key) {
+    if (p.lbs >= 0) return key >> p.lbs;
+    return p.inv_bs != 0u ? static_cast<int>(__umulhi(static_cast<uint32_t>(key), p.inv_bs)) : key / p.bs;
+}
 
 // Row of the cache, in rows of all blocks and heads, of a key whose block-table
 // entry is `page`; entries out of range are taken as block 0.
@@ -103,106 +109,147 @@ constexpr float kMiddle = 7.5f;  // of the codes
 constexpr int kLeastRef = -90;   // (sums of 2^24 weights stay within fp32)
 constexpr float kNever = -1e30f;  // the running maximum before any key
 
-// Block-size modes: 1 a multiple of 16 (a block of 16 keys lies in one page: its
-// entry is a scalar), 2 a multiple of 4 (so do a lane's 4 keys), 0 any.
-template <int D, int BSM>
-struct Block {
-    static constexpr int KW = D / 32;  // 32-bit words of a key row in a lane
+// N words of each lane from `base` + `off` (or `src`) to `dst` in LDS, lane after lane
+// (M0 holds where; a copy has to be a wait state behind its write).
+__device__ __forceinline__ uint32_t lds_address(char *at) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)(at)));
+}
+__device__ __forceinline__ void copy4(const void *base, uint32_t off, char *dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base),
+                 "s"(lds_address(dst))
+                 : "memory");
+}
+__device__ __forceinline__ void copy4(const void *src, char *dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_address(dst))
+                 : "memory");
+}
+__device__ __forceinline__ void copy1(const void *src, char *dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds_address(dst))
+                 : "memory");
+}
+
+// A wave's blocks of 32 keys on their way: keys, values and pairs go from the cache
+// straight into LDS (global_load_lds, no registers), DEPTH blocks in a ring of the
+// wave's own, so that a block is worked on while the next ones are under way.
+//
+//   keys    head_size 128: 16 bytes at 16 (64 h + 16 g + m), the words that lane
+//           (g, m) reads for key 16 h + m; else rows as they are
+//   values  rows, that of key 16 h + 4 g + i at 16 h + 4 i + g: the four rows that a
+//           read touches lie together
+//   pairs   32 of the keys, 32 of the values
+//
+// UNIFORM: pages hold a multiple of 16 keys, so that the pages of a block's halves are
+// scalars, followed from block to block without a division, and where a copy's rows
+// are of one half (head size 128) it costs no vector instruction but itself;
+// else each lane looks its rows' entries up in a copy of the table's part in LDS
+// (kTable entries; what lies behind them, in memory).
+constexpr int kTable = 2048;
+
+template <int D, bool UNIFORM>
+struct Ring {
+    static constexpr int KW = D / 32;               // 32-bit words of a key row in a lane
     static constexpr int N128 = D / 128, N64 = D % 128 / 64, N32 = D % 64 / 32;
-    static constexpr int VP = BSM == 0 ? 4 : 1;  // table entries of a lane's 4 keys
-    uint32_t k[2][KW];
-    uint32_t v[2][4][N128 + N64 + N32];
-    u32x4 ks[2], vs[2];
+    static constexpr int NI = (D + 63) / 64;        // copies of the keys, and of the values
+    static constexpr int PER = 2 * NI + 1;          // copies of a block
+    static constexpr int V_AT = NI * 1024, P_AT = 2 * NI * 1024, BYTES = P_AT + 256;
+    static constexpr int DEPTH = D <= 64 ? 4 : 2;
+    static constexpr int STEP = 32 * kWaves;        // keys from a wave's block to its next
+    static constexpr bool SCALAR = UNIFORM && D == 128;
+    static_assert((DEPTH - 1) * PER < 64, "vmcnt");
 
-    // The block-table entries that a load() needs, fetched one load ahead of it.
-    struct Pages {
-        int kp[2], vp[2][VP];
-    };
+    const Params &p;
+    const int *table, *copy;
+    int kvh, first, limit;
+    const uint32_t *pairs;  // of the lane: the keys' or the values'
+    uint32_t koff, voff;    // SCALAR: the lane's 16 bytes within 16 rows
+    // UNIFORM: the pages and places in them of the block to ask for next
+    uint32_t in, step_in, within[2] = {0, 0};
+    int blk, step_blk, last, page[2] = {0, 0};
 
-    static __device__ __forceinline__ void pages(Pages &g, const Params &p, const int *table, int j0, int limit) {
+    __device__ __forceinline__ Ring(const Params &params, int kv_head, const int *entries, const int *copied, int from,
+                                    int end, int j0)
+        : p(params), table(entries), copy(copied), kvh(kv_head), first(from), limit(end) {
         const int lane = threadIdx.x & 63;
-        int(&kp)[2] = g.kp, (&vp)[2][VP] = g.vp;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            if constexpr (BSM == 1) {
-                const int row = __builtin_amdgcn_readfirstlane(j0 + 16 * b);
-                const auto *t4 = (const __attribute__((address_space(4))) int *)(table);
-                kp[b] = row < limit ? t4[block_at(p, row)] : 0;
-            } else {
-                const int key = j0 + 16 * b + (lane & 15);
-                kp[b] = table[block_at(p, key < limit ? key : 0)];
-#pragma unroll
-                for (int i = 0; i < VP; ++i) {
-                    const int kv = j0 + 16 * b + 4 * (lane >> 4) + i;
-                    vp[b][i] = table[block_at(p, kv < limit ? kv : 0)];
-                }
+        pairs = lane < 32 ? p.ks : p.vs;
+        asm volatile("" : "+v"(pairs));  // (in registers, not loaded again for each block)
+        koff = (lane & 15) * (D / 2) + 16 * (lane >> 4);
+        voff = (4 * (lane >> 2 & 3) + (lane >> 4)) * (D / 2) + 16 * (lane & 3);
+        if constexpr (UNIFORM) {
+            const int b = block_at(p, j0);
+            blk = __builtin_amdgcn_readfirstlane(b);
+            in = __builtin_amdgcn_readfirstlane(j0 - b * p.bs);
+            step_blk = __builtin_amdgcn_readfirstlane(block_at(p, STEP));
+            step_in = __builtin_amdgcn_readfirstlane(STEP - block_at(p, STEP) * p.bs);
+            last = __builtin_amdgcn_readfirstlane(block_at(p, max(limit - 1, 0)));
+        }
+    }
+
+    // Asks for the table entries of the next block's halves (read-only for the launch:
+    // scalar loads).  Behind the last key's page it is that page again.
+    __device__ __forceinline__ void turn() {
+        if constexpr (UNIFORM) {
+            const auto *entry = (const __attribute__((address_space(4))) int *)(table);
+            const bool next = in + 16 >= static_cast<uint32_t>(p.bs);
+            within[0] = in;
+            within[1] = next ? 0u : in + 16;
+            page[0] = entry[min(blk, last)];
+            page[1] = entry[min(next ? blk + 1 : blk, last)];
+            blk += step_blk;
+            in += step_in;
+            if (in >= static_cast<uint32_t>(p.bs)) {
+                in -= p.bs;
+                ++blk;
             }
         }
     }
 
-    // The 32 keys (load_k) or values (load_v) from j0 on; what lies at `limit` or
-    // behind it is some row.
-    __device__ __forceinline__ void load_k(const Pages &pg, const Params &p, int kvh, int j0, int limit) {
-        const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            int key = j0 + 16 * b + (BSM == 1 ? 0 : m);
-            key = key < limit ? key : 0;
-            long long kr = row_of(p, kvh, pg.kp[b], key, block_at(p, key));
-            long long sr = kr + 4 * g;
-            if (BSM == 1) kr += m;
-            const u32_a4 *kw = reinterpret_cast<const u32_a4 *>(p.kc + kr * (D / 2)) + g * KW;
-#pragma unroll
-            for (int w = 0; w < KW; ++w) k[b][w] = __builtin_nontemporal_load(kw + w);
-            if constexpr (BSM != 1) sr = row4(pg, p, kvh, j0, limit, b, 0);
-            ks[b] = pairs4(pg, p, p.ks, kvh, j0, limit, b, sr);
-        }
+    // Row of key j0 + r of a block; half0, half1: the first rows of its halves (UNIFORM).
+    __device__ __forceinline__ long long row(long long half0, long long half1, int j0, int r) const {
+        if constexpr (UNIFORM) return half0 + (r < 16 ? 0 : half1 - half0) + (r & 15);
+        const int key = j0 + r < limit ? j0 + r : first;
+        const int b = block_at(p, key), at = b - block_at(p, first);
+        return row_of(p, kvh, at < kTable ? copy[at] : table[b], key, b);
     }
-    __device__ __forceinline__ void load_v(const Pages &pg, const Params &p, int kvh, int j0, int limit) {
-        const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+
+    // Asks for the 32 keys from j0 on (UNIFORM: of the pages of the last turn()).
+    __device__ __forceinline__ void load(int j0, char *dst) const {
+        const int lane = threadIdx.x & 63;
+        const auto first_row = [&](int pg, uint32_t at) {
+            if (pg < 0 || pg >= p.num_blocks) pg = 0;
+            return static_cast<uint32_t>(pg) * p.page_rows + static_cast<long long>(kvh) * p.bs + at;
+        };
+        const long long half0 = UNIFORM ? first_row(page[0], within[0]) : 0;
+        const long long half1 = UNIFORM ? first_row(page[1], within[1]) : 0;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            long long r0;
-            if constexpr (BSM == 1) {
-                const int key = j0 + 16 * b < limit ? j0 + 16 * b : 0;
-                r0 = row_of(p, kvh, pg.kp[b], key, block_at(p, key)) + 4 * g;
+        for (int n = 0; n < NI; ++n) {
+            if constexpr (SCALAR) {
+                copy4(p.kc + (n == 0 ? half0 : half1) * (D / 2), koff, dst + 1024 * n);
             } else {
-                r0 = row4(pg, p, kvh, j0, limit, b, 0);
+                const int c = min(64 * n + lane, D - 1);  // 16-byte words of 32 rows: D of them
+                const int r = D == 128 ? 16 * n + (lane & 15) : c / KW, w = D == 128 ? lane >> 4 : c - r * KW;
+                copy4(p.kc + row(half0, half1, j0, r) * (D / 2) + 16 * w, dst + 1024 * n);
             }
+        }
+        copy1(pairs + row(half0, half1, j0, lane & 31), dst + P_AT);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint8_t *row = p.vc + (BSM == 0 && i > 0 ? row4(pg, p, kvh, j0, limit, b, i) : r0 + i) * (D / 2);
-#pragma unroll
-                for (int n = 0; n < N128; ++n)
-                    v[b][i][n] = __builtin_nontemporal_load(reinterpret_cast<const u32_a4 *>(row + 64 * n) + m);
-                if constexpr (N64 > 0)
-                    v[b][i][N128] = *(reinterpret_cast<const uint16_t *>(row + 64 * N128) + m);
-                if constexpr (N32 > 0) v[b][i][N128 + N64] = row[64 * N128 + 32 * N64 + m];
+        for (int n = 0; n < NI; ++n) {
+            if constexpr (SCALAR) {
+                copy4(p.vc + (n == 0 ? half0 : half1) * (D / 2), voff, dst + V_AT + 1024 * n);
+            } else {
+                const int c = min(64 * n + lane, D - 1), q = c / KW, w = c - q * KW;
+                const int r = (q & 16) + 4 * (q & 3) + (q >> 2 & 3);
+                copy4(p.vc + row(half0, half1, j0, r) * (D / 2) + 16 * w, dst + V_AT + 1024 * n);
             }
-            vs[b] = pairs4(pg, p, p.vs, kvh, j0, limit, b, r0);
         }
     }
 
-private:
-    // Row of this lane's key i of its four of half b.
-    static __device__ __forceinline__ long long row4(const Pages &pg, const Params &p, int kvh, int j0, int limit, int b,
-                                                     int i) {
-        int key = j0 + 16 * b + 4 * static_cast<int>(threadIdx.x >> 4 & 3) + i;
-        key = key < limit ? key : 0;
-        return row_of(p, kvh, pg.vp[b][BSM == 0 ? i : 0], key, block_at(p, key));
-    }
-    // The pairs of its four keys, the first in row r0.
-    static __device__ __forceinline__ u32x4 pairs4(const Pages &pg, const Params &p, const uint32_t *pairs, int kvh, int j0,
-                                                   int limit, int b, long long r0) {
-        if constexpr (BSM == 0) {
-            u32x4 x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = pairs[i == 0 ? r0 : row4(pg, p, kvh, j0, limit, b, i)];
-            return x;
-        } else {
-            typedef u32x4 __attribute__((aligned(4))) u32x4_a4;
-            return *reinterpret_cast<const u32x4_a4 *>(pairs + r0);
-        }
+    // Waits until at most `newer` blocks asked for after this one are under way (any
+    // other load under way only makes it wait for more).
+    template <int NEWER>
+    static __device__ __forceinline__ void wait() {
+        constexpr int n = NEWER * PER;
+        __builtin_amdgcn_s_waitcnt(((n >> 4) << 14) | 0x0F70 | (n & 15));
+        asm volatile("" ::: "memory");
     }
 };
 
@@ -290,103 +337,158 @@ __device__ __forceinline__ void load_column(const Params &p, Column<D> &c, const
     c.to_log2 = p.scale_log2 * power2(e - 14) * 0x1p24f;
 }
 
-// Scores of the 32 keys from j0 on, held in `b`, before their factor to_log2.  Keys at
-// `limit` or behind it, and keys that a column does not see, score -inf and have pairs
-// of 0, whatever the cache holds there; `edge`: some are among these.
-template <typename T, int D, int CT, int BSM>
-__device__ __forceinline__ void scores(Block<D, BSM> &b, const Column<D> (&col)[CT], f32x4_t (&s)[CT][2], int j0,
-                                       int limit, bool edge) {
-    const int g = (threadIdx.x & 63) >> 4;
+// A column's sum or maximum over the lanes that hold its keys: 4 groups of 16, and
+// with PACK > 1 the lanes n of a group that are alike modulo 16 / PACK.
+template <int PACK>
+__device__ __forceinline__ float column_sum(float v) {
+    if (PACK >= 4) v += dpp<kDppRor4>(v);
+    if (PACK >= 2) v += dpp<kDppRor8>(v);
+    return row_swap_sum(half_swap_sum(v));
+}
+template <int PACK>
+__device__ __forceinline__ float column_max(float v) {
+    if (PACK >= 4) v = fmaxf(v, dpp<kDppRor4>(v));
+    if (PACK >= 2) v = fmaxf(v, dpp<kDppRor8>(v));
+    return row_swap_max(half_swap_max(v));
+}
+
+// Lane l's value from lane l + N of its row of 16 (N 4, 8 or 12; 0 from past its end).
+template <int N>
+__device__ __forceinline__ uint32_t from_right(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x100 + N, 0xF, 0xF, true));
+}
+
+// The 32 keys from j0 on, whose block lies at `blk`, into the state.  Keys at `limit`
+// or behind it, and keys that a column does not see, weigh nothing, whatever the cache
+// holds there; `edge`: some are among these.
+//
+// PACK (one column tile): with at most 16 / PACK columns the matrix core's 16 hold
+// each of them PACK times, all with the same scores, and each of the copies' lanes
+// takes 8 / PACK of its 8 keys through the softmax instead of all: 4 heads of a group
+// are then a quarter of that work (the larger part of what is not a mask or a product).
+template <typename T, int D, int CT, int PACK>
+__device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[CT], State<D, CT> &st, int j0, int limit,
+                                       bool edge) {
+    using R = Ring<D, true>;
+    static_assert(CT == 1 || PACK == 1, "copies of one tile's columns");
+    constexpr int V = 8 / PACK;  // keys of a lane: (half h, i) in order, V from V part on
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+    const int part = PACK == 1 ? 0 : m / (16 / PACK);
+    const int k0 = V * part >= 4 ? 16 + 4 * g : V == 2 ? 4 * g + 2 * (part & 1) : 4 * g;  // its first key
+    const int first = V == 2 && part >= 2 ? 16 + 4 * g + 2 * (part & 1) : k0;
+    const auto key_of = [&](int e) { return PACK == 1 ? 16 * (e >> 2) + 4 * g + (e & 3) : first + e; };
+    const auto pairs = [&](uint32_t(&pair)[V], int at) {
+        if constexpr (V == 2) {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(blk + at + 4 * first);
+            pair[0] = w[0];
+            pair[1] = w[1];
+        } else {
 #pragma unroll
-    for (int t = 0; t < CT; ++t)
+            for (int h = 0; h < V / 4; ++h) {
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(blk + at + 4 * (V == 4 ? first : 16 * h + 4 * g));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) s[t][h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int i = 0; i < 4; ++i) pair[4 * h + i] = w[i];
+            }
+        }
+    };
+    uint32_t k[2][R::KW], kp[V], vp[V];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(blk + (D == 128 ? 1024 * h + 16 * lane
+                                                                                 : (16 * h + m) * (D / 2) + g * (D / 8)));
+        if constexpr (D == 128) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) k[h][i] = w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < R::KW; ++i) k[h][i] = src[i];
+        }
+    }
+    pairs(kp, R::P_AT);
+    pairs(vp, R::P_AT + 128);
+    f32x4_t raw[CT][2];
 #pragma unroll
     for (int w = 0; w < D / 32; ++w)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const u32x4 a = widen8(b.k[h][w]);
+            const u32x4 a = widen8(k[h][w]);
 #pragma unroll
-            for (int t = 0; t < CT; ++t) s[t][h] = mma16(a, col[t].q[w], s[t][h]);
+            for (int t = 0; t < CT; ++t)
+                raw[t][h] = mma16(a, col[t].q[w], w == 0 ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f} : raw[t][h]);
         }
-    if (edge) {
-        asm volatile("");  // (a branch, taken in the last block alone)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (j0 + 16 * h + 4 * g + i >= limit) b.ks[h][i] = 0u;
-    }
+    uint32_t v[2][4][R::N128 + R::N64 + R::N32];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float sk = lo<T>(b.ks[h][i]), ak = hi<T>(b.ks[h][i]);
+            const char *row = blk + R::V_AT + (16 * h + 4 * i + g) * (D / 2);
 #pragma unroll
-            for (int t = 0; t < CT; ++t) s[t][h][i] = fmaf(sk, s[t][h][i], ak * col[t].sum);
+            for (int n = 0; n < R::N128; ++n) v[h][i][n] = *(reinterpret_cast<const uint32_t *>(row + 64 * n) + m);
+            if constexpr (R::N64 > 0)
+                v[h][i][R::N128] = *(reinterpret_cast<const uint16_t *>(row + 64 * R::N128) + m);
+            if constexpr (R::N32 > 0)
+                v[h][i][R::N128 + R::N64] = *(reinterpret_cast<const uint8_t *>(row + 64 * R::N128 + 32 * R::N64) + m);
         }
+    float s[CT][V];
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            float x;
+            if constexpr (PACK == 1) {
+                x = raw[t][e >> 2][e & 3];
+            } else if constexpr (PACK == 2) {
+                x = part ? raw[t][1][e] : raw[t][0][e];
+            } else {
+                const float x0 = part & 1 ? raw[t][0][2 + e] : raw[t][0][e], x1 = part & 1 ? raw[t][1][2 + e] : raw[t][1][e];
+                x = part & 2 ? x1 : x0;
+            }
+            s[t][e] = fmaf(lo<T>(kp[e]), x, hi<T>(kp[e]) * col[t].sum);
+        }
+    // (a branch, taken in the last blocks alone; none stands between a product and the
+    // reads of it, across which the compiler has left out waits that those need)
     if (edge) {
         asm volatile("");
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (j0 + key_of(e) >= limit) vp[e] = 0u;
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (j0 + 16 * h + 4 * g + i >= min(limit, col[t].vis)) s[t][h][i] = kNegInf;
+            for (int e = 0; e < V; ++e)
+                if (j0 + key_of(e) >= min(limit, col[t].vis)) s[t][e] = kNegInf;
     }
-}
-
-// Their values, weighted by the softmax of the scores, into the state.
-template <typename T, int D, int CT, int BSM>
-__device__ __forceinline__ void weigh(Block<D, BSM> &b, const Column<D> (&col)[CT], const f32x4_t (&s)[CT][2],
-                                      State<D, CT> &st, int j0, int limit, bool edge) {
-    const int g = (threadIdx.x & 63) >> 4;
-    if (edge) {
-        asm volatile("");
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (j0 + 16 * h + 4 * g + i >= limit) b.vs[h][i] = 0u;
-    }
-    float sv[2][4], av[2][4];
+    float sv[V], av[V];
     float top = 0.0f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sv[h][i] = lo<T>(b.vs[h][i]);
-            av[h][i] = fmaf(kMiddle, sv[h][i], hi<T>(b.vs[h][i]));
-            top = fmaxf(top, fabsf(sv[h][i]));
-        }
-    // scales relative to a power of two that is at least half of the largest seen
-    if (!__all(top <= st.twice_ref)) {
-        top = row_swap_max(half_swap_max(top));
-        const int e = min(static_cast<int>(__float_as_uint(top) >> 23) - 127, 100);
-        if (e > st.ref) {
-            const float down = e - st.ref > 120 ? 0.0f : power2(st.ref - e);
-            st.ref = e;
-            st.twice_ref = power2(e + 1);
-#pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                st.l[t] *= down;
-                st.r[t] *= down;
-                st.w[t] *= down;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= down;
-            }
-        }
+    for (int e = 0; e < V; ++e) {
+        sv[e] = lo<T>(vp[e]);
+        av[e] = fmaf(kMiddle, sv[e], hi<T>(vp[e]));
+        top = fmaxf(top, fabsf(sv[e]));
     }
-    u32x4 pw[CT];
+    float mx[CT];
+    bool raise = !(top <= st.twice_ref);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
-        float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                         fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3]))) * col[t].to_log2;
-        if (!__all(mx <= st.m[t] + kSlack)) {
-            mx = row_swap_max(half_swap_max(mx));
-            const float next = fmaxf(st.m[t], mx);
-            const float f = __builtin_amdgcn_exp2f(st.m[t] - next);
+        mx[t] = s[t][0];
+#pragma unroll
+        for (int e = 1; e < V; ++e) mx[t] = fmaxf(mx[t], s[t][e]);
+        mx[t] *= col[t].to_log2;
+        raise = raise || !(mx[t] <= st.m[t] + kSlack);
+    }
+    if (__any(raise)) {
+        // scales relative to a power of two that is at least half of the largest seen
+        // (wave-wide: they are the same for all columns)
+        top = column_max<PACK>(top);
+        const int e = max(st.ref, min(static_cast<int>(__float_as_uint(top) >> 23) - 127, 100));
+        const float down = e - st.ref > 120 ? 0.0f : power2(st.ref - e);
+        st.ref = e;
+        st.twice_ref = power2(e + 1);
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const float next = fmaxf(st.m[t], column_max<PACK>(mx[t]));
+            const float f = __builtin_amdgcn_exp2f(st.m[t] - next) * down;
             st.m[t] = next;
             st.l[t] *= f;
             st.r[t] *= f;
@@ -394,25 +496,29 @@ __device__ __forceinline__ void weigh(Block<D, BSM> &b, const Column<D> (&col)[C
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= f;
         }
+    }
+    u32x4 pw[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
         const float shift = kTop - st.m[t] - static_cast<float>(st.ref);
-        float w[2][4];
+        uint32_t w[V / 2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[t][h][i], col[t].to_log2, shift));
-                st.l[t] += e;
-                st.r[t] = fmaf(e, av[h][i], st.r[t]);
-                w[h][i] = e * sv[h][i];
-            }
-        pw[t] = u32x4{Mma<f16>::pack2(w[0][0], w[0][1]), Mma<f16>::pack2(w[0][2], w[0][3]),
-                      Mma<f16>::pack2(w[1][0], w[1][1]), Mma<f16>::pack2(w[1][2], w[1][3])};
+        for (int e = 0; e < V; e += 2) {
+            const float a = __builtin_amdgcn_exp2f(fmaf(s[t][e], col[t].to_log2, shift));
+            const float b = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], col[t].to_log2, shift));
+            st.l[t] += a + b;
+            st.r[t] = fmaf(b, av[e + 1], fmaf(a, av[e], st.r[t]));
+            w[e / 2] = Mma<f16>::pack2(a * sv[e], b * sv[e + 1]);
+        }
+        // (of the copies of a column the first alone has all its weights after this)
+        if constexpr (PACK == 1) pw[t] = u32x4{w[0], w[1], w[2], w[3]};
+        else if constexpr (PACK == 2) pw[t] = u32x4{w[0], w[1], from_right<8>(w[0]), from_right<8>(w[1])};
+        else pw[t] = u32x4{w[0], from_right<4>(w[0]), from_right<8>(w[0]), from_right<12>(w[0])};
         constexpr uint32_t one = 0x3c003c00u;
         st.w[t] = mma16(u32x4{one, one, one, one}, pw[t], st.w[t]);
     }
     // values: words of 8, 4 or 2 channels of a key become, per pair of keys, words
     // of one channel each
-    using B = Block<D, BSM>;
     const auto product = [&](int tile, const u32x4 &a) {
 #pragma unroll
         for (int t = 0; t < CT; ++t) st.acc[t][tile] = mma16(a, pw[t], st.acc[t][tile]);
@@ -424,23 +530,23 @@ __device__ __forceinline__ void weigh(Block<D, BSM> &b, const Column<D> (&col)[C
         product(tile + 2, y & 0x000f000fu);
         product(tile + 3, y & 0x00f000f0u);
     };
-    const auto pairs = [&](int n, uint32_t select) {
+    const auto of_two = [&](int n, uint32_t select) {
         u32x4 x;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            x[i] = __builtin_amdgcn_perm(b.v[i >> 1][2 * (i & 1) + 1][n], b.v[i >> 1][2 * (i & 1)][n], select);
+            x[i] = __builtin_amdgcn_perm(v[i >> 1][2 * (i & 1) + 1][n], v[i >> 1][2 * (i & 1)][n], select);
         return x;
     };
 #pragma unroll
-    for (int n = 0; n < B::N128; ++n) {
-        four(8 * n, pairs(n, 0x05040100u));
-        four(8 * n + 4, pairs(n, 0x07060302u));
+    for (int n = 0; n < R::N128; ++n) {
+        four(8 * n, of_two(n, 0x05040100u));
+        four(8 * n + 4, of_two(n, 0x07060302u));
     }
-    if constexpr (B::N64 > 0) four(8 * B::N128, pairs(B::N128, 0x05040100u));
-    if constexpr (B::N32 > 0) {
-        const u32x4 x = pairs(B::N128 + B::N64, 0x05040100u);
-        product(8 * B::N128 + 4 * B::N64, x & 0x000f000fu);
-        product(8 * B::N128 + 4 * B::N64 + 1, x & 0x00f000f0u);
+    if constexpr (R::N64 > 0) four(8 * R::N128, of_two(R::N128, 0x05040100u));
+    if constexpr (R::N32 > 0) {
+        const u32x4 x = of_two(R::N128 + R::N64, 0x05040100u);
+        product(8 * R::N128 + 4 * R::N64, x & 0x000f000fu);
+        product(8 * R::N128 + 4 * R::N64 + 1, x & 0x00f000f0u);
     }
 }
 
@@ -453,21 +559,27 @@ __device__ __forceinline__ int channel_of(int tile, int m) {
     return 128 * N128 + 64 * N64 + 2 * m + (tile - 8 * N128 - 4 * N64);
 }
 
-template <int D, int CT>
+template <int D, int CT, bool UNIFORM>
 constexpr size_t split_lds() {
-    return sizeof(float) * kWaves * 16 * CT * (D + 2);
+    constexpr size_t states = sizeof(float) * kWaves * 16 * CT * (D + 2);
+    constexpr size_t rings = kWaves * Ring<D, UNIFORM>::DEPTH * Ring<D, UNIFORM>::BYTES + (UNIFORM ? 0 : kTable * 4);
+    return states > rings ? states : rings;
 }
 
-// Columns [c0, c0 + 16 CT) of (sequence, kv head) over the keys [lo, hi): column j
+// Columns of a workgroup.
+template <int CT, int PACK>
+constexpr int kSpan = PACK > 1 ? 16 / PACK : 16 * CT;
+
+// Columns [c0, c0 + kSpan) of (sequence, kv head) over the keys [lo, hi): column j
 // is query row j / G, head j % G of the group.  Leaves the waves' states in LDS,
 // after a barrier: maximum, sum and unnormalised output of each column.
-template <typename T, int D, int CT, int BSM>
+template <typename T, int D, int CT, int PACK, bool UNIFORM>
 __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, int kvh, long long q_off, int L, int S,
                                            int c0, int lo, int hi) {
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q_start = p.causal ? max(S - L, 0) : 0;
-    const int last = min(c0 + 16 * CT, p.G * L) - 1;
+    const int last = min(c0 + kSpan<CT, PACK>, p.G * L) - 1;
     // no column sees more than the last one
     const int limit = p.causal ? min(hi, q_start + last / p.G + 1) : hi;
     const int least = p.causal ? min(limit, q_start + c0 / p.G + 1) : limit;
@@ -475,46 +587,65 @@ __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, i
     Column<D> col[CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
-        const int j = min(c0 + 16 * t + n, last);
+        const int nc = PACK == 1 ? 16 * t + n : n & (16 / PACK - 1);
+        const int j = min(c0 + nc, last);
         const int row = j / p.G, head = j - row * p.G;
-        load_column<T, D>(p, col[t], p.q + ((q_off + row) * p.H + kvh * p.G + head) * D, c0 + 16 * t + n <= last);
+        load_column<T, D>(p, col[t], p.q + ((q_off + row) * p.H + kvh * p.G + head) * D, c0 + nc <= last);
         col[t].vis = p.causal ? q_start + row + 1 : S;
     }
     State<D, CT> st;
     st.clear();
-    // The next block's keys are asked for once this one's scores are done, its values
-    // once these are used: one set of registers each, and more waves, whose loads
-    // overlap, in place of a second set.
-    using B = Block<D, BSM>;
-    B blk;
-    typename B::Pages pages, next;
-    constexpr int STEP = 32 * kWaves;
-    int j0 = lo + 32 * wave;
-    if (j0 < limit) {
-        B::pages(pages, p, table, j0, limit);
-        blk.load_k(pages, p, kvh, j0, limit);
-        blk.load_v(pages, p, kvh, j0, limit);
-        if (j0 + STEP < limit) B::pages(next, p, table, j0 + STEP, limit);
-    }
-    for (; j0 < limit; j0 += STEP) {
-        const bool edge = j0 + 32 > least, more = j0 + STEP < limit;
-        f32x4_t s[CT][2];
-        scores<T, D, CT, BSM>(blk, col, s, j0, limit, edge);
-        pages = next;
-        if (more) {
-            blk.load_k(pages, p, kvh, j0 + STEP, limit);
-            if (j0 + 2 * STEP < limit) B::pages(next, p, table, j0 + 2 * STEP, limit);
+    using R = Ring<D, UNIFORM>;
+    constexpr int STEP = R::STEP, DEPTH = R::DEPTH;
+    char *const ring = reinterpret_cast<char *>(lds) + wave * (DEPTH * R::BYTES);
+    int *const copy = reinterpret_cast<int *>(reinterpret_cast<char *>(lds) + kWaves * DEPTH * R::BYTES);
+    if constexpr (!UNIFORM) {
+        if (lo < limit) {
+            const int b0 = block_at(p, lo), used = min(block_at(p, limit - 1) - b0 + 1, kTable);
+            for (int i = threadIdx.x; i < used; i += 64 * kWaves) copy[i] = table[b0 + i];
         }
-        weigh<T, D, CT, BSM>(blk, col, s, st, j0, limit, edge);
-        if (more) blk.load_v(pages, p, kvh, j0 + STEP, limit);
+        __syncthreads();
     }
+    const int j0 = lo + 32 * wave;
+    R asked(p, kvh, table, copy, lo, limit, j0);
+    const auto load = [&](int i) {
+        asked.load(j0 + i * STEP, ring + __builtin_amdgcn_readfirstlane((i % DEPTH) * R::BYTES));
+        asked.turn();
+    };
+    const int blocks = j0 < limit ? (limit - j0 + STEP - 1) / STEP : 0;
+    // (the queries are there before the first copy: no wait for them among the copies)
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    asm volatile("" ::: "memory");
+    if (blocks > 0) asked.turn();
+#pragma unroll
+    for (int i = 0; i < DEPTH - 1; ++i)
+        if (i < blocks) load(i);
+    for (int i = 0; i < blocks; ++i) {
+        const int j = j0 + i * STEP;
+        // the reads of the block before this one are done: its place is free
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + DEPTH - 1 < blocks) {
+            load(i + DEPTH - 1);
+            R::template wait<DEPTH - 1>();
+        } else {
+            // fewer blocks behind this one than the ring holds
+            if (DEPTH > 3 && i + 2 < blocks) R::template wait<2>();
+            else if (DEPTH > 2 && i + 1 < blocks) R::template wait<1>();
+            else R::template wait<0>();
+        }
+        const char *blk = ring + __builtin_amdgcn_readfirstlane((i % DEPTH) * R::BYTES);
+        const bool edge = j + 32 > least;
+        attend<T, D, CT, PACK>(blk, col, st, j, limit, edge);
+    }
+    __syncthreads();  // the states take the rings' place
     constexpr int COLS = 16 * CT;
     float *lm = lds, *ll = lm + kWaves * COLS, *lout = ll + kWaves * COLS;
     const float ref = power2(st.ref);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
-        const float l = row_swap_sum(half_swap_sum(st.l[t])), r = row_swap_sum(half_swap_sum(st.r[t]));
+        const float l = column_sum<PACK>(st.l[t]), r = column_sum<PACK>(st.r[t]);
         const int c = wave * COLS + 16 * t + n;
+        if (n >= 16 / PACK) continue;  // a copy
         if (g == 0) {
             lm[c] = st.m[t];
             ll[c] = l * ref;
@@ -560,7 +691,7 @@ __device__ __forceinline__ int splits_of(const Params &p, int S) {
 // key past the splits, and rows past the bound that the grid was made for are done
 // by the workgroups of split 0, over all keys, so that the bounds shape the launch
 // alone.
-template <typename T, int D, int CT, int BSM>
+template <typename T, int D, int CT, int PACK, bool UNIFORM>
 __global__ void __launch_bounds__(64 * kWaves, D * CT <= 64 && CT == 1 ? 4 : D * CT <= 128 ? 3 : D * CT <= 256 ? 2 : 1) split_kernel(Params p) {
     extern __shared__ __attribute__((aligned(16))) float states[];
     if (blockIdx.x == 0 && blockIdx.y == 0) zero_tail(p, D);
@@ -579,11 +710,12 @@ __global__ void __launch_bounds__(64 * kWaves, D * CT <= 64 && CT == 1 ? 4 : D *
                 Cvt<T>::from(sum > 0.0f ? out / sum : 0.0f * sum);
         };
     };
-    int c0 = tile * 16 * CT;
+    constexpr int SPAN = kSpan<CT, PACK>;
+    int c0 = tile * SPAN;
     if (c0 < min(all, p.cols) && split < ns) {
         const int lo = split * p.split_len, hi = split == ns - 1 ? S : lo + p.split_len;
-        const int cols = min(16 * CT, min(all, p.cols) - c0);
-        split_pass<T, D, CT, BSM>(p, states, b, kvh, q_off, L, S, c0, lo, hi);
+        const int cols = min(SPAN, min(all, p.cols) - c0);
+        split_pass<T, D, CT, PACK, UNIFORM>(p, states, b, kvh, q_off, L, S, c0, lo, hi);
         if (p.splits == 1) {
             merge_states<D, CT>(states, cols, write(c0));
         } else {
@@ -599,10 +731,10 @@ __global__ void __launch_bounds__(64 * kWaves, D * CT <= 64 && CT == 1 ? 4 : D *
     }
     if (split != 0) return;
     // (p.cols need not be a whole number of tiles: the rest starts at it)
-    for (c0 = p.cols + tile * 16 * CT; c0 < all; c0 += p.tiles * 16 * CT) {
+    for (c0 = p.cols + tile * SPAN; c0 < all; c0 += p.tiles * SPAN) {
         __syncthreads();
-        split_pass<T, D, CT, BSM>(p, states, b, kvh, q_off, L, S, c0, 0, S);
-        merge_states<D, CT>(states, min(16 * CT, all - c0), write(c0));
+        split_pass<T, D, CT, PACK, UNIFORM>(p, states, b, kvh, q_off, L, S, c0, 0, S);
+        merge_states<D, CT>(states, min(SPAN, all - c0), write(c0));
     }
 }
 
@@ -925,12 +1057,11 @@ tecoopsStatus_t launch_combine(const Params &p, const Plan &pl, hipStream_t s) {
     return TECOOPS_STATUS_SUCCESS;
 }
 
-template <typename T, int D, int CT>
+template <typename T, int D, int CT, int PACK>
 tecoopsStatus_t launch_split(const Params &p, const Plan &pl, hipStream_t s) {
-    const size_t lds = split_lds<D, CT>();
-    auto *kern = p.bs % 16 == 0  ? &split_kernel<T, D, CT, 1>
-                 : p.bs % 4 == 0 ? &split_kernel<T, D, CT, 2>
-                                 : &split_kernel<T, D, CT, 0>;
+    const bool uniform = p.bs % 16 == 0;
+    const size_t lds = uniform ? split_lds<D, CT, true>() : split_lds<D, CT, false>();
+    auto *kern = uniform ? &split_kernel<T, D, CT, PACK, true> : &split_kernel<T, D, CT, PACK, false>;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), lds)) return TECOOPS_STATUS_INTERNAL_ERROR;
     hipLaunchKernelGGL(kern, dim3(p.batch * p.Hkv * pl.tiles, pl.splits), dim3(64 * kWaves), lds, s, p);
     TECO_CHECK_LAUNCH("flash_attention_int4");
@@ -950,7 +1081,9 @@ tecoopsStatus_t launch_tiles(const Params &p, const Plan &pl, hipStream_t s) {
 
 template <typename T, int D>
 tecoopsStatus_t launch_size(const Params &p, const Plan &pl, hipStream_t s) {
-    if (pl.split) return pl.ct == 1 ? launch_split<T, D, 1>(p, pl, s) : launch_split<T, D, 2>(p, pl, s);
+    if (pl.split && pl.ct > 1) return launch_split<T, D, 2, 1>(p, pl, s);
+    if (pl.split && pl.cols > 8) return launch_split<T, D, 1, 1>(p, pl, s);
+    if (pl.split) return pl.cols > 4 ? launch_split<T, D, 1, 2>(p, pl, s) : launch_split<T, D, 1, 4>(p, pl, s);
     if (pl.waves == 4) return launch_tiles<T, D, 4, 32>(p, pl, s);
     if constexpr (D <= 128) return launch_tiles<T, D, 12, 96>(p, pl, s);
     else return launch_tiles<T, D, 8, 64>(p, pl, s);
@@ -1028,8 +1161,12 @@ extern "C" tecoopsStatus_t tecoopsFlashAttentionInt4(
     p.bs = block_size;
     p.lbs = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
     p.num_blocks = num_blocks;
+    p.page_rows = static_cast<long long>(num_kv_heads) * block_size;
+    const uint64_t inv = ((1ull << 32) + block_size - 1) / block_size;
+    const uint64_t off = inv * block_size - (1ull << 32);  // exact up to 2^32 / off
     // (a block of keys past the last stays within an int)
     p.kv_cap = static_cast<int>(std::min(static_cast<long long>(blocks_per_seq) * block_size, 0x7fffffffll - 4096));
+    p.inv_bs = block_size > 1 && (static_cast<uint64_t>(p.kv_cap) + 8192) * off < (1ull << 32) ? static_cast<uint32_t>(inv) : 0u;
     const float scale = softmax_scale > 0.0f ? softmax_scale : 1.0f / std::sqrt(static_cast<float>(head_size));
     p.scale_log2 = scale * 1.4426950408889634f;
     p.causal = causal != 0;
