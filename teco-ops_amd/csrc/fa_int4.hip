@@ -152,7 +152,7 @@ struct Ring {
     static constexpr int NI = (D + 63) / 64;        // copies of the keys, and of the values
     static constexpr int PER = 2 * NI + 1;          // copies of a block
     static constexpr int V_AT = NI * 1024, P_AT = 2 * NI * 1024, BYTES = P_AT + 256;
-    static constexpr int DEPTH = D <= 64 ? 4 : 2;
+    static constexpr int DEPTH = D <= 64 ? 4 : 3;
     static constexpr int STEP = 32 * kWaves;        // keys from a wave's block to its next
     static constexpr bool SCALAR = UNIFORM && D == 128;
     static_assert((DEPTH - 1) * PER < 64, "vmcnt");

@@ -124,3 +124,26 @@ def _zeroed(want, slots, bs):
     used[slots] = True
     used = used.view(-1, 1, bs, 1)
     return [torch.where(used, t, torch.zeros_like(t)) for t in want]
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("low", [0.0, -7.0])
+def test_values_at_the_middle_of_two_codes(dt, low):
+    """Middles of codes and their neighbours, at scales from the smallest on: the
+    codes are those of the quotients, ties to even."""
+    T, D, bs, NB = 96, 128, 16, 8
+    dtype = DTYPES[dt]
+    tiny, huge = (-24, 11) if dt == "f16" else (-133, 123)
+    unit = torch.logspace(0, 1, T, base=2, dtype=torch.float64).mul(
+        torch.pow(2.0, torch.linspace(tiny, huge, T, dtype=torch.float64).floor())).to(dtype).double()
+    middle = torch.cat([torch.arange(0, 15) + 0.5, torch.arange(0, 16)]).double()
+    x = (unit[:, None] * (middle + low)[None]).to(dtype)  # [T, 31]
+    bits = x.view(torch.int16)
+    row = torch.cat([x, (bits + 1).view(dtype), (bits - (bits & 0x7fff).clamp(max=1)).view(dtype), x], 1)
+    row = torch.where(torch.isfinite(row), row, torch.zeros_like(row))
+    key = torch.cat([row, row[:, :4]], 1).view(T, 1, D)
+    value = key.flip(0).contiguous()
+    slots = slots_of(T, NB, bs)
+    got = run(key, value, slots, NB, bs)
+    same((got[0], got[2]), expected(key, slots, NB, bs))
+    same((got[1], got[3]), expected(value, slots, NB, bs))
