@@ -21,7 +21,10 @@ struct Plan {
 
 constexpr int kWaves = 4;                 // of a workgroup of the split route
 constexpr int kLeastSplit = 32 * kWaves;  // keys: a block of 32 for each wave
-constexpr int kSplitCols = 64;            // columns that the split route serves
+// Columns that the split route serves: both routes take as long at some 90 of them (split
+// / tile route, us, 16 sequences of 4096 keys, 8 kv heads of 128: 32 columns 35.1 / 49.6,
+// 64 47.0 / 56.2, 96 67.7 / 65.1, 128 84.1 / 71.9).
+constexpr int kSplitCols = 64;
 
 inline size_t state_bytes(int batch, int kv_heads, int splits, int cols, int head_size) {
     return splits <= 1 ? 0
@@ -41,20 +44,26 @@ inline Plan make_plan(int batch, int heads, int kv_heads, int head_size, int row
     if (p.split) {
         p.ct = cols <= 16 ? 1 : 2;
         p.tiles = static_cast<int>((cols + 16 * p.ct - 1) / (16 * p.ct));
-        // as long as the grid has four workgroups a CU, else down to one block a wave
+        // 2048 keys, or as much shorter as gives each CU a workgroup, down to one block a
+        // wave.  What a workgroup costs besides its keys, and the splits' states, are
+        // more than a fuller chip gains (one workgroup a CU / four, us: a sequence of
+        // 16384 keys 12.5 / 23.6, 8 of 2048 9.9 / 14.3, 64 of 1000 18.1 / 23.8, 16 of
+        // 4096 22.6 / 23.9; heads 32 on 8 of 128)
         const long long units = static_cast<long long>(batch) * kv_heads * p.tiles;
         len = 2048;
-        while (len > kLeastSplit && units * splits(len) < 4ll * cus) len /= 2;
+        while (len > kLeastSplit && units * splits(len) < cus) len /= 2;
     } else {
         const int wide = head_size <= 128 ? 12 : 8;
         p.waves = cols <= 128 ? 4 : wide;
         const long long tile = 32 * p.waves;
         p.tiles = static_cast<int>((cols + tile - 1) / tile);
-        // where the tiles leave workgroup slots empty, as many splits as fill them,
-        // of 512 keys or more
+        // where the tiles leave workgroup slots empty, as many splits as fill them, of
+        // two tiles of 96 keys or more (least 512 / 192 / 96 keys, us: one sequence of
+        // 1000 keys, 96 columns 45.1 / 19.8 / 16.6, of 4096 31.9 / 22.2 / 19.7, 256
+        // columns 34.0 / 26.5 / 26.9; 4 of 2048, 96 columns 32.3 / 23.0 / 24.0)
         const long long units = static_cast<long long>(batch) * kv_heads * p.tiles;
         const long long slots = static_cast<long long>(cus) * (p.waves == 4 ? 3 : 1);
-        const long long want = std::min(slots / std::max(units, 1ll), static_cast<long long>(keys) / 512);
+        const long long want = std::min(slots / std::max(units, 1ll), static_cast<long long>(keys) / 192);
         len = want > 1 ? ((keys + want - 1) / want + 95) / 96 * 96 : std::max(keys, 1);
     }
     while (splits(len) > 1 && state_bytes(batch, kv_heads, static_cast<int>(splits(len)), p.cols, head_size) > room)

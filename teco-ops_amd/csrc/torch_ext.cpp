@@ -427,15 +427,17 @@ struct AxesArgs {
     int max_position;
 
     AxesArgs(const Tensor &positions, const Tensor &query, const Tensor *key, int64_t head_size,
-             at::IntArrayRef sec, const Tensor *cos_sin_cache, int64_t rot, c10::string_view lay) {
+             at::IntArrayRef sec, const Tensor *cos_sin_cache, int64_t rot, c10::string_view lay, bool flat = false) {
         need_cuda({&positions, &query, key, cos_sin_cache});
         same_device(query, {&positions, key, cos_sin_cache});
         need_dtype(positions, at::kLong, "positions");
         TORCH_CHECK(head_size > 0, "tecoops: head_size must be positive");
-        TORCH_CHECK(positions.dim() == 2 && positions.size(0) == static_cast<int64_t>(sec.size()) &&
-                        (positions.size(1) <= 1 || positions.stride(1) == 1),
+        // (flat: one axis may come as [tokens])
+        const bool one = flat && positions.dim() == 1 && sec.size() == 1;
+        TORCH_CHECK((one || (positions.dim() == 2 && positions.size(0) == static_cast<int64_t>(sec.size()))) &&
+                        (positions.size(-1) <= 1 || positions.stride(-1) == 1),
                     "tecoops: positions must be [axes, tokens] with adjacent tokens, one axis per section");
-        tokens = fits_int(positions.size(1), "tokens");
+        tokens = fits_int(positions.size(-1), "tokens");
         position_stride = sec.size() > 1 ? positions.stride(0) : tokens;
         for (int64_t s : sec) sections.push_back(static_cast<int>(std::min<int64_t>(std::max<int64_t>(s, -1), 1 << 20)));
         heads = rows(query, query, head_size, "query", &query_stride);
@@ -528,15 +530,15 @@ void rotary_axes_reshape_and_cache(const Tensor &positions, Tensor &query, Tenso
 // The positions and sections of a call in one or several axes: [tokens] and no
 // sections is one axis that all frequencies turn by.
 struct Axes {
-    Tensor positions;
-    std::vector<int64_t> sections;
+    int64_t whole;  // the one section where none are given
+    at::IntArrayRef sections;
 
-    Axes(const Tensor &p, at::IntArrayRef sec, const Tensor *cos_sin_cache, int64_t head_size, int64_t rot)
-        : positions(p.dim() == 1 ? p.unsqueeze(0) : p), sections(sec.vec()) {
-        if (!sections.empty()) return;
+    Axes(at::IntArrayRef sec, const Tensor *cos_sin_cache, int64_t head_size, int64_t rot) : sections(sec) {
         if (cos_sin_cache && cos_sin_cache->dim() == 2) rot = cos_sin_cache->size(1);
-        sections.push_back((rot > 0 ? rot : head_size) / 2);
+        whole = (rot > 0 ? rot : head_size) / 2;
+        if (sections.empty()) sections = at::IntArrayRef(&whole, 1);
     }
+    Axes(const Axes &) = delete;
 };
 
 void need_weight(const Tensor *w, const Tensor &query, int64_t head_size, const char *name) {
@@ -552,14 +554,14 @@ void qk_norm_rotary(const Tensor &positions, Tensor &query, const c10::optional<
     const Tensor *k = given(key), *table = given(cos_sin_cache), *kw = given(key_weight);
     need_cuda({&positions, &query, k, &query_weight, kw});
     same_device(query, {&query_weight, kw});
-    const Axes ax(positions, sections, table, head_size, rot_dim);
-    const AxesArgs a(ax.positions, query, k, head_size, ax.sections, table, rot_dim, layout);
+    const Axes ax(sections, table, head_size, rot_dim);
+    const AxesArgs a(positions, query, k, head_size, ax.sections, table, rot_dim, layout, true);
     need_weight(&query_weight, query, head_size, "query_weight");
     if (k) need_weight(kw, query, head_size, "key_weight");
     if (a.tokens == 0) return;
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(query.device());
     check(tecoopsQkNormRotary(
-              handle_for(query), ax.positions.data_ptr<int64_t>(), a.position_stride,
+              handle_for(query), positions.data_ptr<int64_t>(), a.position_stride,
               static_cast<int>(a.sections.size()), a.sections.data(), a.layout, query.data_ptr(),
               k ? k->data_ptr() : nullptr, query_weight.data_ptr(), k ? kw->data_ptr() : nullptr,
               static_cast<float>(eps), a.tokens, a.heads, a.kv_heads, fits_int(head_size, "head_size"), a.rot_dim,
@@ -577,8 +579,8 @@ void qk_norm_rotary_reshape_and_cache(const Tensor &positions, Tensor &query, Te
     const Tensor *table = given(cos_sin_cache);
     need_cuda({&positions, &query, &key, &value, &query_weight, &key_weight, &slot_mapping, &key_cache, &value_cache});
     same_device(query, {&query_weight, &key_weight, &value, &slot_mapping, &key_cache, &value_cache});
-    const Axes ax(positions, sections, table, head_size, rot_dim);
-    const AxesArgs a(ax.positions, query, &key, head_size, ax.sections, table, rot_dim, layout);
+    const Axes ax(sections, table, head_size, rot_dim);
+    const AxesArgs a(positions, query, &key, head_size, ax.sections, table, rot_dim, layout, true);
     need_weight(&query_weight, query, head_size, "query_weight");
     need_weight(&key_weight, query, head_size, "key_weight");
     need_contiguous({&slot_mapping, &key_cache, &value_cache});
@@ -595,7 +597,7 @@ void qk_norm_rotary_reshape_and_cache(const Tensor &positions, Tensor &query, Te
     if (a.tokens == 0) return;
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(query.device());
     check(tecoopsQkNormRotaryReshapeAndCache(
-              handle_for(query), ax.positions.data_ptr<int64_t>(), a.position_stride,
+              handle_for(query), positions.data_ptr<int64_t>(), a.position_stride,
               static_cast<int>(a.sections.size()), a.sections.data(), a.layout, query.data_ptr(), key.data_ptr(),
               value.data_ptr(), query_weight.data_ptr(), key_weight.data_ptr(), static_cast<float>(eps),
               slot_mapping.data_ptr<int64_t>(), key_cache.data_ptr(), value_cache.data_ptr(), a.tokens, a.heads,
