@@ -508,7 +508,8 @@ tecoopsStatus_t tecoopsQkNormRotaryReshapeAndCache(
  * 2], element 2j in the low half of byte j; key_scales / value_scales dataType
  * [num_blocks, num_kv_heads, block_size, 2].  Slots < 0 or past the cache are not
  * stored; a slot is at most once in a call.  head_size a multiple of 8 up to 512;
- * fewer than 2^26 (token, head) rows; num_tokens = 0 is done without a launch. */
+ * fewer than 2^26 (token, head) rows; strides and num_kv_heads * block_size below 2^32;
+ * num_tokens = 0 is done without a launch. */
 tecoopsStatus_t tecoopsReshapeAndCacheInt4(tecoopsHandle_t handle, const void *key,
                                            const void *value, const int64_t *slot_mapping,
                                            void *key_cache, void *value_cache, void *key_scales,

@@ -21,16 +21,29 @@
 // so that bf16's range is kept and small weights of long contexts lose nothing.
 //   * Scores are computed transposed (keys x columns, 16x16x32), so that a lane
 //     holds 8 keys of one column, which are the operand of the second product as
-//     they are: neither P nor the codes go through LDS.
+//     they are: neither P nor the codes go through LDS.  With at most 8 or 4 columns
+//     the 16 of the matrix core hold each 2 or 4 times, and a lane takes 4 or 2 of the
+//     8 keys through the softmax.
 //   * A wave takes every 4th block of 32 keys, copied into a ring in LDS without
 //     registers while it works on the blocks before.  Partial states meet in LDS,
 //     those of splits in a second kernel.
+//   * [64 sequences of 512 to 8192 keys, 32 heads on 8 of 128, bf16] 72 us, 60 of them this
+//     kernel at 4.8 TB/s (287 MB; a large read alone 5.9) and 5 the second one.  Issue:
+//     per block some 150 vector, 120 scalar and 17 matrix instructions.  Loads through
+//     registers and all 8 keys in each lane took 84; rings of 2 / 3 blocks 72.7 / 71.6;
+//     splits of 4096 / 2048 / 1024 / 512 keys 73.7 / 71.5 / 75.1 / 87.5.
 //
 // Tile route (prefill).  K and V tiles are widened to fp16 once per workgroup, on
 // the way into LDS, and attended as in flash_attention.hip (fa_device.h).  fp16
 // for bf16 models too, 8 times closer than bf16 and a fixed range: rows of the
 // cache are first taken as they are, and a tile in which one is too large or all
-// are too small is done again with a power of two that fits.
+// are too small is done again with a power of two that fits.  Rounded are K, V and the
+// weights, each to 2^-12: unseen beside a bf16 output, in fp16 models 4e-4 to 6e-4 (rms)
+// with the output's own 2.1e-4; second terms of K as those of the split route's weights
+// would be half as many products again.  Matrix cores are busy 37 % of the cycles,
+// vector units 41 %, at the 12 waves a CU that LDS leaves room for: issue and waits in
+// between.  [4 sequences, 2048 rows on up to 4096 keys, 32 heads on 8 of 128] 419 us, 770
+// TFLOP/s of visible pairs; [2 of up to 203 rows on 16300 keys, 40 heads] 150 us, 720.
 #include <cmath>
 
 #include "fa_device.h"
@@ -497,31 +510,43 @@ __device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[C
             for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= f;
         }
     }
-    u32x4 pw[CT];
+    // the weights in fp16, in fp16 models as sums of two terms: one term's rounding,
+    // next to that of such an output, is seen (2.5e-4 to 3.1e-4 against 2.1e-4, rms)
+    constexpr int TERMS = __is_same(T, f16) ? 2 : 1;
+    u32x4 pw[TERMS][CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         const float shift = kTop - st.m[t] - static_cast<float>(st.ref);
-        uint32_t w[V / 2];
+        uint32_t w[TERMS][V / 2];
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
             const float a = __builtin_amdgcn_exp2f(fmaf(s[t][e], col[t].to_log2, shift));
             const float b = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], col[t].to_log2, shift));
             st.l[t] += a + b;
             st.r[t] = fmaf(b, av[e + 1], fmaf(a, av[e], st.r[t]));
-            w[e / 2] = Mma<f16>::pack2(a * sv[e], b * sv[e + 1]);
+            const uint32_t one = Mma<f16>::pack2(a * sv[e], b * sv[e + 1]);
+            w[0][e / 2] = one;
+            if constexpr (TERMS == 2)
+                w[1][e / 2] = Mma<f16>::pack2(fmaf(a, sv[e], -lo<f16>(one)), fmaf(b, sv[e + 1], -hi<f16>(one)));
         }
-        // (of the copies of a column the first alone has all its weights after this)
-        if constexpr (PACK == 1) pw[t] = u32x4{w[0], w[1], w[2], w[3]};
-        else if constexpr (PACK == 2) pw[t] = u32x4{w[0], w[1], from_right<8>(w[0]), from_right<8>(w[1])};
-        else pw[t] = u32x4{w[0], from_right<4>(w[0]), from_right<8>(w[0]), from_right<12>(w[0])};
-        constexpr uint32_t one = 0x3c003c00u;
-        st.w[t] = mma16(u32x4{one, one, one, one}, pw[t], st.w[t]);
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) {
+            // (of the copies of a column the first alone has all its weights after this)
+            const uint32_t *x = w[k];
+            if constexpr (PACK == 1) pw[k][t] = u32x4{x[0], x[1], x[2], x[3]};
+            else if constexpr (PACK == 2) pw[k][t] = u32x4{x[0], x[1], from_right<8>(x[0]), from_right<8>(x[1])};
+            else pw[k][t] = u32x4{x[0], from_right<4>(x[0]), from_right<8>(x[0]), from_right<12>(x[0])};
+            constexpr uint32_t one = 0x3c003c00u;
+            st.w[t] = mma16(u32x4{one, one, one, one}, pw[k][t], st.w[t]);
+        }
     }
     // values: words of 8, 4 or 2 channels of a key become, per pair of keys, words
     // of one channel each
     const auto product = [&](int tile, const u32x4 &a) {
 #pragma unroll
-        for (int t = 0; t < CT; ++t) st.acc[t][tile] = mma16(a, pw[t], st.acc[t][tile]);
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) st.acc[t][tile] = mma16(a, pw[k][t], st.acc[t][tile]);
     };
     const auto four = [&](int tile, const u32x4 &x) {  // x[i]: 16 bits of two keys
         const u32x4 y = x >> 8;

@@ -13,7 +13,21 @@
 // exponent added is taken off with the zero, from the sum of the x of the 32.  x
 // is staged in LDS in the order in which masks yield the codes (0, 4, 1, 5, 2, 6,
 // 3, 7), a plane for each word of the 16 bytes, so that lanes read neighbouring
-// words.
+// words.  [4096, 4096], groups of 128: 6.1 us, 4.2 of them the kernel: the ramp of a
+// launch (8.7 MB at a large read's rate take 1.5).
+//
+// Several rows of x, or a long K or many rows of W: 16x16x32 matrix instructions over
+// 64 rows of W and 8 to 64 of x a workgroup; 8 waves, 2 of rows and 4 of K, whose sums
+// meet in LDS.  Stages of 512 of K go through registers into LDS one stage ahead, x in
+// the order of the masked codes.  Scales are applied to the fp32 sums of a group (at
+// most 128 of K), with the zero's share taken from the sums of x, which one more matrix
+// instruction with ones yields.  [28672, 4096], 16 rows, groups of 64: 23 us, 2.9 TB/s;
+// [4096, 14336], 33 rows, groups of 128: 22, 4 of them for the sum of 4 parts of K.  What
+// bounds them: a workgroup's chain of a few stages (load, barrier, LDS, products) beside a
+// ramp of some 5 us, and x through L2 once for every 64 rows of W.  Tried without a
+// gain: stages copied straight into LDS, four in a ring (19 to 27 us and 19 to 25 over
+// eight shapes of a workgroup; one row of x then 18.4 for 15.5), two stages ahead in
+// registers, two buffers in LDS.
 #include <algorithm>
 
 #include "common.h"

@@ -14,7 +14,9 @@
 // DPP steps and the other halves of the pairs of NeoX order are one exchange
 // between lanes away.  A lane keeps its chunk's place in every head that it
 // works on: its angles and weights are loaded once.  Memory-bound: the loads of
-// kBatch heads are under way before the first is used.
+// kBatch heads are under way before the first is used.  8191 tokens, 32 heads and 8 of
+// 128, bf16, with the store (201 MB): 43.1 us, 4.7 TB/s (a large copy: 4.95); a decode
+// step of 4 tokens 8, of which the kernel 4.5: the ramp of a launch.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -88,10 +90,13 @@ __global__ void __launch_bounds__(kThreads) qk_norm_kernel(AxisPositions angles,
     uint16_t *const q = a.query + t * a.q_stride + 8 * cc;
     uint16_t *const k = a.key + t * a.k_stride + 8 * cc;
     const uint16_t *const v = a.value + t * a.v_stride + 8 * cc;
+    // the head of the wave's first group: where that is past the last, the wave is done
+    const int ahead = __builtin_amdgcn_readfirstlane(first);
     uint4 x[kBatch];
     const auto load = [&](int base) {
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
+            if (base + u * step + ahead >= total) break;
             const int h = min(base + u * step + first, total - 1);
             const uint16_t *row = h < nq ? q + h * a.head_size
                                   : !CACHE || h < nk ? k + (h - nq) * a.head_size
@@ -130,6 +135,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_kernel(AxisPositions angles,
         if (base != 0) load(base);
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
+            if (base + u * step + ahead >= total) break;
             const int h = base + u * step + first;
             const bool is_q = h < nq, is_v = CACHE && h >= nk;
             float f[8], w[8];
