@@ -526,7 +526,8 @@ tecoopsStatus_t tecoopsReshapeAndCacheInt4(tecoopsHandle_t handle, const void *k
  * [batch, blocks_per_seq], rows block_table_stride apart; head_size in {32, 64,
  * 96, 128, 160, 192}.  Up to 64 (query row, head) pairs of a kv head read K and V
  * as they are held; longer queries widen them to fp16 first (one more rounding).
- * What the cache holds behind a sequence's last key is not used, whatever it is.
+ * What the cache holds behind a sequence's last key is not used, whatever it is; a key
+ * or value row of NaN makes the rows that see it NaN and no others.
  * workspace: tecoopsGetFlashAttentionInt4WorkspaceSize() bytes for the same sizes
  * and bounds, 16-byte aligned; with less the keys are cut into fewer splits.  NULL
  * uses the handle's scratch, and none on a stream under capture (unsplit: slower,

@@ -42,8 +42,10 @@
 // with the output's own 2.1e-4; second terms of K as those of the split route's weights
 // would be half as many products again.  Matrix cores are busy 37 % of the cycles,
 // vector units 41 %, at the 12 waves a CU that LDS leaves room for: issue and waits in
-// between.  [4 sequences, 2048 rows on up to 4096 keys, 32 heads on 8 of 128] 419 us, 770
-// TFLOP/s of visible pairs; [2 of up to 203 rows on 16300 keys, 40 heads] 150 us, 720.
+// between.  [4 sequences, 2048 rows on up to 4096 keys, 32 heads on 8 of 128] 426 us, 760
+// TFLOP/s of visible pairs; [2 of up to 203 rows on 16300 keys, 40 heads] 155 us, 700
+// (2 and 3 % of both for value rows of NaN, which are kept from the rows that do not see
+// them: their keys become NaN and they 0).
 #include <cmath>
 
 #include "fa_device.h"
@@ -474,14 +476,16 @@ __device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[C
     }
     float sv[V], av[V];
     float top = 0.0f;
+    bool none = false;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         sv[e] = lo<T>(vp[e]);
         av[e] = fmaf(kMiddle, sv[e], hi<T>(vp[e]));
         top = fmaxf(top, fabsf(sv[e]));
+        none = none || av[e] != av[e];
     }
     float mx[CT];
-    bool raise = !(top <= st.twice_ref);
+    bool raise = none || !(top <= st.twice_ref);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         mx[t] = s[t][0];
@@ -491,6 +495,18 @@ __device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[C
         raise = raise || !(mx[t] <= st.m[t] + kSlack);
     }
     if (__any(raise)) {
+        // a value row that is no number: its score is none either, where it is seen (so
+        // that it reaches the rows that see it), and the values 0 (and no others)
+        if (none) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (av[e] != av[e]) {
+#pragma unroll
+                    for (int t = 0; t < CT; ++t)
+                        if (s[t][e] != kNegInf) s[t][e] = av[e];
+                    sv[e] = av[e] = 0.0f;
+                }
+        }
         // scales relative to a power of two that is at least half of the largest seen
         // (wave-wide: they are the same for all columns)
         top = column_max<PACK>(top);
@@ -819,7 +835,7 @@ struct Widener {
     static constexpr int HALF = TILE * WORDS, TASKS = 2 * HALF;
     static constexpr int PER = (TASKS + NT - 1) / NT;
     u32x4 codes[PER];
-    uint32_t pair[PER];
+    uint32_t kpair[PER], vpair[PER];
     int page[PER];
     float most_k, most_v;  // largest magnitude seen
 
@@ -842,8 +858,9 @@ struct Widener {
             key = there ? key : 0;
             const long long row = row_of(p, kvh, page[i], key, block_at(p, key));
             codes[i] = *reinterpret_cast<const u32x4 *>((is_v ? p.vc : p.kc) + row * (D / 2) + 16 * word);
-            pair[i] = (is_v ? p.vs : p.ks)[row];
-            if (!there) pair[i] = 0u;
+            kpair[i] = p.ks[row];
+            vpair[i] = p.vs[row];
+            if (!there) kpair[i] = vpair[i] = 0u;
         }
     }
     // rows times down_k (keys) and down_v (values)
@@ -854,7 +871,12 @@ struct Widener {
             if (TASKS % NT != 0 && t >= TASKS) continue;
             const int task = t % HALF, word = task % WORDS, row = task / WORDS;
             const bool is_v = t >= HALF;
-            const float s = lo<T>(pair[i]), a = hi<T>(pair[i]);
+            const float vs = lo<T>(vpair[i]), va = hi<T>(vpair[i]), v15 = fmaf(15.0f, vs, va);
+            // a value row that is no number: its key is none (so that it reaches the rows
+            // that see it) and the values 0 (so that it reaches no others)
+            const bool none = v15 != v15;
+            float s = is_v ? vs : lo<T>(kpair[i]), a = is_v ? va : hi<T>(kpair[i]);
+            if (none) s = a = is_v ? 0.0f : v15;
             const float most = fmaxf(fabsf(a), fabsf(fmaf(15.0f, s, a)));
             if (is_v) most_v = fmaxf(most_v, most);
             else most_k = fmaxf(most_k, most);

@@ -150,6 +150,34 @@ def test_nan_rows_reach_their_columns_only(rows):
     assert torch.equal(torch.isnan(got.cpu()).any(-1), seen)
 
 
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("rows,G", [(1, 4), (3, 1), (3, 4), (9, 2), (14, 1), (14, 4), (70, 4)])
+def test_nan_rows_of_keys_and_values(rows, G, which):
+    """The same for keys and values, where rows share a tile of columns (held in one or
+    several copies), and for more of them."""
+    lens, D = [200, 90], 128
+    held = list(cache(lens, 2, D, 16, torch.float16))
+    held[which][held[4][0, 12], 0, 6] = math.nan  # row 198 of kv head 0
+    q = rand(2 * rows, 2 * G, D, dtype=torch.float16)
+    got, cu = run(q, held, lens, [rows, rows])
+    seen = torch.zeros(2 * rows, 2 * G, dtype=torch.bool)
+    for r in range(rows):
+        seen[r, :G] = 200 - rows + r >= 198
+    assert torch.equal(torch.isnan(got.cpu()).all(-1), seen)
+    assert torch.equal(torch.isnan(got.cpu()).any(-1), seen)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192])
+@pytest.mark.parametrize("G,rows", [(1, 1), (2, 1), (4, 1), (3, 1), (8, 1), (5, 1), (12, 1), (16, 1),
+                                    (1, 3), (2, 4), (1, 17), (4, 9)])
+@pytest.mark.parametrize("bs", [16, 48, 20])
+def test_columns_of_every_number(G, rows, bs, D, dt):
+    """Columns that are held once, twice and four times, one and two tiles of them, in
+    pages of whole halves of a block and others, at keys that end inside blocks."""
+    compare(dt, 2 * G, 2, D, bs, [37, 129 + 16 * G, 260], [rows] * 3)
+
+
 def test_long_context_of_small_weights():
     """Many keys of equal weight: none may be lost to fp16's range."""
     S, D = 40000, 64
