@@ -524,8 +524,9 @@ tecoopsStatus_t tecoopsReshapeAndCacheInt4(tecoopsHandle_t handle, const void *k
  * alone), but the softmax has no clamp at 0, so that scores of any size are
  * weighed.  q and out [total_q, num_heads, head_size] packed; block_table int32
  * [batch, blocks_per_seq], rows block_table_stride apart; head_size in {32, 64,
- * 96, 128, 160, 192}.  Up to 64 (query row, head) pairs of a kv head read K and V
- * as they are held; longer queries widen them to fp16 first (one more rounding).
+ * 96, 128, 160, 192}.  fp16, and in bf16 up to 64 (query row, head) pairs of a kv head,
+ * read K and V as they are held; longer queries in bf16 widen them to fp16 first (one
+ * more rounding, finer than the output's; fp16 prompts take up to twice as long).
  * What the cache holds behind a sequence's last key is not used, whatever it is; a key
  * or value row of NaN makes the rows that see it NaN and no others.
  * workspace: tecoopsGetFlashAttentionInt4WorkspaceSize() bytes for the same sizes

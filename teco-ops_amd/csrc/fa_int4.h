@@ -23,7 +23,9 @@ constexpr int kWaves = 4;                 // of a workgroup of the split route
 constexpr int kLeastSplit = 32 * kWaves;  // keys: a block of 32 for each wave
 // Columns that the split route serves: both routes take as long at some 90 of them (split
 // / tile route, us, 16 sequences of 4096 keys, 8 kv heads of 128: 32 columns 35.1 / 49.6,
-// 64 47.0 / 56.2, 96 67.7 / 65.1, 128 84.1 / 71.9).
+// 64 47.0 / 56.2, 96 67.7 / 65.1, 128 84.1 / 71.9).  In fp16 it serves any number: the
+// widened tiles' roundings are seen there (5e-4 against 2.1e-4, rms, of the output's own).
+// 8 sequences of 1000 keys, 400 columns 57 / 47 us, 4 of 4096, 8192 columns 875 / 459.
 constexpr int kSplitCols = 64;
 
 inline size_t state_bytes(int batch, int kv_heads, int splits, int cols, int head_size) {
@@ -32,12 +34,13 @@ inline size_t state_bytes(int batch, int kv_heads, int splits, int cols, int hea
 }
 
 // rows, keys: bounds on a sequence's query rows and keys; room: the workspace's
-// bytes; cus: compute units.
-inline Plan make_plan(int batch, int heads, int kv_heads, int head_size, int rows, int keys, size_t room, int cus) {
+// bytes; cus: compute units; exact: for any number of columns the split route.
+inline Plan make_plan(int batch, int heads, int kv_heads, int head_size, int rows, int keys, size_t room, int cus,
+                      bool exact = false) {
     Plan p{};
     const long long cols = std::min<long long>(static_cast<long long>(heads / kv_heads) * rows, 0x7fffffff);
     p.cols = static_cast<int>(cols);
-    p.split = cols <= kSplitCols;
+    p.split = exact || cols <= kSplitCols;
     p.splits = 1;
     long long len = 0;
     const auto splits = [&](long long l) { return std::max(1ll, (keys + l - 1) / l); };
@@ -50,7 +53,10 @@ inline Plan make_plan(int batch, int heads, int kv_heads, int head_size, int row
         // 16384 keys 12.5 / 23.6, 8 of 2048 9.9 / 14.3, 64 of 1000 18.1 / 23.8, 16 of
         // 4096 22.6 / 23.9; heads 32 on 8 of 128)
         const long long units = static_cast<long long>(batch) * kv_heads * p.tiles;
-        len = 2048;
+        // (many columns in two workgroups a CU or more fill the chip unsplit, and would
+        // write as many states: 2048 keys a split / none, us, fp16: 2 sequences of 16300
+        // keys, 1015 columns 318 / 248, 32 of 6000, 48 columns 127 / 105)
+        len = p.ct > 1 && units >= 2ll * cus ? (std::max(keys, 1) + 127ll) / 128 * 128 : 2048;
         while (len > kLeastSplit && units * splits(len) < cus) len /= 2;
     } else {
         const int wide = head_size <= 128 ? 12 : 8;

@@ -33,19 +33,18 @@
 //     registers and all 8 keys in each lane took 84; rings of 2 / 3 blocks 72.7 / 71.6;
 //     splits of 4096 / 2048 / 1024 / 512 keys 73.7 / 71.5 / 75.1 / 87.5.
 //
-// Tile route (prefill).  K and V tiles are widened to fp16 once per workgroup, on
-// the way into LDS, and attended as in flash_attention.hip (fa_device.h).  fp16
-// for bf16 models too, 8 times closer than bf16 and a fixed range: rows of the
-// cache are first taken as they are, and a tile in which one is too large or all
-// are too small is done again with a power of two that fits.  Rounded are K, V and the
-// weights, each to 2^-12: unseen beside a bf16 output, in fp16 models 4e-4 to 6e-4 (rms)
-// with the output's own 2.1e-4; second terms of K as those of the split route's weights
-// would be half as many products again.  Matrix cores are busy 37 % of the cycles,
-// vector units 41 %, at the 12 waves a CU that LDS leaves room for: issue and waits in
-// between.  [4 sequences, 2048 rows on up to 4096 keys, 32 heads on 8 of 128] 426 us, 760
-// TFLOP/s of visible pairs; [2 of up to 203 rows on 16300 keys, 40 heads] 155 us, 700
-// (2 and 3 % of both for value rows of NaN, which are kept from the rows that do not see
-// them: their keys become NaN and they 0).
+// Tile route (prefill in bf16).  K and V tiles are widened to fp16 once per workgroup, on
+// the way into LDS, and attended as in flash_attention.hip (fa_device.h).  fp16 is 8 times
+// closer than bf16 and a fixed range: rows of the cache are first taken as they are, and a
+// tile in which one is too large or all are too small is done again with a power of two
+// that fits.  Rounded are K, V and the weights, each to 2^-12, which is unseen beside a
+// bf16 output.  Beside an fp16 one it is seen (4e-4 to 6e-4, rms, against 2.1e-4), so
+// that fp16 models have the split route for any number of columns, at up to twice the
+// time.  Matrix cores are busy 37 % of the cycles, vector units 41 %, at the 12 waves a CU
+// that LDS leaves room for: issue and waits in between.  [4 sequences, 2048 rows on up to
+// 4096 keys, 32 heads on 8 of 128] 426 to 436 us, 750 TFLOP/s of visible pairs; [2 of up to
+// 203 rows on 16300 keys, 40 heads] 155 us, 700 (2 and 3 % of both for value rows of NaN,
+// which are kept from the rows that do not see them: their keys become NaN and they 0).
 #include <cmath>
 
 #include "fa_device.h"
@@ -736,7 +735,7 @@ template <typename T, int D, int CT, int PACK, bool UNIFORM>
 __global__ void __launch_bounds__(64 * kWaves, D * CT <= 64 && CT == 1 ? 4 : D * CT <= 128 ? 3 : D * CT <= 256 ? 2 : 1) split_kernel(Params p) {
     extern __shared__ __attribute__((aligned(16))) float states[];
     if (blockIdx.x == 0 && blockIdx.y == 0) zero_tail(p, D);
-    const int tile = blockIdx.x % p.tiles;
+    const int tile = p.tiles - 1 - blockIdx.x % p.tiles;  // (the heaviest first)
     const int kvh = blockIdx.x / p.tiles % p.Hkv;
     const int b = blockIdx.x / p.tiles / p.Hkv;
     const int split = blockIdx.y;
@@ -1131,8 +1130,9 @@ tecoopsStatus_t launch_size(const Params &p, const Plan &pl, hipStream_t s) {
     if (pl.split && pl.ct > 1) return launch_split<T, D, 2, 1>(p, pl, s);
     if (pl.split && pl.cols > 8) return launch_split<T, D, 1, 1>(p, pl, s);
     if (pl.split) return pl.cols > 4 ? launch_split<T, D, 1, 2>(p, pl, s) : launch_split<T, D, 1, 4>(p, pl, s);
-    if (pl.waves == 4) return launch_tiles<T, D, 4, 32>(p, pl, s);
-    if constexpr (D <= 128) return launch_tiles<T, D, 12, 96>(p, pl, s);
+    if constexpr (__is_same(T, f16)) return TECOOPS_STATUS_INTERNAL_ERROR;  // (make_plan's exact)
+    else if (pl.waves == 4) return launch_tiles<T, D, 4, 32>(p, pl, s);
+    else if constexpr (D <= 128) return launch_tiles<T, D, 12, 96>(p, pl, s);
     else return launch_tiles<T, D, 8, 64>(p, pl, s);
 }
 
@@ -1161,9 +1161,11 @@ extern "C" tecoopsStatus_t tecoopsGetFlashAttentionInt4WorkspaceSize(int batch, 
         return TECOOPS_STATUS_BAD_PARAM;
     if (!head_size_ok(head_size)) return TECOOPS_STATUS_NOT_SUPPORTED;
     const int rows = std::max(max_seqlen_q, static_cast<int>(tecoops::ceil_div(std::max(total_q, 1), batch)));
-    *bytes = tecoops::fa4::make_plan(batch, num_heads, num_kv_heads, head_size, rows, max_seqlen_k, ~size_t{0},
-                                     tecoops::device_cus())
-                 .bytes;
+    *bytes = 0;
+    for (const bool exact : {false, true})  // (of either type)
+        *bytes = std::max(*bytes, tecoops::fa4::make_plan(batch, num_heads, num_kv_heads, head_size, rows, max_seqlen_k,
+                                                          ~size_t{0}, tecoops::device_cus(), exact)
+                                      .bytes);
     return TECOOPS_STATUS_SUCCESS;
 }
 
@@ -1224,7 +1226,8 @@ extern "C" tecoopsStatus_t tecoopsFlashAttentionInt4(
                    "flash_attention_int4: too many query rows");
     const int cus = tecoops::device_cus();
     const auto plan = [&](size_t room) {
-        return tecoops::fa4::make_plan(batch, num_heads, num_kv_heads, head_size, rows, keys, room, cus);
+        return tecoops::fa4::make_plan(batch, num_heads, num_kv_heads, head_size, rows, keys, room, cus,
+                                       dataType == TECOOPS_DATA_HALF);
     };
     Plan pl = plan(workspace != nullptr ? workspace_bytes : ~size_t{0});
     if (pl.bytes > 0 && workspace == nullptr) {
