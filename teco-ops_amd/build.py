@@ -143,12 +143,11 @@ def _vector_registers(text):
 def check_matrix_waits(asm_text, src=""):
     """Checks that on every path of each kernel enough wait states lie between a
     v_mfma and the first vector or memory instruction that reads its result or
-    overwrites it (for a product of P passes P + 4, of 2 passes 5;
-    those of 4 x 4 results have 2 passes, of 16 x 16 at most 4 here, of 32 x 32 8, or
-    16 with a depth of 8 or less).  The
-    hardware does not wait by itself, and the compiler has left the wait out where a
-    branch lay between the two.  Returns the number of products; raises
-    RuntimeError on a violation."""
+    overwrites it: for a product of P passes P + 4, of 2 passes 5 (those of 4 x 4
+    results have 2 passes, of 16 x 16 at most 4 here, of 32 x 32 8, or 16 with a
+    depth of 8 or less).  The hardware does not wait by itself, and the compiler
+    has left the wait out where a branch lay between the two.  Returns the number
+    of products; raises RuntimeError on a violation."""
     import re
     count = 0
     for k in re.finditer(r"^(_Z\S*):", asm_text, re.M):

@@ -17,10 +17,9 @@
 // largest are a few DPP steps; each lane has one chunk of a key and one of its value,
 // both loaded before the first is used.  2.5 bytes of memory an element and 4 a row,
 // and some 20 vector instructions an element (least and largest as integers, two at a
-// time):
-// many short waves hide one under the other.  8192 tokens, 8 heads of 128, fp16 (42 MB):
-// 12.9 us, 3.3 TB/s; with 2, 3 and 4 rows a lane 13.8, 15.4 and 15.2, and with a division
-// for each code 16.5 (2 rows).
+// time): many short waves hide one under the other.  8192 tokens, 8 heads of 128, fp16
+// (42 MB): 12.9 us, 3.3 TB/s; with 2, 3 and 4 rows a lane 13.8, 15.4 and 15.2, and with a
+// division for each code 16.5 (2 rows).
 #include "common.h"
 #include "device.h"
 #include "epilogue.h"
