@@ -53,10 +53,15 @@ inline Plan make_plan(int batch, int heads, int kv_heads, int head_size, int row
         // 16384 keys 12.5 / 23.6, 8 of 2048 9.9 / 14.3, 64 of 1000 18.1 / 23.8, 16 of
         // 4096 22.6 / 23.9; heads 32 on 8 of 128)
         const long long units = static_cast<long long>(batch) * kv_heads * p.tiles;
-        // (many columns in two workgroups a CU or more fill the chip unsplit, and would
-        // write as many states: 2048 keys a split / none, us, fp16: 2 sequences of 16300
-        // keys, 1015 columns 318 / 248, 32 of 6000, 48 columns 127 / 105)
-        len = p.ct > 1 && units >= 2ll * cus ? (std::max(keys, 1) + 127ll) / 128 * 128 : 2048;
+        // (two tiles of 16 columns write more states: no splits where there are two
+        // workgroups a CU or more, else no more than make four of them.  2048 keys a split /
+        // none, us, fp16: 2 sequences of 16300 keys, 1015 columns 318 / 248, 32 of 6000, 48
+        // columns 127 / 105)
+        len = 2048;
+        if (p.ct > 1) {
+            const long long most = units >= 2ll * cus ? 1 : 4ll * cus / units, each = (keys + most - 1) / most;
+            len = std::max(len, (each + 127) / 128 * 128);
+        }
         while (len > kLeastSplit && units * splits(len) < cus) len /= 2;
     } else {
         const int wide = head_size <= 128 ? 12 : 8;
