@@ -29,6 +29,7 @@
 // eight shapes of a workgroup; one row of x then 18.4 for 15.5), two stages ahead in
 // registers, two buffers in LDS.
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 #include "device.h"
@@ -79,6 +80,49 @@ struct Args {
 __device__ __forceinline__ u32x4 interleaved(const u32x4 &v) {
     return u32x4{__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
                  __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
+}
+
+// For sums that are no finite number: an infinite x, or one whose multiple by 128 + n
+// passes fp32's range, makes the difference of two sums NaN where the sum of the
+// products is infinite or finite.  Then elements [k0, k1) (whole runs of 32) of output
+// (n, b) are summed by the whole wave, each weight on its own, but for rows of x with a
+// NaN there, whose outputs are NaN.  ([28672, 4096], 16 rows of x, the same call again and
+// again: 20.4 us, one row with a NaN 24, all of them 86.  Looking for such sums costs
+// [4096, 14336], 33 rows 0.7 us, [28672, 4096], 16 rows 0.1.)
+template <typename T>
+__device__ __forceinline__ bool holds_nan(const Args &a, int b, int k0, int k1) {
+    constexpr uint32_t kInf = __is_same(T, f16) ? 0x7c00u : 0x7f80u;
+    bool nan = false;
+#pragma unroll 1
+    for (int q = k0 / 8 + static_cast<int>(threadIdx.x & 63); q < k1 / 8; q += 64) {
+        const u32x4 v = *reinterpret_cast<const u32x4_a2 *>(a.x + static_cast<long long>(b) * a.k + 8ll * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nan = nan || (v[e] & 0x7fffu) > kInf || (v[e] >> 16 & 0x7fffu) > kInf;
+    }
+    return __any(nan);
+}
+
+template <typename T>
+__device__ __forceinline__ float direct_sum(const Args &a, int n, int b, int k0, int k1) {
+    const long long row = n;
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int q = k0 / 32 + static_cast<int>(threadIdx.x & 63); q < k1 / 32; q += 64) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(a.w + row * (a.k / 2) + 16ll * q);
+        const uint16_t *x = a.x + static_cast<long long>(b) * a.k + 32ll * q;
+        const long long at = row * a.groups + 32 * q / a.group;
+        const float s = Cvt<T>::to(a.scales[at]), z = a.zeros != nullptr ? Cvt<T>::to(a.zeros[at]) : 8.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const u32x4 v = *reinterpret_cast<const u32x4_a2 *>(x + 8 * j);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float code = static_cast<float>((w[j] >> (4 * e)) & 15u);
+                sum = fmaf((code - z) * s, e & 1 ? hi<T>(v[e >> 1]) : lo<T>(v[e >> 1]), sum);
+            }
+        }
+    }
+    return wave_sum(sum);
 }
 
 // Bytes of a staged panel: x, and the sums of its runs of 32.
@@ -146,7 +190,9 @@ __global__ void __launch_bounds__(kThreads) dot_kernel(Args a) {
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-        const float v = wave_sum(acc[r]);
+        float v = wave_sum(acc[r]);
+        if (n0 + r < a.n && !(fabsf(v) < INFINITY))
+            v = holds_nan<T>(a, 0, 0, a.k) ? NAN : direct_sum<T>(a, n0 + r, 0, 0, a.k);
         if (lane == 0 && n0 + r < a.n) a.y[n0 + r] = Cvt<T>::from(v);
     }
 }
@@ -356,8 +402,24 @@ __global__ void __launch_bounds__(64 * RS * KS) mma_kernel(Args a) {
             }
         }
     }
-    const auto put = [&](int tile, int t, const float4_t &s) {  // 16 rows and columns
+    const auto put = [&](int tile, int t, float4_t s) {  // 16 rows and columns, a whole wave
         const int n = n0 + tile * 16 + 4 * g, col = 16 * t + c;
+        const auto finite = [](float v) { return fabsf(v) < INFINITY; };
+        const bool whole = finite(s[0]) && finite(s[1]) && finite(s[2]) && finite(s[3]);
+#pragma unroll 1
+        for (uint64_t left = __ballot(!whole && col < nb && n < a.n); left != 0;) {
+            const int at = __builtin_ctzll(left) & 15;  // a column of these
+            left &= ~(0x0001000100010001ull << at);
+            const int k0 = st0 * kStage, k1 = min(st1 * kStage, a.k);
+            const bool nan = holds_nan<T>(a, b0 + 16 * t + at, k0, k1);
+#pragma unroll 1
+            for (int r = 0; r < 16 && n0 + tile * 16 + r < a.n; ++r) {
+                const float sum = nan ? NAN : direct_sum<T>(a, n0 + tile * 16 + r, b0 + 16 * t + at, k0, k1);
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    if (4 * g + v == r && c == at && !finite(s[v])) s[v] = sum;
+            }
+        }
         if (col >= nb || n >= a.n) return;
         const long long at = static_cast<long long>(b0 + col) * a.n + n;
         if (a.parts != nullptr) {
