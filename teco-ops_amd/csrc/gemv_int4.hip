@@ -71,7 +71,7 @@ struct Args {
     int pairs;   // four outputs of a row in one 8-byte word
     int groups;  // of a row
     int slots_a_group = 0;   // uses of a group's scales
-    float inv_slots = 0.0f;  // 1 / that
+    uint32_t inv_slots = 0;  // for gemv_int4_quotient by that
     int split = 0;           // stages of a part of K
     float *parts = nullptr;  // [parts of K][batch][n] sums, null: one part
 };
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(64 * RS * KS) mma_kernel(Args a) {
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rs = wave % RS, kp = wave / RS;
     const int n0 = blockIdx.x * R, b0 = blockIdx.z * XR, nb = min(XR, a.batch - b0);
-    const int st0 = blockIdx.y * a.split, st1 = min(st0 + a.split, (a.k + kStage - 1) / kStage);
+    const int st0 = blockIdx.y * a.split, st1 = min(st0 + a.split, tecoops::gemv_int4_stages(a.k));
 
     // this thread's words of the first stage: of W row / step, of x row / 8
     // elements, of the scales row, and its slot
@@ -282,18 +282,18 @@ __global__ void __launch_bounds__(64 * RS * KS) mma_kernel(Args a) {
     uint16_t sc[S::ST], ze[S::ST];
     const auto load = [&](int st) {
         const int k0 = st * kStage;
-        const bool whole = k0 + kStage <= a.k;  // words past K: the last ones instead
+        const bool whole = a.k - k0 >= kStage;  // words past K: the last ones instead
 #pragma unroll
         for (int i = 0; i < S::XT; ++i) {
             const uint16_t *src = xp[i] + k0;
-            if (!whole) src -= max(0, k0 + (tid + i * NT) % (kStage / 8) * 8 + 8 - a.k);
+            if (!whole) src -= tecoops::gemv_int4_past(k0 + (tid + i * NT) % (kStage / 8) * 8, 8, a.k);
             x[i] = *reinterpret_cast<const u32x4_a2 *>(src);
         }
 #pragma unroll
         for (int i = 0; i < S::ST; ++i) {
             // the group that the slot's first element is in (those past K are not used)
             const int slot = st * S::SLOTS + min((tid + i * NT) / R, S::SLOTS - 1);
-            const int gi = a.slots_a_group == 1 ? slot : static_cast<int>((slot + 0.5f) * a.inv_slots);
+            const int gi = tecoops::gemv_int4_quotient(slot, a.slots_a_group, a.inv_slots);
             const long long at = sp[i] + min(gi, a.groups - 1);
             sc[i] = a.scales[at];
             if (a.zeros != nullptr) ze[i] = a.zeros[at];
@@ -301,12 +301,12 @@ __global__ void __launch_bounds__(64 * RS * KS) mma_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < S::WT; ++i) {
             const uint8_t *src = wp[i] + k0 / 2;
-            if (!whole) src -= max(0, k0 / 2 + (tid + i * NT) % kSteps * 16 + 16 - a.k / 2);
+            if (!whole) src -= tecoops::gemv_int4_past(k0 / 2 + (tid + i * NT) % kSteps * 16, 16, a.k / 2);
             w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src));
         }
     };
     const auto store = [&](int st) {
-        const bool tail = (st + 1) * kStage > a.k;  // past K, x is 0
+        const bool tail = a.k - st * kStage < kStage;  // past K, x is 0
 #pragma unroll
         for (int i = 0; i < S::XT; ++i) {
             const int t = tid + i * NT, row = t / (kStage / 8), q = t % (kStage / 8);
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(64 * RS * KS) mma_kernel(Args a) {
         for (uint64_t left = __ballot(!whole && col < nb && n < a.n); left != 0;) {
             const int at = __builtin_ctzll(left) & 15;  // a column of these
             left &= ~(0x0001000100010001ull << at);
-            const int k0 = st0 * kStage, k1 = min(st1 * kStage, a.k);
+            const int k0 = st0 * kStage, k1 = min(static_cast<long long>(st1) * kStage, static_cast<long long>(a.k));
             const bool nan = holds_nan<T>(a, b0 + 16 * t + at, k0, k1);
 #pragma unroll 1
             for (int r = 0; r < 16 && n0 + tile * 16 + r < a.n; ++r) {
@@ -476,8 +476,8 @@ bool launch_mma(Args a, int splits, hipStream_t s) {
     auto *kern = &mma_kernel<T, XR, RT, RS, KS, PER>;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), S::LDS)) return false;
     a.slots_a_group = a.group / (32 * PER);
-    a.inv_slots = 1.0f / static_cast<float>(a.slots_a_group);
-    const int stages = (a.k + kStage - 1) / kStage;
+    const int stages = tecoops::gemv_int4_stages(a.k);
+    a.inv_slots = tecoops::gemv_int4_inverse(a.slots_a_group, stages * S::SLOTS);
     a.split = (stages + splits - 1) / splits;
     splits = (stages + a.split - 1) / a.split;
     if (splits == 1) a.parts = nullptr;

@@ -68,3 +68,22 @@ def test_rows_beside_one_that_is_none():
     x = rand(b, k, dtype=torch.bfloat16, seed=1)
     x[3, 5], x[17, 900], x[9] = math.nan, math.inf, math.nan
     compare(x, n, group, False, 2)
+
+
+@pytest.mark.parametrize("b", [1, 2])
+def test_groups_of_a_very_long_row(b):
+    """The last groups of a K of 2 * 10^8: x is 0 but there."""
+    n, group, k, used = 2, 96, 201332160, 5472
+    dtype, far = torch.float16, k - 5472
+    g = torch.Generator().manual_seed(3)
+    w = torch.zeros(n, k // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.ones(n, k // group, dtype=dtype, device="cuda")
+    x = torch.zeros(b, k, dtype=dtype, device="cuda")
+    codes = torch.randint(0, 16, (n, used), generator=g)
+    tail = ((torch.rand(n, used // group, generator=g) + 0.5) * 0.1).to(dtype)
+    xt = rand(b, used, dtype=dtype, seed=4)
+    w[:, far // 2:], scales[:, far // group:], x[:, far:] = pack(codes).cuda(), tail.cuda(), xt.cuda()
+    out = torch.empty(b, n, dtype=dtype, device="cuda")
+    tecoops.gemv_int4(w, scales, x, out)
+    ref = xt.double() @ weights(codes, tail, None, group).t()
+    check(out, ref, bound(xt, codes, tail, None, group, ref, dtype), "the end of a long row")
