@@ -724,7 +724,7 @@ __device__ __forceinline__ void merge_states(const float *lds, int cols, Sink si
 }
 
 __device__ __forceinline__ int splits_of(const Params &p, int S) {
-    return min(max((S + p.split_len - 1) / p.split_len, 1), p.splits);
+    return min(max((S - 1) / p.split_len + 1, 1), p.splits);
 }
 
 // Workgroup (sequence, kv head, column tile) and split: the last split holds every
@@ -771,7 +771,8 @@ __global__ void __launch_bounds__(64 * kWaves, D * CT <= 64 && CT == 1 ? 4 : D *
     }
     if (split != 0) return;
     // (p.cols need not be a whole number of tiles: the rest starts at it)
-    for (c0 = p.cols + tile * SPAN; c0 < all; c0 += p.tiles * SPAN) {
+    for (long long past = static_cast<long long>(p.cols) + tile * SPAN; past < all; past += p.tiles * SPAN) {
+        c0 = static_cast<int>(past);
         __syncthreads();
         split_pass<T, D, CT, PACK, UNIFORM>(p, states, b, kvh, q_off, L, S, c0, 0, S);
         merge_states<D, CT>(states, min(SPAN, all - c0), write(c0));
@@ -1059,8 +1060,8 @@ __device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, floa
 }
 
 // Workgroup (sequence, kv head) and (column tile, split), the heaviest tiles first;
-// that of tile 0 and split 0 goes on to the columns past the grid, of which there
-// are none where the bound on the rows holds.
+// those of split 0 go on to the columns past the grid, of which there are none where
+// the bound on the rows holds and the grid has room for it.
 template <typename T, int D, int W, int TILE>
 __global__ void __launch_bounds__(W * 64, W >= 12 ? 3 : D <= 128 && W == 4 ? 3 : 2) tile_kernel(Params p) {
     extern __shared__ __attribute__((aligned(16))) uint16_t tiles_lds[];
@@ -1085,8 +1086,10 @@ __global__ void __launch_bounds__(W * 64, W >= 12 ? 3 : D <= 128 && W == 4 ? 3 :
                                        split == ns - 1 ? S : (split + 1) * p.split_len, p.ws_o + at * p.cols * D,
                                        p.ws_ml + at * p.cols * 2);
     }
-    if (tile != 0 || split != 0) return;
-    for (c0 = p.cols; c0 < all; c0 += COLS) {
+    if (split != 0) return;
+    for (long long past = p.cols + static_cast<long long>(tile) * COLS; past < all;
+         past += static_cast<long long>(p.tiles) * COLS) {
+        c0 = static_cast<int>(past);
         __syncthreads();
         column_tile<T, D, W, TILE>(p, tiles_lds, meet, b, kvh, q_off, L, S, all, c0, 0, S, nullptr, nullptr);
     }
@@ -1160,7 +1163,7 @@ extern "C" tecoopsStatus_t tecoopsGetFlashAttentionInt4WorkspaceSize(int batch, 
         num_heads % num_kv_heads != 0 || max_seqlen_k <= 0)
         return TECOOPS_STATUS_BAD_PARAM;
     if (!head_size_ok(head_size)) return TECOOPS_STATUS_NOT_SUPPORTED;
-    const int rows = std::max(max_seqlen_q, static_cast<int>(tecoops::ceil_div(std::max(total_q, 1), batch)));
+    const int rows = tecoops::fa4::row_bound(max_seqlen_q, total_q, batch);
     *bytes = 0;
     for (const bool exact : {false, true})  // (of either type)
         *bytes = std::max(*bytes, tecoops::fa4::make_plan(batch, num_heads, num_kv_heads, head_size, rows, max_seqlen_k,
@@ -1220,10 +1223,11 @@ extern "C" tecoopsStatus_t tecoopsFlashAttentionInt4(
     p.scale_log2 = scale * 1.4426950408889634f;
     p.causal = causal != 0;
     p.total_q = total_q;
-    const int rows = std::max(max_seqlen_q, static_cast<int>(tecoops::ceil_div(total_q, batch)));
-    const int keys = max_seqlen_k > 0 ? max_seqlen_k : std::max(p.kv_cap, 1);
+    const int rows = tecoops::fa4::row_bound(max_seqlen_q, total_q, batch);
+    const int keys = std::max(max_seqlen_k > 0 ? std::min(max_seqlen_k, p.kv_cap) : p.kv_cap, 1);
     TECO_RETURN_IF(static_cast<long long>(total_q) * p.G >= (1ll << 31), TECOOPS_STATUS_NOT_SUPPORTED,
                    "flash_attention_int4: too many query rows");
+    if (static_cast<long long>(batch) * num_kv_heads > tecoops::fa4::kMostWorkgroups) return TECOOPS_STATUS_NOT_SUPPORTED;
     const int cus = tecoops::device_cus();
     const auto plan = [&](size_t room) {
         return tecoops::fa4::make_plan(batch, num_heads, num_kv_heads, head_size, rows, keys, room, cus,
@@ -1234,8 +1238,6 @@ extern "C" tecoopsStatus_t tecoopsFlashAttentionInt4(
         workspace = tecoops::handle_scratch_if_any(handle, pl.bytes);
         if (workspace == nullptr) pl = plan(0);
     }
-    // the grid within 32-bit thread counts
-    if (static_cast<long long>(batch) * num_kv_heads * pl.tiles * pl.splits > (1ll << 22)) return TECOOPS_STATUS_NOT_SUPPORTED;
     p.cols = pl.cols;
     p.tiles = pl.tiles;
     p.split_len = pl.split_len;
