@@ -91,6 +91,12 @@ __device__ __forceinline__ void sequence(const Params &p, int b, long long &q_of
     S = min(max(p.kv_lens[b], 0), p.kv_cap);
 }
 
+// The power of two that brings a sum of weights next to 2^-10: with it a state's output
+// is at most the largest value, whatever the number of keys.
+__device__ __forceinline__ int near_1024th(float sum) {
+    return sum > 0.0f && sum < INFINITY ? -10 - ilogbf(sum) : 0;
+}
+
 // Output rows of no sequence are written as zeros, as by the 16-bit cache's
 // attention.
 __device__ __forceinline__ void zero_tail(const Params &p, int D) {
@@ -117,10 +123,17 @@ __device__ __forceinline__ long long row_of(const Params &p, int kvh, int page, 
 }
 
 // Weights are at most 2^kTop * 2^kSlack before the maximum is raised; scales at
-// most twice the reference: P s stays below 2^15.
+// most twice the reference: P s stays below 2^15.  Rows of equal elements have scale 0
+// whatever they hold: middles of rows are at most 2^kAside above that, so that P * middle
+// stays below 2^56.
 constexpr float kTop = 10.0f, kSlack = 4.0f;
 constexpr float kMiddle = 7.5f;  // of the codes
 constexpr int kLeastRef = -90;   // (sums of 2^24 weights stay within fp32)
+constexpr float kAside = 0x1p40f;
+// Past a reference of 2^kMostRef (in bf16 alone), sums in the values' units come near
+// fp32's end, and past 2^100 small weights its start: from there on a wave takes its
+// values in units of 2^kFar, and leaves a state whose sum is near 2^-10.
+constexpr int kMostRef = 40, kFar = 64;
 constexpr float kNever = -1e30f;  // the running maximum before any key
 
 // N words of each lane from `base` + `off` (or `src`) to `dst` in LDS, lane after lane
@@ -278,12 +291,14 @@ __device__ __forceinline__ u32x4 widen8(uint32_t w) {
 // the weights and of weight * middle of the row over this lane's keys, and the
 // unnormalised sums of weight * scale * code, all in units of the power of two `ref`
 // that the scales are taken relative to.
-template <int D, int CT>
+template <typename T, int D, int CT>
 struct State {
     f32x4_t acc[CT][D / 16], w[CT];  // w: sums of the weights * scale as rounded
     float m[CT], l[CT], r[CT];
-    float twice_ref;
+    float twice_ref;  // below 0 in units of 2^kFar: every block is looked at
     int ref;
+
+    __device__ __forceinline__ bool far() const { return __is_same(T, bf16) && twice_ref < 0.0f; }
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -381,7 +396,7 @@ __device__ __forceinline__ uint32_t from_right(uint32_t v) {
 // takes 8 / PACK of its 8 keys through the softmax instead of all: 4 heads of a group
 // are then a quarter of that work (the larger part of what is not a mask or a product).
 template <typename T, int D, int CT, int PACK>
-__device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[CT], State<D, CT> &st, int j0, int limit,
+__device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[CT], State<T, D, CT> &st, int j0, int limit,
                                        bool edge) {
     using R = Ring<D, true>;
     static_assert(CT == 1 || PACK == 1, "copies of one tile's columns");
@@ -474,17 +489,16 @@ __device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[C
                 if (j0 + key_of(e) >= min(limit, col[t].vis)) s[t][e] = kNegInf;
     }
     float sv[V], av[V];
-    float top = 0.0f;
-    bool none = false;
+    float top = 0.0f, aside = 0.0f;  // largest scale, middle (NaN where one is)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         sv[e] = lo<T>(vp[e]);
         av[e] = fmaf(kMiddle, sv[e], hi<T>(vp[e]));
         top = fmaxf(top, fabsf(sv[e]));
-        none = none || av[e] != av[e];
+        aside = __builtin_elementwise_maximum(aside, fabsf(av[e]));
     }
     float mx[CT];
-    bool raise = none || !(top <= st.twice_ref);
+    bool raise = !(__builtin_elementwise_maximum(top, aside * (1.0f / kAside)) <= st.twice_ref);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         mx[t] = s[t][0];
@@ -496,33 +510,49 @@ __device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[C
     if (__any(raise)) {
         // a value row that is no number: its score is none either, where it is seen (so
         // that it reaches the rows that see it), and the values 0 (and no others)
-        if (none) {
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (av[e] != av[e]) {
+        for (int e = 0; e < V; ++e) {
+            if (av[e] != av[e]) {
 #pragma unroll
-                    for (int t = 0; t < CT; ++t)
-                        if (s[t][e] != kNegInf) s[t][e] = av[e];
-                    sv[e] = av[e] = 0.0f;
-                }
+                for (int t = 0; t < CT; ++t)
+                    if (s[t][e] != kNegInf) s[t][e] = av[e];
+                sv[e] = av[e] = 0.0f;
+            }
+            top = fmaxf(top, fabsf(av[e]) * (1.0f / kAside));
         }
         // scales relative to a power of two that is at least half of the largest seen
         // (wave-wide: they are the same for all columns)
         top = column_max<PACK>(top);
-        const int e = max(st.ref, min(static_cast<int>(__float_as_uint(top) >> 23) - 127, 100));
-        const float down = e - st.ref > 120 ? 0.0f : power2(st.ref - e);
+        const int old = st.ref;
+        int e = static_cast<int>(__float_as_uint(top) >> 23) - 127, enter = 0;
+        if (__is_same(T, bf16) && (st.far() || e > kMostRef)) {
+            enter = st.far() ? 0 : kFar;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                sv[k] *= power2(-kFar);
+                av[k] *= power2(-kFar);
+            }
+            e = max(old - enter, min(e - kFar, kFar));
+            st.twice_ref = -1.0f;
+        } else {
+            e = max(old, min(e, kMostRef));
+            st.twice_ref = power2(e + 1);
+        }
         st.ref = e;
-        st.twice_ref = power2(e + 1);
+        // (such a power of two may be past a float's, though nothing scaled by it is)
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             const float next = fmaxf(st.m[t], column_max<PACK>(mx[t]));
-            const float f = __builtin_amdgcn_exp2f(st.m[t] - next) * down;
+            const float f = __builtin_amdgcn_exp2f(st.m[t] - next);
             st.m[t] = next;
-            st.l[t] *= f;
-            st.r[t] *= f;
-            st.w[t] *= f;
+            st.l[t] = ldexpf(st.l[t] * f, old - e);
+            st.r[t] = ldexpf(st.r[t] * f, old - e - enter);
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= f;
+            for (int v = 0; v < 4; ++v) {
+                st.w[t][v] = ldexpf(st.w[t][v] * f, old - e - enter);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) st.acc[t][i][v] = ldexpf(st.acc[t][i][v] * f, old - e - enter);
+            }
         }
     }
     // the weights in fp16, in fp16 models as sums of two terms: one term's rounding,
@@ -633,7 +663,7 @@ __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, i
         load_column<T, D>(p, col[t], p.q + ((q_off + row) * p.H + kvh * p.G + head) * D, c0 + nc <= last);
         col[t].vis = p.causal ? q_start + row + 1 : S;
     }
-    State<D, CT> st;
+    State<T, D, CT> st;
     st.clear();
     using R = Ring<D, UNIFORM>;
     constexpr int STEP = R::STEP, DEPTH = R::DEPTH;
@@ -680,23 +710,26 @@ __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, i
     __syncthreads();  // the states take the rings' place
     constexpr int COLS = 16 * CT;
     float *lm = lds, *ll = lm + kWaves * COLS, *lout = ll + kWaves * COLS;
-    const float ref = power2(st.ref);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         const float l = column_sum<PACK>(st.l[t]), r = column_sum<PACK>(st.r[t]);
         const int c = wave * COLS + 16 * t + n;
         if (n >= 16 / PACK) continue;  // a copy
+        // the sum's unit 2^ref, or one that brings it to 2^-10, which the maximum takes up
+        const int unit = st.far() ? near_1024th(l) : st.ref;
+        const float ref = st.far() ? 1.0f : power2(st.ref);
+        const auto value = [&](float x) { return st.far() ? ldexpf(x, unit + kFar) : x * ref; };
         if (g == 0) {
-            lm[c] = st.m[t];
-            ll[c] = l * ref;
+            lm[c] = st.m[t] + static_cast<float>(st.ref - unit);
+            ll[c] = ldexpf(l, unit);
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-            const float unit = (i & 1) ? 0x1p20f : 0x1p24f;
+            const float code = (i & 1) ? 0x1p20f : 0x1p24f;
 #pragma unroll
             for (int v = 0; v < 4; ++v)
                 lout[c * D + channel_of<D>(i, 4 * g + v)] =
-                    ref * (fmaf(st.acc[t][i][v], unit, -kMiddle * st.w[t][v]) + r);
+                    value(fmaf(st.acc[t][i][v], code, -kMiddle * st.w[t][v]) + r);
         }
     }
     __syncthreads();
@@ -1016,7 +1049,7 @@ __device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, floa
         const auto outside = [](float most) { return most < INFINITY && most > 0.0f && (most > 0x1p15f || most < 0x1p-6f); };
         if (!outside(all_k) && !outside(all_v)) break;
         const auto power = [&](float most) {
-            return outside(most) ? min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127 - 10, -110), 110) : 0;
+            return outside(most) ? min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127 - 10, -110), 118) : 0;
         };
         ek = __builtin_amdgcn_readfirstlane(power(all_k));
         ev = __builtin_amdgcn_readfirstlane(power(all_v));
@@ -1025,15 +1058,20 @@ __device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, floa
     if (part != nullptr) {
         if (cw0 + r32 < all) {
             float *dst = part + static_cast<long long>(j) * D;
-            const float unit = power2(ev);
+            // (sums of large values, of any number of keys, stay within fp32)
+            const int up = ev > 40 ? near_1024th(lt) : 0;
 #pragma unroll
             for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    *reinterpret_cast<float4_t *>(dst + 32 * db + 8 * u + 4 * g) =
-                        float4_t{oacc[0][db][4 * u] * unit, oacc[0][db][4 * u + 1] * unit, oacc[0][db][4 * u + 2] * unit,
-                                 oacc[0][db][4 * u + 3] * unit};
-            if (g == 0) *reinterpret_cast<float2_t *>(part_ml + static_cast<long long>(j) * 2) = float2_t{m[0], lt};
+                for (int u = 0; u < 4; ++u) {
+                    float4_t o;
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) o[v] = ldexpf(oacc[0][db][4 * u + v], ev + up);
+                    *reinterpret_cast<float4_t *>(dst + 32 * db + 8 * u + 4 * g) = o;
+                }
+            if (g == 0)
+                *reinterpret_cast<float2_t *>(part_ml + static_cast<long long>(j) * 2) =
+                    float2_t{m[0] - static_cast<float>(up), ldexpf(lt, up)};
         }
         return;  // (the loop's last barrier has passed)
     }
