@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_kernel(AxisPositions angles,
 // Any head size, alignment and order: a wave per head, an element a lane at a time.
 template <typename T, bool NEOX, bool CACHE>
 __global__ void __launch_bounds__(kThreads) qk_norm_any_kernel(AxisPositions angles, Args a) {
-    __shared__ float rows[kThreads / 64][kMaxHead];
+    __shared__ __attribute__((aligned(16))) float rows[kThreads / 64][kMaxHead];
     const int lane = threadIdx.x & 63, D = a.head_size;
     const int nq = a.num_heads, nk = nq + a.num_kv_heads, total = nk + (CACHE ? a.num_kv_heads : 0);
     const long long unit = static_cast<long long>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
@@ -210,16 +210,31 @@ __global__ void __launch_bounds__(kThreads) qk_norm_any_kernel(AxisPositions ang
     }
     float *y = rows[threadIdx.x >> 6];
     const uint16_t *w = is_q ? a.q_weight : a.k_weight;
+    // (the wave's own LDS writes, before it reads them)
+    const auto written = [] {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    for (int e = lane; e < D; e += 64) y[e] = Cvt<T>::to(row[e]);
+    written();
+    // runs of 8 a lane and a tree over the lanes, as in the kernel above: a row comes out
+    // of both with the same bits
     float sum = 0.0f;
-    for (int e = lane; e < D; e += 64) {
-        const float f = Cvt<T>::to(row[e]);
-        sum = fmaf(f, f, sum);
+    for (int c = 8 * lane; c < D; c += 8 * 64) {
+        float run = 0.0f;
+        if (c + 8 <= D) {
+            const float4_t f[2] = {*reinterpret_cast<const float4_t *>(y + c), *reinterpret_cast<const float4_t *>(y + c + 4)};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) run = fmaf(f[e >> 2][e & 3], f[e >> 2][e & 3], run);
+        } else {
+            for (int e = c; e < D; ++e) run = fmaf(y[e], y[e], run);
+        }
+        sum += run;
     }
     const float r = rsqrtf(fmaf(wave_sum(sum), 1.0f / static_cast<float>(D), a.eps));
-    for (int e = lane; e < D; e += 64) y[e] = Cvt<T>::to(row[e]) * r * Cvt<T>::to(w[e]);
-    // the wave's own LDS writes, before it reads them
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    written();
+    for (int e = lane; e < D; e += 64) y[e] = y[e] * r * Cvt<T>::to(w[e]);
+    written();
     const int half = a.rot_dim >> 1;
     for (int e = lane; e < D; e += 64) {
         float o = y[e];
