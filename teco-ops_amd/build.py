@@ -74,8 +74,8 @@ EXTRA_FLAGS = {
 # with a fixed vmcnt that leaves the compiler's own younger loads in flight.
 # The count is right only if those loads stay between the copies and the
 # wait, which the compiler does not promise for loads of read-only memory,
-# so the device assembly of these sources is checked on every build (with it
-# the waits behind matrix products).
+# so the device assembly of these sources is checked on every build (that of
+# every source for the waits behind matrix products).
 # flash_attention.hip, fa_int4.hip, gemv_batch.hip and moe.hip wait for their copies by
 # counting only younger copies (inline assembly, which the compiler keeps in
 # order) and linear.hip for all of its copies at once, so only their use of M0 is
@@ -133,10 +133,14 @@ def check_copy_waits(asm_text, src="", waits=True):
 
 
 def _vector_registers(text):
+    """Vector (v) and accumulation (a) registers that the text names."""
     import re
     regs = set()
-    for m in re.finditer(r"\bv\[(\d+):(\d+)\]|\bv(\d+)\b", text):
-        regs |= {int(m.group(3))} if m.group(3) else set(range(int(m.group(1)), int(m.group(2)) + 1))
+    for m in re.finditer(r"\b([av])\[(\d+):(\d+)\]|\b([av])(\d+)\b", text):
+        if m.group(4):
+            regs.add((m.group(4), int(m.group(5))))
+        else:
+            regs |= {(m.group(1), i) for i in range(int(m.group(2)), int(m.group(3)) + 1)}
     return regs
 
 
@@ -145,9 +149,11 @@ def check_matrix_waits(asm_text, src=""):
     v_mfma and the first vector or memory instruction that reads its result or
     overwrites it: for a product of P passes P + 4, of 2 passes 5 (those of 4 x 4
     results have 2 passes, of 16 x 16 at most 4 here, of 32 x 32 8, or 16 with a
-    depth of 8 or less).  The hardware does not wait by itself, and the compiler
-    has left the wait out where a branch lay between the two.  Returns the number
-    of products; raises RuntimeError on a violation."""
+    depth of 8 or less).  Another product may add to the whole result at once, and to
+    a part of it two states earlier than multiply by it; what it writes is its own from
+    there on.  The hardware does not wait by itself, and the compiler has left the wait
+    out where a branch lay between the two.
+    Returns the number of products; raises RuntimeError on a violation."""
     import re
     count = 0
     for k in re.finditer(r"^(_Z\S*):", asm_text, re.M):
@@ -165,16 +171,16 @@ def check_matrix_waits(asm_text, src=""):
                 continue
             count += 1
             need = 5 if "_4x4x" in op else 8 if "_16x16x" in op else 12 if "_32x32x16" in op else 20
-            result = _vector_registers(args.split(",")[0])
-            paths, seen = [(i + 1, 0)], set()
+            paths, seen = [(i + 1, 0, frozenset(_vector_registers(args.split(",")[0])))], set()
             while paths:
-                j, passed = paths.pop()
-                if j >= len(code) or passed >= need or (j, passed) in seen:
+                j, passed, result = paths.pop()
+                if j >= len(code) or passed >= need or not result or (j, passed, result) in seen:
                     continue
-                seen.add((j, passed))
+                seen.add((j, passed, result))
                 o, a = code[j]
                 if o.startswith("v_mfma"):
-                    used = _vector_registers(",".join(re.findall(r"v\[\d+:\d+\]", a)[1:3]))
+                    written, one, two, added = [_vector_registers(x) for x in a.split(",")[:4]]
+                    used = one | two | (added if added != result and passed < need - 2 else set())
                 elif o.startswith(("v_", "ds_", "global_", "buffer_", "flat_", "scratch_")):
                     used = _vector_registers(a)
                 else:
@@ -182,15 +188,17 @@ def check_matrix_waits(asm_text, src=""):
                 if used & result:
                     raise RuntimeError(f"{src}: {k.group(1)}: {o} {a} only {passed} wait states behind "
                                        f"{op} {args}")
+                if o.startswith("v_mfma"):
+                    result = result - written
                 passed += 1 + (int(a) if o == "s_nop" else 0)
                 if o.startswith(("s_branch", "s_cbranch")):
-                    paths.append((labels[a], passed))
+                    paths.append((labels[a], passed, result))
                 if o not in ("s_branch", "s_endpgm"):
-                    paths.append((j + 1, passed))
+                    paths.append((j + 1, passed, result))
     return count
 
 
-def _check_copies(src, waits):
+def _check_assembly(src):
     out = os.path.join(BUILD, os.path.splitext(src)[0] + ".s")
     cmd = [HIPCC, *CFLAGS, *EXTRA_FLAGS.get(src, []), "--cuda-device-only", "-S",
            os.path.join(CSRC, src), "-o", out]
@@ -199,12 +207,12 @@ def _check_copies(src, waits):
         raise RuntimeError(f"assembly failed: {src}\n{' '.join(cmd)}\n{r.stderr[-4000:]}")
     with open(out) as f:
         asm = f.read()
-    n = check_copy_waits(asm, src, waits)
-    check_matrix_waits(asm, src)
+    n = check_copy_waits(asm, src, COPY_WAIT_CHECKED.get(src, False))
+    products = check_matrix_waits(asm, src)
     os.remove(out)
-    if n == 0:
-        raise RuntimeError(f"{src}: no LDS copies found to check")
-    return out, ""
+    if (n > 0) != (src in COPY_WAIT_CHECKED):
+        raise RuntimeError(f"{src}: {n} kernels with LDS copies; COPY_WAIT_CHECKED lists those that have them")
+    return products
 
 
 def _compile(src):
@@ -276,7 +284,7 @@ def build(verbose=False):
     os.makedirs(BUILD, exist_ok=True)
     jobs = min(len(SOURCES), os.cpu_count() or 4, 16)
     with concurrent.futures.ThreadPoolExecutor(jobs) as ex:
-        checks = [ex.submit(_check_copies, src, w) for src, w in COPY_WAIT_CHECKED.items()]
+        checks = [ex.submit(_check_assembly, src) for src in SOURCES if src.endswith(".hip")]
         results = list(ex.map(_compile, SOURCES))
         for c in checks:
             c.result()
