@@ -94,7 +94,7 @@ __device__ __forceinline__ void sequence(const Params &p, int b, long long &q_of
 // The power of two that brings a sum of weights next to 2^-10: with it a state's output
 // is at most the largest value, whatever the number of keys.
 __device__ __forceinline__ int near_1024th(float sum) {
-    return sum > 0.0f && sum < INFINITY ? -10 - ilogbf(sum) : 0;
+    return sum > 0.0f && sum < INFINITY ? 117 - static_cast<int>(__float_as_uint(sum) >> 23) : 0;
 }
 
 // Output rows of no sequence are written as zeros, as by the 16-bit cache's
@@ -295,10 +295,12 @@ template <typename T, int D, int CT>
 struct State {
     f32x4_t acc[CT][D / 16], w[CT];  // w: sums of the weights * scale as rounded
     float m[CT], l[CT], r[CT];
-    float twice_ref;  // below 0 in units of 2^kFar: every block is looked at
+    float twice_ref;  // 0: no sums yet; below 0: in units of 2^kFar (every block is looked at)
     int ref;
 
-    __device__ __forceinline__ bool far() const { return __is_same(T, bf16) && twice_ref < 0.0f; }
+    // twice_ref's sign, the same in all lanes.
+    __device__ __forceinline__ int state() const { return __builtin_amdgcn_readfirstlane(__float_as_int(twice_ref)); }
+    __device__ __forceinline__ bool far() const { return __is_same(T, bf16) && state() < 0; }
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -310,7 +312,7 @@ struct State {
             for (int i = 0; i < D / 16; ++i) acc[t][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
         ref = kLeastRef;
-        twice_ref = power2(kLeastRef + 1);
+        twice_ref = 0.0f;
     }
 };
 
@@ -510,49 +512,67 @@ __device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[C
     if (__any(raise)) {
         // a value row that is no number: its score is none either, where it is seen (so
         // that it reaches the rows that see it), and the values 0 (and no others)
+        if (__builtin_expect(__any(aside != aside), 0)) {
+            aside = 0.0f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            if (av[e] != av[e]) {
+            for (int e = 0; e < V; ++e) {
+                if (av[e] != av[e]) {
 #pragma unroll
-                for (int t = 0; t < CT; ++t)
-                    if (s[t][e] != kNegInf) s[t][e] = av[e];
-                sv[e] = av[e] = 0.0f;
+                    for (int t = 0; t < CT; ++t)
+                        if (s[t][e] != kNegInf) s[t][e] = av[e];
+                    sv[e] = av[e] = 0.0f;
+                }
+                aside = fmaxf(aside, fabsf(av[e]));
             }
-            top = fmaxf(top, fabsf(av[e]) * (1.0f / kAside));
         }
         // scales relative to a power of two that is at least half of the largest seen
         // (wave-wide: they are the same for all columns)
-        top = column_max<PACK>(top);
-        const int old = st.ref;
-        int e = static_cast<int>(__float_as_uint(top) >> 23) - 127, enter = 0;
-        if (__is_same(T, bf16) && (st.far() || e > kMostRef)) {
-            enter = st.far() ? 0 : kFar;
+        top = column_max<PACK>(fmaxf(top, aside * (1.0f / kAside)));
+        int e = __builtin_amdgcn_readfirstlane(static_cast<int>(__float_as_uint(top) >> 23) - 127);
+        const int before = st.state(), old = st.ref;
+        st.ref = max(old, min(e, kMostRef));
+        st.twice_ref = power2(st.ref + 1);
+        int down = before == 0 ? 0 : old - st.ref, down_l = down;  // (without a sum: any)
+        if (__builtin_expect(before < 0 || e > kMostRef || down < -80, 0)) {
+            int enter = 0;
+            if (__is_same(T, bf16) && (before < 0 || e > kMostRef)) {
+                enter = before < 0 ? 0 : kFar;
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                sv[k] *= power2(-kFar);
-                av[k] *= power2(-kFar);
+                for (int k = 0; k < V; ++k) {
+                    sv[k] *= power2(-kFar);
+                    av[k] *= power2(-kFar);
+                }
+                st.ref = max(old - enter, min(e - kFar, kFar));
+                st.twice_ref = -1.0f;
             }
-            e = max(old - enter, min(e - kFar, kFar));
-            st.twice_ref = -1.0f;
-        } else {
-            e = max(old, min(e, kMostRef));
-            st.twice_ref = power2(e + 1);
+            down_l = before == 0 ? 0 : old - st.ref;
+            down = before == 0 ? 0 : down_l - enter;
+            // (such a power of two may be past a float's, though nothing scaled by it is: in
+            // steps.  What a factor above 2^-80 and a fall of the weights make 0 is nothing)
+#pragma unroll 1
+            for (; down < -80; down += 80)
+#pragma unroll
+                for (int t = 0; t < CT; ++t) {
+                    st.r[t] *= 0x1p-80f;
+                    st.w[t] *= 0x1p-80f;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= 0x1p-80f;
+                }
+#pragma unroll 1
+            for (; down_l < -80; down_l += 80)
+#pragma unroll
+                for (int t = 0; t < CT; ++t) st.l[t] *= 0x1p-80f;
         }
-        st.ref = e;
-        // (such a power of two may be past a float's, though nothing scaled by it is)
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             const float next = fmaxf(st.m[t], column_max<PACK>(mx[t]));
-            const float f = __builtin_amdgcn_exp2f(st.m[t] - next);
+            const float fall = __builtin_amdgcn_exp2f(st.m[t] - next), f = fall * power2(down);
             st.m[t] = next;
-            st.l[t] = ldexpf(st.l[t] * f, old - e);
-            st.r[t] = ldexpf(st.r[t] * f, old - e - enter);
+            st.l[t] *= fall * power2(down_l);
+            st.r[t] *= f;
+            st.w[t] *= f;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                st.w[t][v] = ldexpf(st.w[t][v] * f, old - e - enter);
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) st.acc[t][i][v] = ldexpf(st.acc[t][i][v] * f, old - e - enter);
-            }
+            for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= f;
         }
     }
     // the weights in fp16, in fp16 models as sums of two terms: one term's rounding,
@@ -717,11 +737,10 @@ __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, i
         if (n >= 16 / PACK) continue;  // a copy
         // the sum's unit 2^ref, or one that brings it to 2^-10, which the maximum takes up
         const int unit = st.far() ? near_1024th(l) : st.ref;
-        const float ref = st.far() ? 1.0f : power2(st.ref);
-        const auto value = [&](float x) { return st.far() ? ldexpf(x, unit + kFar) : x * ref; };
+        const float value = power2(st.far() ? unit + kFar : unit);
         if (g == 0) {
             lm[c] = st.m[t] + static_cast<float>(st.ref - unit);
-            ll[c] = ldexpf(l, unit);
+            ll[c] = l * power2(unit);
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
@@ -729,7 +748,7 @@ __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, i
 #pragma unroll
             for (int v = 0; v < 4; ++v)
                 lout[c * D + channel_of<D>(i, 4 * g + v)] =
-                    value(fmaf(st.acc[t][i][v], code, -kMiddle * st.w[t][v]) + r);
+                    value * (fmaf(st.acc[t][i][v], code, -kMiddle * st.w[t][v]) + r);
         }
     }
     __syncthreads();
@@ -1060,18 +1079,17 @@ __device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, floa
             float *dst = part + static_cast<long long>(j) * D;
             // (sums of large values, of any number of keys, stay within fp32)
             const int up = ev > 40 ? near_1024th(lt) : 0;
+            const float unit = power2(ev + up);
 #pragma unroll
             for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    float4_t o;
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) o[v] = ldexpf(oacc[0][db][4 * u + v], ev + up);
-                    *reinterpret_cast<float4_t *>(dst + 32 * db + 8 * u + 4 * g) = o;
-                }
+                for (int u = 0; u < 4; ++u)
+                    *reinterpret_cast<float4_t *>(dst + 32 * db + 8 * u + 4 * g) =
+                        float4_t{oacc[0][db][4 * u] * unit, oacc[0][db][4 * u + 1] * unit, oacc[0][db][4 * u + 2] * unit,
+                                 oacc[0][db][4 * u + 3] * unit};
             if (g == 0)
                 *reinterpret_cast<float2_t *>(part_ml + static_cast<long long>(j) * 2) =
-                    float2_t{m[0] - static_cast<float>(up), ldexpf(lt, up)};
+                    float2_t{m[0] - static_cast<float>(up), lt * power2(up)};
         }
         return;  // (the loop's last barrier has passed)
     }
