@@ -527,8 +527,9 @@ tecoopsStatus_t tecoopsReshapeAndCacheInt4(tecoopsHandle_t handle, const void *k
  * 96, 128, 160, 192}.  fp16, and in bf16 up to 64 (query row, head) pairs of a kv head,
  * read K and V as they are held; longer queries in bf16 widen them to fp16 first (one
  * more rounding, finer than the output's; fp16 prompts take up to twice as long).
- * What the cache holds behind a sequence's last key is not used, whatever it is; a key
- * or value row of NaN makes the rows that see it NaN and no others.
+ * What the cache holds behind a sequence's last key is not used, whatever it is.  A key
+ * or value row of NaN, or a value row whose pair is infinite, makes the rows that see it
+ * NaN and no others; large rows change nothing for the query rows that do not see them.
  * workspace: tecoopsGetFlashAttentionInt4WorkspaceSize() bytes for the same sizes
  * and bounds, 16-byte aligned; with less the keys are cut into fewer splits.  NULL
  * uses the handle's scratch, and none on a stream under capture (unsplit: slower,

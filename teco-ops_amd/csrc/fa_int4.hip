@@ -17,8 +17,9 @@
 // which for rows around 0 is 3 times as far.  A nibble in bits 4-7 is 16 n; the 1/16 goes into
 // q's elements and into the sums of those value channels.  q and the weights P s
 // are fp16, scaled by powers of two to the top of its range (q by its largest
-// element in its column, P s by the running maximum and the largest scale so far),
-// so that bf16's range is kept and small weights of long contexts lose nothing.
+// element in its column, P s by the running maximum and the largest scale that the
+// column has seen), so that bf16's range is kept and small weights of long contexts lose
+// nothing.
 //   * Scores are computed transposed (keys x columns, 16x16x32), so that a lane
 //     holds 8 keys of one column, which are the operand of the second product as
 //     they are: neither P nor the codes go through LDS.  With at most 8 or 4 columns
@@ -35,16 +36,13 @@
 //
 // Tile route (prefill in bf16).  K and V tiles are widened to fp16 once per workgroup, on
 // the way into LDS, and attended as in flash_attention.hip (fa_device.h).  fp16 is 8 times
-// closer than bf16 and a fixed range: rows of the cache are first taken as they are, and a
-// tile in which one is too large or all are too small is done again with a power of two
-// that fits.  Rounded are K, V and the weights, each to 2^-12, which is unseen beside a
-// bf16 output.  Beside an fp16 one it is seen (4e-4 to 6e-4, rms, against 2.1e-4), so
-// that fp16 models have the split route for any number of columns, at up to twice the
-// time.  Matrix cores are busy 37 % of the cycles, vector units 41 %, at the 12 waves a CU
-// that LDS leaves room for: issue and waits in between.  [4 sequences, 2048 rows on up to
-// 4096 keys, 32 heads on 8 of 128] 426 to 436 us, 750 TFLOP/s of visible pairs; [2 of up to
-// 203 rows on 16300 keys, 40 heads] 155 us, 700 (2 and 3 % of both for value rows of NaN,
-// which are kept from the rows that do not see them: their keys become NaN and they 0).
+// closer than bf16 and a fixed range: rows of the cache are first taken as they are.  A
+// tile of columns in which a row is too large, all are too small, or all that some column
+// sees have too few bits is done again with powers of two that fit, and where its largest
+// row is more than 2^24 above all that some column sees, key by key in fp32.  Rounded are
+// K, V and the weights, each to 2^-11, which is unseen beside a bf16 output.  Beside an
+// fp16 one it is seen (4e-4 to 6e-4, rms, against 2.1e-4), so that fp16 models have the
+// split route for any number of columns, at up to twice the time.
 #include <cmath>
 
 #include "fa_device.h"
@@ -289,17 +287,20 @@ __device__ __forceinline__ u32x4 widen8(uint32_t w) {
 
 // State of a wave: per column tile the running maximum (log2 domain), the sums of
 // the weights and of weight * middle of the row over this lane's keys, and the
-// unnormalised sums of weight * scale * code, all in units of the power of two `ref`
-// that the scales are taken relative to.
+// unnormalised sums of weight * scale * code, all in units of the power of two ref()
+// that the scales of the rows that the column sees are taken relative to.
 template <typename T, int D, int CT>
 struct State {
     f32x4_t acc[CT][D / 16], w[CT];  // w: sums of the weights * scale as rounded
     float m[CT], l[CT], r[CT];
-    float twice_ref;  // 0: no sums yet; below 0: in units of 2^kFar (every block is looked at)
-    int ref;
+    float shift[CT];      // of a score to its weight: kTop - maximum - ref
+    float twice_ref[CT];  // 0: no sums yet; below 0: in units of 2^kFar (every block is looked at)
 
-    // twice_ref's sign, the same in all lanes.
-    __device__ __forceinline__ int state() const { return __builtin_amdgcn_readfirstlane(__float_as_int(twice_ref)); }
+    __device__ __forceinline__ int ref(int t) const {
+        return max(static_cast<int>(__float_as_uint(twice_ref[t]) >> 23 & 255u) - 128, kLeastRef);
+    }
+    // twice_ref's sign, the same in all columns.
+    __device__ __forceinline__ int state() const { return __builtin_amdgcn_readfirstlane(__float_as_int(twice_ref[0])); }
     __device__ __forceinline__ bool far() const { return __is_same(T, bf16) && state() < 0; }
 
     __device__ __forceinline__ void clear() {
@@ -310,9 +311,9 @@ struct State {
             w[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) acc[t][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            shift[t] = -kNever;
+            twice_ref[t] = 0.0f;
         }
-        ref = kLeastRef;
-        twice_ref = 0.0f;
     }
 };
 
@@ -500,9 +501,11 @@ __device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[C
         aside = __builtin_elementwise_maximum(aside, fabsf(av[e]));
     }
     float mx[CT];
-    bool raise = !(__builtin_elementwise_maximum(top, aside * (1.0f / kAside)) <= st.twice_ref);
+    const float size = __builtin_elementwise_maximum(top, aside * (1.0f / kAside));
+    bool raise = false;
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
+        raise = raise || !(size <= st.twice_ref[t]);
         mx[t] = s[t][0];
 #pragma unroll
         for (int e = 1; e < V; ++e) mx[t] = fmaxf(mx[t], s[t][e]);
@@ -510,65 +513,93 @@ __device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[C
         raise = raise || !(mx[t] <= st.m[t] + kSlack);
     }
     if (__any(raise)) {
-        // a value row that is no number: its score is none either, where it is seen (so
-        // that it reaches the rows that see it), and the values 0 (and no others)
-        if (__builtin_expect(__any(aside != aside), 0)) {
+        // a value row that is no finite number: its score is none, where it is seen (so that
+        // it reaches the rows that see it), and the values 0 (and no others)
+        if (__builtin_expect(__any(!(aside < INFINITY)), 0)) {
             aside = 0.0f;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                if (av[e] != av[e]) {
+                if (!(fabsf(av[e]) < INFINITY)) {
 #pragma unroll
                     for (int t = 0; t < CT; ++t)
-                        if (s[t][e] != kNegInf) s[t][e] = av[e];
+                        if (s[t][e] != kNegInf) s[t][e] = NAN;
                     sv[e] = av[e] = 0.0f;
                 }
                 aside = fmaxf(aside, fabsf(av[e]));
             }
         }
-        // scales relative to a power of two that is at least half of the largest seen
-        // (wave-wide: they are the same for all columns)
-        top = column_max<PACK>(fmaxf(top, aside * (1.0f / kAside)));
-        int e = __builtin_amdgcn_readfirstlane(static_cast<int>(__float_as_uint(top) >> 23) - 127);
-        const int before = st.state(), old = st.ref;
-        st.ref = max(old, min(e, kMostRef));
-        st.twice_ref = power2(st.ref + 1);
-        int down = before == 0 ? 0 : old - st.ref, down_l = down;  // (without a sum: any)
-        if (__builtin_expect(before < 0 || e > kMostRef || down < -80, 0)) {
-            int enter = 0;
-            if (__is_same(T, bf16) && (before < 0 || e > kMostRef)) {
-                enter = before < 0 ? 0 : kFar;
+        // scales relative to a power of two that is at least half of the largest that the
+        // column sees (a larger one behind its mask would leave nothing of the others)
+        const int before = st.state();
+        const auto exponent = [](float most) {
+            return static_cast<int>(__float_as_uint(column_max<PACK>(most)) >> 23) - 127;
+        };
+        int e[CT], old[CT], now[CT], down[CT], down_l[CT];
+        const int all = exponent(fmaxf(top, aside * (1.0f / kAside)));
+#pragma unroll
+        for (int t = 0; t < CT; ++t) e[t] = all;
+        if (edge) {
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                float most = 0.0f;
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    most = s[t][k] == kNegInf ? most : fmaxf(most, fmaxf(fabsf(sv[k]), fabsf(av[k]) * (1.0f / kAside)));
+                e[t] = exponent(most);
+            }
+        }
+        bool strange = before < 0;
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            old[t] = st.ref(t);
+            now[t] = max(old[t], min(e[t], kMostRef));
+            st.twice_ref[t] = power2(now[t] + 1);
+            down[t] = down_l[t] = before == 0 ? 0 : old[t] - now[t];  // (without a sum: any)
+            strange = strange || e[t] > kMostRef || down[t] < -80;
+        }
+        if (__builtin_expect(__any(strange), 0)) {
+            bool far = before < 0;
+#pragma unroll
+            for (int t = 0; t < CT; ++t) far = far || e[t] > kMostRef;
+            if (__is_same(T, bf16) && __any(far)) {
+                const int enter = before < 0 ? 0 : kFar;
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     sv[k] *= power2(-kFar);
                     av[k] *= power2(-kFar);
                 }
-                st.ref = max(old - enter, min(e - kFar, kFar));
-                st.twice_ref = -1.0f;
-            }
-            down_l = before == 0 ? 0 : old - st.ref;
-            down = before == 0 ? 0 : down_l - enter;
-            // (such a power of two may be past a float's, though nothing scaled by it is: in
-            // steps.  What a factor above 2^-80 and a fall of the weights make 0 is nothing)
-#pragma unroll 1
-            for (; down < -80; down += 80)
 #pragma unroll
                 for (int t = 0; t < CT; ++t) {
-                    st.r[t] *= 0x1p-80f;
-                    st.w[t] *= 0x1p-80f;
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= 0x1p-80f;
+                    now[t] = max(max(old[t] - enter, kLeastRef), min(e[t] - kFar, kFar));
+                    st.twice_ref[t] = -power2(now[t] + 1);
+                    down_l[t] = before == 0 ? 0 : old[t] - now[t];
+                    down[t] = before == 0 ? 0 : down_l[t] - enter;
                 }
-#pragma unroll 1
-            for (; down_l < -80; down_l += 80)
+            }
+            // (such a power of two may be past a float's, though nothing scaled by it is: in
+            // steps.  What a factor above 2^-80 and a fall of the weights make 0 is nothing)
 #pragma unroll
-                for (int t = 0; t < CT; ++t) st.l[t] *= 0x1p-80f;
+            for (int t = 0; t < CT; ++t) {
+#pragma unroll 1
+                for (int step = 0; step < 4; ++step) {
+                    const float f = down[t] < -80 ? 0x1p-80f : 1.0f, fl = down_l[t] < -80 ? 0x1p-80f : 1.0f;
+                    down[t] += down[t] < -80 ? 80 : 0;
+                    down_l[t] += down_l[t] < -80 ? 80 : 0;
+                    st.l[t] *= fl;
+                    st.r[t] *= f;
+                    st.w[t] *= f;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) st.acc[t][i] *= f;
+                }
+            }
         }
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             const float next = fmaxf(st.m[t], column_max<PACK>(mx[t]));
-            const float fall = __builtin_amdgcn_exp2f(st.m[t] - next), f = fall * power2(down);
+            const float fall = __builtin_amdgcn_exp2f(st.m[t] - next), f = fall * power2(down[t]);
             st.m[t] = next;
-            st.l[t] *= fall * power2(down_l);
+            st.shift[t] = kTop - next - static_cast<float>(now[t]);
+            st.l[t] *= fall * power2(down_l[t]);
             st.r[t] *= f;
             st.w[t] *= f;
 #pragma unroll
@@ -581,12 +612,11 @@ __device__ __forceinline__ void attend(const char *blk, const Column<D> (&col)[C
     u32x4 pw[TERMS][CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
-        const float shift = kTop - st.m[t] - static_cast<float>(st.ref);
         uint32_t w[TERMS][V / 2];
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
-            const float a = __builtin_amdgcn_exp2f(fmaf(s[t][e], col[t].to_log2, shift));
-            const float b = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], col[t].to_log2, shift));
+            const float a = __builtin_amdgcn_exp2f(fmaf(s[t][e], col[t].to_log2, st.shift[t]));
+            const float b = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], col[t].to_log2, st.shift[t]));
             st.l[t] += a + b;
             st.r[t] = fmaf(b, av[e + 1], fmaf(a, av[e], st.r[t]));
             const uint32_t one = Mma<f16>::pack2(a * sv[e], b * sv[e + 1]);
@@ -736,10 +766,10 @@ __device__ __forceinline__ void split_pass(const Params &p, float *lds, int b, i
         const int c = wave * COLS + 16 * t + n;
         if (n >= 16 / PACK) continue;  // a copy
         // the sum's unit 2^ref, or one that brings it to 2^-10, which the maximum takes up
-        const int unit = st.far() ? near_1024th(l) : st.ref;
+        const int unit = st.far() ? near_1024th(l) : st.ref(t);
         const float value = power2(st.far() ? unit + kFar : unit);
         if (g == 0) {
-            lm[c] = st.m[t] + static_cast<float>(st.ref - unit);
+            lm[c] = st.m[t] + static_cast<float>(st.ref(t) - unit);
             ll[c] = l * power2(unit);
         }
 #pragma unroll
@@ -876,6 +906,36 @@ __global__ void __launch_bounds__(256) combine_kernel(Params p) {
 
 // ---------------------------------------------------------------- tile route
 
+// The largest magnitude that a row of this pair can hold.
+template <typename T>
+__device__ __forceinline__ float magnitude(uint32_t pair) {
+    return fmaxf(fabsf(hi<T>(pair)), fabsf(fmaf(15.0f, lo<T>(pair), hi<T>(pair))));
+}
+// fp16 holds a row to 2^-11 of this and more, which is enough for columns that see one
+// such key and such a value.
+constexpr float kEnough = 0x1p-14f;
+// Out of what fp16 holds well, of the largest magnitude of all rows.
+__device__ __forceinline__ bool outside(float most) {
+    return most < INFINITY && most > 0.0f && (most > 0x1p15f || most < 0x1p-6f);
+}
+
+// Maxima over the workgroup, through `meet` [N][W].
+template <int N, int W>
+__device__ __forceinline__ void over_waves(float (&x)[N], float *meet) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        x[i] = wave_max(x[i]);
+        if (lane == 0) meet[i * W + wave] = x[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int w = 0; w < W; ++w) x[i] = fmaxf(x[i], meet[i * W + w]);
+    __syncthreads();
+}
+
 // K and V tiles of TILE keys from the cache into LDS as fp16, both row-major (the
 // layout that wave_attend reads with transposing loads): a thread's tasks are
 // 16-byte words of codes, 32 elements of a row.
@@ -915,6 +975,17 @@ struct Widener {
             if (!there) kpair[i] = vpair[i] = 0u;
         }
     }
+    // Whether a key, and a value, of the loaded tile's first `rows` is at least kEnough.
+    __device__ __forceinline__ void enough(int rows, bool &key, bool &value) const {
+        key = value = false;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int t = static_cast<int>(threadIdx.x) + i * NT;
+            if (t % HALF / WORDS >= rows) continue;
+            key = key || magnitude<T>(kpair[i]) >= kEnough;
+            value = value || magnitude<T>(vpair[i]) >= kEnough;
+        }
+    }
     // rows times down_k (keys) and down_v (values)
     __device__ __forceinline__ void store(uint16_t *buf, float down_k, float down_v) {
 #pragma unroll
@@ -923,12 +994,12 @@ struct Widener {
             if (TASKS % NT != 0 && t >= TASKS) continue;
             const int task = t % HALF, word = task % WORDS, row = task / WORDS;
             const bool is_v = t >= HALF;
-            const float vs = lo<T>(vpair[i]), va = hi<T>(vpair[i]), v15 = fmaf(15.0f, vs, va);
-            // a value row that is no number: its key is none (so that it reaches the rows
-            // that see it) and the values 0 (so that it reaches no others)
-            const bool none = v15 != v15;
+            const float vs = lo<T>(vpair[i]), va = hi<T>(vpair[i]);
+            // a value row that is no finite number: its key is none (so that it reaches the
+            // rows that see it) and the values 0 (so that it reaches no others)
+            const bool none = !(fabsf(fmaf(kMiddle, vs, va)) < INFINITY);
             float s = is_v ? vs : lo<T>(kpair[i]), a = is_v ? va : hi<T>(kpair[i]);
-            if (none) s = a = is_v ? 0.0f : v15;
+            if (none) s = a = is_v ? 0.0f : NAN;
             const float most = fmaxf(fabsf(a), fabsf(fmaf(15.0f, s, a)));
             if (is_v) most_v = fmaxf(most_v, most);
             else most_k = fmaxf(most_k, most);
@@ -959,14 +1030,88 @@ constexpr size_t tile_lds() {
     return sizeof(uint16_t) * (kv > o ? kv : o);
 }
 
+// Columns [c, end) of (sequence, kv head) over the keys [from, to), one key after the other
+// in fp32, into the output rows or the states as by column_tile: for sequences whose rows
+// have magnitudes too far apart for one power of two, where a row that a column does not
+// see would leave nothing of those that it sees.
+template <typename T, int D>
+__device__ __forceinline__ void plain_columns(const Params &p, int b, int kvh, long long q_off, int q_start, int c, int end,
+                                              int from, int to, float *part, float *part_ml) {
+    constexpr int N = (D + 63) / 64, AHEAD = 4;
+    const int lane = threadIdx.x & 63;
+    const int *table = p.bt + b * p.bt_stride;
+#pragma unroll 1
+    for (; c < end; ++c) {
+        const int row = c / p.G, seen = p.causal ? min(to, q_start + row + 1) : to;
+        const long long at = ((q_off + row) * p.H + kvh * p.G + (c - row * p.G)) * D;
+        float q[N], out[N], m = kNever, sum = 0.0f;  // out: the mean of the values so far
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int d = lane + 64 * i;
+            q[i] = d < D ? Cvt<T>::to(p.q[at + d]) * p.scale_log2 : 0.0f;
+            out[i] = 0.0f;
+        }
+#pragma unroll 1
+        for (int j0 = from; j0 < seen; j0 += AHEAD) {
+            uint32_t kp[AHEAD], vp[AHEAD];
+            uint8_t k[AHEAD][N], v[AHEAD][N];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int key = min(j0 + u, seen - 1), blk = block_at(p, key);
+                const long long r = row_of(p, kvh, table[blk], key, blk);
+                kp[u] = p.ks[r];
+                vp[u] = p.vs[r];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const long long byte = r * (D / 2) + min(lane + 64 * i, D - 1) / 2;
+                    k[u][i] = p.kc[byte];
+                    v[u][i] = p.vc[byte];
+                }
+            }
+            const auto code = [&](uint8_t x) { return static_cast<float>(lane & 1 ? x >> 4 : x & 15); };
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (j0 + u >= seen) break;
+                float score = 0.0f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) score = fmaf(q[i], fmaf(lo<T>(kp[u]), code(k[u][i]), hi<T>(kp[u])), score);
+                score = wave_sum(score);
+                const float next = fmaxf(m, score), before = sum * __builtin_amdgcn_exp2f(m - next);
+                const float weight = __builtin_amdgcn_exp2f(score - next);
+                m = next;
+                sum = before + weight;
+                const float now = weight / sum, rest = before / sum;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    out[i] = fmaf(out[i], rest, now * fmaf(lo<T>(vp[u]), code(v[u][i]), hi<T>(vp[u])));
+            }
+        }
+        // (as a state: the mean of weights of sum 2^-10)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int d = lane + 64 * i;
+            if (d >= D) continue;
+            if (part != nullptr) part[static_cast<long long>(c) * D + d] = out[i] * 0x1p-10f;
+            else p.o[at + d] = Cvt<T>::from(out[i]);
+        }
+        if (part != nullptr && lane == 0) {
+            part_ml[static_cast<long long>(c) * 2] = sum == 0.0f ? kNever : m + log2f(sum) + 10.0f;
+            part_ml[static_cast<long long>(c) * 2 + 1] = sum == 0.0f ? 0.0f : sum == sum ? 0x1p-10f : sum;
+        }
+    }
+}
+
 // Columns [c0, c0 + 32 W) below `all` of (sequence, kv head) over the keys [from, to): wave w
 // serves columns 32 w .. + 31, column j being query row j / G, head j % G of the
 // group, so that heads of any number fill the waves.  Into the output rows, or with
 // `part` into the states [column][D], (maximum, sum) [column].  Ends with a barrier.
-template <typename T, int D, int W, int TILE>
-__device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, float *meet, int b, int kvh, long long q_off,
+// Keys and values are taken times 2^-ek and 2^-ev.  LOOK: as they are, and false, with
+// nothing written, where fp16 does not hold them well: rows out of its range, or all that
+// some column sees down where it has few bits.
+template <typename T, int D, int W, int TILE, bool LOOK>
+__device__ __forceinline__ bool column_tile(const Params &p, uint16_t *lds, float *meet, int b, int kvh, long long q_off,
                                             int L, int S, int all, int c0, int from, int to, float *part,
-                                            float *part_ml) {
+                                            float *part_ml, int ek = 0, int ev = 0) {
     constexpr int NKB = TILE % 64 == 0 ? 2 : 1, KB = 32 * NKB, COLS = 32 * W;
     using Wd = Widener<T, D, TILE, W * 64>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5, r32 = lane & 31;
@@ -1011,67 +1156,51 @@ __device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, floa
     float m[1], lsum[1];
     f32x16_t oacc[1][D / 32];
     Wd wd;
-    int ek = 0, ev = 0;
+    if (LOOK) ek = ev = 0;
+    bool enough_k = true, enough_v = true;  // among the first tile's keys that all columns see
     const int ntiles = kv_end > from ? (kv_end - from + TILE - 1) / TILE : 0;
-    for (int pass = 0;; ++pass) {
-        const float down_k = power2(-ek), down_v = power2(-ev);
-        const float scale = p.scale_log2 * q_unit * power2(ek), inv_scale = 1.0f / scale;
-        m[0] = kNever;
-        lsum[0] = 0.0f;
+    const float down_k = power2(-ek), down_v = power2(-ev);
+    const float scale = p.scale_log2 * q_unit * power2(ek), inv_scale = 1.0f / scale;
+    m[0] = kNever;
+    lsum[0] = 0.0f;
 #pragma unroll
-        for (int db = 0; db < D / 32; ++db)
+    for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) oacc[0][db][v] = 0.0f;
-        wd.most_k = wd.most_v = 0.0f;
-        const auto buf = [&](int t) { return lds + __builtin_amdgcn_readfirstlane((t & 1) * Wd::ELEMS); };
-        if (ntiles > 0) {
-            wd.pages(p, table, from, to);
-            wd.load(p, kvh, from, to);
-            wd.pages(p, table, from + TILE, to);
-            wd.store(buf(0), down_k, down_v);
+        for (int v = 0; v < 16; ++v) oacc[0][db][v] = 0.0f;
+    wd.most_k = wd.most_v = 0.0f;
+    const auto buf = [&](int t) { return lds + __builtin_amdgcn_readfirstlane((t & 1) * Wd::ELEMS); };
+    if (ntiles > 0) {
+        wd.pages(p, table, from, to);
+        wd.load(p, kvh, from, to);
+        wd.pages(p, table, from + TILE, to);
+        // (the first column that sees a key sees the first)
+        if (LOOK) wd.enough(max(seen(c0) - from, 1), enough_k, enough_v);
+        wd.store(buf(0), down_k, down_v);
+    }
+    const bool wave_k = __any(enough_k), wave_v = __any(enough_v);
+    __syncthreads();
+    for (int it = 0; it < ntiles; ++it) {
+        const uint16_t *cur = buf(it);
+        if (it + 1 < ntiles) {
+            wd.load(p, kvh, from + (it + 1) * TILE, to);
+            wd.pages(p, table, from + (it + 2) * TILE, to);
         }
-        __syncthreads();
-        for (int it = 0; it < ntiles; ++it) {
-            const uint16_t *cur = buf(it);
-            if (it + 1 < ntiles) {
-                wd.load(p, kvh, from + (it + 1) * TILE, to);
-                wd.pages(p, table, from + (it + 2) * TILE, to);
+#pragma unroll
+        for (int hb = 0; hb < TILE / KB; ++hb) {
+            const int j0 = from + it * TILE + KB * hb;
+            if (j0 < wave_end) {
+                const int lim[1] = {vis - j0 - 4 * g};
+                wave_attend<f16, D, Wd::KP, 0, Wd::VR, NKB, 1, true>(cur, cur + Wd::VOFF, KB * hb, qf, oacc, m, lsum,
+                                                                    lim, scale, inv_scale, j0 + KB > wave_least);
             }
-#pragma unroll
-            for (int hb = 0; hb < TILE / KB; ++hb) {
-                const int j0 = from + it * TILE + KB * hb;
-                if (j0 < wave_end) {
-                    const int lim[1] = {vis - j0 - 4 * g};
-                    wave_attend<f16, D, Wd::KP, 0, Wd::VR, NKB, 1, true>(cur, cur + Wd::VOFF, KB * hb, qf, oacc, m, lsum,
-                                                                        lim, scale, inv_scale, j0 + KB > wave_least);
-                }
-            }
-            if (it + 1 < ntiles) wd.store(buf(it + 1), down_k, down_v);
-            __syncthreads();
         }
-        // rows out of fp16's range, or all of them down where it has few bits: once
-        // more, with the power of two that their largest asks for
-        if (pass == 1) break;
-        const float mk = wave_max(wd.most_k), mv = wave_max(wd.most_v);
-        if (lane == 0) {
-            meet[wave] = mk;
-            meet[W + wave] = mv;
-        }
+        if (it + 1 < ntiles) wd.store(buf(it + 1), down_k, down_v);
         __syncthreads();
-        float all_k = 0.0f, all_v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            all_k = fmaxf(all_k, meet[w]);
-            all_v = fmaxf(all_v, meet[W + w]);
-        }
-        __syncthreads();
-        const auto outside = [](float most) { return most < INFINITY && most > 0.0f && (most > 0x1p15f || most < 0x1p-6f); };
-        if (!outside(all_k) && !outside(all_v)) break;
-        const auto power = [&](float most) {
-            return outside(most) ? min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127 - 10, -110), 118) : 0;
-        };
-        ek = __builtin_amdgcn_readfirstlane(power(all_k));
-        ev = __builtin_amdgcn_readfirstlane(power(all_v));
+    }
+    if (LOOK) {
+        float of[4] = {wd.most_k, wd.most_v, wave_k ? 1.0f : 0.0f, wave_v ? 1.0f : 0.0f};
+        over_waves<4, W>(of, meet);
+        if (outside(of[0]) || outside(of[1]) || of[2] * of[3] == 0.0f) return false;
     }
     const float lt = half_swap_sum(lsum[0]);
     if (part != nullptr) {
@@ -1091,7 +1220,7 @@ __device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, floa
                 *reinterpret_cast<float2_t *>(part_ml + static_cast<long long>(j) * 2) =
                     float2_t{m[0] - static_cast<float>(up), lt * power2(up)};
         }
-        return;  // (the loop's last barrier has passed)
+        return true;  // (the loop's last barrier has passed)
     }
     // O leaves through LDS, a column at a time
     constexpr int OROW = D + 8, RCH = D / 8, NOC = (COLS * RCH + W * 64 - 1) / (W * 64);
@@ -1113,6 +1242,67 @@ __device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, floa
             *reinterpret_cast<const u32x4 *>(lds + c * OROW + (t - c * RCH) * 8);
     }
     __syncthreads();
+    return true;
+}
+
+// The tiles of a workgroup once more (from the start, so that nothing is kept for it
+// through them), with the powers of two that their rows ask for.  A tile whose largest row
+// is more than 2^24 above all that some column sees is done without: one power of two
+// would leave that column less than 11 bits.
+template <typename T, int D, int W, int TILE>
+__device__ __forceinline__ void careful_tiles(const Params &p, uint16_t *lds, float *meet) {
+    constexpr long long COLS = 32 * W;
+    const int kvh = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, wave = threadIdx.x >> 6;
+    const int split = blockIdx.y % p.splits, tile = p.tiles - 1 - blockIdx.y / p.splits;
+    const int *table = p.bt + b * p.bt_stride;
+    long long q_off;
+    int L, S;
+    sequence(p, b, q_off, L, S);
+    const int all = p.G * L, q_start = p.causal ? max(S - L, 0) : 0, ns = splits_of(p, S);
+    const long long at = (static_cast<long long>(b) * p.Hkv + kvh) * p.splits + split, step = COLS * p.tiles;
+#pragma unroll 1
+    for (long long c = tile * COLS; c < all; c += step) {
+        const bool in_grid = c < p.cols, split_up = in_grid && p.splits > 1;
+        if (split >= ns || (split != 0 && !in_grid)) return;
+        const int c0 = static_cast<int>(c), end = in_grid ? min(all, p.cols) : all;
+        const int from = split_up ? split * p.split_len : 0, to = split_up && split < ns - 1 ? from + p.split_len : S;
+        float *const part = split_up ? p.ws_o + at * p.cols * D : nullptr;
+        float *const part_ml = split_up ? p.ws_ml + at * p.cols * 2 : nullptr;
+        const auto seen = [&](int j) { return p.causal ? min(to, q_start + j / p.G + 1) : to; };
+        const int last = seen(static_cast<int>(min(c + COLS, static_cast<long long>(end))) - 1);
+        const int first_end = max(seen(c0), from + 1);
+        // of keys and values: the largest, the largest that all columns see, the least of the rest
+        float most[2] = {0.0f, 0.0f}, own[4] = {0.0f, 0.0f, -INFINITY, -INFINITY};
+        for (int key = from + static_cast<int>(threadIdx.x); key < last; key += W * 64) {
+            const int blk = block_at(p, key);
+            const long long r = row_of(p, kvh, table[blk], key, blk);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float x = magnitude<T>(i == 0 ? p.ks[r] : p.vs[r]);
+                if (!(x < INFINITY)) continue;
+                most[i] = fmaxf(most[i], x);
+                if (key < first_end) own[i] = fmaxf(own[i], x);
+                else if (x > 0.0f) own[2 + i] = fmaxf(own[2 + i], -x);
+            }
+        }
+        over_waves<2, W>(most, meet);
+        over_waves<4, W>(own, meet);
+        int e[2];
+        bool apart = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float least = own[i] > 0.0f ? own[i] : -own[2 + i];  // (rows of zeros are held whole)
+            const bool again = outside(most[i]) || least < kEnough;
+            apart = apart || (again && least < most[i] * 0x1p-24f);
+            e[i] = __builtin_amdgcn_readfirstlane(
+                again ? min(max(static_cast<int>(__float_as_uint(most[i]) >> 23) - 127 - 10, -110), 118) : 0);
+        }
+        const int cw0 = c0 + 32 * wave;
+        if (apart) plain_columns<T, D>(p, b, kvh, q_off, q_start, cw0, min(cw0 + 32, end), from, to, part, part_ml);
+        else column_tile<T, D, W, TILE, false>(p, lds, meet, b, kvh, q_off, L, S, end, c0, from, to, part, part_ml, e[0], e[1]);
+        __syncthreads();
+        if (in_grid) c = p.cols + tile * COLS - step;  // (those past the grid start at its end)
+    }
 }
 
 // Workgroup (sequence, kv head) and (column tile, split), the heaviest tiles first;
@@ -1121,7 +1311,7 @@ __device__ __forceinline__ void column_tile(const Params &p, uint16_t *lds, floa
 template <typename T, int D, int W, int TILE>
 __global__ void __launch_bounds__(W * 64, W >= 12 ? 3 : D <= 128 && W == 4 ? 3 : 2) tile_kernel(Params p) {
     extern __shared__ __attribute__((aligned(16))) uint16_t tiles_lds[];
-    __shared__ float meet[2 * W];
+    __shared__ float meet[4 * W];
     if (blockIdx.x == 0 && blockIdx.y == 0) zero_tail(p, D);
     constexpr int COLS = 32 * W;
     const int kvh = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
@@ -1132,23 +1322,27 @@ __global__ void __launch_bounds__(W * 64, W >= 12 ? 3 : D <= 128 && W == 4 ? 3 :
     if (L <= 0) return;
     const int all = p.G * L, bound = min(all, p.cols);
     int c0 = tile * COLS;
+    bool done = true;
     if (c0 < bound && p.splits == 1) {
-        column_tile<T, D, W, TILE>(p, tiles_lds, meet, b, kvh, q_off, L, S, bound, c0, 0, S, nullptr, nullptr);
+        done = column_tile<T, D, W, TILE, true>(p, tiles_lds, meet, b, kvh, q_off, L, S, bound, c0, 0, S, nullptr, nullptr);
     } else if (c0 < bound) {
         const int ns = splits_of(p, S);
         const long long at = (static_cast<long long>(b) * p.Hkv + kvh) * p.splits + split;
         if (split < ns)
-            column_tile<T, D, W, TILE>(p, tiles_lds, meet, b, kvh, q_off, L, S, bound, c0, split * p.split_len,
-                                       split == ns - 1 ? S : (split + 1) * p.split_len, p.ws_o + at * p.cols * D,
-                                       p.ws_ml + at * p.cols * 2);
+            done = column_tile<T, D, W, TILE, true>(p, tiles_lds, meet, b, kvh, q_off, L, S, bound, c0, split * p.split_len,
+                                              split == ns - 1 ? S : (split + 1) * p.split_len, p.ws_o + at * p.cols * D,
+                                              p.ws_ml + at * p.cols * 2);
     }
-    if (split != 0) return;
-    for (long long past = p.cols + static_cast<long long>(tile) * COLS; past < all;
-         past += static_cast<long long>(p.tiles) * COLS) {
-        c0 = static_cast<int>(past);
-        __syncthreads();
-        column_tile<T, D, W, TILE>(p, tiles_lds, meet, b, kvh, q_off, L, S, all, c0, 0, S, nullptr, nullptr);
+    if (split == 0) {
+        for (long long past = p.cols + static_cast<long long>(tile) * COLS; past < all;
+             past += static_cast<long long>(p.tiles) * COLS) {
+            c0 = static_cast<int>(past);
+            __syncthreads();
+            if (!column_tile<T, D, W, TILE, true>(p, tiles_lds, meet, b, kvh, q_off, L, S, all, c0, 0, S, nullptr, nullptr))
+                done = false;
+        }
     }
+    if (!done) careful_tiles<T, D, W, TILE>(p, tiles_lds, meet);
 }
 
 // ------------------------------------------------------------------- host
@@ -1176,7 +1370,7 @@ tecoopsStatus_t launch_split(const Params &p, const Plan &pl, hipStream_t s) {
 template <typename T, int D, int W, int TILE>
 tecoopsStatus_t launch_tiles(const Params &p, const Plan &pl, hipStream_t s) {
     constexpr size_t lds = tile_lds<D, TILE, W>();
-    static_assert(lds + 8 * W <= tecoops::kLdsMax, "fits the LDS");
+    static_assert(lds + 16 * W <= tecoops::kLdsMax, "fits the LDS");
     auto *kern = &tile_kernel<T, D, W, TILE>;
     if (!tecoops::reserve_lds(reinterpret_cast<const void *>(kern), lds)) return TECOOPS_STATUS_INTERNAL_ERROR;
     hipLaunchKernelGGL(kern, dim3(p.batch * p.Hkv, pl.tiles * pl.splits), dim3(W * 64), lds, s, p);
