@@ -1125,7 +1125,7 @@ __device__ __forceinline__ bool column_tile(const Params &p, uint16_t *lds, floa
     const int j = min(cw0 + r32, all - 1), row = j / p.G;
     const int vis = seen(j);
 
-    // the wave's queries in fp16, their largest element to [2^8, 2^9)
+    // the wave's queries in fp16, each with its largest element to [2^8, 2^9)
     u32x4 qf[1][D / 16];
     float q_unit;
     {
@@ -1141,7 +1141,7 @@ __device__ __forceinline__ bool column_tile(const Params &p, uint16_t *lds, floa
                 most = max(most, max(a & 0xffffu, a >> 16));
             }
         }
-        const float big = wave_max(Cvt<T>::to(static_cast<uint16_t>(most)));
+        const float big = half_swap_max(Cvt<T>::to(static_cast<uint16_t>(most)));
         int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
         e = min(max(e, -100), 120);
         const float up = power2(8 - e);

@@ -98,3 +98,25 @@ def test_nan_and_far_rows():
     nan = torch.zeros(70, 8, dtype=torch.bool)
     nan[60:, :4] = True  # (row r sees keys up to 20 + r)
     assert torch.equal(torch.isnan(got.cpu()).all(-1), nan) and torch.equal(torch.isnan(got.cpu()).any(-1), nan)
+
+
+@pytest.mark.parametrize("dt,what", [(t, x) for t in ("f16", "bf16") for x in (float("inf"), float("nan"), 2.0 ** 13)] +
+                         [("bf16", 2.0 ** 30), ("bf16", 2.0 ** 100)])
+@pytest.mark.parametrize("rows,H,lens,D", SHAPES)
+def test_query_rows_of_other_sizes(rows, H, lens, D, what, dt):
+    """One query row (of one head) infinite, none or large: the others are what they are."""
+    dtype = DTYPES[dt]
+    held = cache(lens, 2, D, 16, dtype, seed=1)
+    q = rand(sum(rows), H, D, dtype=dtype, seed=2)
+    ref, mass, reach = attention(q, *held[:4], [0, rows[0], sum(rows)], lens, held[4])
+    r, h = rows[0] // 2, H - 1
+    if what - what == 0:
+        q[r, h] *= what / 4
+    else:
+        q[r, h, 3] = what
+    got, _ = run(q, held, lens, rows)
+    others = torch.ones(sum(rows), H, dtype=torch.bool)
+    others[r, h] = False
+    check(got.cpu()[others], ref[others], bound(ref, mass, reach, dtype, widened(dtype, H // 2, rows))[others], "others")
+    if what - what != 0:
+        assert torch.isnan(got[r, h]).all()
