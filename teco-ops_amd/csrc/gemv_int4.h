@@ -8,7 +8,7 @@
 namespace tecoops {
 
 constexpr int kGemvInt4Stage = 512;  // of K, staged at a time by the matrix-core kernel
-constexpr int kGemvInt4DotK = 4096;  // the longest K of the kernel of one row of x
+constexpr int kGemvInt4DotK = 8192;  // the longest K of the kernel of one row of x
 constexpr int kGemvInt4Rows = 64;    // rows of W of its workgroups
 
 // Stages of a K of up to 2^31 - 1.
@@ -51,10 +51,11 @@ inline GemvInt4Plan gemv_int4_plan(int batch, int n, int k, size_t room, int cus
     // as many parts as leave a workgroup a CU, two stages each or more
     const long long most = std::min<long long>(cus / std::max(wgs, 1ll), stages / 2);
     p.parts = static_cast<int>(std::max(1ll, std::min<long long>(most, static_cast<long long>(room / part))));
-    // one row over a short K takes about as long in either kernel, but two launches
-    // here where K is split (us, dot / this and the sums of its parts: 4096 x 4096
-    // 6.8 / 4.6 + 1.8, 2048 x 2048 5.9 / 4.9 + 2.0; 28672 x 4096 20.7 / 15.5,
-    // 4096 x 14336 18.4 / 10.2 + 2.0)
+    // one row where K would be split, which takes a second launch (us, dot / this and
+    // the sums of its parts, fp16, groups of 128, calls of a graph: 2048 x 2048 3.6 / 6.5,
+    // 4096 x 4096 4.6 / 7.5, 256 x 8192 5.3 / 7.0, 8192 x 8192 9.8 / 13.0; past that a few
+    // long rows are faster split, 256 x 14336 7.9 / 7.0, and many are not, 4096 x 14336
+    // 9.7 / 12.7).  Unsplit, this is the faster: 28672 x 4096 20.7 / 15.5
     p.dot = batch == 1 && most > 1 && k <= kGemvInt4DotK;
     if (p.dot) p.parts = 1;
     p.bytes = p.parts > 1 ? part * p.parts : 0;

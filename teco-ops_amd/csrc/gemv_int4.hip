@@ -87,8 +87,8 @@ __device__ __forceinline__ u32x4 interleaved(const u32x4 &v) {
 // products is infinite or finite.  Then elements [k0, k1) (whole runs of 32) of output
 // (n, b) are summed by the whole wave, each weight on its own, but for rows of x with a
 // NaN there, whose outputs are NaN.  ([28672, 4096], 16 rows of x, the same call again and
-// again: 20.4 us, one row with a NaN 24, all of them 86.  Looking for such sums costs
-// [4096, 14336], 33 rows 0.7 us, [28672, 4096], 16 rows 0.1.)
+// again: 20.4 us, one row with a NaN 24, all of them 86.  Looking for such sums costs less
+// than 0.2.)
 template <typename T>
 __device__ __forceinline__ bool holds_nan(const Args &a, int b, int k0, int k1) {
     constexpr uint32_t kInf = __is_same(T, f16) ? 0x7c00u : 0x7f80u;
@@ -188,13 +188,25 @@ __global__ void __launch_bounds__(kThreads) dot_kernel(Args a) {
             }
         }
     }
+    bool whole = true;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-        float v = wave_sum(acc[r]);
-        if (n0 + r < a.n && !(fabsf(v) < INFINITY))
-            v = holds_nan<T>(a, 0, 0, a.k) ? NAN : direct_sum<T>(a, n0 + r, 0, 0, a.k);
-        if (lane == 0 && n0 + r < a.n) a.y[n0 + r] = Cvt<T>::from(v);
+        acc[r] = wave_sum(acc[r]);
+        whole = whole && (fabsf(acc[r]) < INFINITY || n0 + r >= a.n);
     }
+    if (__builtin_expect(!whole, 0)) {
+        const bool nan = holds_nan<T>(a, 0, 0, a.k);
+#pragma unroll 1
+        for (int i = 0; i < kRows && n0 + i < a.n; ++i) {
+            const float sum = nan ? NAN : direct_sum<T>(a, n0 + i, 0, 0, a.k);
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+                if (r == i && !(fabsf(acc[r]) < INFINITY)) acc[r] = sum;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+        if (lane == 0 && n0 + r < a.n) a.y[n0 + r] = Cvt<T>::from(acc[r]);
 }
 
 template <typename T>
