@@ -473,8 +473,9 @@ tecoopsStatus_t tecoopsRotaryAxesReshapeAndCache(tecoopsHandle_t handle, const i
  * NULL, with key_weight.  Positions, sections and layout are those of
  * tecoopsRotaryEmbeddingAxes; sections may be NULL for one axis.  A token with a
  * position outside the cos_sin_cache is left as it is, not normalised either.
- * head_size up to 1024, fewer than 2^24 tokens (head sizes in whole 16-byte words,
- * aligned, up to 512 are fastest; others up to 2^25 heads of all tokens). */
+ * head_size up to 1024, fewer than 2^24 tokens, up to 2^20 heads a token (head sizes in
+ * whole 16-byte words, aligned, up to 512 are fastest; others up to 2^25 heads of all
+ * tokens). */
 tecoopsStatus_t tecoopsQkNormRotary(tecoopsHandle_t handle, const int64_t *positions,
                                     long long position_stride, int axes, const int *sections,
                                     tecoopsRotaryLayout_t layout, void *query, void *key,
@@ -508,7 +509,8 @@ tecoopsStatus_t tecoopsQkNormRotaryReshapeAndCache(
  * 2], element 2j in the low half of byte j; key_scales / value_scales dataType
  * [num_blocks, num_kv_heads, block_size, 2].  Slots < 0 or past the cache are not
  * stored; a slot is at most once in a call.  head_size a multiple of 8 up to 512;
- * fewer than 2^26 (token, head) rows; strides and num_kv_heads * block_size below 2^32;
+ * fewer than 2^26 (token, head) rows; strides and num_kv_heads * block_size below 2^32,
+ * num_kv_heads * head_size below 2^30, num_blocks * block_size below 2^31;
  * num_tokens = 0 is done without a launch. */
 tecoopsStatus_t tecoopsReshapeAndCacheInt4(tecoopsHandle_t handle, const void *key,
                                            const void *value, const int64_t *slot_mapping,
@@ -524,9 +526,12 @@ tecoopsStatus_t tecoopsReshapeAndCacheInt4(tecoopsHandle_t handle, const void *k
  * alone), but the softmax has no clamp at 0, so that scores of any size are
  * weighed.  q and out [total_q, num_heads, head_size] packed; block_table int32
  * [batch, blocks_per_seq], rows block_table_stride apart; head_size in {32, 64,
- * 96, 128, 160, 192}.  fp16, and in bf16 up to 64 (query row, head) pairs of a kv head,
+ * 96, 128, 160, 192}; total_q * num_heads / num_kv_heads below 2^31, batch * num_kv_heads
+ * up to 2^22.  fp16, and in bf16 up to 64 (query row, head) pairs of a kv head,
  * read K and V as they are held; longer queries in bf16 widen them to fp16 first (one
  * more rounding, finer than the output's; fp16 prompts take up to twice as long).
+ * Weights and values are held relative to the largest that a query row sees: rows 2^24
+ * below it and further lose digits.
  * What the cache holds behind a sequence's last key is not used, whatever it is.  A key
  * or value row of NaN, or a value row whose pair is infinite, makes the rows that see it
  * NaN and no others; large rows change nothing for the query rows that do not see them.
@@ -551,7 +556,9 @@ tecoopsStatus_t tecoopsGetFlashAttentionInt4WorkspaceSize(int batch, int total_q
  * low half of byte j; scales and zeros dataType [n, k / group_size] (zeros NULL: 8
  * everywhere; they need not be whole); x [batch, k], y [batch, n].  group_size a
  * multiple of 32 that divides k.  For decode batches: the weights are read again
- * for every 64 rows of x; batch = 0 is done without a launch.
+ * for every 64 rows of x; batch = 0 is done without a launch.  n up to 2^26, batch up to
+ * 2^16, n * batch below 2^27 (more rows of x in slices).  Infinite and very large x are
+ * taken as the formula has them (their sums again, one weight at a time: slower).
  * workspace: tecoopsGetGemvInt4WorkspaceSize() bytes for the same sizes let few rows
  * of W be split along k; with less, or NULL, there are fewer splits (slower, the
  * same result up to fp32 rounding).  Nothing is allocated. */

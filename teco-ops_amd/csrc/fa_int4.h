@@ -21,11 +21,13 @@ struct Plan {
 
 constexpr int kWaves = 4;                 // of a workgroup of the split route
 constexpr int kLeastSplit = 32 * kWaves;  // keys: a block of 32 for each wave
-// Columns that the split route serves: both routes take as long at some 90 of them (split
-// / tile route, us, 16 sequences of 4096 keys, 8 kv heads of 128: 32 columns 35.1 / 49.6,
-// 64 47.0 / 56.2, 96 67.7 / 65.1, 128 84.1 / 71.9).  In fp16 it serves any number: the
+// Columns that the split route serves: two tiles of 32, past which it takes a third and the
+// other is faster (split / tile route, us, bf16, 8 kv heads of 128: 16 sequences of 4096
+// keys, 32 columns 38.5 / 49.7, 64 53.2 / 56.0, 72 72.2 / 63.4, 96 73.2 / 66.6; 4 of 2048, 64
+// columns 20.1 / 20.2, 72 26.0 / 20.7; one of 16384, 64 columns 27.8 / 33.7, 72 34.6 / 35.3;
+// 64 of 1000, 64 columns 60.1 / 56.6, 72 83.1 / 57.9).  In fp16 it serves any number: the
 // widened tiles' roundings are seen there (5e-4 against 2.1e-4, rms, of the output's own).
-// 8 sequences of 1000 keys, 400 columns 57 / 47 us, 4 of 4096, 8192 columns 875 / 459.
+// 8 sequences of 1000 keys, 400 columns 60 / 48 us, 4 of 4096, 8192 columns 934 / 435.
 constexpr int kSplitCols = 64;
 
 constexpr long long kMostWorkgroups = 1ll << 22;  // of a grid, whose threads stay within 32 bits

@@ -42,7 +42,11 @@
 // row is more than 2^24 above all that some column sees, key by key in fp32.  Rounded are
 // K, V and the weights, each to 2^-11, which is unseen beside a bf16 output.  Beside an
 // fp16 one it is seen (4e-4 to 6e-4, rms, against 2.1e-4), so that fp16 models have the
-// split route for any number of columns, at up to twice the time.
+// split route for any number of columns, at up to twice the time.  Matrix cores are busy
+// 39 % of the cycles, vector units 44 %, at the 12 waves a CU that LDS leaves room for: issue
+// and waits in between.  [4 sequences, 2048 rows on up to 4096 keys, 32 heads on 8 of 128]
+// 404 us, 800 TFLOP/s of visible pairs (fp16 by the split route 700); [2 of up to 203 rows on
+// 16300 keys, 40 heads] 142 us, 760 (fp16 220).
 #include <cmath>
 
 #include "fa_device.h"
