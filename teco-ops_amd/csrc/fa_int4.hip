@@ -1080,6 +1080,7 @@ __device__ __forceinline__ void plain_columns(const Params &p, int b, int kvh, l
 #pragma unroll
                 for (int i = 0; i < N; ++i) score = fmaf(q[i], fmaf(lo<T>(kp[u]), code(k[u][i]), hi<T>(kp[u])), score);
                 score = wave_sum(score);
+                if (!(fabsf(fmaf(kMiddle, lo<T>(vp[u]), hi<T>(vp[u]))) < INFINITY)) score = NAN;  // (as in the tiles)
                 const float next = fmaxf(m, score), before = sum * __builtin_amdgcn_exp2f(m - next);
                 const float weight = __builtin_amdgcn_exp2f(score - next);
                 m = next;

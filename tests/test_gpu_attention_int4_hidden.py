@@ -120,3 +120,19 @@ def test_query_rows_of_other_sizes(rows, H, lens, D, what, dt):
     check(got.cpu()[others], ref[others], bound(ref, mass, reach, dtype, widened(dtype, H // 2, rows))[others], "others")
     if what - what != 0:
         assert torch.isnan(got[r, h]).all()
+
+
+@pytest.mark.parametrize("power", [0, 60])
+@pytest.mark.parametrize("rows,H", [(3, 4), (9, 8), (70, 8), (100, 8)])
+def test_infinite_value_rows_are_none(power, rows, H):
+    """A value row whose pair is infinite makes the rows that see it NaN, and no others, in
+    every form (2^60 apart: key by key)."""
+    held = larger(cache([130], 2, 128, 16, torch.bfloat16, seed=1), [130], 3, power)
+    for i, (key, pair) in enumerate(((127, (float("inf"), 0.0)), (128, (0.0, -float("inf"))))):
+        held[3][held[4][0, key // 16], i, key % 16] = torch.tensor(pair, dtype=torch.bfloat16)
+    q = rand(rows, H, 128, dtype=torch.bfloat16)
+    got, _ = run(q, held, [130], [rows])
+    nan = torch.zeros(rows, H, dtype=torch.bool)
+    nan[rows - 3:, :H // 2] = True  # (row r sees keys up to 130 - rows + r)
+    nan[rows - 2:, H // 2:] = True
+    assert torch.equal(torch.isnan(got.cpu()).all(-1), nan) and torch.isfinite(got.cpu()[~nan]).all()
